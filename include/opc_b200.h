@@ -350,6 +350,118 @@ int opc_coo_gemv(int32_t M, const int32_t* row_ptr, const int32_t* cols, const f
 int opc_coo_scatter(int32_t M, const int32_t* row_ptr, const int32_t* cols, const void* values_f16, void* w, int64_t ldw,
                     void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Paged key/value cache held in 4 bits: append (with the rotary embedding), read back, attention.
+ *
+ * The cache is n_pages pages of page_size tokens.  A page holds, for each kv head, one block of
+ * head_bytes = page_size * (head_dim + 8) bytes:
+ *   key codes    [page_size][head_dim/2]  4-bit codes: dimension d is the low (d even) or high
+ *                                         (d odd) nibble of byte d/2
+ *   value codes  [page_size][head_dim/2]
+ *   key pairs    [page_size]              fp16 scale (low half), fp16 zero (high half)
+ *   value pairs  [page_size]
+ * A stored value stands for scale * (code + zero).  opc_kv_append stores a head x as
+ *   scale = max(fp16(max((max x - min x) / 15, max |x| / 1024)), 2^-24)
+ *   zero  = fp16(min x / scale)
+ *   code  = clamp(round(x / scale - zero), 0, 15)        (round to even, in fp32)
+ * -- the max |x| / 1024 term keeps |zero| <= 1024, so the pair's own rounding stays below half a
+ * step for heads whose values lie far from 0.  A head with an infinity or NaN (or beyond the
+ * range of an fp16 scale) is stored with a NaN scale, zero and codes 0: what attends to it is NaN.
+ * --------------------------------------------------------------------------------------------- */
+enum { OPC_F16 = 0, OPC_BF16 = 1, OPC_F32 = 2 };  /* element types */
+
+typedef struct opc_kv_cache {
+  int32_t kv_heads, head_dim;     /* head_dim 32, 64, 96, 128, 192 or 256 */
+  int32_t page_size, n_pages;     /* tokens per page: 16, 32, 64, 128 or 256 */
+  int64_t head_bytes;             /* one page of one kv head: page_size * (head_dim + 8) */
+  int64_t total_bytes;            /* n_pages * kv_heads * head_bytes */
+  void* pages;                    /* device, 16-byte aligned: [n_pages][kv_heads][head_bytes] */
+} opc_kv_cache;
+
+/* The rows (tokens) of one call, packed: rows q_start[s] .. q_start[s+1] are the last q_len rows
+ * of sequence s, which holds kv_len[s] tokens once they are appended.  Row i of them is at
+ * position kv_len - q_len + i, in page page_table[s][position / page_size].  Sequences may be
+ * empty.  Rows outside [q_start[0], q_start[n_seqs]) and rows at negative positions belong to
+ * nothing: no call reads or writes anything for the first, and the second (kv_len < q_len) are
+ * not stored and attend to nothing.  Table entries past a sequence's last page are not read.
+ * max_q and max_kv bound the sequences' q_len and kv_len on the host (they size the grids; the
+ * lengths themselves are read on the device, so a captured graph replays with new ones): keys
+ * beyond max_kv or beyond the table are not read, and a row that would be stored there, a page
+ * outside [0, n_pages) and a q_len above max_q raise device error 2 (opc_take_device_error) and
+ * are skipped. */
+typedef struct opc_kv_batch {
+  int32_t n_seqs, n_tokens;       /* sequences; rows in q, k, v and out */
+  int32_t max_q, max_kv;
+  const int32_t* q_start;         /* device [n_seqs + 1], not decreasing */
+  const int32_t* kv_len;          /* device [n_seqs] */
+  const int32_t* page_table;      /* device [n_seqs][table_stride] */
+  int64_t table_stride;
+  int32_t max_pages;              /* table entries per sequence that may be read */
+} opc_kv_batch;
+
+/* Rotary embedding: the first rot_dim dimensions of a head (a multiple of 16) are turned in pairs,
+ * pair i by the angle position * f_i; pairs are (i, i + rot_dim/2), or (2i, 2i+1) when
+ * interleaved.  turns[i] is f_i / 2pi as a 64-bit binary fraction (opc_rope_turns): position *
+ * turns modulo 2^64 is the angle modulo one turn without rounding, at any position. */
+typedef struct opc_rope {
+  int32_t rot_dim, interleaved;
+  const uint64_t* turns;          /* device [rot_dim / 2] */
+} opc_rope;
+
+/* Sizes of a cache (host only; `pages` is left for the caller). */
+int opc_kv_plan(int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t n_pages, opc_kv_cache* cache);
+
+/* f[n] (radians per position, host) as 64-bit fractions of a turn (host). */
+int opc_rope_turns(const double* f, int32_t n, uint64_t* turns);
+
+/* Append the batch's rows: k (turned by `rope`, NULL: not turned) and v, quantized into the pages;
+ * q, if given, is turned into q_out (which may be q itself).  Row r, head h of k is at
+ * k + r * ldk + h * head_dim (likewise v, q, q_out; leading dimensions in elements), so the parts
+ * of one fused q|k|v row can be passed as they are.  dtype OPC_F16 or OPC_BF16, one for all.  The
+ * turned values are formed in fp32; angles are exact and their sine and cosine correctly rounded.
+ * Two rows of a call must not fall on the same place of a page. */
+int opc_kv_append(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads, int32_t dtype,
+                  const opc_rope* rope, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* q,
+                  int64_t ldq, void* q_out, int64_t ldqo, void* stream);
+
+/* What the cache holds at the batch's rows, as OPC_F16 or OPC_BF16 (k is as stored: turned; a
+ * value that lies a fraction of a step beyond fp16's range is read as its largest).
+ * Rows without a place in the cache (see opc_kv_batch) are left as they were. */
+int opc_kv_read(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t dtype, void* k, int64_t ldk, void* v,
+                int64_t ldv, void* stream);
+
+/* Causal grouped-query attention of the batch's rows over the cache:
+ *   out[r][h] = sum_j softmax_j(scale * q[r][h] . k[j][h / (heads/kv_heads)]) v[j][...]
+ * over the positions j <= the row's own, with k and v as the cache holds them.  lse (may be NULL):
+ * [n_tokens][heads] fp32, the natural logarithm of the softmax's sum.  A row that sees no key
+ * gives out 0 and lse -infinity.  dtype (of q and out) OPC_F16 or OPC_BF16.  Statistics and sums in
+ * fp32; deterministic.  The workspace (opc_kv_attention_workspace_bytes; 0 for a refused request)
+ * is zero-filled once before first use (opc_workspace_init), is not to be shared with opc_gemv, and
+ * serves any calls that are ordered on one stream; calls that may overlap, replays of two graphs
+ * among them, need one each. */
+size_t opc_kv_attention_workspace_bytes(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads,
+                                        int32_t device);
+int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads, int32_t dtype, float scale,
+                     const void* q, int64_t ldq, void* out, int64_t ldo, float* lse, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* Log probabilities of given tokens under the rows of a [rows][vocab] logits matrix (row r at
+ * logits + r * ld; OPC_F16, OPC_BF16 or OPC_F32):
+ *   logprob[r]  = x[targets[r]] - lse(x)       a negative target gives 0 (no token there)
+ *   entropy[r]  = -sum p log p                 (natural logarithms, p log p = 0 at p = 0)
+ *   top_ids[r][i], top_logprobs[r][i], i < top_k: the largest logits in order, equal ones by the
+ *                                              lower id
+ * targets/logprob, entropy and the two top arrays may be NULL (top_k 0); top_k at most 32 and at
+ * most vocab.  Logits of -infinity are tokens of probability 0.  A row of nothing else gives
+ * logprob and top_logprobs -infinity and entropy 0; a row with a NaN or +infinity gives NaN for
+ * all of them (its ids are ordered with NaN below everything).  A target >= vocab gives NaN and
+ * device error 2.  Sums in fp32; deterministic.  The workspace
+ * (opc_token_logprobs_workspace_bytes) follows opc_kv_attention's rules. */
+size_t opc_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top_k, int32_t device);
+int opc_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int32_t rows, int32_t vocab,
+                       const int32_t* targets, float* logprob, float* entropy, int32_t top_k, int32_t* top_ids,
+                       float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
+
 /* XXH64 (seed `seed`) of a HOST buffer: the checksum that the .bf2 layout places after the last
  * layer (opacc1ty/format/header.py:26; the reference documents it but never writes it).  Files
  * written with it set bit 0 of the file header's flags.  A format helper, not a kernel. */

@@ -101,6 +101,43 @@ class DeviceProps(ctypes.Structure):
     ]
 
 
+OPC_F16, OPC_BF16, OPC_F32 = 0, 1, 2
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = [
+        ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("n_pages", ctypes.c_int32),
+        ("head_bytes", ctypes.c_int64),
+        ("total_bytes", ctypes.c_int64),
+        ("pages", ctypes.c_void_p),
+    ]
+
+
+class KvBatch(ctypes.Structure):
+    _fields_ = [
+        ("n_seqs", ctypes.c_int32),
+        ("n_tokens", ctypes.c_int32),
+        ("max_q", ctypes.c_int32),
+        ("max_kv", ctypes.c_int32),
+        ("q_start", ctypes.c_void_p),
+        ("kv_len", ctypes.c_void_p),
+        ("page_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_int64),
+        ("max_pages", ctypes.c_int32),
+    ]
+
+
+class Rope(ctypes.Structure):
+    _fields_ = [
+        ("rot_dim", ctypes.c_int32),
+        ("interleaved", ctypes.c_int32),
+        ("turns", ctypes.c_void_p),
+    ]
+
+
 # Exported symbols and their prototypes: (restype, argtypes).  Kept in the order of the header.
 _c = ctypes
 PROTOTYPES = {
@@ -165,6 +202,29 @@ PROTOTYPES = {
                                _c.c_void_p, _c.c_int64, _c.c_int32, _c.c_void_p]),
     "opc_coo_scatter": (_c.c_int, [_c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int64,
                                   _c.c_void_p]),
+    "opc_kv_plan": (_c.c_int, [_c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32, _c.POINTER(KvCache)]),
+    "opc_rope_turns": (_c.c_int, [_c.c_void_p, _c.c_int32, _c.c_void_p]),
+    "opc_kv_append": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p,
+         _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p],
+    ),
+    "opc_kv_read": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_void_p],
+    ),
+    "opc_kv_attention_workspace_bytes": (_c.c_size_t, [_c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32]),
+    "opc_kv_attention": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_int32, _c.c_float, _c.c_void_p, _c.c_int64, _c.c_void_p,
+         _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p],
+    ),
+    "opc_token_logprobs_workspace_bytes": (_c.c_size_t, [_c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32]),
+    "opc_token_logprobs": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_int64, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_void_p,
+         _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p],
+    ),
     "opc_take_device_error": (_c.c_int, [_c.c_int32, _c.POINTER(_c.c_int32)]),
 }
 

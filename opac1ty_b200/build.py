@@ -10,7 +10,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
-SOURCES = [CSRC / "opc_lib.cu", CSRC / "opc_engine.cu"]
+SOURCES = [CSRC / "opc_lib.cu", CSRC / "opc_engine.cu", CSRC / "opc_kv.cu", CSRC / "opc_score.cu"]
 DEPENDS = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
 OUTPUT = PKG / "libopc_b200.so"
 
@@ -19,6 +19,7 @@ NVCC_FLAGS = [
     "-O3", "-lineinfo", "-std=c++17",
     "-shared", "-Xcompiler", "-fPIC",
     "--expt-relaxed-constexpr",
+    "--threads", "0",  # the sources side by side
 ]
 
 

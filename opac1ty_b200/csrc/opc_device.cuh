@@ -328,8 +328,8 @@ __device__ __forceinline__ uint32_t ld_nc_u16(const void* p) {
 __device__ __forceinline__ int frexp_exponent(float m) { return ((__float_as_int(m) >> 23) & 0xff) - 126; }
 
 
-// Device error word (one per device, lives in the module; the library is one translation
-// unit).  Codes:
+// Device error word (one per device; it lives in opc_lib.cu's module, the kernels of the other
+// translation units get its address as an argument).  Codes:
 //   1  a ring / shared-memory barrier wait gave up
 //   2  an index out of range was skipped
 //   3  a grid or cross-rank barrier of the decode chain gave up (a CTA or rank did not arrive)
@@ -341,6 +341,8 @@ enum DeviceError : int {
   kDevErrBarrierTimeout = 3,
   kDevErrChainPoisoned = 4
 };
+#ifndef OPC_WITHOUT_ERROR_WORD  // defined by the translation units that get the address
 __device__ int g_opc_device_error = 0;
+#endif
 
 }  // namespace opc

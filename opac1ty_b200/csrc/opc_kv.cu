@@ -1,0 +1,277 @@
+// opc_kv.cu -- C ABI of the 4-bit paged cache (include/opc_b200.h): opc_kv_plan, opc_rope_turns,
+// opc_kv_append, opc_kv_read, opc_kv_attention.
+#define OPC_WITHOUT_ERROR_WORD
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "../../include/opc_b200.h"
+#include "opc_internal.h"
+#include "opc_kv.cuh"
+#include "opc_kv_attention.cuh"
+
+namespace {
+
+using opc_host::cuda_fail;
+using opc_host::fail;
+
+#define KV_CUDA(call, what)                            \
+  do {                                                 \
+    cudaError_t e_ = (call);                           \
+    if (e_ != cudaSuccess) return cuda_fail(e_, what); \
+  } while (0)
+
+bool head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 192 || hd == 256; }
+bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128 || p == 256; }
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+// The checks of a cache and a batch that every call makes.
+int check_cache(const char* who, const opc_kv_cache* c) {
+  if (!c) return fail(OPC_ERR_INVALID, "%s: cache is NULL", who);
+  if (c->kv_heads < 1 || c->kv_heads > 65535 || !head_dim_ok(c->head_dim) || !page_size_ok(c->page_size) || c->n_pages < 1 ||
+      c->head_bytes != static_cast<int64_t>(c->page_size) * (c->head_dim + 8) ||
+      c->total_bytes != c->n_pages * (c->kv_heads * c->head_bytes))
+    return fail(OPC_ERR_INVALID, "%s: the cache is not one that opc_kv_plan filled (kv_heads %d, head_dim %d, page_size %d, n_pages %d)",
+                who, c->kv_heads, c->head_dim, c->page_size, c->n_pages);
+  if (!c->pages || !aligned16(c->pages)) return fail(OPC_ERR_INVALID, "%s: cache.pages must be a 16-byte aligned device pointer", who);
+  return OPC_OK;
+}
+int check_batch(const char* who, const opc_kv_batch* b) {
+  if (!b) return fail(OPC_ERR_INVALID, "%s: batch is NULL", who);
+  if (b->n_seqs < 0 || b->n_tokens < 0 || b->max_q < 0 || b->max_kv < 0 || b->max_pages < 0)
+    return fail(OPC_ERR_INVALID, "%s: negative size in the batch (n_seqs %d, n_tokens %d, max_q %d, max_kv %d, max_pages %d)", who,
+                b->n_seqs, b->n_tokens, b->max_q, b->max_kv, b->max_pages);
+  if (b->n_seqs > 65535) return fail(OPC_ERR_INVALID, "%s: n_seqs %d above 65535", who, b->n_seqs);
+  if (b->table_stride < b->max_pages)
+    return fail(OPC_ERR_INVALID, "%s: table_stride %lld below max_pages %d", who, static_cast<long long>(b->table_stride), b->max_pages);
+  if (b->n_seqs > 0 && b->n_tokens > 0 && (!b->q_start || !b->kv_len || (b->max_pages > 0 && !b->page_table)))
+    return fail(OPC_ERR_INVALID, "%s: the batch's q_start, kv_len or page_table is NULL", who);
+  return OPC_OK;
+}
+int check_type(const char* who, int32_t dtype) {
+  if (dtype == OPC_F16 || dtype == OPC_BF16) return OPC_OK;
+  return fail(OPC_ERR_UNSUPPORTED, "%s: element type %d (OPC_F16 and OPC_BF16 are supported)", who, dtype);
+}
+int check_matrix(const char* who, const char* name, const void* p, int64_t ld, int64_t cols) {
+  if (!p) return fail(OPC_ERR_INVALID, "%s: %s is NULL", who, name);
+  if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(OPC_ERR_INVALID, "%s: %s is not aligned to its elements", who, name);
+  if (ld < cols) return fail(OPC_ERR_INVALID, "%s: leading dimension %lld of %s below its %lld columns", who, static_cast<long long>(ld), name, static_cast<long long>(cols));
+  return OPC_OK;
+}
+#define KV_CHECK(call)                 \
+  do {                                 \
+    const int rc_ = (call);            \
+    if (rc_ != OPC_OK) return rc_;     \
+  } while (0)
+
+opc::KvGeom geom_of(const opc_kv_cache& c) {
+  opc::KvGeom g;
+  g.pages = static_cast<uint8_t*>(c.pages);
+  g.head_bytes = c.head_bytes;
+  g.kv_heads = c.kv_heads;
+  g.hd = c.head_dim;
+  g.page_size = c.page_size;
+  g.page_shift = __builtin_ctz(static_cast<unsigned>(c.page_size));
+  g.n_pages = c.n_pages;
+  return g;
+}
+opc::KvRows rows_of(const opc_kv_batch& b, const opc_kv_cache& c, int* err) {
+  opc::KvRows r;
+  r.q_start = b.q_start;
+  r.kv_len = b.kv_len;
+  r.table = b.page_table;
+  r.table_stride = b.table_stride;
+  r.n_seqs = b.n_seqs;
+  r.n_tokens = b.n_tokens;
+  r.max_q = b.max_q;
+  // (page counts are kept below 2^31 positions, so positions and their sums stay in 32 bits)
+  r.max_pages = static_cast<int32_t>(std::min<int64_t>(b.max_pages, INT32_MAX / c.page_size));
+  r.max_kv = std::min(b.max_kv, r.max_pages * c.page_size);
+  r.err = err;
+  return r;
+}
+
+// Lanes that take one head: head_dim / 8, rounded up to a power of two.
+int lanes_per_head(int hd) {
+  int n = 4;
+  while (n < hd / 8) n *= 2;
+  return n;
+}
+
+template <int kLpr, int kTok>
+auto append_of(bool bf, bool vec) {
+  return bf ? (vec ? opc::kv_append_kernel<kLpr, kTok, true, true> : opc::kv_append_kernel<kLpr, kTok, true, false>)
+            : (vec ? opc::kv_append_kernel<kLpr, kTok, false, true> : opc::kv_append_kernel<kLpr, kTok, false, false>);
+}
+template <int kTok>
+auto append_for(int lpr, bool bf, bool vec) {
+  return lpr == 4 ? append_of<4, kTok>(bf, vec) : lpr == 8 ? append_of<8, kTok>(bf, vec)
+       : lpr == 16 ? append_of<16, kTok>(bf, vec) : append_of<32, kTok>(bf, vec);
+}
+template <int kLpr>
+auto read_of(bool bf, bool vec) {
+  return bf ? (vec ? opc::kv_read_kernel<kLpr, true, true> : opc::kv_read_kernel<kLpr, true, false>)
+            : (vec ? opc::kv_read_kernel<kLpr, false, true> : opc::kv_read_kernel<kLpr, false, false>);
+}
+auto read_for(int lpr, bool bf, bool vec) {
+  return lpr == 4 ? read_of<4>(bf, vec) : lpr == 8 ? read_of<8>(bf, vec) : lpr == 16 ? read_of<16>(bf, vec) : read_of<32>(bf, vec);
+}
+
+}  // namespace
+
+extern "C" {
+
+int opc_kv_plan(int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t n_pages, opc_kv_cache* cache) {
+  if (!cache) return fail(OPC_ERR_INVALID, "opc_kv_plan: cache is NULL");
+  if (kv_heads < 1 || kv_heads > 65535 || n_pages < 1)
+    return fail(OPC_ERR_INVALID, "opc_kv_plan: kv_heads %d, n_pages %d", kv_heads, n_pages);
+  if (!head_dim_ok(head_dim)) return fail(OPC_ERR_UNSUPPORTED, "opc_kv_plan: head_dim %d (32, 64, 96, 128, 192 and 256 are supported)", head_dim);
+  if (!page_size_ok(page_size)) return fail(OPC_ERR_UNSUPPORTED, "opc_kv_plan: page_size %d (16, 32, 64, 128 and 256 are supported)", page_size);
+  cache->kv_heads = kv_heads;
+  cache->head_dim = head_dim;
+  cache->page_size = page_size;
+  cache->n_pages = n_pages;
+  cache->head_bytes = static_cast<int64_t>(page_size) * (head_dim + 8);
+  cache->total_bytes = n_pages * (kv_heads * cache->head_bytes);
+  cache->pages = nullptr;
+  return OPC_OK;
+}
+
+int opc_rope_turns(const double* f, int32_t n, uint64_t* turns) {
+  if (n < 0 || (n > 0 && (!f || !turns))) return fail(OPC_ERR_INVALID, "opc_rope_turns: NULL argument or n %d", n);
+  for (int32_t i = 0; i < n; ++i) {
+    if (!std::isfinite(f[i])) return fail(OPC_ERR_INVALID, "opc_rope_turns: frequency %d is not finite", i);
+    // f / 2pi modulo 1 in the 64-bit mantissa of long double, as a fraction of 2^64
+    long double t = static_cast<long double>(f[i]) / 6.283185307179586476925286766559L;
+    t -= std::floor(t);
+    const long double u = std::nearbyint(t * 18446744073709551616.0L);
+    turns[i] = u >= 18446744073709551616.0L ? 0u : static_cast<uint64_t>(u);
+  }
+  return OPC_OK;
+}
+
+int opc_kv_append(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads, int32_t dtype,
+                  const opc_rope* rope, const void* k, int64_t ldk, const void* v, int64_t ldv, const void* q,
+                  int64_t ldq, void* q_out, int64_t ldqo, void* stream) {
+  const char* who = "opc_kv_append";
+  KV_CHECK(check_cache(who, cache));
+  KV_CHECK(check_batch(who, batch));
+  KV_CHECK(check_type(who, dtype));
+  const int hd = cache->head_dim, kvh = cache->kv_heads;
+  if (heads < 0 || heads > 65535) return fail(OPC_ERR_INVALID, "%s: heads %d", who, heads);
+  if ((q != nullptr) != (q_out != nullptr)) return fail(OPC_ERR_INVALID, "%s: q and q_out go together", who);
+  if (q && heads < 1) return fail(OPC_ERR_INVALID, "%s: q given with %d heads", who, heads);
+  if (rope) {
+    if (rope->rot_dim < 16 || rope->rot_dim % 16 || rope->rot_dim > hd)
+      return fail(OPC_ERR_UNSUPPORTED, "%s: rot_dim %d (a multiple of 16 up to head_dim %d)", who, rope->rot_dim, hd);
+    if (!rope->turns || (reinterpret_cast<uintptr_t>(rope->turns) & 7u))
+      return fail(OPC_ERR_INVALID, "%s: rope.turns must be an 8-byte aligned device pointer", who);
+  }
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return OPC_OK;
+  KV_CHECK(check_matrix(who, "k", k, ldk, static_cast<int64_t>(kvh) * hd));
+  KV_CHECK(check_matrix(who, "v", v, ldv, static_cast<int64_t>(kvh) * hd));
+  if (q) {
+    KV_CHECK(check_matrix(who, "q", q, ldq, static_cast<int64_t>(heads) * hd));
+    KV_CHECK(check_matrix(who, "q_out", q_out, ldqo, static_cast<int64_t>(heads) * hd));
+  }
+  opc_host::Device dev;
+  KV_CHECK(opc_host::current_device(&dev));
+  opc::KvAppendArgs a;
+  a.C = geom_of(*cache);
+  a.B = rows_of(*batch, *cache, dev.error_word);
+  a.k = static_cast<const uint16_t*>(k);
+  a.v = static_cast<const uint16_t*>(v);
+  a.q = static_cast<const uint16_t*>(q);
+  a.q_out = static_cast<uint16_t*>(q_out);
+  a.ldk = ldk;
+  a.ldv = ldv;
+  a.ldq = ldq;
+  a.ldqo = ldqo;
+  a.heads = q ? heads : 0;
+  a.rot_dim = rope ? rope->rot_dim : 0;
+  a.interleaved = rope ? rope->interleaved != 0 : 0;
+  a.turns = rope ? rope->turns : nullptr;
+  const bool vec = aligned16(k) && aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0 &&
+                   (!q || (aligned16(q) && aligned16(q_out) && ldq % 8 == 0 && ldqo % 8 == 0));
+  const int lpr = lanes_per_head(hd), groups = opc::kKvAppendThreads / lpr, all = 2 * kvh + a.heads;
+  const bool bf = dtype == OPC_BF16;
+  // few rows: a CTA per row and `groups` heads; many: four rows per CTA, which share its set-up
+  const bool few = batch->n_tokens < 4 * dev.sm_count;
+  const int tok = few ? 1 : 4;
+  const dim3 grid((batch->n_tokens + tok - 1) / tok, few ? (all + groups - 1) / groups : 1);
+  auto kern = few ? append_for<1>(lpr, bf, vec) : append_for<4>(lpr, bf, vec);
+  kern<<<grid, opc::kKvAppendThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  KV_CUDA(cudaGetLastError(), "opc_kv_append launch");
+  return OPC_OK;
+}
+
+int opc_kv_read(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t dtype, void* k, int64_t ldk, void* v,
+                int64_t ldv, void* stream) {
+  const char* who = "opc_kv_read";
+  KV_CHECK(check_cache(who, cache));
+  KV_CHECK(check_batch(who, batch));
+  KV_CHECK(check_type(who, dtype));
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return OPC_OK;
+  const int64_t cols = static_cast<int64_t>(cache->kv_heads) * cache->head_dim;
+  KV_CHECK(check_matrix(who, "k", k, ldk, cols));
+  KV_CHECK(check_matrix(who, "v", v, ldv, cols));
+  opc_host::Device dev;
+  KV_CHECK(opc_host::current_device(&dev));
+  opc::KvReadArgs a;
+  a.C = geom_of(*cache);
+  a.B = rows_of(*batch, *cache, dev.error_word);
+  a.k = static_cast<uint16_t*>(k);
+  a.v = static_cast<uint16_t*>(v);
+  a.ldk = ldk;
+  a.ldv = ldv;
+  const bool vec = aligned16(k) && aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0;
+  auto kern = read_for(lanes_per_head(cache->head_dim), dtype == OPC_BF16, vec);
+  kern<<<batch->n_tokens, opc::kKvAppendThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  KV_CUDA(cudaGetLastError(), "opc_kv_read launch");
+  return OPC_OK;
+}
+
+size_t opc_kv_attention_workspace_bytes(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads,
+                                        int32_t device) {
+  (void)device;
+  if (!cache || !batch || heads < 1 || cache->kv_heads < 1 || heads % cache->kv_heads) return 0;
+  return 256;
+}
+
+int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads, int32_t dtype, float scale,
+                     const void* q, int64_t ldq, void* out, int64_t ldo, float* lse, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  const char* who = "opc_kv_attention";
+  KV_CHECK(check_cache(who, cache));
+  KV_CHECK(check_batch(who, batch));
+  KV_CHECK(check_type(who, dtype));
+  if (heads < 1 || heads > 65535 || heads % cache->kv_heads)
+    return fail(OPC_ERR_INVALID, "%s: %d heads over %d kv heads", who, heads, cache->kv_heads);
+  if (!std::isfinite(scale)) return fail(OPC_ERR_INVALID, "%s: scale is not finite", who);
+  if (batch->n_tokens == 0 || batch->n_seqs == 0) return OPC_OK;
+  const int64_t cols = static_cast<int64_t>(heads) * cache->head_dim;
+  KV_CHECK(check_matrix(who, "q", q, ldq, cols));
+  KV_CHECK(check_matrix(who, "out", out, ldo, cols));
+  opc_host::Device dev;
+  KV_CHECK(opc_host::current_device(&dev));
+  if (!workspace || workspace_bytes < 256) return fail(OPC_ERR_WORKSPACE, "%s: workspace of %zu bytes", who, workspace_bytes);
+  opc::KvAttnArgs a;
+  a.C = geom_of(*cache);
+  a.B = rows_of(*batch, *cache, dev.error_word);
+  a.q = static_cast<const uint16_t*>(q);
+  a.out = static_cast<uint16_t*>(out);
+  a.lse = lse;
+  a.ldq = ldq;
+  a.ldo = ldo;
+  a.scale = scale;
+  a.heads = heads;
+  a.group = heads / cache->kv_heads;
+  a.bf16 = dtype == OPC_BF16;
+  opc::kv_attention_plain_kernel<<<dim3(batch->n_tokens, heads), opc::kKvPlainThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  KV_CUDA(cudaGetLastError(), "opc_kv_attention launch");
+  return OPC_OK;
+}
+
+}  // extern "C"

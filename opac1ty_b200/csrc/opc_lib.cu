@@ -1,5 +1,5 @@
-// opc_lib.cu -- C ABI (include/opc_b200.h) over the sm_100a kernels.  Single translation
-// unit: the kernels live in the included .cuh files.
+// opc_lib.cu -- C ABI (include/opc_b200.h) over the sm_100a kernels, which live in the included
+// .cuh files.  The paged-cache and log-probability entry points are in opc_kv.cu and opc_score.cu.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <cuda_runtime.h>
@@ -16,6 +16,7 @@
 #include <vector>
 
 #include "../../include/opc_b200.h"
+#include "opc_internal.h"
 #include "opc_device.cuh"
 #include "opc_chain.cuh"
 #include "opc_chain2.cuh"
@@ -72,6 +73,8 @@ int device_cache(int dev, DeviceCache* out) {
   *out = c;
   return OPC_OK;
 }
+
+std::map<int, int*> g_error_words;  // by device; under g_mu
 
 // k columns per index unit: 128 (svs = 1, 512-byte units), 256 (svs = 8, 128-byte units)
 int unit_cols(int svs) { return svs == 8 ? opc::kVq8BlockCols : opc::kPackedCols; }
@@ -341,6 +344,40 @@ int launch_gemvq(const opc::GemvQArgs& args, int64_t grid, size_t smem, cudaStre
 }
 
 }  // namespace
+
+// What the other translation units use (opc_internal.h).
+namespace opc_host {
+
+int fail(int code, const char* fmt, ...) {
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(g_last_error, sizeof(g_last_error), fmt, ap);
+  va_end(ap);
+  return code;
+}
+
+int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+
+int current_device(Device* out) {
+  int dev = 0;
+  OPC_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
+  DeviceCache dc;
+  const int rc = device_cache(dev, &dc);
+  if (rc != OPC_OK) return rc;
+  std::lock_guard<std::mutex> lk(g_mu);
+  int*& word = g_error_words[dev];
+  if (!word) {
+    void* p = nullptr;
+    OPC_CUDA(cudaGetSymbolAddress(&p, opc::g_opc_device_error), "cudaGetSymbolAddress(device error word)");
+    word = static_cast<int*>(p);
+  }
+  out->sm_count = dc.sm_count;
+  out->max_smem_optin = dc.max_smem_optin;
+  out->error_word = word;
+  return OPC_OK;
+}
+
+}  // namespace opc_host
 
 extern "C" {
 
