@@ -119,6 +119,74 @@ auto read_for(int lpr, bool bf, bool vec) {
   return lpr == 4 ? read_of<4>(bf, vec) : lpr == 8 ? read_of<8>(bf, vec) : lpr == 16 ? read_of<16>(bf, vec) : read_of<32>(bf, vec);
 }
 
+// ------------------------------------------------------------------------------------------------
+// Attention: how a call is divided
+// ------------------------------------------------------------------------------------------------
+struct AttentionPlan {
+  int step_nt;          // row tiles of the step kernel, 0: not launched
+  int step_q;           // the step kernel takes sequences of at most this many rows
+  opc::KvSplit step;    // part and count are set per call
+  size_t bytes;
+};
+
+constexpr size_t kCounterBytes = opc::kKvCounters * sizeof(int32_t);
+
+AttentionPlan plan_attention(const opc_kv_cache& c, const opc_kv_batch& b, int group, int sms) {
+  AttentionPlan p{};
+  // Row tiles of 8 (query token, head) pairs: two where the accumulators leave registers for them.
+  const int most = c.head_dim <= 128 ? 16 : 8;
+  const int max_q = std::max(b.max_q, 0);
+  p.step_q = std::min(max_q, most / group);
+  p.bytes = kCounterBytes;
+  if (p.step_q > 0) {
+    p.step_nt = p.step_q * group > 8 ? 2 : 1;
+    // Chunks: one wave of four CTAs per SM for a single sequence, whose chunks are all alike; four
+    // waves where lengths differ, so that short ones fill up what long ones leave.
+    const int64_t pairs = std::max<int64_t>(1, static_cast<int64_t>(b.n_seqs) * c.kv_heads);
+    const int64_t stages = std::max<int64_t>(1, (static_cast<int64_t>(b.max_kv) + opc::kKvStage - 1) / opc::kKvStage);
+    const int64_t want = static_cast<int64_t>(sms) * 4 * (b.n_seqs == 1 ? 1 : 4);
+    int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({want / pairs, 128, (stages + 1) / 2}));
+    if (pairs > opc::kKvCounters) chunks = 1;
+    const int64_t per = (stages + chunks - 1) / chunks;
+    p.step.chunk = static_cast<int32_t>(per * opc::kKvStage);
+    p.step.chunks = static_cast<int32_t>((stages + per - 1) / per);
+    p.step.rows = p.step_q * group;
+    if (p.step.chunks > 1) p.bytes += static_cast<size_t>(pairs) * p.step.chunks * p.step.rows * (c.head_dim + 4) * 4;
+  }
+  return p;
+}
+
+template <int kNT>
+auto step_of(int hd) {
+  if constexpr (kNT == 1) {
+    if (hd == 192) return opc::kv_attention_step_kernel<192, 1>;
+    if (hd == 256) return opc::kv_attention_step_kernel<256, 1>;
+  }
+  return hd == 32 ? opc::kv_attention_step_kernel<32, kNT> : hd == 64 ? opc::kv_attention_step_kernel<64, kNT>
+       : hd == 96 ? opc::kv_attention_step_kernel<96, kNT> : opc::kv_attention_step_kernel<128, kNT>;
+}
+
+// Launched with programmatic serialization: set-up overlaps the kernel before, which each of these
+// kernels waits for before it reads anything.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
+  if (smem > 48 * 1024) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
+}
+
 }  // namespace
 
 extern "C" {
@@ -235,9 +303,16 @@ int opc_kv_read(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t dt
 
 size_t opc_kv_attention_workspace_bytes(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads,
                                         int32_t device) {
-  (void)device;
-  if (!cache || !batch || heads < 1 || cache->kv_heads < 1 || heads % cache->kv_heads) return 0;
-  return 256;
+  if (!cache || !batch || heads < 1 || heads > 65535 || cache->kv_heads < 1 || heads % cache->kv_heads ||
+      !head_dim_ok(cache->head_dim) || !page_size_ok(cache->page_size) || batch->n_seqs < 0 || batch->max_q < 0 ||
+      batch->max_kv < 0)
+    return 0;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return plan_attention(*cache, *batch, heads / cache->kv_heads, sms).bytes;
 }
 
 int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads, int32_t dtype, float scale,
@@ -256,7 +331,10 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
   KV_CHECK(check_matrix(who, "out", out, ldo, cols));
   opc_host::Device dev;
   KV_CHECK(opc_host::current_device(&dev));
-  if (!workspace || workspace_bytes < 256) return fail(OPC_ERR_WORKSPACE, "%s: workspace of %zu bytes", who, workspace_bytes);
+  const int group = heads / cache->kv_heads;
+  AttentionPlan p = plan_attention(*cache, *batch, group, dev.sm_count);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < p.bytes)
+    return fail(OPC_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", who, p.bytes, workspace_bytes);
   opc::KvAttnArgs a;
   a.C = geom_of(*cache);
   a.B = rows_of(*batch, *cache, dev.error_word);
@@ -267,9 +345,25 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
   a.ldo = ldo;
   a.scale = scale;
   a.heads = heads;
-  a.group = heads / cache->kv_heads;
+  a.group = group;
   a.bf16 = dtype == OPC_BF16;
-  opc::kv_attention_plain_kernel<<<dim3(batch->n_tokens, heads), opc::kKvPlainThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+  a.vec = aligned16(q) && aligned16(out) && ldq % 8 == 0 && ldo % 8 == 0;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (p.step_nt) {
+    a.lo_q = 1;
+    a.hi_q = p.step_q;
+    p.step.count = static_cast<int32_t*>(workspace);
+    p.step.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+    auto kern = p.step_nt == 2 ? step_of<2>(cache->head_dim) : step_of<1>(cache->head_dim);
+    KV_CUDA(launch_pdl(kern, dim3(p.step.chunks, cache->kv_heads, batch->n_seqs), opc::kKvStepThreads,
+                       opc::kv_step_smem(cache->head_dim), s, a, p.step),
+            "opc_kv_attention launch (steps)");
+  }
+  if (a.B.max_q > p.step_q) {
+    a.lo_q = p.step_q + 1;
+    a.hi_q = a.B.max_q;
+    opc::kv_attention_plain_kernel<<<dim3(batch->n_tokens, heads), opc::kKvPlainThreads, 0, s>>>(a);
+  }
   KV_CUDA(cudaGetLastError(), "opc_kv_attention launch");
   return OPC_OK;
 }
