@@ -125,33 +125,22 @@ auto read_for(int lpr, bool bf, bool vec) {
 struct AttentionPlan {
   int step_nt;          // row tiles of the step kernel, 0: not launched
   int step_q;           // the step kernel takes sequences of at most this many rows
-  opc::KvSplit step;    // part and count are set per call
-  size_t bytes;
+  int step_grid;
+  size_t bytes;         // workspace: the counters, then the records
 };
 
-constexpr size_t kCounterBytes = opc::kKvCounters * sizeof(int32_t);
+constexpr size_t kCounterBytes = 4096;  // one per CTA of a launch
 
 AttentionPlan plan_attention(const opc_kv_cache& c, const opc_kv_batch& b, int group, int sms) {
   AttentionPlan p{};
   // Row tiles of 8 (query token, head) pairs: two where the accumulators leave registers for them.
   const int most = c.head_dim <= 128 ? 16 : 8;
-  const int max_q = std::max(b.max_q, 0);
-  p.step_q = std::min(max_q, most / group);
+  p.step_q = std::min(std::max(b.max_q, 0), most / group);
   p.bytes = kCounterBytes;
   if (p.step_q > 0) {
     p.step_nt = p.step_q * group > 8 ? 2 : 1;
-    // Chunks: one wave of four CTAs per SM for a single sequence, whose chunks are all alike; four
-    // waves where lengths differ, so that short ones fill up what long ones leave.
-    const int64_t pairs = std::max<int64_t>(1, static_cast<int64_t>(b.n_seqs) * c.kv_heads);
-    const int64_t stages = std::max<int64_t>(1, (static_cast<int64_t>(b.max_kv) + opc::kKvStage - 1) / opc::kKvStage);
-    const int64_t want = static_cast<int64_t>(sms) * 4 * (b.n_seqs == 1 ? 1 : 4);
-    int64_t chunks = std::max<int64_t>(1, std::min<int64_t>({want / pairs, 128, (stages + 1) / 2}));
-    if (pairs > opc::kKvCounters) chunks = 1;
-    const int64_t per = (stages + chunks - 1) / chunks;
-    p.step.chunk = static_cast<int32_t>(per * opc::kKvStage);
-    p.step.chunks = static_cast<int32_t>((stages + per - 1) / per);
-    p.step.rows = p.step_q * group;
-    if (p.step.chunks > 1) p.bytes += static_cast<size_t>(pairs) * p.step.chunks * p.step.rows * (c.head_dim + 4) * 4;
+    p.step_grid = std::min<int>(sms * opc::kv_step_ctas(c.head_dim, p.step_nt), kCounterBytes / 4);
+    p.bytes += static_cast<size_t>(p.step_grid) * 2 * (p.step_q * group) * (c.head_dim + 4) * 4;
   }
   return p;
 }
@@ -332,6 +321,10 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
   opc_host::Device dev;
   KV_CHECK(opc_host::current_device(&dev));
   const int group = heads / cache->kv_heads;
+  // (the work of a call is counted in 32 bits, in stages of 128 keys)
+  if (static_cast<double>(batch->n_seqs) * cache->kv_heads * (batch->max_kv / opc::kKvStage + 2) > 4e9)
+    return fail(OPC_ERR_INVALID, "%s: %d sequences of up to %d keys over %d kv heads are too many for one call", who,
+                batch->n_seqs, batch->max_kv, cache->kv_heads);
   AttentionPlan p = plan_attention(*cache, *batch, group, dev.sm_count);
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.bytes)
     return fail(OPC_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", who, p.bytes, workspace_bytes);
@@ -352,11 +345,12 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
   if (p.step_nt) {
     a.lo_q = 1;
     a.hi_q = p.step_q;
-    p.step.count = static_cast<int32_t*>(workspace);
-    p.step.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+    opc::KvSplit sp;
+    sp.count = static_cast<int32_t*>(workspace);
+    sp.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+    sp.rows = p.step_q * group;
     auto kern = p.step_nt == 2 ? step_of<2>(cache->head_dim) : step_of<1>(cache->head_dim);
-    KV_CUDA(launch_pdl(kern, dim3(p.step.chunks, cache->kv_heads, batch->n_seqs), opc::kKvStepThreads,
-                       opc::kv_step_smem(cache->head_dim), s, a, p.step),
+    KV_CUDA(launch_pdl(kern, dim3(p.step_grid), opc::kKvStepThreads, opc::kv_step_smem(cache->head_dim, p.step_nt), s, a, sp),
             "opc_kv_attention launch (steps)");
   }
   if (a.B.max_q > p.step_q) {

@@ -142,29 +142,39 @@ __global__ void __launch_bounds__(kKvPlainThreads) kv_attention_plain_kernel(con
 //   maximum   m and e move only when a score passes m + 8 or a scale 2^(e+5) (one vote per tile):
 //             weights stay below 2^13, and the common tile has no shuffles and no rescaling.
 //
-// A CTA takes one chunk of the keys: a producer warp brings 64 keys per stage (one bulk copy per
-// page and head, or four where a page is larger than a stage) into a ring, four consumer warps take
-// 16 keys each.  Their results are merged in shared memory; where a sequence has several chunks
-// the records (m, sum, weighted sums) go to the workspace and the last CTA to arrive merges them in
-// order.
+// The work -- for every sequence and kv head the stages of 128 keys -- is one line that the CTAs
+// (persistent, two or three per SM) cut into equal contiguous ranges, whatever the sequences'
+// lengths.  A producer warp walks the CTA's range: per item (the part of one sequence and kv head)
+// it leaves a description and the item's q rows in one of two slots, and streams the keys through
+// a ring (one bulk copy per page, or four where a page is larger than a stage), running ahead of
+// the consumers across items.  Four consumer warps take 32 keys of a stage each and merge in shared
+// memory at the end of the item.  An item that is a whole sequence and head is written out; else
+// its record (m, sum, weighted sums) goes to the workspace -- a CTA has at most two -- and the last
+// CTA of that sequence and head to arrive merges the records in order.
 // ------------------------------------------------------------------------------------------------
-constexpr int kKvStage = 64;                  // keys per stage
+constexpr int kKvStage = 128;                 // keys per stage, 32 for each consumer
+constexpr int kKvStageShift = 7;
 constexpr int kKvStepWarps = 4;               // consumers
 constexpr int kKvStepThreads = (kKvStepWarps + 1) * 32;
-constexpr int kKvCounters = 65536;            // (sequence, kv head) pairs that may be split
+constexpr int kKvMinStages = 2;               // stages per CTA below which fewer CTAs take part
+constexpr int kKvItemCost = 3;                // what an item costs beside its stages, in stages
 __host__ __device__ constexpr int kv_stage_bytes(int hd) { return kKvStage * (hd + 8); }
-// As many stages as fit four CTAs into an SM's shared memory, 3 to 10.
-__host__ __device__ constexpr int kv_stages(int hd) {
-  return 53000 / kv_stage_bytes(hd) > 10 ? 10 : 53000 / kv_stage_bytes(hd);
+// CTAs per SM: bounded by the accumulators' registers and the shared memory of a record.
+__host__ __device__ constexpr int kv_step_ctas(int hd, int nt) { return hd <= 128 && nt == 1 ? 3 : 2; }
+__host__ __device__ constexpr int kv_rec_bytes(int hd, int nt) { return kKvStepWarps * 8 * nt * (hd + 4) * 4; }
+__host__ __device__ constexpr int kv_slot_bytes(int hd, int nt) { return 8 * nt * (hd * 2 + 8) + 64; }  // q, its factors, description
+__host__ __device__ constexpr int kv_stages(int hd, int nt) {
+  const int room = (kv_step_ctas(hd, nt) == 3 ? 75000 : 113000) - kv_rec_bytes(hd, nt) - 2 * kv_slot_bytes(hd, nt) - 512;
+  return room / kv_stage_bytes(hd) > 8 ? 8 : room / kv_stage_bytes(hd);
 }
-__host__ __device__ constexpr int kv_step_smem(int hd) { return kv_stages(hd) * kv_stage_bytes(hd) + 256; }
+__host__ __device__ constexpr int kv_step_smem(int hd, int nt) {
+  return kv_stages(hd, nt) * kv_stage_bytes(hd) + kv_rec_bytes(hd, nt) + 2 * kv_slot_bytes(hd, nt) + 512;
+}
 
 struct KvSplit {
-  int32_t chunk;    // keys per CTA, a multiple of kKvStage
-  int32_t chunks;   // records per (sequence, kv head) in the workspace
-  int32_t rows;     // rows of a record
-  float* part;      // [n_seqs][kv_heads][chunks][rows][head_dim + 4]: weighted sums, then m, sum, -, -
-  int32_t* count;   // [n_seqs * kv_heads], zero between calls
+  float* part;      // [CTAs][2][rows][head_dim + 4]: weighted sums, then m, sum, -, -
+  int32_t* count;   // [CTAs], zero between calls
+  int32_t rows;
 };
 
 __device__ __forceinline__ uint32_t movmatrix_trans(uint32_t x) {
@@ -178,6 +188,8 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 __device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }  // -126 <= e <= 127
+
+__device__ __forceinline__ float2 unpack_half2(uint32_t w) { return __half22float2(*reinterpret_cast<const __half2*>(&w)); }
 
 // kW consecutive 32-bit words of shared memory.
 template <int kW>
@@ -230,207 +242,413 @@ __device__ __forceinline__ void kv_finish_row(const KvAttnArgs& a, int r0, int k
     a.lse[static_cast<int64_t>(r0 + i) * a.heads + head] = T == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(T);
 }
 
-// The CTA has written its record; the last one of its (sequence, kv head) merges all of them, in
-// order, and leaves the count at 0.  Called by the kThreads consumer threads, barrier 1; smem holds
-// chunks * R + R float2.
+// Merge the records of an item that `n` CTAs share, the first of them `c_first`, in order (record 1
+// of the first CTA, record 0 of the others), by the kThreads consumer threads (barrier 1).  Records
+// are brought to shared memory, as many as `smem` holds, by asynchronous copies that are all in
+// flight together; what they merge to takes the place of the first, and the next ones follow it.
+// The code is kept small (one short loop each for the copies and for the sums): it runs once per
+// launch and SM, and fetching it is what it costs -- unrolled by 14 and 20 records it took 7 and 15 us
+// for the 56 records of 131071 keys over 8 heads.
 template <int kHd, int kThreads>
-__device__ __forceinline__ void kv_merge_chunks(const KvAttnArgs& a, const KvSplit& sp, int r0, int kvh, int64_t pair_id,
-                                                int n_chunks, int R, unsigned char* smem, int* sm_last) {
+__device__ __forceinline__ void kv_merge_records(const KvAttnArgs& a, const KvSplit& sp, int r0, int kvh, int c_first, int n,
+                                                 int R, float* smem, int smem_floats) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  __threadfence();
-  named_barrier(1, kThreads);
-  if (tid == 0) *sm_last = atom_add_acq_rel_gpu(sp.count + pair_id, 1) == n_chunks - 1;
-  named_barrier(1, kThreads);
-  if (!*sm_last) return;
-  __threadfence();
-  if (tid == 0) sp.count[pair_id] = 0;
-  constexpr int kRec = kHd + 4;
+  constexpr int kRec = kHd + 4, kQ = kHd / 4;
+  const int size = R * kRec, most = smem_floats / size;  // floats per record here, records at once
   const int64_t stride = static_cast<int64_t>(sp.rows) * kRec;
-  const float* part = sp.part + pair_id * sp.chunks * stride;
-  float2* f = reinterpret_cast<float2*>(smem);  // [row][chunk]: (m, sum), then (factor, sum)
-  float2* total = f + R * n_chunks;             // [row]: (M, T)
-  for (int i = tid; i < R * n_chunks; i += kThreads) {
-    const int row = i / n_chunks, c = i - row * n_chunks;
-    f[i] = __ldcg(reinterpret_cast<const float2*>(part + c * stride + row * kRec + kHd));
-  }
-  named_barrier(1, kThreads);
-  for (int row = warp; row < R; row += kThreads / 32) {
-    float M = -1e30f, T = 0.f;
-    for (int c = lane; c < n_chunks; c += 32) M = fmaxf(M, f[row * n_chunks + c].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-    for (int c = lane; c < n_chunks; c += 32) {
-      const float w = ex2(f[row * n_chunks + c].x - M);
-      T += w * f[row * n_chunks + c].y;
-      f[row * n_chunks + c].x = w;
+  const float* part = sp.part + static_cast<int64_t>(c_first) * 2 * stride;
+  const uint32_t base = smem_u32(smem);
+  // (the first place's (m, sum) alternate between two spots, so that a row's threads need not agree on
+  // when to overwrite them)
+  for (int c0 = 0, have = 0, spot = 0; c0 < n; have = 1, spot ^= 2) {
+    const int m = min(most - have, n - c0);
+#pragma unroll 1
+    for (int c = warp; c < m; c += kThreads / 32) {
+      const float* src = part + (2 * (c0 + c) + (c0 + c == 0)) * stride;
+#pragma unroll 1
+      for (int x = 4 * lane; x < size; x += 128)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(base + 4 * ((have + c) * size + x)), "l"(src + x) : "memory");
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) T += __shfl_xor_sync(0xffffffffu, T, o);
-    if (lane == 0) total[row] = make_float2(M, T);
-  }
-  named_barrier(1, kThreads);
-  constexpr int kQ = kHd / 4;
-  for (int i = tid; i < R * kQ; i += kThreads) {
-    const int row = i / kQ, d = 4 * (i - row * kQ);
-    const float* src = part + row * kRec + d;
-    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-    for (int c = 0; c < n_chunks; ++c) {
-      const float4 v = __ldcg(reinterpret_cast<const float4*>(src + c * stride));
-      const float w = f[row * n_chunks + c].x;
-      o.x += w * v.x;
-      o.y += w * v.y;
-      o.z += w * v.z;
-      o.w += w * v.w;
+    asm volatile("cp.async.wait_all;" ::: "memory");
+    named_barrier(1, kThreads);
+    c0 += m;
+#pragma unroll 1
+    for (int i = tid; i < R * kQ; i += kThreads) {
+      const int row = i / kQ, d = 4 * (i - row * kQ);
+      float M = -1e30f, T = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      const float* src = smem + row * kRec;
+#pragma unroll 4
+      for (int c = 0; c < have + m; ++c) M = fmaxf(M, src[c * size + kHd + (c == 0 ? spot : 0)]);
+#pragma unroll 4
+      for (int c = 0; c < have + m; ++c) {
+        const float2 w = *reinterpret_cast<const float2*>(src + c * size + kHd + (c == 0 ? spot : 0));
+        const float4 v = *reinterpret_cast<const float4*>(src + c * size + d);
+        const float f = ex2(w.x - M);
+        T += f * w.y;
+        o.x += f * v.x;
+        o.y += f * v.y;
+        o.z += f * v.z;
+        o.w += f * v.w;
+      }
+      if (c0 == n) {
+        kv_finish_row(a, r0, kvh, row, d, o, M, T);
+      } else {
+        *reinterpret_cast<float4*>(smem + row * kRec + d) = o;
+        if (d == 0) *reinterpret_cast<float2*>(smem + row * kRec + kHd + (spot ^ 2)) = make_float2(M, T);
+      }
     }
-    kv_finish_row(a, r0, kvh, row, d, o, total[row].x, total[row].y);
+    named_barrier(1, kThreads);
+  }
+}
+
+// An item that the CTA shares with others.
+struct KvShared {
+  int32_t r0, kvh, c_first, contributors, rows;
+};
+
+// One thread's arrival for a record: it releases what the CTA's threads wrote before their last
+// barrier; the arrival that completes the count has acquired the others' records.
+__device__ __forceinline__ void kv_arrive(const KvSplit& sp, const KvShared& sh, int* last) {
+  const bool all = atom_add_acq_rel_gpu(sp.count + sh.c_first, 1) == sh.contributors - 1;
+  if (all) sp.count[sh.c_first] = 0;
+  *last = all;
+}
+
+// What the producer tells the consumers of an item.
+struct KvItem {
+  int32_t n_st;       // stages here; -1: no more items
+  int32_t k0, k1;     // keys [k0, k1)
+  int32_t seq_end;    // keys the sequence holds (the last row's limit)
+  int32_t hidden;     // seq_end - (position of row 0 + 1): row i sees keys below seq_end - hidden + i
+  int32_t r0, rows, kvh;
+  int32_t c_first, contributors, record;
+};
+
+// The rows of q as B fragments in an item's slot, from the elements each lane holds (row g of each
+// row tile, dimensions q*kHd/4 + 8d + 0..7): multiplication s of code word d meets codes (2s, 2s + 4)
+// in the first register, (2s + 1, 2s + 5), which are 16 times larger, in the second.  fp16 queries go
+// in as they are (a sixteenth of one below 2^-10 is rounded, by 2^-25 at most); bf16 ones, whose
+// range is wider, are first multiplied by the power of two that puts the row's largest near 2^14.
+// Behind the fragments, per row: the factor of its scores (log2 units) and the sum of its elements.
+template <int kHd, int kNT, bool kBf>
+__device__ __forceinline__ void kv_stage_q(const uint4 (&raw)[kNT][kHd / 32], uint32_t slot_s, float scale, int lane) {
+  const __half2 sixteenth = __float2half2_rn(0.0625f);
+#pragma unroll
+  for (int t = 0; t < kNT; ++t) {
+    int e2 = 0;
+    if (kBf) {
+      float big = 0.f;
+#pragma unroll
+      for (int d = 0; d < kHd / 32; ++d) {
+        float x[8];
+        unpack_halves<kBf>(raw[t][d], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+      }
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+      // |e2| is kept below 100 (a query beyond fp32's reach overflows)
+      e2 = max(-99, min(99, big > 0.f ? 14 - ((__float_as_int(big) >> 23) - 127) : 0));
+    }
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int d = 0; d < kHd / 32; ++d) {
+      uint32_t w[4] = {raw[t][d].x, raw[t][d].y, raw[t][d].z, raw[t][d].w};
+      if (kBf) {
+        const float up = pow2i(e2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = pack_halves<false>(half_lo<true>(w[i]) * up, half_hi<true>(w[i]) * up);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack_half2(w[i]);
+        sum[0] += f.x;
+        sum[1] += f.y;
+      }
+      const uint32_t lo0 = prmt(w[0], w[2], 0x5410u), hi0 = prmt(w[0], w[2], 0x7632u);
+      const uint32_t lo1 = prmt(w[1], w[3], 0x5410u), hi1 = prmt(w[1], w[3], 0x7632u);
+      const __half2 h0 = __hmul2(*reinterpret_cast<const __half2*>(&hi0), sixteenth);
+      const __half2 h1 = __hmul2(*reinterpret_cast<const __half2*>(&hi1), sixteenth);
+      sts128(slot_s + ((t * (kHd / 32) + d) * 32 + lane) * 16,
+             make_uint4(lo0, *reinterpret_cast<const uint32_t*>(&h0), lo1, *reinterpret_cast<const uint32_t*>(&h1)));
+    }
+    float total = sum[0] + sum[1];
+    total += __shfl_xor_sync(0xffffffffu, total, 1);
+    total += __shfl_xor_sync(0xffffffffu, total, 2);
+    if ((lane & 3) == 0)  // (q carries 2^e2, the codes 2^-24)
+      sts64(slot_s + 8 * kNT * kHd * 2 + 8 * (8 * t + (lane >> 2)),
+            __float_as_uint(scale * 1.4426950408889634f * pow2i(12 - e2) * 4096.0f), __float_as_uint(total * 0x1p-24f));
   }
 }
 
 template <int kHd, int kNT>
-__global__ void __launch_bounds__(kKvStepThreads) kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
-  constexpr int kS = kv_stages(kHd), kStageBytes = kv_stage_bytes(kHd);
+__global__ void __launch_bounds__(kKvStepThreads, kv_step_ctas(kHd, kNT))
+kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
+  constexpr int kS = kv_stages(kHd, kNT), kStageBytes = kv_stage_bytes(kHd);
+  static_assert(kS >= 2, "two stages at least");
   constexpr int kRow = kHd / 2;          // bytes of one key's codes
   constexpr int kKW = kHd / 32;          // words of a key row per lane (4 lanes per row)
   constexpr int kMt = kHd / 16;          // 16-dimension tiles of the values
   constexpr int kRows = 8 * kNT;
+  constexpr int kSlotBytes = kv_slot_bytes(kHd, kNT);
+  constexpr int kItemAt = kRows * (kHd * 2 + 8);  // of a slot: the fragments of q, (factor, sum) per row, the description
   extern __shared__ __align__(128) unsigned char smem[];
-  __shared__ int sm_last;
-  const uint32_t ring = smem_u32(smem), bars = ring + kS * kStageBytes;
-  const uint32_t full_b = bars, empty_b = bars + 8 * kS, valid_s = bars + 16 * kS;  // valid_s: [kS] masks
+  __shared__ int sm_last[2];
+  __shared__ volatile int sm_failed;
+  __shared__ KvShared sm_shared[2];
+  float* rec = reinterpret_cast<float*>(smem + kS * kStageBytes);  // [warp][row][kHd + 4]
+  unsigned char* slots = smem + kS * kStageBytes + kv_rec_bytes(kHd, kNT);
+  const uint32_t ring = smem_u32(smem), bars = smem_u32(slots) + 2 * kSlotBytes;
+  const uint32_t full_b = bars, empty_b = bars + 8 * kS, item_b = bars + 16 * kS, free_b = item_b + 16;
+  const uint32_t valid_s = free_b + 16;  // [kS] masks of the pieces that are there
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, q = lane & 3;
-  const int chunk = blockIdx.x, kvh = blockIdx.y, seq = blockIdx.z;
 
   if (tid == 0) {
+    sm_failed = 0;
     for (int s = 0; s < kS; ++s) {
       mbar_init(full_b + 8 * s, 1);
       mbar_init(empty_b + 8 * s, kKvStepWarps);
     }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(item_b + 8 * s, 1);
+      mbar_init(free_b + 8 * s, kKvStepWarps);
+    }
     fence_mbar_init();
   }
+  __syncthreads();
   griddep_wait();
   griddep_launch_dependents();
-  const int r0 = __ldg(a.B.q_start + seq), q_all = __ldg(a.B.q_start + seq + 1) - r0, kv_all = __ldg(a.B.kv_len + seq);
-  const int q_len = min(q_all, a.B.max_q);  // rows beyond the batch's bound are skipped
-  if (q_len < a.lo_q || q_len > a.hi_q) return;
-  if (r0 < 0 || r0 > a.B.n_tokens - q_len) {  // starts that lead outside q and out
-    if (tid == 0) kv_bad_index(a.B);
-    return;
-  }
-  const int n = max(0, min(kv_all, a.B.max_kv));
-  if ((q_all > a.B.max_q || kv_all > a.B.max_kv) && chunk == 0 && kvh == 0 && tid == 0) kv_bad_index(a.B);
-  const int n_chunks = max(1, (n + sp.chunk - 1) / sp.chunk);
-  if (chunk >= n_chunks) return;
-  const int k0 = chunk * sp.chunk, k1 = min(n, k0 + sp.chunk);
-  const int n_st = (k1 - k0 + kKvStage - 1) / kKvStage;
-  const int pe = min(a.C.page_size, kKvStage), pe_shift = min(a.C.page_shift, 6);  // keys per piece of a stage
-  __syncthreads();
+  const int pe = min(a.C.page_size, kKvStage), pe_shift = min(a.C.page_shift, kKvStageShift);  // keys per piece of a stage
   bool ok = true;
 
   if (warp == kKvStepWarps) {
     // ---------------------------------------------------------------- producer
-    const int pieces = kKvStage >> pe_shift;          // per stage
-    const int ahead = 32 >> (6 - pe_shift);           // stages whose page numbers the warp holds
-    const uint32_t piece_bytes = static_cast<uint32_t>(pe) * (kHd + 8);
-    int pages = -1;
-    for (int st = 0; st < n_st && ok; ++st) {
-      if (st % ahead == 0) {  // lane i: the page of piece i from here on
-        const int pos = k0 + st * kKvStage + lane * pe;
-        pages = -1;
-        if (pos < k1) {
-          pages = __ldg(a.B.table + seq * a.B.table_stride + (pos >> a.C.page_shift));
-          if (static_cast<uint32_t>(pages) >= static_cast<uint32_t>(a.C.n_pages)) {
-            kv_bad_index(a.B);
-            pages = -1;
-          }
+    const int n_seqs = a.B.n_seqs, kvh_n = a.C.kv_heads;
+    const uint64_t once = l2_policy_evict_first();  // every key is read once
+    // lane i: sequence s0 + i; its stages (one at least, so that rows without keys are written), 0
+    // when the launch does not take it
+    int my_r0 = 0, my_q = 0, my_kv = 0, my_n = 0, my_st = 0;
+    auto load_seqs = [&](int s0) {
+      const int s = s0 + lane;
+      my_st = 0;
+      if (s < n_seqs) {
+        my_r0 = __ldg(a.B.q_start + s);
+        const int all = __ldg(a.B.q_start + s + 1) - my_r0;
+        my_kv = __ldg(a.B.kv_len + s);
+        my_q = min(all, a.B.max_q);  // rows beyond the batch's bound are skipped
+        my_n = max(0, min(my_kv, a.B.max_kv));
+        my_kv -= all;                // the position of row 0
+        if (my_q >= a.lo_q && my_q <= a.hi_q) {
+          const bool inside = my_r0 >= 0 && my_r0 <= a.B.n_tokens - my_q;
+          if (blockIdx.x == 0 && (all > a.B.max_q || my_kv + all > a.B.max_kv || !inside)) kv_bad_index(a.B);
+          if (inside) my_st = max(1, (my_n + kKvStage - 1) >> kKvStageShift);
         }
       }
-      const int slot = st % kS;
-      if (st >= kS && !mbar_wait_bounded(empty_b + 8 * slot, ((st / kS) - 1) & 1)) {
+    };
+    // The line of work: a (sequence, kv head) takes its stages and kKvItemCost places before them, for
+    // what an item costs beside its stages.  CTA c takes the stages at places [place(c), place(c + 1)).
+    uint32_t W = 0;
+    for (int s0 = 0; s0 < n_seqs; s0 += 32) {
+      load_seqs(s0);
+      W += __reduce_add_sync(0xffffffffu, my_st ? my_st + kKvItemCost : 0);
+    }
+    W *= kvh_n;
+    const uint32_t G = min(static_cast<uint32_t>(gridDim.x), max(1u, W / kKvMinStages));
+    const uint32_t per = W / G, rest = W - per * G;  // the first `rest` CTAs take one place more
+    const auto place_of = [&](uint32_t c) { return c * per + min(c, rest); };
+    const auto cta_of = [&](uint32_t x) {
+      return static_cast<int>(x < rest * (per + 1) ? x / (per + 1) : rest + (x - rest * (per + 1)) / per);
+    };
+    const uint32_t c = blockIdx.x;
+    uint32_t w = 0, w_end = 0;
+    if (c < G) {
+      w = place_of(c);
+      w_end = place_of(c + 1);
+    }
+    // the first sequence of the range: base = places before sequence s0 + i
+    int s0 = 0, i = 0, n_items = 0;
+    uint32_t base = 0;
+    if (w < w_end) {
+      for (;; s0 += 32) {
+        if (n_seqs > 32) load_seqs(s0);
+        const uint32_t sum = __reduce_add_sync(0xffffffffu, my_st ? my_st + kKvItemCost : 0) * kvh_n;
+        if (base + sum > w) break;
+        base += sum;
+      }
+    }
+    int st_all = 0;  // stages issued
+    while (w < w_end && ok) {
+      const uint32_t st = __shfl_sync(0xffffffffu, my_st, i), cost = st ? st + kKvItemCost : 0;
+      if (base + cost * kvh_n <= w) {  // the next sequence
+        base += cost * kvh_n;
+        if (++i == 32) {
+          i = 0;
+          s0 += 32;
+          load_seqs(s0);
+        }
+        continue;
+      }
+      const int head = static_cast<int>((w - base) / cost), seq = s0 + i;
+      const uint32_t pair0 = base + head * cost + kKvItemCost, pair1 = pair0 + st;  // the places of its stages
+      const uint32_t begin = max(w, pair0), end = min(w_end, pair1);
+      if (begin >= end) break;  // (only the places before an item's stages: another CTA's item)
+      const int r0 = __shfl_sync(0xffffffffu, my_r0, i), q_len = __shfl_sync(0xffffffffu, my_q, i);
+      const int n = __shfl_sync(0xffffffffu, my_n, i), pos0 = __shfl_sync(0xffffffffu, my_kv, i);
+      const int k0 = static_cast<int>(begin - pair0) * kKvStage, n_st = static_cast<int>(end - begin);
+      const int k1 = min(n, k0 + n_st * kKvStage);
+      const int is = n_items & 1, R = q_len * a.group;
+      uint4 raw[kNT][kHd / 32];
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) {
+        const int row = 8 * t + g, tok = row / a.group;
+        const uint16_t* src = a.q + static_cast<int64_t>(r0 + tok) * a.ldq + (head * a.group + row - tok * a.group) * kHd + q * (kHd / 4);
+#pragma unroll
+        for (int d = 0; d < kHd / 32; ++d) {
+          raw[t][d] = make_uint4(0, 0, 0, 0);
+          if (row < R) raw[t][d] = a.vec ? ld_row8<true>(src + 8 * d) : ld_row8<false>(src + 8 * d);
+        }
+      }
+      // Its stages.  Those whose slots are surely free (all of the ring for the first item, one for
+      // the others) are requested before q is turned into fragments.
+      const int pieces = kKvStage >> pe_shift;                   // per stage
+      const int ahead = 32 >> (kKvStageShift - pe_shift);        // stages whose page numbers the warp holds
+      const uint32_t piece_bytes = static_cast<uint32_t>(pe) * (kHd + 8);
+      int pages = -1;
+      const auto issue = [&](int t) {
+        if (t % ahead == 0) {  // lane l: the page of piece l from here on
+          const int pos = k0 + t * kKvStage + lane * pe;
+          pages = -1;
+          if (pos < k1) {
+            pages = __ldg(a.B.table + seq * a.B.table_stride + (pos >> a.C.page_shift));
+            if (static_cast<uint32_t>(pages) >= static_cast<uint32_t>(a.C.n_pages)) {
+              kv_bad_index(a.B);
+              pages = -1;
+            }
+          }
+        }
+        const int slot = st_all % kS;
+        if (st_all >= kS && !mbar_wait_bounded(empty_b + 8 * slot, ((st_all / kS) - 1) & 1)) {
+          ok = false;
+          return;
+        }
+        const int page = __shfl_sync(0xffffffffu, pages, ((t % ahead) << (kKvStageShift - pe_shift)) + min(lane, pieces - 1));
+        const uint32_t mask = __ballot_sync(0xffffffffu, lane < pieces && page >= 0);
+        if (lane == 0) {
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(valid_s + 4 * slot), "r"(mask) : "memory");
+          mbar_expect_tx(full_b + 8 * slot, piece_bytes * __popc(mask));
+        }
+        __syncwarp();
+        if (lane < pieces && page >= 0) {
+          const uint8_t* block = a.C.pages + (static_cast<int64_t>(page) * kvh_n + head) * a.C.head_bytes;
+          const uint32_t dst = ring + slot * kStageBytes + lane * piece_bytes, bar = full_b + 8 * slot;
+          if (a.C.page_size <= kKvStage) {
+            bulk_g2s_hint(dst, block, piece_bytes, bar, once);
+          } else {  // part of a larger page
+            const int off = (k0 + t * kKvStage) & (a.C.page_size - 1);
+            const uint8_t* pairs = block + a.C.page_size * kHd;
+            bulk_g2s_hint(dst, block + off * kRow, kKvStage * kRow, bar, once);
+            bulk_g2s_hint(dst + kKvStage * kRow, block + (a.C.page_size + off) * kRow, kKvStage * kRow, bar, once);
+            bulk_g2s_hint(dst + kKvStage * kHd, pairs + 4 * off, 4 * kKvStage, bar, once);
+            bulk_g2s_hint(dst + kKvStage * (kHd + 4), pairs + 4 * (a.C.page_size + off), 4 * kKvStage, bar, once);
+          }
+        }
+        ++st_all;
+      };
+      const int first = min(n_st, st_all == 0 ? kS : 1);
+      for (int t = 0; t < first && ok; ++t) issue(t);
+      if (!ok) break;
+      // The item's slot: the description, and q as fragments (once per item here instead of once per
+      // consumer; the consumers read them back for every 32 keys, which costs them less than holding
+      // them in registers).
+      if (n_items >= 2 && !mbar_wait_bounded(free_b + 8 * is, ((n_items >> 1) - 1) & 1)) {
         ok = false;
         break;
       }
-      const int page = __shfl_sync(0xffffffffu, pages, ((st % ahead) << (6 - pe_shift)) + min(lane, pieces - 1));
-      const uint32_t mask = __ballot_sync(0xffffffffu, lane < pieces && page >= 0);
       if (lane == 0) {
-        asm volatile("st.shared.u32 [%0], %1;" ::"r"(valid_s + 4 * slot), "r"(mask) : "memory");
-        mbar_expect_tx(full_b + 8 * slot, piece_bytes * __popc(mask));
+        KvItem it;
+        it.n_st = n_st;
+        it.k0 = k0;
+        it.k1 = k1;
+        it.seq_end = n;
+        it.hidden = n - (pos0 + 1);
+        it.r0 = r0;
+        it.rows = R;
+        it.kvh = head;
+        it.c_first = cta_of(pair0);
+        it.contributors = cta_of(pair1 - 1) - it.c_first + 1;
+        it.record = 2 * c + (static_cast<int>(c) == it.c_first);
+        *reinterpret_cast<KvItem*>(slots + is * kSlotBytes + kItemAt) = it;
       }
+      const uint32_t slot_s = smem_u32(slots) + is * kSlotBytes;
+      if (a.bf16) kv_stage_q<kHd, kNT, true>(raw, slot_s, a.scale, lane);
+      else kv_stage_q<kHd, kNT, false>(raw, slot_s, a.scale, lane);
       __syncwarp();
-      if (lane < pieces && page >= 0) {
-        const uint8_t* block = a.C.pages + (static_cast<int64_t>(page) * a.C.kv_heads + kvh) * a.C.head_bytes;
-        const uint32_t dst = ring + slot * kStageBytes + lane * piece_bytes, bar = full_b + 8 * slot;
-        if (a.C.page_size <= kKvStage) {
-          bulk_g2s(dst, block, piece_bytes, bar);
-        } else {  // part of a larger page
-          const int off = (k0 + st * kKvStage) & (a.C.page_size - 1);
-          const uint8_t* pairs = block + a.C.page_size * kHd;
-          bulk_g2s(dst, block + off * kRow, kKvStage * kRow, bar);
-          bulk_g2s(dst + kKvStage * kRow, block + (a.C.page_size + off) * kRow, kKvStage * kRow, bar);
-          bulk_g2s(dst + kKvStage * kHd, pairs + 4 * off, 4 * kKvStage, bar);
-          bulk_g2s(dst + kKvStage * (kHd + 4), pairs + 4 * (a.C.page_size + off), 4 * kKvStage, bar);
-        }
-      }
+      if (lane == 0) mbar_arrive(item_b + 8 * is);
+      ++n_items;
+      for (int t = first; t < n_st && ok; ++t) issue(t);
+      w = end;
     }
-    if (ok)  // every copy has landed before the CTA can end, whatever its consumers did
-      for (int st = max(0, n_st - kS); st < n_st; ++st) ok = mbar_wait_bounded(full_b + 8 * (st % kS), (st / kS) & 1) && ok;
+    // no more items
+    const int is = n_items & 1;
+    if (ok && n_items >= 2) ok = mbar_wait_bounded(free_b + 8 * is, ((n_items >> 1) - 1) & 1);
+    if (ok && lane == 0) {
+      reinterpret_cast<KvItem*>(slots + is * kSlotBytes + kItemAt)->n_st = -1;
+      mbar_arrive(item_b + 8 * is);
+    }
+    // every copy has landed before the CTA can end, whatever its consumers did
+    for (int t = max(0, st_all - kS); t < st_all; ++t) ok = mbar_wait_bounded(full_b + 8 * (t % kS), (t / kS) & 1) && ok;
     if (!ok && lane == 0) atomicCAS(a.B.err, 0, kDevErrTmaTimeout);
     return;
   }
 
   // ------------------------------------------------------------------ consumers
-  const int R = q_len * a.group;  // live rows
-  // q as B fragments: lane (g, q) has row g of each row tile at dimensions q*kHd/4 + 8w + i, word w;
-  // multiplication s of a word meets codes (2s, 2s + 4) in the first register, (2s + 1, 2s + 5) in
-  // the second
-  uint32_t bq[kNT][2 * kKW][2];
-  float cf[kNT][2], qs[kNT][2];  // of rows 2q, 2q + 1: factor of the scores (log2 units), sum of q
-  int lim[kNT][2];               // keys that the row sees
+  // Score row r of 16 keys is key r ^ ((r >> 1) & 1), an order in which both code reads spread over
+  // the banks: rows g and 8 + g are keys perm and 8 + perm, the weights 2q and 2q + 1 the keys pk and
+  // pk +- 1.
+  const int perm = g ^ ((g >> 1) & 1), pk = 2 * q + (q & 1);
+  const int vnext = (q & 1) ? -kRow : kRow;
+  // This lane's addresses for the first 16 of the warp's 32 keys of a stage, and the way to the others
+  // (the same piece of the stage, or with pages of 16 the next).
+  const uint32_t piece = ring + ((32 * warp) >> pe_shift) * pe * (kHd + 8);
+  const int place = (32 * warp) & (pe - 1);
+  const uint32_t ka = piece + (place + perm) * kRow + q * (kHd / 8);
+  const uint32_t pa = piece + pe * kHd + 4 * (place + perm);
+  const uint32_t va = piece + (pe + place + pk) * kRow + g * (kHd / 16);
+  const uint32_t next_code = pe == 16 ? 16 * (kHd + 8) : 16 * kRow, next_pair = pe == 16 ? 16 * (kHd + 8) : 64;
+  int slot = 0, n_shared = 0, n_arrived = 0;
+  uint32_t phase = 0;
+#pragma unroll 1
+  for (int item = 0;; ++item) {
+  // (a wait that gives up is told to all four warps, which leave together: none waits at a barrier for another)
+  if (!mbar_wait_bounded(item_b + 8 * (item & 1), (item >> 1) & 1)) sm_failed = 1;
+  named_barrier(1, kKvStepWarps * 32);  // ... and the last item's records have been read
+  if (sm_failed) break;
+  if (n_arrived < n_shared) {  // the last item's record is complete
+    if (tid == 0) kv_arrive(sp, sm_shared[n_arrived], &sm_last[n_arrived]);
+    ++n_arrived;
+  }
+  const unsigned char* slot_p = slots + (item & 1) * kSlotBytes;
+  // (the description is read where it is needed: it stays in its slot until the item's end)
+  const volatile KvItem& it = *reinterpret_cast<const volatile KvItem*>(slot_p + kItemAt);
+  int left = it.n_st;
+  if (left < 0) break;
+  int kb = it.k0 + 32 * warp;  // this warp's first key of a stage
+  const int k1 = it.k1;
+  const uint32_t bq = smem_u32(slot_p) + lane * 16;  // q's fragments
+  float cf[kNT][2], qs[kNT][2];  // of rows 2q, 2q + 1: factor of the scores, sum of q
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
-    const int row = 8 * t + g, i = row / a.group;
-    float x[kHd / 4];
-    float big = 0.f, sum = 0.f;
-    const uint16_t* src = a.q + static_cast<int64_t>(r0 + i) * a.ldq + (kvh * a.group + row - i * a.group) * kHd + q * (kHd / 4);
-#pragma unroll
-    for (int d = 0; d < kHd / 4; d += 8) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (row < R) v = a.vec ? ld_row8<true>(src + d) : ld_row8<false>(src + d);
-      if (a.bf16) unpack_halves<true>(v, x + d);
-      else unpack_halves<false>(v, x + d);
-    }
-#pragma unroll
-    for (int d = 0; d < kHd / 4; ++d) big = fmaxf(big, fabsf(x[d]));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-    // e with big * 2^e in [2^14, 2^15); |e| is kept below 100 (a query beyond fp32's reach overflows)
-    const int e = max(-99, min(99, big > 0.f ? 14 - ((__float_as_int(big) >> 23) - 127) : 0));
-    const float up = pow2i(e);
-#pragma unroll
-    for (int d = 0; d < kHd / 4; ++d) {
-      x[d] = __half2float(__float2half_rn(x[d] * up));
-      sum += x[d];
-    }
-    sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-    sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-#pragma unroll
-    for (int w = 0; w < kKW; ++w)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        bq[t][2 * w + s][0] = pack_halves<false>(x[8 * w + 2 * s], x[8 * w + 2 * s + 4]);
-        bq[t][2 * w + s][1] = pack_halves<false>(x[8 * w + 2 * s + 1] * 0.0625f, x[8 * w + 2 * s + 5] * 0.0625f);
-      }
-    // the scores' rows are 2q and 2q + 1 of the tile: fetch their numbers from the lanes of those rows
-    const float f = a.scale * 1.4426950408889634f * pow2i(12 - e);  // the other half of 2^(24 - e): below
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      cf[t][c] = __shfl_sync(0xffffffffu, f, (2 * q + c) * 4) * 4096.0f;
-      qs[t][c] = __shfl_sync(0xffffffffu, sum, (2 * q + c) * 4) * 0x1p-24f;
-      const int rr = 8 * t + 2 * q + c;
-      lim[t][c] = rr < R ? max(0, min(n, kv_all - q_all + rr / a.group + 1)) : 0;
-    }
+    const float4 v = *reinterpret_cast<const float4*>(slot_p + kRows * kHd * 2 + 8 * (8 * t + 2 * q));
+    cf[t][0] = v.x;
+    qs[t][0] = v.y;
+    cf[t][1] = v.z;
+    qs[t][1] = v.w;
   }
-  const int all_see = max(0, min(n, kv_all - q_all + 1));  // keys below this are seen by every live row
+  // keys that row r sees (none where there is no row)
+  const auto limit = [&](int r) { return r < it.rows ? min(it.seq_end, it.seq_end - it.hidden + r / a.group) : 0; };
+  // keys below this need no mask: every live row sees them
+  const int plain_end = min(k1, it.seq_end - it.hidden);
 
   float acc[kNT][kMt][4], az[kNT][2], sum[kNT][2], m[kNT][2];
 #pragma unroll
@@ -447,69 +665,86 @@ __global__ void __launch_bounds__(kKvStepThreads) kv_attention_step_kernel(const
   }
   int ve = -30;             // the weights carry scale_v * 2^-ve
   float vinv = 0x1p30f;
-  const int perm = g ^ ((g >> 1) & 1);      // the key of score row g (and 8 + perm of row 8 + g): an
-  const int pk = 2 * q + (q & 1);           // order in which both code reads spread over the banks;
-  const int pk1 = 2 * q + 1 - (q & 1);      // the keys of weights 2q, 2q + 1
-  const uint32_t woff = static_cast<uint32_t>(((16 * warp) >> pe_shift) * pe * (kHd + 8));
-  const int koff = (16 * warp) & (pe - 1);
-
-  for (int st = 0; st < n_st; ++st) {
-    const int slot = st % kS;
-    if (!mbar_wait_bounded(full_b + 8 * slot, (st / kS) & 1)) {
-      ok = false;
+  for (; left > 0; --left, kb += kKvStage) {
+    if (!mbar_wait_bounded(full_b + 8 * slot, phase)) {
+      sm_failed = 1;
       break;
     }
-    const int kb = k0 + st * kKvStage + 16 * warp;  // this warp's first key
-    const uint32_t base = ring + slot * kStageBytes + woff;
-    if (kb < k1 && ((lds32(valid_s + 4 * slot) >> ((16 * warp) >> pe_shift)) & 1u)) {
-      const uint32_t pairs = base + pe * kHd + 4 * (koff + perm);
-      uint32_t kp[2], vp[2];
-      kp[0] = lds32(pairs);
-      kp[1] = lds32(pairs + 32);
-      vp[0] = lds32(pairs + 4 * pe);
-      vp[1] = lds32(pairs + 4 * pe + 32);
-      const bool whole = kb + 16 <= min(k1, all_see);  // no mask in this tile (rows that are not live see garbage)
-      if (kb + perm >= k1) kp[0] = vp[0] = 0;           // places past the end hold anything
-      if (kb + perm + 8 >= k1) kp[1] = vp[1] = 0;
+    const uint32_t so = slot * kStageBytes;
+    const uint32_t valid = lds32(valid_s + 4 * slot);
+    const bool v0 = (valid >> ((32 * warp) >> pe_shift)) & 1u, v1 = (valid >> ((32 * warp + 16) >> pe_shift)) & 1u;
+    if (kb < k1 && (v0 || v1)) {
+      const bool whole = kb + 32 <= plain_end && v0 && v1;  // no mask (rows that are not live see garbage)
+      uint32_t kp[2][2], vp[2][2];
+      float s[2][kNT][4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint32_t pairs = pa + so + j * next_pair;
+        kp[j][0] = lds32(pairs);
+        kp[j][1] = lds32(pairs + 32);
+        vp[j][0] = lds32(pairs + 4 * pe);
+        vp[j][1] = lds32(pairs + 4 * pe + 32);
+#pragma unroll
+        for (int t = 0; t < kNT; ++t)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) s[j][t][c] = 0.f;
+      }
       // ---- scores
-      float s[kNT][4];
-#pragma unroll
-      for (int t = 0; t < kNT; ++t)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) s[t][c] = 0.f;
       {
-        uint32_t w0[kKW], w1[kKW];
-        const uint32_t ka = base + (koff + perm) * kRow + q * (kHd / 8);
-        lds_words<kKW>(ka, w0);
-        lds_words<kKW>(ka + 8 * kRow, w1);
+        uint32_t w[2][2][kKW];
 #pragma unroll
-        for (int w = 0; w < kKW; ++w)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t u0 = w0[w] >> (8 * h), u1 = w1[w] >> (8 * h);
-            const uint32_t A[4] = {u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u};
-#pragma unroll
-            for (int t = 0; t < kNT; ++t) mma16816(s[t], A, bq[t][2 * w + h][0], bq[t][2 * w + h][1]);
-          }
-      }
-      const float ks0 = half_lo<false>(kp[0]), kz0 = half_hi<false>(kp[0]), ks1 = half_lo<false>(kp[1]), kz1 = half_hi<false>(kp[1]);
-      const float vs0 = half_lo<false>(vp[0]), vz0 = half_hi<false>(vp[0]), vs1 = half_lo<false>(vp[1]), vz1 = half_hi<false>(vp[1]);
-      bool move = fmaxf(fabsf(vs0), fabsf(vs1)) * vinv > 32.f;
-#pragma unroll
-      for (int t = 0; t < kNT; ++t) {
-        s[t][0] = (s[t][0] + kz0 * qs[t][0]) * (ks0 * cf[t][0]);
-        s[t][1] = (s[t][1] + kz0 * qs[t][1]) * (ks0 * cf[t][1]);
-        s[t][2] = (s[t][2] + kz1 * qs[t][0]) * (ks1 * cf[t][0]);
-        s[t][3] = (s[t][3] + kz1 * qs[t][1]) * (ks1 * cf[t][1]);
-        if (!whole) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c)
-            if (kb + perm + 8 * (c >> 1) >= lim[t][c & 1]) s[t][c] = -INFINITY;
+        for (int j = 0; j < 2; ++j) {
+          lds_words<kKW>(ka + so + j * next_code, w[j][0]);
+          lds_words<kKW>(ka + so + j * next_code + 8 * kRow, w[j][1]);
         }
-        move |= fmaxf(s[t][0], s[t][2]) > m[t][0] + 8.f || fmaxf(s[t][1], s[t][3]) > m[t][1] + 8.f;
+#pragma unroll
+        for (int i = 0; i < kKW; ++i) {
+          uint4 b[kNT];
+#pragma unroll
+          for (int t = 0; t < kNT; ++t) b[t] = lds128(bq + (t * (kHd / 32) + i) * 512);
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint32_t u0 = w[j][0][i] >> (8 * h), u1 = w[j][1][i] >> (8 * h);
+              const uint32_t A[4] = {u0 & 0x000f000fu, u1 & 0x000f000fu, u0 & 0x00f000f0u, u1 & 0x00f000f0u};
+#pragma unroll
+              for (int t = 0; t < kNT; ++t) mma16816(s[j][t], A, h ? b[t].z : b[t].x, h ? b[t].w : b[t].y);
+            }
+        }
       }
+      if (!whole) {  // places past the end, or of a page that does not exist, hold anything
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (kb + 16 * j + perm + 8 * e >= k1 || !(j ? v1 : v0)) kp[j][e] = vp[j][e] = 0;
+      }
+      float2 vf[2][2];  // (scale, zero) of the values
+      float top[kNT][2], vmax = 0.f;
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) top[t][0] = top[t][1] = -INFINITY;
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 kf = unpack_half2(kp[j][e]);
+          vf[j][e] = unpack_half2(vp[j][e]);
+          vmax = fmaxf(vmax, fabsf(vf[j][e].x));
+#pragma unroll
+          for (int t = 0; t < kNT; ++t)
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+              float x = (s[j][t][2 * e + c] + kf.y * qs[t][c]) * (kf.x * cf[t][c]);
+              if (!whole && (kb + 16 * j + perm + 8 * e >= limit(8 * t + 2 * q + c) || !(j ? v1 : v0))) x = -INFINITY;
+              s[j][t][2 * e + c] = x;
+              top[t][c] = fmaxf(top[t][c], x);
+            }
+        }
+      bool move = vmax * vinv > 32.f;
+#pragma unroll
+      for (int t = 0; t < kNT; ++t) move |= top[t][0] > m[t][0] + 8.f || top[t][1] > m[t][1] + 8.f;
       if (__any_sync(0xffffffffu, move)) {
-        float vmax = fmaxf(fmaxf(fabsf(vs0), fabsf(vs1)), 0.f);  // (NaN scales have no size)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
         const int e = max(ve, min(17, (__float_as_int(vmax) >> 23) - 126));  // 2^e above every scale so far
@@ -520,7 +755,7 @@ __global__ void __launch_bounds__(kKvStepThreads) kv_attention_step_kernel(const
         for (int t = 0; t < kNT; ++t)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            float x = fmaxf(s[t][c], s[t][c + 2]);
+            float x = top[t][c];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
             const float mn = fmaxf(m[t][c], x), corr = ex2(m[t][c] - mn);
@@ -534,70 +769,73 @@ __global__ void __launch_bounds__(kKvStepThreads) kv_attention_step_kernel(const
             }
           }
       }
-      // ---- weights
-      const float u0 = vs0 * vinv, u1 = vs1 * vinv;
-      uint32_t bp[kNT][2];
 #pragma unroll
-      for (int t = 0; t < kNT; ++t) {
-        float p[4], w[4];
+      for (int j = 0; j < 2; ++j) {
+        // ---- weights
+        const float u0 = vf[j][0].x * vinv, u1 = vf[j][1].x * vinv;
+        uint32_t bp[kNT][2];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          p[c] = ex2(s[t][c] - m[t][c & 1]);
-          w[c] = p[c] * (c < 2 ? u0 : u1);
-          // (a hidden key's scale may be NaN)
-          if (!whole && kb + perm + 8 * (c >> 1) >= lim[t][c & 1]) p[c] = w[c] = 0.f;
+        for (int t = 0; t < kNT; ++t) {
+          float p[4], w[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            p[c] = ex2(s[j][t][c] - m[t][c & 1]);
+            w[c] = p[c] * (c < 2 ? u0 : u1);
+            if (!whole && s[j][t][c] == -INFINITY) w[c] = 0.f;  // (a hidden key's scale may be NaN)
+          }
+          sum[t][0] += p[0] + p[2];
+          sum[t][1] += p[1] + p[3];
+          const uint32_t h0 = pack_halves<false>(w[0], w[1]), h1 = pack_halves<false>(w[2], w[3]);
+          const float2 r0 = unpack_half2(h0), r1 = unpack_half2(h1);
+          az[t][0] += r0.x * vf[j][0].y + r1.x * vf[j][1].y;
+          az[t][1] += r0.y * vf[j][0].y + r1.y * vf[j][1].y;
+          bp[t][0] = movmatrix_trans(h0);
+          bp[t][1] = movmatrix_trans(h1);
         }
-        sum[t][0] += p[0] + p[2];
-        sum[t][1] += p[1] + p[3];
-        const uint32_t h0 = pack_halves<false>(w[0], w[1]), h1 = pack_halves<false>(w[2], w[3]);
-        az[t][0] += half_lo<false>(h0) * vz0 + half_lo<false>(h1) * vz1;
-        az[t][1] += half_hi<false>(h0) * vz0 + half_hi<false>(h1) * vz1;
-        bp[t][0] = movmatrix_trans(h0);
-        bp[t][1] = movmatrix_trans(h1);
+        // ---- values: half word h (4 dimensions) of the lane's kHd/8 dimensions, of four keys
+        const uint32_t v0a = va + so + j * next_code, v1a = v0a + vnext;
+        constexpr int kH = kHd / 32;  // half words per key
+        uint32_t lo[kH], hi[kH];      // (key pk | key pk +- 1) of the first and the second eight keys
+        if constexpr (kH % 2 == 0) {
+          uint32_t x[4][kH / 2];
+          lds_words<kH / 2>(v0a, x[0]);
+          lds_words<kH / 2>(v1a, x[1]);
+          lds_words<kH / 2>(v0a + 8 * kRow, x[2]);
+          lds_words<kH / 2>(v1a + 8 * kRow, x[3]);
+#pragma unroll
+          for (int h = 0; h < kH; ++h) {
+            const uint32_t sel = (h & 1) ? 0x7632u : 0x5410u;
+            lo[h] = prmt(x[0][h >> 1], x[1][h >> 1], sel);
+            hi[h] = prmt(x[2][h >> 1], x[3][h >> 1], sel);
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < kH; ++h) {
+            lo[h] = lds16(v0a + 2 * h) | (lds16(v1a + 2 * h) << 16);
+            hi[h] = lds16(v0a + 8 * kRow + 2 * h) | (lds16(v1a + 8 * kRow + 2 * h) << 16);
+          }
+        }
+#pragma unroll
+        for (int h = 0; h < kH; ++h)
+#pragma unroll
+          for (int z = 0; z < 2; ++z) {
+            const uint32_t u = lo[h] >> (8 * z), v = hi[h] >> (8 * z);
+            const uint32_t A[4] = {u & 0x000f000fu, u & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u};
+#pragma unroll
+            for (int t = 0; t < kNT; ++t) mma16816(acc[t][2 * h + z], A, bp[t][0], bp[t][1]);
+          }
       }
-      // ---- values: half word h (4 dimensions) of the lane's kHd/8 dimensions, of four keys
-      const uint32_t va = base + pe * kRow + koff * kRow + g * (kHd / 16);
-      constexpr int kH = kHd / 32;  // half words per key
-      uint32_t lo[kH], hi[kH];      // (key pk | key pk1) of the first and the second eight keys
-      if constexpr (kH % 2 == 0) {
-        uint32_t x[4][kH / 2];
-        lds_words<kH / 2>(va + pk * kRow, x[0]);
-        lds_words<kH / 2>(va + pk1 * kRow, x[1]);
-        lds_words<kH / 2>(va + (8 + pk) * kRow, x[2]);
-        lds_words<kH / 2>(va + (8 + pk1) * kRow, x[3]);
-#pragma unroll
-        for (int h = 0; h < kH; ++h) {
-          const uint32_t sel = (h & 1) ? 0x7632u : 0x5410u;
-          lo[h] = prmt(x[0][h >> 1], x[1][h >> 1], sel);
-          hi[h] = prmt(x[2][h >> 1], x[3][h >> 1], sel);
-        }
-      } else {
-#pragma unroll
-        for (int h = 0; h < kH; ++h) {
-          lo[h] = lds16(va + pk * kRow + 2 * h) | (lds16(va + pk1 * kRow + 2 * h) << 16);
-          hi[h] = lds16(va + (8 + pk) * kRow + 2 * h) | (lds16(va + (8 + pk1) * kRow + 2 * h) << 16);
-        }
-      }
-#pragma unroll
-      for (int h = 0; h < kH; ++h)
-#pragma unroll
-        for (int z = 0; z < 2; ++z) {
-          const uint32_t u = lo[h] >> (8 * z), v = hi[h] >> (8 * z);
-          const uint32_t A[4] = {u & 0x000f000fu, u & 0x00f000f0u, v & 0x000f000fu, v & 0x00f000f0u};
-#pragma unroll
-          for (int t = 0; t < kNT; ++t) mma16816(acc[t][2 * h + z], A, bp[t][0], bp[t][1]);
-        }
     }
     __syncwarp();
     if (lane == 0) mbar_arrive(empty_b + 8 * slot);
+    if (++slot == kS) {
+      slot = 0;
+      phase ^= 1u;
+    }
   }
-  if (!ok && lane == 0) atomicCAS(a.B.err, 0, kDevErrTmaTimeout);
-
   // ------------------------------------------------------------------ merge of the four warps
-  // (the ring is free: every copy was waited for)
-  named_barrier(1, kKvStepWarps * 32);
-  float* rec = reinterpret_cast<float*>(smem);  // [warp][row][kHd + 4]: the sums, then m and the sum of weights
   constexpr int kRec = kHd + 4;
+  const int R = it.rows;
   const float back = pow2i(ve);
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
@@ -627,9 +865,11 @@ __global__ void __launch_bounds__(kKvStepThreads) kv_attention_step_kernel(const
     }
   }
   named_barrier(1, kKvStepWarps * 32);
-  const bool single = n_chunks == 1;
-  const int64_t pair_id = static_cast<int64_t>(seq) * a.C.kv_heads + kvh;
-  float* part = single ? nullptr : sp.part + (pair_id * sp.chunks + chunk) * (static_cast<int64_t>(sp.rows) * (kHd + 4));
+  const int r0 = it.r0, kvh = it.kvh, c_first = it.c_first, contributors = it.contributors;
+  const bool single = contributors == 1;
+  float* part = sp.part + static_cast<int64_t>(it.record) * sp.rows * kRec;
+  __syncwarp();
+  if (lane == 0) mbar_arrive(free_b + 8 * (item & 1));
   constexpr int kQ = kHd / 4;  // float4 columns of a row
   for (int i = tid; i < R * kQ; i += kKvStepWarps * 32) {
     const int row = i / kQ, d = 4 * (i - row * kQ);
@@ -655,12 +895,30 @@ __global__ void __launch_bounds__(kKvStepThreads) kv_attention_step_kernel(const
     if (single) {
       kv_finish_row(a, r0, kvh, row, d, o, M, T);
     } else {
-      *reinterpret_cast<float4*>(part + row * (kHd + 4) + d) = o;
-      if (d == 0) *reinterpret_cast<float2*>(part + row * (kHd + 4) + kHd) = make_float2(M, T);
+      *reinterpret_cast<float4*>(part + row * kRec + d) = o;
+      if (d == 0) *reinterpret_cast<float2*>(part + row * kRec + kHd) = make_float2(M, T);
     }
   }
-  if (single) return;
-  kv_merge_chunks<kHd, kKvStepWarps * 32>(a, sp, r0, kvh, pair_id, n_chunks, R, smem, &sm_last);
+  if (!single) {
+    if (tid == 0) sm_shared[n_shared] = {r0, kvh, c_first, contributors, R};
+    ++n_shared;
+  }
+  }
+  // Merges come after the loop: in it their registers would push the tile's to local memory
+  // (attention over 131071 keys 44 -> 68 us).
+  named_barrier(1, kKvStepWarps * 32);  // sm_shared and sm_failed are final; rec may be overwritten
+  if (sm_failed) {
+    if (tid == 0) atomicCAS(a.B.err, 0, kDevErrTmaTimeout);
+    return;
+  }
+  if (tid == 0 && n_arrived < n_shared) kv_arrive(sp, sm_shared[n_arrived], &sm_last[n_arrived]);
+  named_barrier(1, kKvStepWarps * 32);
+  for (int i = 0; i < n_shared; ++i) {
+    if (!sm_last[i]) continue;
+    const KvShared& sh = sm_shared[i];
+    kv_merge_records<kHd, kKvStepWarps * 32>(a, sp, sh.r0, sh.kvh, sh.c_first, sh.contributors, sh.rows,
+                                             reinterpret_cast<float*>(smem), (kS * kStageBytes + kv_rec_bytes(kHd, kNT)) / 4);
+  }
 }
 
 }  // namespace opc
