@@ -11,6 +11,7 @@
 #include "opc_internal.h"
 #include "opc_kv.cuh"
 #include "opc_kv_attention.cuh"
+#include "opc_kv_prompt.cuh"
 
 namespace {
 
@@ -126,7 +127,9 @@ struct AttentionPlan {
   int step_nt;          // row tiles of the step kernel, 0: not launched
   int step_q;           // the step kernel takes sequences of at most this many rows
   int step_grid;
-  size_t bytes;         // workspace: the counters, then the records
+  int pairs;            // row tile groups of the longest sequence in the prompt kernel, 0: not launched
+  int splits, tiles;    // CTAs per row tile group, key tiles of each
+  size_t bytes;         // workspace: the counters, then the records (of one kernel after the other)
 };
 
 constexpr size_t kCounterBytes = 4096;  // one per CTA of a launch
@@ -142,6 +145,19 @@ AttentionPlan plan_attention(const opc_kv_cache& c, const opc_kv_batch& b, int g
     p.step_grid = std::min<int>(sms * opc::kv_step_ctas(c.head_dim, p.step_nt), kCounterBytes / 4);
     p.bytes += static_cast<size_t>(p.step_grid) * 2 * (p.step_q * group) * (c.head_dim + 4) * 4;
   }
+  if (b.max_q > p.step_q) {
+    const int64_t rows = static_cast<int64_t>(opc::kv_p_qt(c.head_dim)) * opc::kKvPM;
+    const int64_t pairs = (static_cast<int64_t>(b.max_q) * group + rows - 1) / rows;
+    const int64_t items = std::max<int64_t>(1, pairs * c.kv_heads * std::max(b.n_seqs, 1));
+    const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(b.max_kv) + opc::kKvPN - 1) / opc::kKvPN);
+    // Fewer row tile groups than SMs are split over the keys, down to two tiles for each CTA.
+    const int64_t splits = std::max<int64_t>(1, std::min(sms / items, tiles / 2));
+    p.pairs = static_cast<int>(std::min<int64_t>(pairs, INT32_MAX / splits));
+    p.tiles = static_cast<int>((tiles + splits - 1) / splits);
+    p.splits = static_cast<int>((tiles + p.tiles - 1) / p.tiles);
+    if (p.splits > 1)
+      p.bytes = std::max(p.bytes, kCounterBytes + static_cast<size_t>(items) * p.splits * rows * (c.head_dim + 4) * 4);
+  }
   return p;
 }
 
@@ -153,6 +169,12 @@ auto step_of(int hd) {
   }
   return hd == 32 ? opc::kv_attention_step_kernel<32, kNT> : hd == 64 ? opc::kv_attention_step_kernel<64, kNT>
        : hd == 96 ? opc::kv_attention_step_kernel<96, kNT> : opc::kv_attention_step_kernel<128, kNT>;
+}
+
+auto prompt_of(int hd) {
+  return hd == 32 ? opc::kv_attention_prompt_kernel<32> : hd == 64 ? opc::kv_attention_prompt_kernel<64>
+       : hd == 96 ? opc::kv_attention_prompt_kernel<96> : hd == 128 ? opc::kv_attention_prompt_kernel<128>
+       : hd == 192 ? opc::kv_attention_prompt_kernel<192> : opc::kv_attention_prompt_kernel<256>;
 }
 
 // Launched with programmatic serialization: set-up overlaps the kernel before, which each of these
@@ -353,10 +375,17 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
     KV_CUDA(launch_pdl(kern, dim3(p.step_grid), opc::kKvStepThreads, opc::kv_step_smem(cache->head_dim, p.step_nt), s, a, sp),
             "opc_kv_attention launch (steps)");
   }
-  if (a.B.max_q > p.step_q) {
+  if (p.pairs) {
     a.lo_q = p.step_q + 1;
     a.hi_q = a.B.max_q;
-    opc::kv_attention_plain_kernel<<<dim3(batch->n_tokens, heads), opc::kKvPlainThreads, 0, s>>>(a);
+    opc::KvPromptSplit sp;
+    sp.tiles = p.tiles;
+    sp.splits = p.splits;
+    sp.count = static_cast<int32_t*>(workspace);
+    sp.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
+    KV_CUDA(launch_pdl(prompt_of(cache->head_dim), dim3(p.pairs * p.splits, cache->kv_heads, batch->n_seqs), opc::kKvPThreads,
+                       opc::kv_p_smem(cache->head_dim), s, a, sp),
+            "opc_kv_attention launch (prompts)");
   }
   KV_CUDA(cudaGetLastError(), "opc_kv_attention launch");
   return OPC_OK;

@@ -98,9 +98,12 @@ def quantize32(x):
 
 
 def attention64(su: Setup, pages_np, q, scale, table_ok=None):
-    """(out, lse, weighted |v|, bound of the scores' error) per row in float64; rows of no sequence
-    are NaN.  The last two feed the tolerances."""
+    """(out, lse, weighted |v|, bound of the scores' error, bound of the values' error) per row in
+    float64; rows of no sequence are NaN.  The last three feed the tolerances."""
     k, v = values(pages_np, su.page, su.hd)
+    with np.errstate(invalid="ignore"):
+        off_k, off_v = (np.abs(s * (np.float64(1) * cz.astype(np.float16) - cz))
+                        for s, cz in _codes_plus_zero(pages_np, su.page, su.hd))
     _, _, kp, _ = parts(pages_np, su.page, su.hd)
     R, H, hd = q.shape
     G = H // su.kv_heads
@@ -108,6 +111,7 @@ def attention64(su: Setup, pages_np, q, scale, table_ok=None):
     lse = np.full((R, H), np.nan)
     mag = np.zeros((R, H, hd))
     dlt = np.zeros((R, H))
+    dv = np.zeros((R, H, hd))
     for r in range(R):
         p = su.place(r)
         if p is None:
@@ -116,6 +120,9 @@ def attention64(su: Setup, pages_np, q, scale, table_ok=None):
         if pos < 0:
             out[r], lse[r] = 0.0, -np.inf
             continue
+        # many rows per kv head (more than the 16, or with large heads 8, of the form for steps): code +
+        # zero goes to the tensor cores rounded to fp16, which moves the scores and values by this
+        rounded = su.q_lens[s] * G > (16 if hd <= 128 else 8)
         idx = np.arange(pos + 1)
         pg, off = su.table[s, idx // su.page], idx % su.page
         for h in range(H):
@@ -134,17 +141,26 @@ def attention64(su: Setup, pages_np, q, scale, table_ok=None):
             mag[r, h] = w @ np.abs(vv)
             # fp32 sums of up to hd products q * code (at most 15) and q * zero, a few roundings each
             dlt[r, h] = abs(scale) * np.max(np.abs(pr[:, 0]) * (15.0 + np.abs(pr[:, 1]))) * np.abs(qq).sum() * 2.0 ** -21
-    return out, lse, mag, dlt
+            if rounded:
+                dlt[r, h] += abs(scale) * np.max(off_k[pg, h // G, off] @ np.abs(qq))
+                dv[r, h] = w @ off_v[pg, h // G, off]
+    return out, lse, mag, dlt, dv
 
 
-def check_attention(got, got_lse, ref, eps, live=None, rounded_keys=0.0):
+def _codes_plus_zero(pages, page, hd):
+    """(scale, code + zero) of keys and of values, float64."""
+    kc, vc, kp, vp = parts(pages, page, hd)
+    for c, p in ((kc, kp), (vc, vp)):
+        yield p[..., :1].astype(np.float64), nibbles(c).astype(np.float64) + p[..., 1:].astype(np.float64)
+
+
+def check_attention(got, got_lse, ref, eps, live=None):
     """Tolerance: the output's rounding (eps/2 of it); each weight rounded once to fp16 (2^-11, plus
     what the fp32 exponential and sums add, 2^-18) and off by twice the scores' error, which moves
-    the result by at most that times sum w |v|; `rounded_keys`: a further error of the scores."""
-    out, lse, mag, dlt = ref
+    the result by at most that times sum w |v|; the values' own error."""
+    out, lse, mag, d, dv = ref
     live = np.isfinite(lse) if live is None else live
-    d = dlt + rounded_keys
-    tol = eps / 2 * np.abs(out) + (2.0 ** -11 + 2.0 ** -18 + 2 * d[..., None]) * mag * (1 + eps) + 2.0 ** -24
+    tol = eps / 2 * np.abs(out) + ((2.0 ** -11 + 2.0 ** -18 + 2 * d[..., None]) * mag + dv) * (1 + eps) + 2.0 ** -24
     err = np.abs(got.astype(np.float64) - out)
     bad = ~(err <= tol) & live[..., None]
     assert not bad.any(), (np.argwhere(bad)[:4], err[bad][:4], tol[bad][:4])
