@@ -10,7 +10,8 @@ namespace opc {
 // The rows of one sequence and kv head (query token i, head j of the group: row i * group + j) in
 // tiles of 128; a CTA takes kQt tiles against the keys they see, 128 at a time:
 //
-//   S = Q K'^T     K' = code + zero in fp16: exact for |zero| < 8, one rounding otherwise.  The key's
+//   S = Q K'^T     (in halves of 64 keys, so that the next half's scores are there while one is evaluated)
+//                  K' = code + zero in fp16: exact for |zero| < 8, one rounding otherwise.  The key's
 //                  scale multiplies its column of S in fp32, so nothing of a key is rounded.
 //   P = exp2(S * scale_k - m) * scale_v, rounded once to fp16, written over S in tensor memory
 //   O += P V'      V' = code + zero in fp16, as above
@@ -18,7 +19,9 @@ namespace opc {
 // 4 * 128 * 128 * head_dim operations per tile pair, against 128 * 128 exponentials, which the
 // special-function units take as long for as the tensor cores for the products at head_dim 128: two
 // row tiles alternate, one in the tensor cores while the other is in the softmax.  Roles:
-//   warps 0..3, 4..7  softmax of row tile 0 and 1: thread = row (TMEM lane).  The reference m of a row
+//   warps 0..3, 4..7  softmax of row tile 0 and 1, 32 rows a warp in the 16-row fragment shapes: a lane has a
+//                     quarter of the columns of four rows, so it holds its keys' scales in registers (with
+//                     thread = row every thread would read all of them from shared memory).  The reference m of a row
 //                     moves only when a score passes m + 12 (with the largest scale_v of the tile):
 //                     the tile is first evaluated with the old m, and again, with O rescaled, where a
 //                     row of the warp passed it -- always in the first tile, hardly ever later.
@@ -26,8 +29,8 @@ namespace opc {
 //                     rows in the 128-byte-swizzled layout -- the same bytes are K-major for K' (rows
 //                     are the N dimension) and MN-major for V' (rows are the K dimension)
 //   warp 12           one lane issues the MMAs and commits them to the roles' barriers (13..15 idle)
-// The warpgroups trade registers: 128 a thread at the launch, then 192 for the softmax (which holds a
-// tile's weights until it knows that m stands), 88 and 40 for the others.
+// The warpgroups trade registers: 128 a thread at the launch, then 176 for the softmax (which holds a
+// tile's weights until it knows that m stands), 88 and 72 for the others.
 // The codes of a word come out in the order 0 4 1 5 2 6 3 7 (one mask per pair); q is staged in that
 // order too, and the output columns are put back in order by the epilogue.
 // Few CTAs are split over the keys: the partial results go to the workspace as records of the step
@@ -50,22 +53,41 @@ struct KvPromptSplit {
   int32_t* count;     // [items]
 };
 
-// D[tmem] (+)= A[tmem] * B[smem]: kind::f16, A fp16 packed in pairs along K.
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+// MMAs issued by one lane of a converged warp (`leader`, from elect.sync): outside a divergent branch
+// their operands can be formed in uniform registers, which brought a key tile's 48 instructions and
+// their barriers from ~6300 cycles to what the tensor cores take.
+__device__ __forceinline__ uint32_t elect_leader() {
+  uint32_t p;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
+  return p;
+}
+__device__ __forceinline__ void umma_f16_by(uint32_t leader, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum)
+      "{\n .reg .pred p, l;\n setp.ne.b32 l, %5, 0;\n setp.ne.b32 p, %4, 0;\n"
+      " @l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* v) {
+// The same with A in tensor memory, fp16 packed in pairs along K.
+__device__ __forceinline__ void umma_f16_ts_by(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                               uint32_t accum) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,"
-      "%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "{\n .reg .pred p, l;\n setp.ne.b32 l, %5, 0;\n setp.ne.b32 p, %4, 0;\n"
+      " @l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accum), "r"(leader)
       : "memory");
+}
+__device__ __forceinline__ void umma_commit_by(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred l;\n setp.ne.b32 l, %1, 0;\n"
+      " @l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}\n" ::"r"(bar), "r"(leader)
+      : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void swap_values(T& a, T& b) {
+  const T t = a;
+  a = b;
+  b = t;
 }
 template <int kRegs>
 __device__ __forceinline__ void regs_up() {
@@ -88,6 +110,128 @@ __host__ __device__ constexpr uint32_t kv_idesc(int n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kKvPM >> 4) << 24);
 }
 
+// Two fp32 values per instruction.
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t v) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+// The 16-row fragment shapes: of 8 fp32 columns lane (g, q) = (lane / 4, lane % 4) holds (row g, columns
+// 2q, 2q + 1) and (row g + 8, the same); of 4 32-bit columns (16x128b) column q of rows g and g + 8.
+__device__ __forceinline__ void tmem_ld_rows64(uint32_t taddr, uint32_t* v) {  // 64 columns
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17,"
+      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+      "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]),
+      "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
+      "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_ld_rows32(uint32_t taddr, uint32_t* v) {  // 32 columns
+  asm volatile(
+      "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
+      "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_rows32(uint32_t taddr, const uint32_t* v) {  // 32 columns
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x256b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+      "%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_pairs32(uint32_t taddr, const uint32_t* v) {  // 32 columns of fp16 pairs
+  asm volatile(
+      "tcgen05.st.sync.aligned.16x128b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15,"
+      "%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+
+// The weights of 16 rows (lane (g, q): rows g and g + 8) for 64 keys: pk the fp16 pairs
+// exp2(S * scale_k - m) * scale_v; the lane's share of the rows' sums of the weights without scale_v.
+// ks, vs: the scales of the lane's 16 keys (8i + 2q, 8i + 2q + 1).  kMask: a row sees its first `seen`
+// keys only.
+template <bool kMask>
+__device__ __forceinline__ void kv_weights(uint32_t s_addr, const uint64_t* ks, const uint64_t* vs, const float* m, const int* seen,
+                                           int q, uint32_t* pk, float* add) {
+  uint32_t v[32];
+  tmem_ld_rows64(s_addr, v);
+  tmem_wait_ld();
+  const uint64_t minus[2] = {pack2(-m[0], -m[0]), pack2(-m[1], -m[1])};
+  uint64_t sum[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      float2 y = unpack2(fma2(pack2(__uint_as_float(v[4 * i + 2 * a]), __uint_as_float(v[4 * i + 2 * a + 1])), ks[i], minus[a]));
+      if (kMask) {
+        if (8 * i + 2 * q >= seen[a]) y.x = -INFINITY;
+        if (8 * i + 2 * q + 1 >= seen[a]) y.y = -INFINITY;
+      }
+      const uint64_t p = pack2(ex2(y.x), ex2(y.y));
+      sum[a] = add2(sum[a], p);
+      float2 w = unpack2(mul2(p, vs[i]));
+      if (kMask) {  // (a hidden key's scale may be NaN)
+        if (8 * i + 2 * q >= seen[a]) w.x = 0.f;
+        if (8 * i + 2 * q + 1 >= seen[a]) w.y = 0.f;
+      }
+      pk[2 * i + a] = pack_halves<false>(w.x, w.y);
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    const float2 x = unpack2(sum[a]);
+    add[a] = x.x + x.y;
+  }
+}
+// The largest S * scale_k of the two rows over the 64 keys (whole rows: all four lanes get it).
+__device__ __forceinline__ void kv_row_max(uint32_t s_addr, const uint64_t* ks, const int* seen, int q, float* mx) {
+  uint32_t v[32];
+  tmem_ld_rows64(s_addr, v);
+  tmem_wait_ld();
+  mx[0] = mx[1] = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float2 k = unpack2(ks[i]);
+#pragma unroll
+    for (int a = 0; a < 2; ++a) {
+      if (8 * i + 2 * q < seen[a]) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * i + 2 * a]) * k.x);
+      if (8 * i + 2 * q + 1 < seen[a]) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * i + 2 * a + 1]) * k.y);
+    }
+  }
+#pragma unroll
+  for (int a = 0; a < 2; ++a) {
+    mx[a] = fmaxf(mx[a], __shfl_xor_sync(0xffffffffu, mx[a], 1));
+    mx[a] = fmaxf(mx[a], __shfl_xor_sync(0xffffffffu, mx[a], 2));
+  }
+}
+
 // Eight codes of a word plus the zero, as four pairs of fp16 in the order 04 15 26 37.
 __device__ __forceinline__ uint4 kv_codes_plus(uint32_t w, __half2 zero) {
   const __half2 big = __float2half2_rn(-1024.f), small = __float2half2_rn(-64.f), sixteenth = __float2half2_rn(0.0625f);
@@ -103,6 +247,13 @@ __device__ __forceinline__ uint4 kv_codes_plus(uint32_t w, __half2 zero) {
   }
   return make_uint4(r[0], r[1], r[2], r[3]);
 }
+// Eight results times a factor, as 16-bit elements.
+__device__ __forceinline__ uint4 kv_out8(const float* x, float f, int bf16) {
+  return bf16 ? make_uint4(pack_halves<true>(x[0] * f, x[1] * f), pack_halves<true>(x[2] * f, x[3] * f),
+                           pack_halves<true>(x[4] * f, x[5] * f), pack_halves<true>(x[6] * f, x[7] * f))
+              : make_uint4(pack_halves<false>(x[0] * f, x[1] * f), pack_halves<false>(x[2] * f, x[3] * f),
+                           pack_halves<false>(x[4] * f, x[5] * f), pack_halves<false>(x[6] * f, x[7] * f));
+}
 // Eight elements in natural order to that order.
 __device__ __forceinline__ uint4 kv_order8(const uint4& v) {
   return make_uint4(prmt(v.x, v.z, 0x5410u), prmt(v.x, v.z, 0x7632u), prmt(v.y, v.w, 0x5410u), prmt(v.y, v.w, 0x7632u));
@@ -116,13 +267,14 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ uint32_t sm_big, sm_tmem;
   __shared__ int sm_last;
+  __shared__ float2 sm_rows[kQt * kKvPM];  // (m, sum) of the rows
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = base, sK = sQ + kQt * kTile, sV = sK + kSt * kTile, sScale = sV + kSt * kTile;
   const uint32_t sTop = sScale + kKvPScales * kKvPN * 8;  // [ring][4] largest scale_v of the warps' keys
   const uint32_t bars = sTop + kKvPScales * 16;
   const uint32_t kfull_b = bars, kempty_b = bars + 16, vfull_b = bars + 32, vempty_b = bars + 48;
   // (per row tile t and half h of a key tile: [t][h], one phase per key tile each)
-  const uint32_t sfull_b = bars + 64, pfull_b = bars + 80, odone_b = bars + 112, drain_b = bars + 144;
+  const uint32_t sfull_b = bars + 64, pfull_b = bars + 96, odone_b = bars + 128, drain_b = bars + 160;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
@@ -131,8 +283,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       mbar_init(kempty_b + 8 * i, 1);
       mbar_init(vfull_b + 8 * i, 4);
       mbar_init(vempty_b + 8 * i, 1);
-      mbar_init(sfull_b + 8 * i, 1);
       for (int h = 0; h < 2; ++h) {
+        mbar_init(sfull_b + 16 * i + 8 * h, 1);
         mbar_init(pfull_b + 16 * i + 8 * h, 4);
         mbar_init(odone_b + 16 * i + 8 * h, 1);
       }
@@ -172,49 +324,81 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   }
   __syncthreads();
 
-  // ---------------------------------------------------------------- q: thread = row
-  const bool softmax = warp < 4 * kQt;
-  const int my_row = row0 + tid;  // of the softmax threads
-  const bool live = softmax && my_row < R;
-  const int tok = my_row / a.group;
-  float qf = a.scale * 1.4426950408889634f;  // factor of the scores (log2 units)
-  if (softmax) {
-    const uint16_t* src = a.q + static_cast<int64_t>(r0 + tok) * a.ldq + (kvh * a.group + my_row - tok * a.group) * kHd;
-    const uint32_t dst = sQ + (tid >> 7) * kTile;
-    const int r = tid & 127;
-    float up = 1.f;
-    if (a.bf16) {  // fp16 has less range: a power of two for the whole tile pair puts its largest near 2^14
-      float big = 0.f;
-      if (live) {
-        for (int c = 0; c < kHd / 8; ++c) {
-          float x[8];
-          unpack_halves<true>(a.vec ? ld_row8<true>(src + 8 * c) : ld_row8<false>(src + 8 * c), x);
+  // ---------------------------------------------------------------- the converters' first loads
+  const bool softmax = warp < 4 * kQt, converter = warp >= 8 && warp < 12;
+  const int key = tid & 127;  // of the tile
+  const int codes = a.C.page_size * (kHd / 2);
+  uint4 rk[kRaw], rv[kRaw];
+  uint32_t pk = 0, pv = 0;
+  int64_t off = -1;  // the key's page in the tile to load next
+  const auto find = [&](int kt) {
+    const int pos = (t0 + kt) * kKvPN + key;
+    off = kt < nt && pos < n ? kv_page_offset(a.C, a.B, seq, pos >> a.C.page_shift) : -1;
+  };
+  const auto load = [&](int kt) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
-        }
+    for (int i = 0; i < kRaw; ++i) rk[i] = rv[i] = make_uint4(0, 0, 0, 0);
+    pk = pv = 0;  // places past the end: scale and zero 0
+    if (off >= 0) {
+      const int in = ((t0 + kt) * kKvPN + key) & (a.C.page_size - 1);
+      const uint8_t* block = a.C.pages + off + kvh * a.C.head_bytes;
+#pragma unroll
+      for (int i = 0; i < kRaw; ++i) {
+        rk[i] = __ldg(reinterpret_cast<const uint4*>(block + in * (kHd / 2) + 16 * i));
+        rv[i] = __ldg(reinterpret_cast<const uint4*>(block + codes + in * (kHd / 2) + 16 * i));
       }
-      atomicMax(&sm_big, __float_as_uint(big));
-      named_barrier(2, kQt * 128);
-      const float top = __uint_as_float(sm_big);
-      const int e = max(-99, min(99, top > 0.f ? 14 - ((__float_as_int(top) >> 23) - 127) : 0));
-      up = pow2i(e);
-      qf *= pow2i(-e);
+      pk = __ldg(reinterpret_cast<const uint32_t*>(block + 2 * codes + 4 * in));
+      pv = __ldg(reinterpret_cast<const uint32_t*>(block + 2 * codes + 4 * (a.C.page_size + in)));
     }
-#pragma unroll 4
-    for (int c = 0; c < kHd / 8; ++c) {
-      uint4 v = make_uint4(0, 0, 0, 0);
-      if (live) {
-        v = a.vec ? ld_row8<true>(src + 8 * c) : ld_row8<false>(src + 8 * c);
-        if (a.bf16) {
-          float x[8];
-          unpack_halves<true>(v, x);
-          v = make_uint4(pack_halves<false>(x[0] * up, x[1] * up), pack_halves<false>(x[2] * up, x[3] * up),
-                         pack_halves<false>(x[4] * up, x[5] * up), pack_halves<false>(x[6] * up, x[7] * up));
-        }
+  };
+  if (converter) find(0);
+
+  // ---------------------------------------------------------------- q, by all threads
+  // the power of two that q is multiplied by (bf16: fp16 has less range; one for the whole tile pair, that
+  // puts its largest near 2^14)
+  const auto q_power = [&]() {
+    const float top = __uint_as_float(*const_cast<volatile uint32_t*>(&sm_big));
+    return a.bf16 ? max(-99, min(99, top > 0.f ? 14 - ((__float_as_int(top) >> 23) - 127) : 0)) : 0;
+  };
+  {
+    constexpr int kChunks = kHd / 8, kMine = kQt * kKvPM * kChunks / kKvPThreads;
+    uint4 v[kMine];
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int x = i * kKvPThreads + tid, row = row0 + x / kChunks, c = x % kChunks, tok = row / a.group;
+      const uint16_t* src = a.q + static_cast<int64_t>(r0 + tok) * a.ldq + (kvh * a.group + row - tok * a.group) * kHd + 8 * c;
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (row < R) v[i] = a.vec ? ld_row8<true>(src) : ld_row8<false>(src);
+    }
+    if (converter) load(0);
+    if (a.bf16) {
+      float big = 0.f;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        float x[8];
+        unpack_halves<true>(v[i], x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
       }
-      sts128(dst + (c >> 3) * kBlock + sw128_off(r, c & 7), kv_order8(v));
+      big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+      if (lane == 0) atomicMax(&sm_big, __float_as_uint(big));
+      __syncthreads();
+      const float up = pow2i(q_power());
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        float x[8];
+        unpack_halves<true>(v[i], x);
+        v[i] = make_uint4(pack_halves<false>(x[0] * up, x[1] * up), pack_halves<false>(x[2] * up, x[3] * up),
+                          pack_halves<false>(x[4] * up, x[5] * up), pack_halves<false>(x[6] * up, x[7] * up));
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kMine; ++i) {
+      const int x = i * kKvPThreads + tid, row = x / kChunks, c = x % kChunks;
+      sts128(sQ + (row >> 7) * kTile + (c >> 3) * kBlock + sw128_off(row & 127, c & 7), kv_order8(v[i]));
     }
     fence_proxy_async_smem();
+    if (converter) find(1);
   }
   tc_fence_before();
   __syncthreads();
@@ -223,102 +407,144 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   const uint32_t tS = tmem, tO = tmem + kQt * kKvPN;  // row tile t: S at + 128 t, O at + kHdp t
   bool ok = true;
 
-  // (every warpgroup trades before its role: two at 192, 88 and 40, or with one row tile 192, 24, 168, 40
+  // (every warpgroup trades before its role: two at 176, 88 and 72, or with one row tile 176, 24, 168, 72
   // -- at most 512 = 4 * 128 together)
   if (softmax) {
     // ---------------------------------------------------------------- softmax
-    regs_up<192>();
-    float m = -1e30f, T = 0.f;
-    const int t = tid >> 7;
+    regs_up<176>();
+    const int t = tid >> 7, g = lane >> 2, q = lane & 3;
     const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
     const uint32_t s_addr = tS + t * kKvPN + lanes, o_addr = tO + t * kHdp + lanes;
-    const int lim = live ? max(0, min(n, pos0 + tok + 1)) : 0;   // keys below it are seen by this row
-    // (rows that do not exist see nothing; a warp's first live row sees the fewest)
+    constexpr uint32_t kHalfLanes = 16u << 16;
+    // rows in the fragment shapes: r = 2b + a is row 16b + 8a + g of the warp's 32
     const int first_row = row0 + (tid & ~31);
-    const int plain = first_row + 31 < R ? max(0, min(n, pos0 + first_row / a.group + 1)) : 0;  // tiles below need no mask
+    float m[4], T[4];
+    int lim[4];         // keys below it are seen by the row
+    bool fresh[4];      // no key seen yet, but one will be: m means nothing
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      m[r] = T[r] = 0.f;
+      const int row = first_row + 16 * (r >> 1) + 8 * (r & 1) + g;
+      lim[r] = row < R ? max(0, min(n, pos0 + row / a.group + 1)) : 0;
+      fresh[r] = lim[r] > 0;
+    }
+    // tiles below need no mask (rows that do not exist see nothing; the first row sees the fewest)
+    const int plain = first_row + 31 < R ? max(0, min(n, pos0 + first_row / a.group + 1)) : 0;
     for (int kt = 0; kt < nt; ++kt) {
       const int kb = (t0 + kt) * kKvPN, ring = kt % kKvPScales;
-      if (!mbar_wait_bounded(sfull_b + 8 * t, kt & 1)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
       const uint32_t sc = sScale + ring * kKvPN * 8;
-      const uint4 tops = lds128(sTop + ring * 16);
-      // log2 of the largest scale_v of the tile, rounded up (NaN scales are left out; all zero: 2^-30)
-      const uint32_t top = max(max(tops.x, tops.y), max(tops.z, tops.w));
-      const float ev = static_cast<float>(max(-30, static_cast<int>(top >> 23) - 126));
+      float ev = 0.f;
       const bool whole = kb + kKvPN <= plain;
-      // in halves of 64 keys: the weights of the first are multiplied while the second is evaluated
+      // In halves of 64 keys (the weights of the first are multiplied while the second is evaluated), 16
+      // rows at a time: after each the rows' registers change places, so that the code, which has to
+      // stay in the instruction cache beside the other roles', is there once.
+      uint64_t ks[8], vs[8];  // the scales of the lane's 16 keys of the half
 #pragma unroll 1
-      for (int h = 0; h < 2 && ok; ++h) {
-        uint32_t pk[32];
-        float add;
-#pragma unroll 1
-        for (int pass = 0; pass < 2; ++pass) {
-          float mx = -INFINITY;
-          add = 0.f;
-#pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            uint32_t v[32];
-            tmem_ld32(s_addr + 64 * h + 32 * c, v);
-#pragma unroll
-            for (int e = 0; e < 32; e += 2) {
-              const int j = 32 * c + e;  // of the half
-              const uint4 f = lds128(sc + (64 * h + j) * 8);  // (scale_k, scale_v) of two keys
-              float x0 = __uint_as_float(v[e]) * (__uint_as_float(f.x) * qf), x1 = __uint_as_float(v[e + 1]) * (__uint_as_float(f.z) * qf);
-              if (!whole) {
-                if (kb + 64 * h + j >= lim) x0 = -INFINITY;
-                if (kb + 64 * h + j + 1 >= lim) x1 = -INFINITY;
-              }
-              mx = fmaxf(mx, fmaxf(x0, x1));
-              const float p0 = ex2(x0 - m), p1 = ex2(x1 - m);
-              add += p0 + p1;
-              float w0 = p0 * __uint_as_float(f.y), w1 = p1 * __uint_as_float(f.w);
-              if (!whole) {  // (a hidden key's scale may be NaN)
-                if (x0 == -INFINITY) w0 = 0.f;
-                if (x1 == -INFINITY) w1 = 0.f;
-              }
-              pk[j >> 1] = pack_halves<false>(w0, w1);
-            }
+      for (int hb = 0; hb < 4 && ok; ++hb) {
+        const int h = hb >> 1, b = hb & 1;
+        if (b == 0) {
+          if (!mbar_wait_bounded(sfull_b + 16 * t + 8 * h, kt & 1)) {
+            ok = false;
+            break;
           }
-          if (pass || !__any_sync(0xffffffffu, mx + ev > m + 12.f)) break;
-          const float mn = fmaxf(m, mx + ev), corr = ex2(m - mn);
-          m = mn;
-          T *= corr;
-          if (kt + h > 0) {  // O holds the halves before
-            if (!mbar_wait_bounded(odone_b + 16 * t + 8 * (1 - h), (kt + h - 1) & 1)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-#pragma unroll 1
-            for (int c = 0; c < kHd / 32; ++c) {
-              uint32_t v[32];
-              tmem_ld32(o_addr + 32 * c, v);
+          tc_fence_after();
+          // log2 of the largest scale_v of the tile, rounded up (NaN scales are left out; all zero: 2^-30)
+          const uint4 tops = lds128(sTop + ring * 16);
+          const uint32_t top = max(max(tops.x, tops.y), max(tops.z, tops.w));
+          ev = static_cast<float>(max(-30, static_cast<int>(top >> 23) - 126));
 #pragma unroll
-              for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * corr);
-              tmem_st32(o_addr + 32 * c, v);
-            }
+          for (int i = 0; i < 8; i += 2) {
+            const uint4 k4 = lds128(sc + 256 * h + 64 * q + 8 * i), v4 = lds128(sc + 512 + 256 * h + 64 * q + 8 * i);
+            ks[i] = pack2(__uint_as_float(k4.x), __uint_as_float(k4.y));
+            ks[i + 1] = pack2(__uint_as_float(k4.z), __uint_as_float(k4.w));
+            vs[i] = pack2(__uint_as_float(v4.x), __uint_as_float(v4.y));
+            vs[i + 1] = pack2(__uint_as_float(v4.z), __uint_as_float(v4.w));
           }
         }
-        T += add;
-        tmem_st32(s_addr + 32 * h, pk);  // over scores that have been read
-        tmem_wait_st();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(pfull_b + 16 * t + 8 * h);
+        uint32_t pk[16];
+        float add[2];
+        const uint32_t addr = s_addr + b * kHalfLanes + 64 * h;
+        const int seen[2] = {lim[0] - kb - 64 * h, lim[1] - kb - 64 * h};
+        // A row moves m when its weights' sum (the lane's share) says that one times scale_v may pass 2^12,
+        // or when it has seen no key yet.
+        bool moved = __any_sync(0xffffffffu, (fresh[0] && seen[0] > 0) || (fresh[1] && seen[1] > 0));
+#pragma unroll 1
+        for (;;) {
+          if (moved) {
+            float mx[2], corr[2];
+            kv_row_max(addr, ks, seen, q, mx);
+#pragma unroll
+            for (int r = 0; r < 2; ++r) {
+              const bool first = fresh[r] && mx[r] > -INFINITY;
+              const float up = first || mx[r] + ev > m[r] ? mx[r] + ev - m[r] : 0.f;
+              corr[r] = first ? 1.f : ex2(-up);
+              m[r] += up;
+              T[r] *= corr[r];
+              fresh[r] = fresh[r] && !first;
+            }
+            if (kt + h > 0) {  // O holds the halves before
+              if (!mbar_wait_bounded(odone_b + 16 * t + 8 * (1 - h), (kt + h - 1) & 1)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+#pragma unroll 1
+              for (int c = 0; c < kHd / 32; ++c) {
+                uint32_t v[16];
+                tmem_ld_rows32(o_addr + b * kHalfLanes + 32 * c, v);
+                tmem_wait_ld();
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * corr[(e >> 1) & 1]);
+                tmem_st_rows32(o_addr + b * kHalfLanes + 32 * c, v);
+              }
+            }
+          }
+          if (whole) kv_weights<false>(addr, ks, vs, m, seen, q, pk, add);
+          else kv_weights<true>(addr, ks, vs, m, seen, q, pk, add);
+          if (moved || !__any_sync(0xffffffffu, fmaxf(add[0], add[1]) > ex2(12.f - ev))) break;
+          moved = true;
+        }
+        T[0] += add[0];
+        T[1] += add[1];
+        tmem_st_pairs32(addr, pk);  // over the half's scores, which have been read
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          swap_values(m[r], m[r + 2]);
+          swap_values(T[r], T[r + 2]);
+          swap_values(lim[r], lim[r + 2]);
+          swap_values(fresh[r], fresh[r + 2]);
+        }
+        if (b == 1) {
+          tmem_wait_st();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pfull_b + 16 * t + 8 * h);
+        }
       }
       if (!ok) break;
     }
     // -------------------------------------------------------------- results
     if (ok && nt > 0) ok = mbar_wait_bounded(odone_b + 16 * t + 8, (nt - 1) & 1);
     tc_fence_after();
+    // from the fragments' rows to lane = row
+    float2* rows_mt = sm_rows + (tid & ~31);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      T[r] += __shfl_xor_sync(0xffffffffu, T[r], 1);
+      T[r] += __shfl_xor_sync(0xffffffffu, T[r], 2);
+      if (q == 0) rows_mt[16 * (r >> 1) + 8 * (r & 1) + g] = make_float2(lim[r] > 0 && !fresh[r] ? m[r] : -1e30f, T[r]);
+    }
+    __syncwarp();
+    const float row_m = rows_mt[lane].x, row_T = rows_mt[lane].y;
+    const int row = row0 + tid;
+    const bool live = row < R;
     const bool single = splits == 1;
     const int64_t item = (static_cast<int64_t>(seq) * gridDim.y + kvh) * (gridDim.x / sp.splits) + pair_from_end;
-    constexpr int kRec = kHd + 4;
-    float* rec = single ? nullptr : sp.part + ((item * sp.splits + split) * (kQt * kKvPM) + tid) * kRec;
-    const int row = my_row;  // of the sequence and kv head
+    // a record: the weighted sums [head_dim / 4][rows] x 4, then (m, sum) [rows]
+    constexpr int kRows = kQt * kKvPM;
+    float* rec = sp.part + (item * sp.splits + split) * (kRows * (kHd + 4));
+    const uint32_t out_s = sQ + t * kTile;  // the row tile's output, laid out like q, which is no longer needed
+    const float inv = row_T == 0.f ? 0.f : 1.0f / row_T;  // a row that sees nothing: 0 (a NaN sum stays NaN)
 #pragma unroll 1
     for (int c = 0; c < kHd / 32; ++c) {
       uint32_t v[32];
@@ -328,86 +554,86 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
 #pragma unroll
         for (int e = 0; e < 32; ++e) v[e] = 0;
       }
-      if (live && ok) {
 #pragma unroll
-        for (int e = 0; e < 32; e += 8) {  // columns 0 4 1 5 2 6 3 7 of eight dimensions
-          const float x[8] = {__uint_as_float(v[e]),     __uint_as_float(v[e + 2]), __uint_as_float(v[e + 4]), __uint_as_float(v[e + 6]),
-                              __uint_as_float(v[e + 1]), __uint_as_float(v[e + 3]), __uint_as_float(v[e + 5]), __uint_as_float(v[e + 7])};
-          const float4 lo = make_float4(x[0], x[1], x[2], x[3]), hi = make_float4(x[4], x[5], x[6], x[7]);
-          const int d = 32 * c + e;
-          if (single) {
-            kv_finish_row(a, r0, kvh, row, d, lo, m, T);
-            kv_finish_row(a, r0, kvh, row, d + 4, hi, m, T);
-          } else {
-            *reinterpret_cast<float4*>(rec + d) = lo;
-            *reinterpret_cast<float4*>(rec + d + 4) = hi;
-          }
+      for (int e = 0; e < 32; e += 8) {  // columns 0 4 1 5 2 6 3 7 of eight dimensions
+        const float x[8] = {__uint_as_float(v[e]),     __uint_as_float(v[e + 2]), __uint_as_float(v[e + 4]), __uint_as_float(v[e + 6]),
+                            __uint_as_float(v[e + 1]), __uint_as_float(v[e + 3]), __uint_as_float(v[e + 5]), __uint_as_float(v[e + 7])};
+        if (single) {
+          sts128(out_s + ((32 * c + e) >> 6) * kBlock + sw128_off(tid & 127, ((32 * c + e) >> 3) & 7), kv_out8(x, inv, a.bf16));
+        } else if (live) {
+          *reinterpret_cast<float4*>(rec + ((32 * c + e) / 4 * kRows + tid) * 4) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(rec + ((32 * c + e) / 4 * kRows + kRows + tid) * 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
       }
     }
-    if (!single) {
-      if (live) *reinterpret_cast<float2*>(rec + kHd) = make_float2(m, T);
-      named_barrier(2, kQt * 128);
+    const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
+    uint16_t* dst = a.out + static_cast<int64_t>(r0 + tok) * a.ldo + static_cast<int64_t>(head) * kHd;
+    if (single) {
+      if (live && ok && a.lse)
+        a.lse[static_cast<int64_t>(r0 + tok) * a.heads + head] = row_T == 0.f ? -INFINITY : row_m * 0.6931471805599453f + logf(row_T);
+      __syncwarp();
+      constexpr int kChunks = kHd / 8;
+#pragma unroll 4
+      for (int i = 0; i < kChunks; ++i) {  // whole rows at a time
+        const int x = i * 32 + lane, r = x / kChunks, c = x % kChunks;
+        const uint64_t to = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), r);
+        const uint4 w = lds128(out_s + (c >> 3) * kBlock + sw128_off((tid & 96) + r, c & 7));
+        uint16_t* o = reinterpret_cast<uint16_t*>(to) + 8 * c;
+        if (row0 + (tid & ~31) + r < R && ok) {
+          if (a.vec) st_row8<true>(o, w);
+          else st_row8<false>(o, w);
+        }
+      }
+    } else {
+      if (live) *reinterpret_cast<float2*>(rec + kRows * kHd + 2 * tid) = make_float2(row_m, row_T);
+      named_barrier(2, kRows);
       if (tid == 0) {
         const bool last = atom_add_acq_rel_gpu(sp.count + item, 1) == splits - 1;
         if (last) sp.count[item] = 0;
         sm_last = last;
       }
-      named_barrier(2, kQt * 128);
-      if (sm_last && ok) {  // merge, in order: thread = (row, four dimensions)
-        const float* part = sp.part + item * sp.splits * (kQt * kKvPM) * kRec;
-        const int rows = row_end - row0;
-        for (int i = tid; i < rows * (kHd / 4); i += kQt * 128) {
-          const int r = i / (kHd / 4), d = 4 * (i - r * (kHd / 4));
-          float M = -1e30f, S = 0.f;
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-          for (int s = 0; s < splits; ++s) M = fmaxf(M, __ldcg(part + (static_cast<int64_t>(s) * kQt * kKvPM + r) * kRec + kHd));
-          for (int s = 0; s < splits; ++s) {
-            const float* src = part + (static_cast<int64_t>(s) * kQt * kKvPM + r) * kRec;
-            const float2 w = __ldcg(reinterpret_cast<const float2*>(src + kHd));
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(src + d));
-            const float f = ex2(w.x - M);
-            S += f * w.y;
-            o.x += f * v.x;
-            o.y += f * v.y;
-            o.z += f * v.z;
-            o.w += f * v.w;
-          }
-          kv_finish_row(a, r0, kvh, row0 + r, d, o, M, S);
+      named_barrier(2, kRows);
+      if (sm_last && live && ok) {  // merge, in order: thread = row
+        const float* part = sp.part + item * sp.splits * (kRows * (kHd + 4));
+        float M = -1e30f, S = 0.f;
+        for (int i = 0; i < splits; ++i) M = fmaxf(M, __ldcg(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tid));
+        for (int i = 0; i < splits; ++i) {
+          const float2 w = __ldcg(reinterpret_cast<const float2*>(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tid));
+          S += ex2(w.x - M) * w.y;
         }
+        const float scale = S == 0.f ? 0.f : 1.0f / S;
+#pragma unroll 1
+        for (int d = 0; d < kHd; d += 16) {
+          float o[16] = {};
+#pragma unroll 2
+          for (int i = 0; i < splits; ++i) {
+            const float* src = part + i * (kRows * (kHd + 4));
+            const float f = ex2(__ldcg(src + kRows * kHd + 2 * tid) - M);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(src + ((d / 4 + e) * kRows + tid) * 4));
+              o[4 * e] += f * v.x;
+              o[4 * e + 1] += f * v.y;
+              o[4 * e + 2] += f * v.z;
+              o[4 * e + 3] += f * v.w;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 16; e += 8) {
+            const uint4 w = kv_out8(o + e, scale, a.bf16);
+            if (a.vec) st_row8<true>(dst + d + e, w);
+            else st_row8<false>(dst + d + e, w);
+          }
+        }
+        if (a.lse) a.lse[static_cast<int64_t>(r0 + tok) * a.heads + head] = S == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(S);
       }
     }
-    } else if (warp < 8) {
+  } else if (warp < 8) {
     regs_down<24>();
   } else if (warp < 12) {
     // ---------------------------------------------------------------- keys: thread = key of the tile
     if constexpr (kQt == 2) regs_down<88>();
     else regs_up<168>();
-    const int key = tid - 8 * 32, w4 = warp - 8;
-    const int codes = a.C.page_size * (kHd / 2);
-    uint4 rk[kRaw], rv[kRaw];
-    uint32_t pk = 0, pv = 0;
-    int64_t off = -1;  // the key's page in the tile to load next
-    const auto find = [&](int kt) {
-      const int pos = (t0 + kt) * kKvPN + key;
-      off = kt < nt && pos < n ? kv_page_offset(a.C, a.B, seq, pos >> a.C.page_shift) : -1;
-    };
-    const auto load = [&](int kt) {
-#pragma unroll
-      for (int i = 0; i < kRaw; ++i) rk[i] = rv[i] = make_uint4(0, 0, 0, 0);
-      pk = pv = 0;  // places past the end: scale and zero 0
-      if (off >= 0) {
-        const int in = ((t0 + kt) * kKvPN + key) & (a.C.page_size - 1);
-        const uint8_t* block = a.C.pages + off + kvh * a.C.head_bytes;
-#pragma unroll
-        for (int i = 0; i < kRaw; ++i) {
-          rk[i] = __ldg(reinterpret_cast<const uint4*>(block + in * (kHd / 2) + 16 * i));
-          rv[i] = __ldg(reinterpret_cast<const uint4*>(block + codes + in * (kHd / 2) + 16 * i));
-        }
-        pk = __ldg(reinterpret_cast<const uint32_t*>(block + 2 * codes + 4 * in));
-        pv = __ldg(reinterpret_cast<const uint32_t*>(block + 2 * codes + 4 * (a.C.page_size + in)));
-      }
-    };
     const auto convert = [&](const uint4 (&raw)[kRaw], uint32_t pair, uint32_t tile) {
       const __half2 zero = __half2half2(__ushort_as_half(static_cast<unsigned short>(pair >> 16)));
 #pragma unroll
@@ -420,9 +646,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         }
       }
     };
-    find(0);
-    load(0);
-    find(1);
+    const float qf = a.scale * 1.4426950408889634f * pow2i(-q_power());  // factor of the scores (log2 units)
     for (int kt = 0; kt < nt; ++kt) {
       const int st = kt % kSt, ring = kt % kKvPScales;
       const uint32_t par = ((kt / kSt) - 1) & 1;
@@ -431,38 +655,48 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         break;
       }
       const float2 kf = unpack_half2(pk), vf = unpack_half2(pv);
-      sts64(sScale + (ring * kKvPN + key) * 8, __float_as_uint(kf.x), __float_as_uint(vf.x));
+      // (in the order of the softmax's lanes: by half, then (key % 8) / 2, key / 8, key % 2)
+      const uint32_t at = sScale + ring * kKvPN * 8 + 4 * ((key & 64) + 16 * ((key >> 1) & 3) + 2 * ((key >> 3) & 7) + (key & 1));
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(kf.x * qf) : "memory");
+      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 512), "f"(vf.x) : "memory");
       const float size = fminf(fmaxf(fabsf(vf.x), 0.f), 65504.f);  // (a NaN has no size)
       const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size));
-      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * w4), "r"(top) : "memory");
-      convert(rk, pk, sK + st * kTile);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(kfull_b + 8 * st);
-      if (kt >= kSt && !mbar_wait_bounded(vempty_b + 8 * st, par)) {
-        ok = false;
-        break;
+      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - 8)), "r"(top) : "memory");
+#pragma unroll 1
+      for (int v = 0; v < 2; ++v) {  // K', then V' (one copy of the code)
+        if (v && kt >= kSt && !mbar_wait_bounded(vempty_b + 8 * st, par)) {
+          ok = false;
+          break;
+        }
+        convert(rk, pk, (v ? sV : sK) + st * kTile);
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive((v ? vfull_b : kfull_b) + 8 * st);
+#pragma unroll
+        for (int i = 0; i < kRaw; ++i) rk[i] = rv[i];
+        pk = pv;
       }
-      convert(rv, pv, sV + st * kTile);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(vfull_b + 8 * st);
+      if (!ok) break;
       load(kt + 1);
       find(kt + 2);
     }
   } else {
     // ---------------------------------------------------------------- MMA issuer
-    regs_down<40>();
-    if (warp == 12 && lane == 0) {
-      const auto scores = [&](int t, int kt) {
+    regs_down<72>();
+    if (warp == 12) {  // (all lanes wait and count, one issues)
+      const uint32_t leader = elect_leader();
+      // the scores of row tile t for half h of key tile kt
+      const auto scores = [&](int t, int kt, int h) {
         const int st = kt % kSt;
-#pragma unroll 2
+        const uint64_t qd = kv_desc_k(sQ + t * kTile), kd = kv_desc_k(sK + st * kTile + 8192 * h);  // (in units of 16 bytes)
+#pragma unroll
         for (int k = 0; k < kHd / 16; ++k) {
-          const uint32_t o = (k >> 2) * kBlock + (k & 3) * 32;
-          umma_f16(tS + t * kKvPN, kv_desc_k(sQ + t * kTile + o), kv_desc_k(sK + st * kTile + o), kv_idesc(kKvPN, false), k > 0);
+          constexpr int kB = kBlock / 16;
+          umma_f16_by(leader, tS + t * kKvPN + 64 * h, qd + ((k >> 2) * kB + (k & 3) * 2), kd + ((k >> 2) * kB + (k & 3) * 2),
+                   kv_idesc(kKvPN / 2, false), k > 0);
         }
-        umma_commit(sfull_b + 8 * t);
-        if (t == kQt - 1) umma_commit(kempty_b + 8 * st);
+        umma_commit_by(leader, sfull_b + 16 * t + 8 * h);
+        if (t == kQt - 1 && h == 1) umma_commit_by(leader, kempty_b + 8 * st);
       };
       const auto wait = [&](uint32_t bar, uint32_t par) {
         if (ok) ok = mbar_wait_bounded(bar, par);
@@ -470,25 +704,28 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         return ok;
       };
       if (nt > 0 && wait(kfull_b, 0))
-        for (int t = 0; t < kQt; ++t) scores(t, 0);
+        for (int i = 0; i < 2 * kQt; ++i) scores(i % kQt, 0, i / kQt);
       for (int kt = 0; kt < nt && ok; ++kt) {
         const int st = kt % kSt;
         if (!wait(vfull_b + 8 * st, (kt / kSt) & 1)) break;
-        for (int t = 0; t < kQt && ok; ++t) {
-          for (int h = 0; h < 2 && wait(pfull_b + 16 * t + 8 * h, kt & 1); ++h) {
-#pragma unroll 1
-            for (int k = 0; k < kKvPN / 32; ++k)
-              umma_f16_ts(tO + t * kHdp, tS + t * kKvPN + 32 * h + 8 * k, kv_desc_mn(sV + st * kTile + 8192 * h + 2048 * k),
-                          kv_idesc(kHdp, true), kt > 0 || h > 0 || k > 0);
-            umma_commit(odone_b + 16 * t + 8 * h);
+        if (kt + 1 < nt && kSt > 1 && !wait(kfull_b + 8 * ((kt + 1) % kSt), ((kt + 1) / kSt) & 1)) break;
+        for (int i = 0; i < 2 * kQt; ++i) {
+          const int t = i % kQt, h = i / kQt;
+          if (!wait(pfull_b + 16 * t + 8 * h, kt & 1)) break;
+          const uint64_t vd = kv_desc_mn(sV + st * kTile + 8192 * h);
+#pragma unroll
+          for (int k = 0; k < kKvPN / 32; ++k)
+            umma_f16_ts_by(leader, tO + t * kHdp, tS + t * kKvPN + 64 * h + 8 * k, vd + 128 * k, kv_idesc(kHdp, true), kt + h + k > 0);
+          umma_commit_by(leader, odone_b + 16 * t + 8 * h);
+          if (t == kQt - 1 && h == 1) umma_commit_by(leader, vempty_b + 8 * st);
+          if (kt + 1 < nt) {
+            if (kSt == 1 && i == 0 && !wait(kfull_b, (kt + 1) & 1)) break;
+            scores(t, kt + 1, h);
           }
-          if (!ok) break;
-          if (t == kQt - 1) umma_commit(vempty_b + 8 * st);
-          if (kt + 1 < nt && wait(kfull_b + 8 * ((kt + 1) % kSt), ((kt + 1) / kSt) & 1)) scores(t, kt + 1);
         }
       }
       // no tensor-core operation of this CTA is in flight past this point
-      umma_commit(drain_b);
+      umma_commit_by(leader, drain_b);
       mbar_wait_bounded(drain_b, 0);
     }
   }
