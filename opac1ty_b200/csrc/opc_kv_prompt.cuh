@@ -19,24 +19,28 @@ namespace opc {
 // 4 * 128 * 128 * head_dim operations per tile pair, against 128 * 128 exponentials, which the
 // special-function units take as long for as the tensor cores for the products at head_dim 128: two
 // row tiles alternate, one in the tensor cores while the other is in the softmax.  Roles:
-//   warps 0..3, 4..7  softmax of row tile 0 and 1, 32 rows a warp in the 16-row fragment shapes: a lane has a
-//                     quarter of the columns of four rows, so it holds its keys' scales in registers (with
-//                     thread = row every thread would read all of them from shared memory).  The reference m of a row
-//                     moves only when a score passes m + 12 (with the largest scale_v of the tile):
-//                     the tile is first evaluated with the old m, and again, with O rescaled, where a
-//                     row of the warp passed it -- always in the first tile, hardly ever later.
-//   warps 8..11       thread = key: reads its codes (one tile ahead, in registers), writes K' and V'
-//                     rows in the 128-byte-swizzled layout -- the same bytes are K-major for K' (rows
-//                     are the N dimension) and MN-major for V' (rows are the K dimension)
-//   warp 12           one lane issues the MMAs and commits them to the roles' barriers (13..15 idle)
-// The warpgroups trade registers: 128 a thread at the launch, then 176 for the softmax (which holds a
-// tile's weights until it knows that m stands), 88 and 72 for the others.
+//   warps 0..15   softmax: four warps for rows 0..15 of each 32 TMEM lanes of row tile 0, four for rows
+//                 16..31, then the same for row tile 1.  In the 16-row fragment shapes a lane has a
+//                 quarter of the columns of two rows, so that it reads a quarter of the keys' scales
+//                 from shared memory (with thread = row every thread would read all of them), and four
+//                 warps per SM sub-partition hide each other's latencies (two took twice as long).
+//                 The reference m of a row moves only when the sum of a half's weights says that one
+//                 times the tile's largest scale_v may pass 2^12: then the row's maximum is looked for,
+//                 O rescaled and the half evaluated again -- always in the first tile, hardly ever later.
+//   warps 16..19  thread = key: reads its codes (one tile ahead, in registers), writes K' and V' rows in
+//                 the 128-byte-swizzled layout -- the same bytes are K-major for K' (rows are the N
+//                 dimension) and MN-major for V' (rows are the K dimension)
+//   warp 20       issues the MMAs and commits them to the roles' barriers (21..23 idle)
+// The warpgroups trade registers: 80 a thread at the launch, then 88 for the softmax and the
+// converters, 40 for the MMA warp; with one row tile (head_dim 192 and 256) two warpgroups less are
+// in the softmax and the converters take more.
 // The codes of a word come out in the order 0 4 1 5 2 6 3 7 (one mask per pair); q is staged in that
 // order too, and the output columns are put back in order by the epilogue.
 // Few CTAs are split over the keys: the partial results go to the workspace as records of the step
 // kernel's form, merged by the last CTA of a row tile pair.
 constexpr int kKvPM = 128, kKvPN = 128;            // rows per tile, keys per tile
-constexpr int kKvPThreads = 16 * 32;
+constexpr int kKvPThreads = 24 * 32;
+constexpr int kKvPConv = 16, kKvPMma = 20;         // first converter warp, the MMA warp
 constexpr int kKvPScales = 4;                      // ring of the tiles' scales
 __host__ __device__ constexpr int kv_p_hdp(int hd) { return (hd + 63) / 64 * 64; }       // whole swizzle blocks
 __host__ __device__ constexpr int kv_p_qt(int hd) { return hd <= 128 ? 2 : 1; }          // row tiles per CTA
@@ -138,16 +142,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 }
 // The 16-row fragment shapes: of 8 fp32 columns lane (g, q) = (lane / 4, lane % 4) holds (row g, columns
 // 2q, 2q + 1) and (row g + 8, the same); of 4 32-bit columns (16x128b) column q of rows g and g + 8.
-__device__ __forceinline__ void tmem_ld_rows64(uint32_t taddr, uint32_t* v) {  // 64 columns
-  asm volatile(
-      "tcgen05.ld.sync.aligned.16x256b.x8.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17,"
-      "%18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]), "=r"(v[7]), "=r"(v[8]),
-      "=r"(v[9]), "=r"(v[10]), "=r"(v[11]), "=r"(v[12]), "=r"(v[13]), "=r"(v[14]), "=r"(v[15]), "=r"(v[16]), "=r"(v[17]),
-      "=r"(v[18]), "=r"(v[19]), "=r"(v[20]), "=r"(v[21]), "=r"(v[22]), "=r"(v[23]), "=r"(v[24]), "=r"(v[25]), "=r"(v[26]),
-      "=r"(v[27]), "=r"(v[28]), "=r"(v[29]), "=r"(v[30]), "=r"(v[31])
-      : "r"(taddr));
-}
 __device__ __forceinline__ void tmem_ld_rows32(uint32_t taddr, uint32_t* v) {  // 32 columns
   asm volatile(
       "tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
@@ -175,33 +169,41 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 
 // The weights of 16 rows (lane (g, q): rows g and g + 8) for 64 keys: pk the fp16 pairs
 // exp2(S * scale_k - m) * scale_v; the lane's share of the rows' sums of the weights without scale_v.
-// ks, vs: the scales of the lane's 16 keys (8i + 2q, 8i + 2q + 1).  kMask: a row sees its first `seen`
-// keys only.
+// sk, sv: shared-memory addresses of the scales of the lane's 16 keys (8i + 2q, 8i + 2q + 1).  kMask: a
+// row sees its first `seen` keys only.
 template <bool kMask>
-__device__ __forceinline__ void kv_weights(uint32_t s_addr, const uint64_t* ks, const uint64_t* vs, const float* m, const int* seen,
-                                           int q, uint32_t* pk, float* add) {
-  uint32_t v[32];
-  tmem_ld_rows64(s_addr, v);
-  tmem_wait_ld();
+__device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_t sv, const float* m, const int* seen, int q, uint32_t* pk,
+                                           float* add) {
   const uint64_t minus[2] = {pack2(-m[0], -m[0]), pack2(-m[1], -m[1])};
   uint64_t sum[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
+  for (int c = 0; c < 2; ++c) {
+    uint32_t v[16];
+    tmem_ld_rows32(s_addr + 32 * c, v);
+    const uint4 k4[2] = {lds128(sk + 32 * c), lds128(sk + 32 * c + 16)}, v4[2] = {lds128(sv + 32 * c), lds128(sv + 32 * c + 16)};
+    tmem_wait_ld();
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      float2 y = unpack2(fma2(pack2(__uint_as_float(v[4 * i + 2 * a]), __uint_as_float(v[4 * i + 2 * a + 1])), ks[i], minus[a]));
-      if (kMask) {
-        if (8 * i + 2 * q >= seen[a]) y.x = -INFINITY;
-        if (8 * i + 2 * q + 1 >= seen[a]) y.y = -INFINITY;
+    for (int j = 0; j < 4; ++j) {
+      const int col = 32 * c + 8 * j + 2 * q;
+      const uint4 &kk = k4[j >> 1], &vv = v4[j >> 1];
+      const uint64_t ks = pack2(__uint_as_float((j & 1) ? kk.z : kk.x), __uint_as_float((j & 1) ? kk.w : kk.y));
+      const uint64_t vs = pack2(__uint_as_float((j & 1) ? vv.z : vv.x), __uint_as_float((j & 1) ? vv.w : vv.y));
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        float2 y = unpack2(fma2(pack2(__uint_as_float(v[4 * j + 2 * a]), __uint_as_float(v[4 * j + 2 * a + 1])), ks, minus[a]));
+        if (kMask) {
+          if (col >= seen[a]) y.x = -INFINITY;
+          if (col + 1 >= seen[a]) y.y = -INFINITY;
+        }
+        const uint64_t p = pack2(ex2(y.x), ex2(y.y));
+        sum[a] = add2(sum[a], p);
+        float2 w = unpack2(mul2(p, vs));
+        if (kMask) {  // (a hidden key's scale may be NaN)
+          if (col >= seen[a]) w.x = 0.f;
+          if (col + 1 >= seen[a]) w.y = 0.f;
+        }
+        pk[8 * c + 2 * j + a] = pack_halves<false>(w.x, w.y);
       }
-      const uint64_t p = pack2(ex2(y.x), ex2(y.y));
-      sum[a] = add2(sum[a], p);
-      float2 w = unpack2(mul2(p, vs[i]));
-      if (kMask) {  // (a hidden key's scale may be NaN)
-        if (8 * i + 2 * q >= seen[a]) w.x = 0.f;
-        if (8 * i + 2 * q + 1 >= seen[a]) w.y = 0.f;
-      }
-      pk[2 * i + a] = pack_halves<false>(w.x, w.y);
     }
   }
 #pragma unroll
@@ -211,18 +213,22 @@ __device__ __forceinline__ void kv_weights(uint32_t s_addr, const uint64_t* ks, 
   }
 }
 // The largest S * scale_k of the two rows over the 64 keys (whole rows: all four lanes get it).
-__device__ __forceinline__ void kv_row_max(uint32_t s_addr, const uint64_t* ks, const int* seen, int q, float* mx) {
-  uint32_t v[32];
-  tmem_ld_rows64(s_addr, v);
-  tmem_wait_ld();
+__device__ __forceinline__ void kv_row_max(uint32_t s_addr, uint32_t sk, const int* seen, int q, float* mx) {
   mx[0] = mx[1] = -INFINITY;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 k = unpack2(ks[i]);
+  for (int c = 0; c < 2; ++c) {
+    uint32_t v[16];
+    tmem_ld_rows32(s_addr + 32 * c, v);
+    tmem_wait_ld();
 #pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      if (8 * i + 2 * q < seen[a]) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * i + 2 * a]) * k.x);
-      if (8 * i + 2 * q + 1 < seen[a]) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * i + 2 * a + 1]) * k.y);
+    for (int j = 0; j < 4; ++j) {
+      const uint2 k = lds64(sk + 32 * c + 8 * j);
+#pragma unroll
+      for (int a = 0; a < 2; ++a) {
+        const int col = 32 * c + 8 * j + 2 * q;
+        if (col < seen[a]) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a]) * __uint_as_float(k.x));
+        if (col + 1 < seen[a]) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a + 1]) * __uint_as_float(k.y));
+      }
     }
   }
 #pragma unroll
@@ -285,7 +291,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       mbar_init(vempty_b + 8 * i, 1);
       for (int h = 0; h < 2; ++h) {
         mbar_init(sfull_b + 16 * i + 8 * h, 1);
-        mbar_init(pfull_b + 16 * i + 8 * h, 4);
+        mbar_init(pfull_b + 16 * i + 8 * h, 8);
         mbar_init(odone_b + 16 * i + 8 * h, 1);
       }
     }
@@ -318,14 +324,14 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   if (split >= splits) return;
   const int t0 = split * sp.tiles, nt = min(tiles, t0 + sp.tiles) - t0;    // key tiles [t0, t0 + nt)
 
-  if (warp == 12) {
+  if (warp == kKvPMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm_tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   __syncthreads();
 
   // ---------------------------------------------------------------- the converters' first loads
-  const bool softmax = warp < 4 * kQt, converter = warp >= 8 && warp < 12;
+  const bool softmax = warp < 8 * kQt, converter = warp >= kKvPConv && warp < kKvPMma;
   const int key = tid & 127;  // of the tile
   const int codes = a.C.page_size * (kHd / 2);
   uint4 rk[kRaw], rv[kRaw];
@@ -361,16 +367,15 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     return a.bf16 ? max(-99, min(99, top > 0.f ? 14 - ((__float_as_int(top) >> 23) - 127) : 0)) : 0;
   };
   {
-    constexpr int kChunks = kHd / 8, kMine = kQt * kKvPM * kChunks / kKvPThreads;
+    constexpr int kChunks = kHd / 8, kAll = kQt * kKvPM * kChunks, kMine = (kAll + kKvPThreads - 1) / kKvPThreads;
     uint4 v[kMine];
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int x = i * kKvPThreads + tid, row = row0 + x / kChunks, c = x % kChunks, tok = row / a.group;
       const uint16_t* src = a.q + static_cast<int64_t>(r0 + tok) * a.ldq + (kvh * a.group + row - tok * a.group) * kHd + 8 * c;
       v[i] = make_uint4(0, 0, 0, 0);
-      if (row < R) v[i] = a.vec ? ld_row8<true>(src) : ld_row8<false>(src);
+      if (x < kAll && row < R) v[i] = a.vec ? ld_row8<true>(src) : ld_row8<false>(src);
     }
-    if (converter) load(0);
     if (a.bf16) {
       float big = 0.f;
 #pragma unroll
@@ -395,11 +400,11 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
 #pragma unroll
     for (int i = 0; i < kMine; ++i) {
       const int x = i * kKvPThreads + tid, row = x / kChunks, c = x % kChunks;
-      sts128(sQ + (row >> 7) * kTile + (c >> 3) * kBlock + sw128_off(row & 127, c & 7), kv_order8(v[i]));
+      if (x < kAll) sts128(sQ + (row >> 7) * kTile + (c >> 3) * kBlock + sw128_off(row & 127, c & 7), kv_order8(v[i]));
     }
     fence_proxy_async_smem();
-    if (converter) find(1);
   }
+  if (kQt == 2 && converter) load(0);  // (large heads: when the converters have their registers)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -407,63 +412,47 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   const uint32_t tS = tmem, tO = tmem + kQt * kKvPN;  // row tile t: S at + 128 t, O at + kHdp t
   bool ok = true;
 
-  // (every warpgroup trades before its role: two at 176, 88 and 72, or with one row tile 176, 24, 168, 72
-  // -- at most 512 = 4 * 128 together)
+  // (every warpgroup trades before its role: 4 * 88 + 88 + 40 = 6 * 80, or with one row tile
+  // 2 * 88 + 2 * 24 + 168 + 40 below it)
   if (softmax) {
     // ---------------------------------------------------------------- softmax
-    regs_up<176>();
-    const int t = tid >> 7, g = lane >> 2, q = lane & 3;
-    const uint32_t lanes = static_cast<uint32_t>(32 * (warp & 3)) << 16;
+    regs_up<88>();
+    const int t = warp >> 3, b = (warp >> 2) & 1, g = lane >> 2, q = lane & 3;
+    const int lane0 = 32 * (warp & 3) + 16 * b;  // the warp's first row (TMEM lane) of the tile
+    const uint32_t lanes = static_cast<uint32_t>(lane0) << 16;
     const uint32_t s_addr = tS + t * kKvPN + lanes, o_addr = tO + t * kHdp + lanes;
-    constexpr uint32_t kHalfLanes = 16u << 16;
-    // rows in the fragment shapes: r = 2b + a is row 16b + 8a + g of the warp's 32
-    const int first_row = row0 + (tid & ~31);
-    float m[4], T[4];
-    int lim[4];         // keys below it are seen by the row
-    bool fresh[4];      // no key seen yet, but one will be: m means nothing
+    const int first_row = row0 + t * kKvPM + lane0;
+    float m[2], T[2];   // of rows g and g + 8
+    int lim[2];         // keys below it are seen by the row
+    bool fresh[2];      // no key seen yet, but one will be: m means nothing
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 2; ++r) {
       m[r] = T[r] = 0.f;
-      const int row = first_row + 16 * (r >> 1) + 8 * (r & 1) + g;
+      const int row = first_row + 8 * r + g;
       lim[r] = row < R ? max(0, min(n, pos0 + row / a.group + 1)) : 0;
       fresh[r] = lim[r] > 0;
     }
     // tiles below need no mask (rows that do not exist see nothing; the first row sees the fewest)
-    const int plain = first_row + 31 < R ? max(0, min(n, pos0 + first_row / a.group + 1)) : 0;
+    const int plain = first_row + 15 < R ? max(0, min(n, pos0 + first_row / a.group + 1)) : 0;
     for (int kt = 0; kt < nt; ++kt) {
       const int kb = (t0 + kt) * kKvPN, ring = kt % kKvPScales;
       const uint32_t sc = sScale + ring * kKvPN * 8;
-      float ev = 0.f;
       const bool whole = kb + kKvPN <= plain;
-      // In halves of 64 keys (the weights of the first are multiplied while the second is evaluated), 16
-      // rows at a time: after each the rows' registers change places, so that the code, which has to
-      // stay in the instruction cache beside the other roles', is there once.
-      uint64_t ks[8], vs[8];  // the scales of the lane's 16 keys of the half
+      // in halves of 64 keys: the weights of the first are multiplied while the second is evaluated
 #pragma unroll 1
-      for (int hb = 0; hb < 4 && ok; ++hb) {
-        const int h = hb >> 1, b = hb & 1;
-        if (b == 0) {
-          if (!mbar_wait_bounded(sfull_b + 16 * t + 8 * h, kt & 1)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
-          // log2 of the largest scale_v of the tile, rounded up (NaN scales are left out; all zero: 2^-30)
-          const uint4 tops = lds128(sTop + ring * 16);
-          const uint32_t top = max(max(tops.x, tops.y), max(tops.z, tops.w));
-          ev = static_cast<float>(max(-30, static_cast<int>(top >> 23) - 126));
-#pragma unroll
-          for (int i = 0; i < 8; i += 2) {
-            const uint4 k4 = lds128(sc + 256 * h + 64 * q + 8 * i), v4 = lds128(sc + 512 + 256 * h + 64 * q + 8 * i);
-            ks[i] = pack2(__uint_as_float(k4.x), __uint_as_float(k4.y));
-            ks[i + 1] = pack2(__uint_as_float(k4.z), __uint_as_float(k4.w));
-            vs[i] = pack2(__uint_as_float(v4.x), __uint_as_float(v4.y));
-            vs[i + 1] = pack2(__uint_as_float(v4.z), __uint_as_float(v4.w));
-          }
+      for (int h = 0; h < 2; ++h) {
+        if (!mbar_wait_bounded(sfull_b + 16 * t + 8 * h, kt & 1)) {
+          ok = false;
+          break;
         }
+        tc_fence_after();
+        // log2 of the largest scale_v of the tile, rounded up (NaN scales are left out; all zero: 2^-30)
+        const uint4 tops = lds128(sTop + ring * 16);
+        const uint32_t top = max(max(tops.x, tops.y), max(tops.z, tops.w));
+        const float ev = static_cast<float>(max(-30, static_cast<int>(top >> 23) - 126));
         uint32_t pk[16];
         float add[2];
-        const uint32_t addr = s_addr + b * kHalfLanes + 64 * h;
+        const uint32_t addr = s_addr + 64 * h, sk = sc + 256 * h + 64 * q, sv = sk + 512;
         const int seen[2] = {lim[0] - kb - 64 * h, lim[1] - kb - 64 * h};
         // A row moves m when its weights' sum (the lane's share) says that one times scale_v may pass 2^12,
         // or when it has seen no key yet.
@@ -472,7 +461,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         for (;;) {
           if (moved) {
             float mx[2], corr[2];
-            kv_row_max(addr, ks, seen, q, mx);
+            kv_row_max(addr, sk, seen, q, mx);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const bool first = fresh[r] && mx[r] > -INFINITY;
@@ -483,60 +472,50 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
               fresh[r] = fresh[r] && !first;
             }
             if (kt + h > 0) {  // O holds the halves before
-              if (!mbar_wait_bounded(odone_b + 16 * t + 8 * (1 - h), (kt + h - 1) & 1)) {
-                ok = false;
-                break;
-              }
+              if (!mbar_wait_bounded(odone_b + 16 * t + 8 * (1 - h), (kt + h - 1) & 1)) ok = false;
               tc_fence_after();
 #pragma unroll 1
               for (int c = 0; c < kHd / 32; ++c) {
                 uint32_t v[16];
-                tmem_ld_rows32(o_addr + b * kHalfLanes + 32 * c, v);
+                tmem_ld_rows32(o_addr + 32 * c, v);
                 tmem_wait_ld();
 #pragma unroll
                 for (int e = 0; e < 16; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * corr[(e >> 1) & 1]);
-                tmem_st_rows32(o_addr + b * kHalfLanes + 32 * c, v);
+                tmem_st_rows32(o_addr + 32 * c, v);
               }
             }
           }
-          if (whole) kv_weights<false>(addr, ks, vs, m, seen, q, pk, add);
-          else kv_weights<true>(addr, ks, vs, m, seen, q, pk, add);
+          if (whole) kv_weights<false>(addr, sk, sv, m, seen, q, pk, add);
+          else kv_weights<true>(addr, sk, sv, m, seen, q, pk, add);
           if (moved || !__any_sync(0xffffffffu, fmaxf(add[0], add[1]) > ex2(12.f - ev))) break;
           moved = true;
         }
         T[0] += add[0];
         T[1] += add[1];
         tmem_st_pairs32(addr, pk);  // over the half's scores, which have been read
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-          swap_values(m[r], m[r + 2]);
-          swap_values(T[r], T[r + 2]);
-          swap_values(lim[r], lim[r + 2]);
-          swap_values(fresh[r], fresh[r + 2]);
-        }
-        if (b == 1) {
-          tmem_wait_st();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(pfull_b + 16 * t + 8 * h);
-        }
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(pfull_b + 16 * t + 8 * h);
       }
       if (!ok) break;
     }
     // -------------------------------------------------------------- results
     if (ok && nt > 0) ok = mbar_wait_bounded(odone_b + 16 * t + 8, (nt - 1) & 1);
     tc_fence_after();
-    // from the fragments' rows to lane = row
-    float2* rows_mt = sm_rows + (tid & ~31);
+    // From here on thread = row of the tile, the tile's second four warps taking other columns than the
+    // first: (m, sum) of the rows through shared memory.
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
+    for (int r = 0; r < 2; ++r) {
       T[r] += __shfl_xor_sync(0xffffffffu, T[r], 1);
       T[r] += __shfl_xor_sync(0xffffffffu, T[r], 2);
-      if (q == 0) rows_mt[16 * (r >> 1) + 8 * (r & 1) + g] = make_float2(lim[r] > 0 && !fresh[r] ? m[r] : -1e30f, T[r]);
+      if (q == 0) sm_rows[t * kKvPM + lane0 + 8 * r + g] = make_float2(lim[r] > 0 && !fresh[r] ? m[r] : -1e30f, T[r]);
     }
-    __syncwarp();
-    const float row_m = rows_mt[lane].x, row_T = rows_mt[lane].y;
-    const int row = row0 + tid;
+    named_barrier(2 + t, 256);
+    const int in = tid & 127, tile_row = t * kKvPM + in;
+    const float row_m = sm_rows[tile_row].x, row_T = sm_rows[tile_row].y;
+    const uint32_t row_addr = tO + t * kHdp + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
+    const int row = row0 + tile_row;
     const bool live = row < R;
     const bool single = splits == 1;
     const int64_t item = (static_cast<int64_t>(seq) * gridDim.y + kvh) * (gridDim.x / sp.splits) + pair_from_end;
@@ -546,72 +525,73 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     const uint32_t out_s = sQ + t * kTile;  // the row tile's output, laid out like q, which is no longer needed
     const float inv = row_T == 0.f ? 0.f : 1.0f / row_T;  // a row that sees nothing: 0 (a NaN sum stays NaN)
 #pragma unroll 1
-    for (int c = 0; c < kHd / 32; ++c) {
-      uint32_t v[32];
+    for (int c = b; c < kHd / 16; c += 2) {
+      uint32_t v[16];
       if (nt > 0) {
-        tmem_ld32(o_addr + 32 * c, v);
+        tmem_ld16(row_addr + 16 * c, v);
       } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] = 0;
+        for (int e = 0; e < 16; ++e) v[e] = 0;
       }
 #pragma unroll
-      for (int e = 0; e < 32; e += 8) {  // columns 0 4 1 5 2 6 3 7 of eight dimensions
+      for (int e = 0; e < 16; e += 8) {  // columns 0 4 1 5 2 6 3 7 of eight dimensions
+        const int d = 16 * c + e;
         const float x[8] = {__uint_as_float(v[e]),     __uint_as_float(v[e + 2]), __uint_as_float(v[e + 4]), __uint_as_float(v[e + 6]),
                             __uint_as_float(v[e + 1]), __uint_as_float(v[e + 3]), __uint_as_float(v[e + 5]), __uint_as_float(v[e + 7])};
         if (single) {
-          sts128(out_s + ((32 * c + e) >> 6) * kBlock + sw128_off(tid & 127, ((32 * c + e) >> 3) & 7), kv_out8(x, inv, a.bf16));
+          sts128(out_s + (d >> 6) * kBlock + sw128_off(in, (d >> 3) & 7), kv_out8(x, inv, a.bf16));
         } else if (live) {
-          *reinterpret_cast<float4*>(rec + ((32 * c + e) / 4 * kRows + tid) * 4) = make_float4(x[0], x[1], x[2], x[3]);
-          *reinterpret_cast<float4*>(rec + ((32 * c + e) / 4 * kRows + kRows + tid) * 4) = make_float4(x[4], x[5], x[6], x[7]);
+          *reinterpret_cast<float4*>(rec + (d / 4 * kRows + tile_row) * 4) = make_float4(x[0], x[1], x[2], x[3]);
+          *reinterpret_cast<float4*>(rec + (d / 4 * kRows + kRows + tile_row) * 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
       }
     }
     const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
     uint16_t* dst = a.out + static_cast<int64_t>(r0 + tok) * a.ldo + static_cast<int64_t>(head) * kHd;
     if (single) {
-      if (live && ok && a.lse)
+      if (b == 0 && live && ok && a.lse)
         a.lse[static_cast<int64_t>(r0 + tok) * a.heads + head] = row_T == 0.f ? -INFINITY : row_m * 0.6931471805599453f + logf(row_T);
-      __syncwarp();
+      named_barrier(2 + t, 256);
       constexpr int kChunks = kHd / 8;
-#pragma unroll 4
-      for (int i = 0; i < kChunks; ++i) {  // whole rows at a time
-        const int x = i * 32 + lane, r = x / kChunks, c = x % kChunks;
+#pragma unroll 2
+      for (int i = 0; i < kChunks / 2; ++i) {  // whole rows at a time, of the warp's 16 (in lanes 16b..16b + 15)
+        const int x = i * 32 + lane, r = 16 * b + x / kChunks, c = x % kChunks;
         const uint64_t to = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(dst), r);
-        const uint4 w = lds128(out_s + (c >> 3) * kBlock + sw128_off((tid & 96) + r, c & 7));
+        const uint4 w = lds128(out_s + (c >> 3) * kBlock + sw128_off((in & 96) + r, c & 7));
         uint16_t* o = reinterpret_cast<uint16_t*>(to) + 8 * c;
-        if (row0 + (tid & ~31) + r < R && ok) {
+        if (row - lane + r < R && ok) {
           if (a.vec) st_row8<true>(o, w);
           else st_row8<false>(o, w);
         }
       }
     } else {
-      if (live) *reinterpret_cast<float2*>(rec + kRows * kHd + 2 * tid) = make_float2(row_m, row_T);
-      named_barrier(2, kRows);
+      if (b == 0 && live) *reinterpret_cast<float2*>(rec + kRows * kHd + 2 * tile_row) = make_float2(row_m, row_T);
+      named_barrier(4, 2 * kRows);
       if (tid == 0) {
         const bool last = atom_add_acq_rel_gpu(sp.count + item, 1) == splits - 1;
         if (last) sp.count[item] = 0;
         sm_last = last;
       }
-      named_barrier(2, kRows);
-      if (sm_last && live && ok) {  // merge, in order: thread = row
+      named_barrier(4, 2 * kRows);
+      if (sm_last && live && ok) {  // merge, in order: thread = row and every other 16 dimensions
         const float* part = sp.part + item * sp.splits * (kRows * (kHd + 4));
         float M = -1e30f, S = 0.f;
-        for (int i = 0; i < splits; ++i) M = fmaxf(M, __ldcg(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tid));
+        for (int i = 0; i < splits; ++i) M = fmaxf(M, __ldcg(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tile_row));
         for (int i = 0; i < splits; ++i) {
-          const float2 w = __ldcg(reinterpret_cast<const float2*>(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tid));
+          const float2 w = __ldcg(reinterpret_cast<const float2*>(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tile_row));
           S += ex2(w.x - M) * w.y;
         }
         const float scale = S == 0.f ? 0.f : 1.0f / S;
 #pragma unroll 1
-        for (int d = 0; d < kHd; d += 16) {
+        for (int d = 16 * b; d < kHd; d += 32) {
           float o[16] = {};
 #pragma unroll 2
           for (int i = 0; i < splits; ++i) {
             const float* src = part + i * (kRows * (kHd + 4));
-            const float f = ex2(__ldcg(src + kRows * kHd + 2 * tid) - M);
+            const float f = ex2(__ldcg(src + kRows * kHd + 2 * tile_row) - M);
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const float4 v = __ldcg(reinterpret_cast<const float4*>(src + ((d / 4 + e) * kRows + tid) * 4));
+              const float4 v = __ldcg(reinterpret_cast<const float4*>(src + ((d / 4 + e) * kRows + tile_row) * 4));
               o[4 * e] += f * v.x;
               o[4 * e + 1] += f * v.y;
               o[4 * e + 2] += f * v.z;
@@ -625,15 +605,21 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
             else st_row8<false>(dst + d + e, w);
           }
         }
-        if (a.lse) a.lse[static_cast<int64_t>(r0 + tok) * a.heads + head] = S == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(S);
+        if (b == 0 && a.lse)
+          a.lse[static_cast<int64_t>(r0 + tok) * a.heads + head] = S == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(S);
       }
     }
-  } else if (warp < 8) {
+  } else if (warp < kKvPConv) {
     regs_down<24>();
-  } else if (warp < 12) {
+  } else if (warp < kKvPMma) {
     // ---------------------------------------------------------------- keys: thread = key of the tile
-    if constexpr (kQt == 2) regs_down<88>();
-    else regs_up<168>();
+    if constexpr (kQt == 2) {
+      regs_up<88>();
+    } else {
+      regs_up<168>();
+      load(0);
+    }
+    find(1);
     const auto convert = [&](const uint4 (&raw)[kRaw], uint32_t pair, uint32_t tile) {
       const __half2 zero = __half2half2(__ushort_as_half(static_cast<unsigned short>(pair >> 16)));
 #pragma unroll
@@ -661,7 +647,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 512), "f"(vf.x) : "memory");
       const float size = fminf(fmaxf(fabsf(vf.x), 0.f), 65504.f);  // (a NaN has no size)
       const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size));
-      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - 8)), "r"(top) : "memory");
+      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - kKvPConv)), "r"(top) : "memory");
 #pragma unroll 1
       for (int v = 0; v < 2; ++v) {  // K', then V' (one copy of the code)
         if (v && kt >= kSt && !mbar_wait_bounded(vempty_b + 8 * st, par)) {
@@ -682,8 +668,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     }
   } else {
     // ---------------------------------------------------------------- MMA issuer
-    regs_down<72>();
-    if (warp == 12) {  // (all lanes wait and count, one issues)
+    regs_down<40>();
+    if (warp == kKvPMma) {  // (all lanes wait and count, one issues)
       const uint32_t leader = elect_leader();
       // the scores of row tile t for half h of key tile kt
       const auto scores = [&](int t, int kt, int h) {
@@ -733,7 +719,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   if (!ok && lane == 0) atomicCAS(a.B.err, 0, kDevErrTmaTimeout);
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) {
+  if (warp == kKvPMma) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
   }
