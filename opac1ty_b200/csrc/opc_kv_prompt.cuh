@@ -114,32 +114,6 @@ __host__ __device__ constexpr uint32_t kv_idesc(int n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kKvPM >> 4) << 24);
 }
 
-// Two fp32 values per instruction.
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t d;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t v) {
-  float2 d;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(v));
-  return d;
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-  return d;
-}
 // The 16-row fragment shapes: of 8 fp32 columns lane (g, q) = (lane / 4, lane % 4) holds (row g, columns
 // 2q, 2q + 1) and (row g + 8, the same); of 4 32-bit columns (16x128b) column q of rows g and g + 8.
 __device__ __forceinline__ void tmem_ld_rows32(uint32_t taddr, uint32_t* v) {  // 32 columns

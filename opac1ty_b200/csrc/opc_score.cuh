@@ -5,8 +5,8 @@
 //   logprob = x_t - m - ln2 log2 Z,  entropy = ln2 (log2 Z - W / Z)
 // in one pass: a thread takes groups of 16 bytes, and moves its own m only when a group passes it (the
 // sums are then rescaled); the threads' (m, Z, W) are joined at the end.  At 2 bytes a logit HBM leaves
-// about 11 issue slots per logit on an SM; the pass takes about 8 (unpack, maximum, difference, product,
-// clamp, exp2, sum, fma).
+// about 11 issue slots per logit on an SM; two 16-bit logits take about 9 instructions (packed maximum
+// and clamp, unpack, packed fp32 fma, two exp2, packed sum and fma).
 //
 // Top alternatives without a second pass: every thread also keeps the largest logit of its share.  The
 // top_k-th largest of these maxima bounds the answer from below (top_k different logits reach it), so
@@ -79,8 +79,40 @@ __device__ __forceinline__ float score_value(uint64_t key) {  // (NaN comes back
 }
 __device__ __forceinline__ int score_id(uint64_t key) { return static_cast<int>(~static_cast<uint32_t>(key)); }
 
+// The larger of two pairs of 16-bit elements, ignoring NaN, or handing it on.
+template <bool kBf>
+__device__ __forceinline__ uint32_t max_pair(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (kBf) asm("max.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("max.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+template <bool kBf>
+__device__ __forceinline__ uint32_t max_pair_nan(uint32_t a, uint32_t b) {
+  uint32_t d;
+  if constexpr (kBf) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
+// The largest of a group, ignoring NaN.
+template <int kType>
+__device__ __forceinline__ float score_max(const uint4& w) {
+  if constexpr (kType == 2) {
+    return fmaxf(fmaxf(__uint_as_float(w.x), __uint_as_float(w.y)), fmaxf(__uint_as_float(w.z), __uint_as_float(w.w)));
+  } else {
+    const uint32_t b = max_pair<kType == 1>(max_pair<kType == 1>(w.x, w.y), max_pair<kType == 1>(w.z, w.w));
+    return fmaxf(half_lo<kType == 1>(b), half_hi<kType == 1>(b));
+  }
+}
+
 struct ScoreSums {
-  float m, z, w, bad;  // m = -inf: nothing but -infinity so far
+  float m, z, w, bad;  // bad: a NaN or +infinity was seen; m = -inf: nothing but -infinity so far
 };
 __device__ __forceinline__ ScoreSums score_join(const ScoreSums& a, const ScoreSums& b) {
   ScoreSums r;
@@ -104,15 +136,14 @@ __device__ __forceinline__ ScoreSums score_shfl(const ScoreSums& s, int o) {
   r.bad = __shfl_xor_sync(0xffffffffu, s.bad, o);
   return r;
 }
-__device__ __forceinline__ uint64_t score_shfl64(uint64_t v, int o) { return __shfl_xor_sync(0xffffffffu, v, o); }
-
 // 32 keys of a warp in descending order (bitonic).
-__device__ __forceinline__ uint64_t score_sort32(uint64_t v, int lane) {
+template <typename T>
+__device__ __forceinline__ T score_sort32(T v, int lane) {
 #pragma unroll
   for (int k = 2; k <= 32; k *= 2) {
 #pragma unroll
     for (int j = k / 2; j > 0; j /= 2) {
-      const uint64_t o = score_shfl64(v, j);
+      const T o = __shfl_xor_sync(0xffffffffu, v, j);
       const bool up = (lane & k) != 0, low = (lane & j) == 0;  // descending blocks, ascending where up
       v = (low != up) ? (v > o ? v : o) : (v < o ? v : o);
     }
@@ -120,12 +151,13 @@ __device__ __forceinline__ uint64_t score_sort32(uint64_t v, int lane) {
   return v;
 }
 // Two descending sequences of 32 (lane i: element i of each) to the 32 largest of both, descending.
-__device__ __forceinline__ uint64_t score_merge32(uint64_t a, uint64_t b, int lane) {
-  const uint64_t r = __shfl_sync(0xffffffffu, b, 31 - lane);
-  uint64_t v = a > r ? a : r;
+template <typename T>
+__device__ __forceinline__ T score_merge32(T a, T b, int lane) {
+  const T r = __shfl_sync(0xffffffffu, b, 31 - lane);
+  T v = a > r ? a : r;
 #pragma unroll
   for (int j = 16; j > 0; j /= 2) {
-    const uint64_t o = score_shfl64(v, j);
+    const T o = __shfl_xor_sync(0xffffffffu, v, j);
     v = (lane & j) == 0 ? (v > o ? v : o) : (v < o ? v : o);
   }
   return v;
@@ -162,14 +194,15 @@ __device__ __forceinline__ void score_write(const ScoreArgs& a, int64_t r, const
 }
 
 template <int kType, bool kVec, bool kTop>
-__global__ void __launch_bounds__(kScoreThreads) score_kernel(const ScoreArgs a) {
+__global__ void __launch_bounds__(kScoreThreads, 5) score_kernel(const ScoreArgs a) {
   constexpr int kN = kType == 2 ? 4 : 8, kWarps = kScoreThreads / 32, kU = 4;  // groups in flight per thread
   constexpr int kSize = kType == 2 ? 4 : 2;
   __shared__ ScoreSums sm_sums[kWarps];
   __shared__ uint64_t sm_keys[kWarps][32];
   __shared__ uint64_t sm_cand[kTop ? kScoreCand : 1];
   __shared__ uint32_t sm_share[kScoreThreads];
-  __shared__ int sm_n, sm_shares;
+  __shared__ uint32_t sm_top[kWarps][32];
+  __shared__ int sm_n, sm_shares, sm_last;
   __shared__ uint64_t sm_best[kWarps];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int64_t r = blockIdx.x / a.split;
@@ -182,42 +215,73 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const ScoreArgs a)
   if (kTop && tid == 0) sm_n = sm_shares = 0;
 
   // ---------------------------------------------------------------- one pass over the logits
-  ScoreSums s = {-INFINITY, 0.f, 0.f, 0.f};
+  constexpr float kLog2e = 1.4426950408889634f;
+  // The thread's m, and Z and W in two halves each (even and odd logits).  For an ordinary m, y is one
+  // fma, fma(x, log2 e, -M), M = m log2 e rounded; the rounding c = m log2 e - M shifts every y alike and
+  // is taken out when m moves and at the end.  -infinity goes in as -65504 (fp16) or -1e30, far enough below kPlainLow for a weight of 0; a NaN turns
+  // Z into one.  Other m (nothing but -infinity or NaN so far, masks of the type's lowest value, absurd
+  // logits) take logit by logit.
+  constexpr float kPlain = 1e6f, kPlainLow = kType == 0 ? -6e4f : -1e6f, kNothing = -1e30f;
+  float m = -INFINITY, c = 0.f, bad = 0.f;
+  uint64_t z2 = 0, w2 = 0, ml2 = 0;  // ml2: -M, twice
   float top = -INFINITY;  // largest logit of this thread's share (thread t: groups t, t + 256, ..., and the tail's)
   bool any = false;       // whether the share holds anything but NaN
-  const auto take = [&](const float* x, int n) {
-    constexpr float kLog2e = 1.4426950408889634f;
-    float big = x[0];
-    bool nan = !(x[0] < INFINITY);
-#pragma unroll
-    for (int i = 1; i < kN; ++i)
-      if (i < n) {
-        big = fmaxf(big, x[i]);
-        nan |= !(x[i] < INFINITY);
+  const uint64_t l2 = pack2(kLog2e, kLog2e);
+  const auto move = [&](float big) {  // the share's maximum moves (seldom after the first groups)
+    top = fmaxf(top, big);
+    any |= big == big;
+    if (big > m && big < INFINITY) {
+      const float ml = big * kLog2e, cn = fabsf(big) <= kPlain ? fmaf(big, kLog2e, -ml) : 0.f;
+      if (m > -INFINITY) {  // y falls by (big - m) log2 e, and its shift changes
+        const float d = fmaxf((m - big) * kLog2e + (cn - c), -200.f), f = exp2f(d);
+        w2 = mul2(pack2(f, f), fma2(pack2(d, d), z2, w2));
+        z2 = mul2(pack2(f, f), z2);
       }
-    if (nan) s.bad = 1.f;
-    if (big > top || !any) {  // the share's maximum moves (seldom after the first groups)
-      top = fmaxf(top, big);
-      any |= big == big;
-      if (big > s.m && big < INFINITY) {
-        if (s.m > -INFINITY) {
-          const float d = fmaxf((s.m - big) * kLog2e, -200.f), f = exp2f(d);
-          s.w = f * (s.w + d * s.z);
-          s.z *= f;
-        }
-        s.m = big;
-      }
+      m = big;
+      c = cn;
+      ml2 = pack2(-ml, -ml);
     }
-    if (s.m > -INFINITY) {
+  };
+  const auto one = [&](float x) {  // any logit, any m
+    if (x > top || !any) move(x);
+    if (x != x) bad = 1.f;
+    if (m > -INFINITY && x == x) {
+      const float y = fmaxf((x - m) * kLog2e + c, -200.f), e = exp2f(y);  // (2^-200 is 0, and so is its product with y)
+      z2 = add2(z2, pack2(e, 0.f));
+      w2 = add2(w2, pack2(e * y, 0.f));
+    }
+  };
+  const auto pair = [&](float x0, float x1) {
+    const uint64_t y = fma2(pack2(x0, x1), l2, ml2);
+    const float2 f = unpack2(y);
+    float e0, e1;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(f.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(f.y));
+    const uint64_t e = pack2(e0, e1);
+    z2 = add2(z2, e);
+    w2 = fma2(e, y, w2);
+  };
+  const auto take = [&](const uint4& raw) {
+    const uint32_t r4[4] = {raw.x, raw.y, raw.z, raw.w};
+    const float big = score_max<kType>(raw);
+    if (big > top || !any) move(big);
+    if (m >= kPlainLow && m <= kPlain) {
+      if constexpr (kType == 2) {
+        pair(max_nan(__uint_as_float(raw.x), kNothing), max_nan(__uint_as_float(raw.y), kNothing));
+        pair(max_nan(__uint_as_float(raw.z), kNothing), max_nan(__uint_as_float(raw.w), kNothing));
+      } else {
+        const uint32_t low = kType == 1 ? 0xf149f149u : 0xfbfffbffu;  // about -1e30; -65504
 #pragma unroll
-      for (int i = 0; i < kN; ++i)
-        if (i < n) {
-          const float y = fmaxf((x[i] - s.m) * kLog2e, -200.f);  // (2^-200 is 0, and so is its product with y)
-          float e;
-          asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(y));
-          s.z += e;
-          s.w = fmaf(e, y, s.w);
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t c = max_pair_nan<kType == 1>(r4[i], low);
+          pair(half_lo<kType == 1>(c), half_hi<kType == 1>(c));
         }
+      }
+    } else {
+      float x[kN];
+      score_unpack<kType>(raw, x);
+#pragma unroll 1
+      for (int i = 0; i < kN; ++i) one(i == 0 ? x[0] : i == 1 ? x[1] : i == 2 ? x[2] : i == 3 ? x[3] : i == 4 ? x[4 % kN] : i == 5 ? x[5 % kN] : i == 6 ? x[6 % kN] : x[7 % kN]);
     }
   };
   const auto group = [&](int g) {
@@ -237,72 +301,68 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const ScoreArgs a)
 #pragma unroll
     for (int u = 0; u < kU; ++u) w[u] = group(g + u * kScoreThreads);
 #pragma unroll
-    for (int u = 0; u < kU; ++u) {
-      float x[kN];
-      score_unpack<kType>(w[u], x);
-      take(x, kN);
-    }
+    for (int u = 0; u < kU; ++u) take(w[u]);
   }
-  for (; g < groups; g += kScoreThreads) {
-    float x[kN];
-    score_unpack<kType>(group(g), x);
-    take(x, kN);
-  }
-  for (int i = tail + tid; i < end; i += kScoreThreads) {
-    const float x[kN] = {score_load<kType>(row, i)};
-    take(x, 1);
-  }
+  for (; g < groups; g += kScoreThreads) take(group(g));
+  for (int i = tail + tid; i < end; i += kScoreThreads) one(score_load<kType>(row, i));
 
   // ---------------------------------------------------------------- join the threads
-  ScoreSums all = s;
+  const float2 zz = unpack2(z2), ww = unpack2(w2);
+  ScoreSums all = {m, zz.x + zz.y, ww.x + ww.y, bad};
+  all.z *= exp2f(-c);  // 2^(y + c), and 2^(y + c) (y + c), without c
+  all.w = fmaf(all.w, exp2f(-c), -c * all.z);
+  if (all.z != all.z || top == INFINITY) all.bad = 1.f;
+  if (all.bad != 0.f) all.z = all.w = 0.f;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) all = score_join(all, score_shfl(all, o));
   if (lane == 0) sm_sums[warp] = all;
   uint64_t mine = 0;
   if (kTop) {
-    // the maxima in order: the top_k-th bounds the answer from below.  (id: the thread, so that keys
-    // differ; a share of NaN alone counts as the lowest)
-    const uint64_t own = (static_cast<uint64_t>(any ? score_order(top) : 0u) << 32) | static_cast<uint32_t>(~tid);
-    sm_keys[warp][lane] = score_sort32(own, lane);
+    // the maxima in order: the top_k-th bounds the answer from below (shares of NaN alone count as 0)
+    sm_top[warp][lane] = score_sort32(any ? score_order(top) : 0u, lane);
   }
   __syncthreads();
   all = sm_sums[0];
   for (int i = 1; i < kWarps; ++i) all = score_join(all, sm_sums[i]);
   if (kTop) {
+    if (warp == 0) {
+      uint32_t v = sm_top[0][lane];
 #pragma unroll 1
-    for (int h = kWarps / 2; h > 0; h /= 2) {  // merge the warps' lists pairwise
-      uint64_t v = 0;
-      if (warp < h) v = score_merge32(sm_keys[warp][lane], sm_keys[warp + h][lane], lane);
-      __syncthreads();
-      if (warp < h) sm_keys[warp][lane] = v;
-      __syncthreads();
+      for (int w = 1; w < kWarps; ++w) v = score_merge32(v, sm_top[w][lane], lane);
+      sm_top[0][lane] = v;
     }
+    __syncthreads();
     const int want = min(a.top_k, max(0, end - begin));
     // (where fewer shares hold something it is 0: everything is a candidate)
-    const uint32_t bound = want > 0 ? static_cast<uint32_t>(sm_keys[0][want - 1] >> 32) : ~0u;
+    const uint32_t bound = want > 0 ? sm_top[0][want - 1] : ~0u;
     // the shares that reach it
     if ((any ? score_order(top) : 0u) >= bound) sm_share[atomicAdd(&sm_shares, 1)] = tid;
     __syncthreads();
     const int shares = sm_shares, per = (groups + kScoreThreads - 1) / kScoreThreads;
     const int n_tail = end - tail;
-    // element k of the shares: group k of them all, and the tail (once)
+    // the groups of those shares, and the tail (once)
     const auto scan = [&](auto&& f) {
+#pragma unroll 1
       for (int i = tid; i < shares * per; i += kScoreThreads) {
         const int gg = static_cast<int>(sm_share[i / per]) + (i % per) * kScoreThreads;
-        if (gg < groups) {
-          float x[kN];
-          score_unpack<kType>(group(gg), x);
-#pragma unroll
-          for (int e = 0; e < kN; ++e) f(x[e], begin + gg * kN + e);
-        }
+        if (gg < groups) f(group(gg), begin + gg * kN, kN);
       }
-      for (int i = tid; i < n_tail; i += kScoreThreads) f(score_load<kType>(row, tail + i), tail + i);
+      for (int i = tid; i < n_tail; i += kScoreThreads) {
+        uint4 w = make_uint4(0, 0, 0, 0);  // (only the first element counts)
+        w.x = kType == 2 ? __float_as_uint(score_load<kType>(row, tail + i)) : static_cast<const uint16_t*>(static_cast<const void*>(row))[tail + i];
+        f(w, tail + i, 1);
+      }
     };
-    scan([&](float x, int id) {
-      if (score_order(x) >= bound) {
-        const int at = atomicAdd(&sm_n, 1);
-        if (at < kScoreCand) sm_cand[at] = score_key(x, id);
-      }
+    scan([&](const uint4& w, int id, int n) {
+      if (n == kN && bound != 0 && score_order(score_max<kType>(w)) < bound) return;
+      float x[kN];
+      score_unpack<kType>(w, x);
+#pragma unroll
+      for (int e = 0; e < kN; ++e)
+        if (e < n && score_order(x[e]) >= bound) {
+          const int at = atomicAdd(&sm_n, 1);
+          if (at < kScoreCand) sm_cand[at] = score_key(x[e], id + e);
+        }
     });
     __syncthreads();
     const int n = sm_n;
@@ -322,14 +382,19 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const ScoreArgs a)
 #pragma unroll 1
       for (int k = 0; k < want; ++k) {
         uint64_t best = 0;
-        scan([&](float x, int id) {
-          const uint64_t key = score_key(x, id);
-          if (key < last && key > best) best = key;
+        scan([&](const uint4& w, int id, int n) {
+          float x[kN];
+          score_unpack<kType>(w, x);
+#pragma unroll
+          for (int e = 0; e < kN; ++e) {
+            const uint64_t key = score_key(x[e], id + e);
+            if (e < n && key < last && key > best) best = key;
+          }
         });
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) {
-          const uint64_t o64 = score_shfl64(best, o);
-          best = best > o64 ? best : o64;
+          const uint64_t other = __shfl_xor_sync(0xffffffffu, best, o);
+          best = best > other ? best : other;
         }
         if (lane == 0) sm_best[warp] = best;
         __syncthreads();
@@ -350,26 +415,33 @@ __global__ void __launch_bounds__(kScoreThreads) score_kernel(const ScoreArgs a)
     if (lane == 0) a.part[r * a.split + part] = make_float4(all.m, all.z, all.w, all.bad);
     if (kTop) a.cand[(r * a.split + part) * kScoreMaxTop + lane] = mine;
     __syncwarp();
-    int last = 0;
-    if (lane == 0) last = atom_add_acq_rel_gpu(a.count + r, 1) == a.split - 1;
-    if (__shfl_sync(0xffffffffu, last, 0)) {
-      __syncwarp();
-      if (lane == 0) a.count[r] = 0;
-      ScoreSums sums = {-INFINITY, 0.f, 0.f, 0.f};
-      for (int i = lane; i < a.split; i += 32) {  // (at most two each; lanes joined in a fixed order)
-        const float4 p = __ldcg(a.part + r * a.split + i);
-        sums = score_join(sums, ScoreSums{p.x, p.y, p.z, p.w});
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sums = score_join(sums, score_shfl(sums, o));
-      uint64_t v = 0;
-      if (kTop) {
-        const uint64_t* c = a.cand + r * a.split * kScoreMaxTop;
-#pragma unroll 4
-        for (int i = 0; i < a.split; ++i) v = score_merge32(v, __ldcg(c + i * kScoreMaxTop + lane), lane);
-      }
-      score_write<kType>(a, r, row, sums, v, lane);
+    if (lane == 0) {
+      sm_last = atom_add_acq_rel_gpu(a.count + r, 1) == a.split - 1;
+      if (sm_last) a.count[r] = 0;
     }
+  }
+  __syncthreads();
+  if (!sm_last) return;
+  if (kTop) {  // the CTAs' candidates: lists w, w + 8, ... per warp, then the warps'
+    const uint64_t* c = a.cand + r * a.split * kScoreMaxTop;
+    uint64_t v = 0;
+#pragma unroll 4
+    for (int i = warp; i < a.split; i += kWarps) v = score_merge32(v, __ldcg(c + i * kScoreMaxTop + lane), lane);
+    sm_keys[warp][lane] = v;
+    __syncthreads();
+  }
+  if (warp == 0) {
+    ScoreSums sums = {-INFINITY, 0.f, 0.f, 0.f};
+    for (int i = lane; i < a.split; i += 32) {  // (at most two each; lanes joined in a fixed order)
+      const float4 p = __ldcg(a.part + r * a.split + i);
+      sums = score_join(sums, ScoreSums{p.x, p.y, p.z, p.w});
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) sums = score_join(sums, score_shfl(sums, o));
+    uint64_t v = 0;
+    if (kTop)
+      for (int w = 0; w < kWarps; ++w) v = score_merge32(v, sm_keys[w][lane], lane);
+    score_write<kType>(a, r, row, sums, v, lane);
   }
 }
 

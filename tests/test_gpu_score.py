@@ -115,6 +115,40 @@ def test_special_rows(cuda_device):
 
 
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
+def test_rows_near_the_lowest_value(cuda_device, dtype):
+    # masks of the lowest value beside -infinity: rows of nothing else, and few ordinary logits among them
+    low, vocab = torch.finfo(dtype).min, 5000
+    x = torch.full((5, vocab), low, dtype=dtype)
+    x[0, ::2] = float("-inf")
+    x[1, 3:4990] = float("-inf")
+    x[2, 17] = -5.0
+    x[3, 1000:] = float("-inf")
+    x[3, 5] = low * 0.75
+    x[4, ::3] = float("-inf")
+    x[4, 4999] = float("nan")
+    x = x.to(cuda_device)
+    t = [1, 0, 17, 5, 1]
+    check(x, t, 6, token_logprobs(x, torch.tensor(t, device=cuda_device), top_k=6))
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("rows", [1, 400])
+def test_one_nan_or_infinity_anywhere(cuda_device, dtype, rows):
+    # in the first group of a thread, a later one, the tail, a masked region
+    vocab = 20011
+    base = torch.randn(rows, vocab, generator=torch.Generator().manual_seed(rows)) * 2
+    base[:, 9000:12000] = float("-inf")
+    for bad in (float("nan"), float("inf")):
+        for at in (0, 7, 5000, 9500, 11999, 15000, 20010):
+            x = base.clone().to(dtype)
+            x[0, at] = bad
+            x = x.to(cuda_device)
+            r = token_logprobs(x, torch.full((rows,), 3, device=cuda_device), top_k=2)
+            for v in (r.logprob, r.entropy, r.top_logprobs[:, 0]):
+                assert v[0].isnan() and v[1:].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
 @pytest.mark.parametrize("ld,off", [(1003, 0), (1008, 0), (1024, 3), (1001, 1)])
 def test_strides_and_alignment(cuda_device, dtype, ld, off):
     rows, vocab = 6, 1000
