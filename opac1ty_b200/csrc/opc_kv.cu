@@ -6,6 +6,9 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <mutex>
+#include <set>
+#include <utility>
 
 #include "../../include/opc_b200.h"
 #include "opc_internal.h"
@@ -181,9 +184,19 @@ auto prompt_of(int hd) {
 // kernels waits for before it reads anything.
 template <typename... KArgs, typename... Args>
 cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, int threads, int smem, cudaStream_t s, Args... args) {
-  if (smem > 48 * 1024) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (smem > 48 * 1024) {  // (once per kernel and device: the size is the kernel's own)
+    static std::mutex mu;
+    static std::set<std::pair<const void*, int>> done;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
+    const std::pair<const void*, int> key(reinterpret_cast<const void*>(kern), dev);
+    std::lock_guard<std::mutex> lk(mu);
+    if (!done.count(key)) {
+      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+      if (e != cudaSuccess) return e;
+      done.insert(key);
+    }
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
@@ -281,8 +294,7 @@ int opc_kv_append(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t 
   const int tok = few ? 1 : 4;
   const dim3 grid((batch->n_tokens + tok - 1) / tok, few ? (all + groups - 1) / groups : 1);
   auto kern = few ? append_for<1>(lpr, bf, vec) : append_for<4>(lpr, bf, vec);
-  kern<<<grid, opc::kKvAppendThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  KV_CUDA(cudaGetLastError(), "opc_kv_append launch");
+  KV_CUDA(launch_pdl(kern, grid, opc::kKvAppendThreads, 0, static_cast<cudaStream_t>(stream), a), "opc_kv_append launch");
   return OPC_OK;
 }
 
@@ -307,8 +319,7 @@ int opc_kv_read(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t dt
   a.ldv = ldv;
   const bool vec = aligned16(k) && aligned16(v) && ldk % 8 == 0 && ldv % 8 == 0;
   auto kern = read_for(lanes_per_head(cache->head_dim), dtype == OPC_BF16, vec);
-  kern<<<batch->n_tokens, opc::kKvAppendThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
-  KV_CUDA(cudaGetLastError(), "opc_kv_read launch");
+  KV_CUDA(launch_pdl(kern, dim3(batch->n_tokens), opc::kKvAppendThreads, 0, static_cast<cudaStream_t>(stream), a), "opc_kv_read launch");
   return OPC_OK;
 }
 
@@ -387,7 +398,6 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
                        opc::kv_p_smem(cache->head_dim), s, a, sp),
             "opc_kv_attention launch (prompts)");
   }
-  KV_CUDA(cudaGetLastError(), "opc_kv_attention launch");
   return OPC_OK;
 }
 

@@ -121,8 +121,14 @@ __device__ __forceinline__ void unpack_halves(const uint4& w, float x[8]) {
   const uint32_t v[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    x[2 * i] = half_lo<kBf>(v[i]);
-    x[2 * i + 1] = half_hi<kBf>(v[i]);
+    if constexpr (kBf) {
+      x[2 * i] = half_lo<true>(v[i]);
+      x[2 * i + 1] = half_hi<true>(v[i]);
+    } else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v[i]));
+      x[2 * i] = f.x;
+      x[2 * i + 1] = f.y;
+    }
   }
 }
 
@@ -171,10 +177,12 @@ struct KvAppendArgs {
 };
 
 // One CTA takes kTok rows (tokens); kLpr lanes (a power of two, head_dim / 8 of them at work) take
-// one head with 16 bytes each.  Memory bound for prompts (2 bytes in and out per element of q, 2 in
-// and 0.5 out per element of k and v), latency bound for steps: there gridDim.y spreads a row's
-// heads over CTAs so that each group of lanes has one head, and its load is issued before the
-// row's place is looked up (three dependent loads: starts, length, page table).
+// one head with 16 bytes each, one after the other of the CTA's heads, with the loads of the next
+// kAhead heads in flight (one load at a time held 16 KB in flight on an SM, a third of what HBM's
+// latency asks for).  Memory bound for prompts (2 bytes in and out per element of q, 2 in and 0.5 out
+// per element of k and v), latency bound for steps: there gridDim.y spreads a row's heads over CTAs so
+// that each group of lanes has one head, loaded before the row's place is looked up (three dependent
+// loads: starts, length, page table).
 //
 // Angles: position * turns (64-bit product) is the angle in turns modulo 1, exact; sine and cosine
 // are formed in double from it, once per row and pair, shared by all heads, and rounded to fp32.
@@ -182,26 +190,54 @@ struct KvAppendArgs {
 // whatever lane computes it and equals the one an elementwise fp32 evaluation gives.
 template <int kLpr, int kTok, bool kBf, bool kVec>
 __global__ void __launch_bounds__(kKvAppendThreads) kv_append_kernel(const KvAppendArgs a) {
-  __shared__ float2 cs[kTok][kKvMaxHd / 2];  // (cos, sin) of the rows' angles
+  // per row and turned dimension e: (cos, sin) of its pair, sin with the sign that its partner enters
+  // with; in the order [e % 8][lane], which a head's lanes read without bank conflicts
+  __shared__ float2 cs[kTok][8][kKvMaxHd / 8];
   __shared__ int64_t place[kTok];
   __shared__ int place_pos[kTok], place_seq[kTok];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  constexpr int kGroups = kKvAppendThreads / kLpr;
+  constexpr int kGroups = kKvAppendThreads / kLpr, kAhead = kTok == 1 ? 1 : 3;
   const int grp = tid / kLpr, c = tid % kLpr;
   const int hd = a.C.hd, kvh = a.C.kv_heads, chunks = hd >> 3;
   const bool on = c < chunks;
   const int heads_all = 2 * kvh + a.heads;  // a row's heads: k, then v, then q
-  const int r0 = blockIdx.x * kTok;
+  const int r0 = blockIdx.x * kTok, rows = min(kTok, a.B.n_tokens - r0);
   const uint32_t gmask = kLpr == 32 ? 0xffffffffu : ((1u << (kLpr & 31)) - 1u) << (lane & ~(kLpr - 1));
 
-  auto load = [&](int r, int h) {
-    const uint16_t* p = h < kvh ? a.k + r * a.ldk + h * hd
-                                : h < 2 * kvh ? a.v + r * a.ldv + (h - kvh) * hd : a.q + r * a.ldq + (h - 2 * kvh) * hd;
+  // this group's heads: (row t, head h) in steps of the CTAs' groups
+  const int step = kGroups * gridDim.y;
+  struct At {
+    int t, h;
+  };
+  const auto advance = [&](At& x) {
+    x.h += step;
+    while (x.h >= heads_all && x.t < rows) {
+      x.h -= heads_all;
+      ++x.t;
+      if (kTok == 1) x.t = rows;  // (one row: its heads are spread over the CTAs)
+    }
+  };
+  const auto load = [&](const At& x) {
+    if (!on || x.t >= rows) return make_uint4(0, 0, 0, 0);
+    const int64_t r = r0 + x.t;
+    const uint16_t* p = x.h < kvh ? a.k + r * a.ldk + x.h * hd
+                                  : x.h < 2 * kvh ? a.v + r * a.ldv + (x.h - kvh) * hd : a.q + r * a.ldq + (x.h - 2 * kvh) * hd;
     return ld_row8<kVec>(p + 8 * c);
   };
-  const int h0 = blockIdx.y * kGroups + grp;
-  uint4 first = make_uint4(0, 0, 0, 0);
-  if (on && h0 < heads_all && r0 < a.B.n_tokens) first = load(r0, h0);
+  At cur{0, static_cast<int>(blockIdx.y) * kGroups + grp}, ahead;
+  while (cur.h >= heads_all && cur.t < rows) {
+    cur.h -= heads_all;
+    cur.t = kTok == 1 ? rows : cur.t + 1;
+  }
+  griddep_wait();
+  griddep_launch_dependents();
+  uint4 raws[kAhead];
+  ahead = cur;
+#pragma unroll
+  for (int i = 0; i < kAhead; ++i) {
+    raws[i] = load(ahead);
+    advance(ahead);
+  }
 
   if (warp < kTok) {
     KvRowPlace p;
@@ -221,116 +257,106 @@ __global__ void __launch_bounds__(kKvAppendThreads) kv_append_kernel(const KvApp
       const uint64_t turn = static_cast<uint64_t>(place_pos[t]) * __ldg(a.turns + j);
       double s, co;  // the signed 64-bit fraction of a turn, in half turns
       sincospi(static_cast<double>(static_cast<int64_t>(turn)) * 0x1p-63, &s, &co);
-      cs[t][j] = make_float2(static_cast<float>(co), static_cast<float>(s));
+      const int e0 = a.interleaved ? 2 * j : j, e1 = a.interleaved ? 2 * j + 1 : j + half;
+      cs[t][e0 & 7][e0 >> 3] = make_float2(static_cast<float>(co), -static_cast<float>(s));
+      cs[t][e1 & 7][e1 >> 3] = make_float2(static_cast<float>(co), static_cast<float>(s));
     }
   }
   __syncthreads();
 
   const int hc = a.rot_dim >> 4;  // lanes holding the first halves of the pairs (not interleaved)
+  const bool turned = on && c < (a.rot_dim >> 3);
+  // the lane with the other half of the pairs
+  const int src = (lane & ~(kLpr - 1)) + (a.interleaved || c >= 2 * hc ? c : c < hc ? c + hc : c - hc);
 #pragma unroll 1
-  for (int t = 0; t < kTok; ++t) {
-    const int r = r0 + t;
-    if (r >= a.B.n_tokens) break;
+  while (cur.t < rows) {
+    const uint4 raw = raws[0];
+#pragma unroll
+    for (int i = 0; i + 1 < kAhead; ++i) raws[i] = raws[i + 1];
+    raws[kAhead - 1] = load(ahead);
+    advance(ahead);
+    const int t = cur.t, h = cur.h;
+    advance(cur);
     // a row without a position is left alone; one without a page is not stored, its q still turned
     if (place_seq[t] < 0 || place_pos[t] < 0) continue;
-    // this lane's eight angles (four when interleaved) are the same for every head
-    float co[8], si[8];
-    const bool turned = on && c < (a.rot_dim >> 3);
-    if (turned) {
+    const int64_t r = r0 + t;
+    float x[8];
+    unpack_halves<kBf>(raw, x);
+    const bool is_v = h >= kvh && h < 2 * kvh;
+    if (!is_v && a.rot_dim) {  // x cos + partner (-+ sin)
+      uint4 other;
+      other.x = __shfl_sync(gmask, raw.x, src);
+      other.y = __shfl_sync(gmask, raw.y, src);
+      other.z = __shfl_sync(gmask, raw.z, src);
+      other.w = __shfl_sync(gmask, raw.w, src);
+      if (a.interleaved) {  // the partners are the neighbours
+        other.x = __funnelshift_l(other.x, other.x, 16);
+        other.y = __funnelshift_l(other.y, other.y, 16);
+        other.z = __funnelshift_l(other.z, other.z, 16);
+        other.w = __funnelshift_l(other.w, other.w, 16);
+      }
+      if (turned) {
+        float y[8];
+        unpack_halves<kBf>(other, y);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = a.interleaved ? 4 * c + (e >> 1) : 8 * (c < hc ? c : c - hc) + e;
-        const float2 v = cs[t][j];
-        co[e] = v.x;
-        si[e] = v.y;
+        for (int e = 0; e < 8; ++e) {  // (one by one: the packed forms are contracted to a fused multiply-add)
+          const float2 f = cs[t][e][c];
+          x[e] = __fadd_rn(__fmul_rn(x[e], f.x), __fmul_rn(y[e], f.y));
+        }
       }
     }
-#pragma unroll 1
-    for (int h = h0; h < heads_all; h += kGroups * gridDim.y) {
-      uint4 raw = make_uint4(0, 0, 0, 0);
-      if (on) raw = (t == 0 && h == h0) ? first : load(r, h);
-      float x[8];
-      unpack_halves<kBf>(raw, x);
-      const bool is_v = h >= kvh && h < 2 * kvh;
-      if (!is_v && a.rot_dim) {
-        if (a.interleaved) {
-          if (turned) {
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const float u = x[e], w = x[e + 1];
-              x[e] = __fsub_rn(__fmul_rn(u, co[e]), __fmul_rn(w, si[e]));
-              x[e + 1] = __fadd_rn(__fmul_rn(w, co[e]), __fmul_rn(u, si[e]));
-            }
-          }
-        } else {  // the other half of the pair is hc lanes away
-          const int src = (lane & ~(kLpr - 1)) + (c < hc ? c + hc : c < 2 * hc ? c - hc : c);
-          uint4 other;
-          other.x = __shfl_sync(gmask, raw.x, src);
-          other.y = __shfl_sync(gmask, raw.y, src);
-          other.z = __shfl_sync(gmask, raw.z, src);
-          other.w = __shfl_sync(gmask, raw.w, src);
-          if (turned) {
-            float y[8];
-            unpack_halves<kBf>(other, y);
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              x[e] = c < hc ? __fsub_rn(__fmul_rn(x[e], co[e]), __fmul_rn(y[e], si[e]))
-                            : __fadd_rn(__fmul_rn(x[e], co[e]), __fmul_rn(y[e], si[e]));
-          }
-        }
-      }
-      if (h >= 2 * kvh) {  // q
-        if (on) {
-          const uint4 w = make_uint4(pack_halves<kBf>(x[0], x[1]), pack_halves<kBf>(x[2], x[3]),
-                                     pack_halves<kBf>(x[4], x[5]), pack_halves<kBf>(x[6], x[7]));
-          st_row8<kVec>(a.q_out + r * a.ldqo + (h - 2 * kvh) * hd + 8 * c, w);
-        }
-        continue;
-      }
-      if (place[t] < 0) continue;
-      // scale, zero and codes of the head
-      float lo = INFINITY, hi = -INFINITY;
-      bool bad = false;
-      if (on) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          lo = fminf(lo, x[e]);
-          hi = fmaxf(hi, x[e]);
-          bad |= !(fabsf(x[e]) < INFINITY);
-        }
-      }
-#pragma unroll
-      for (int o = kLpr / 2; o > 0; o >>= 1) {
-        lo = fminf(lo, __shfl_xor_sync(gmask, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(gmask, hi, o));
-      }
-      bad = (__ballot_sync(gmask, bad) & gmask) != 0;
-      const float big = fmaxf(fabsf(lo), fabsf(hi));
-      const float want = fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), big * 0x1p-10f);
-      const float scale = fmaxf(__half2float(__float2half_rn(want)), 0x1p-24f);
-      bad |= !(scale < INFINITY);
-      const __half zero16 = __float2half_rn(__fdiv_rn(lo, scale));
-      const float zero = __half2float(zero16), inv = __frcp_rn(scale);
-      uint32_t word = 0;
+    if (h >= 2 * kvh) {  // q
+      if (on)
+        st_row8<kVec>(a.q_out + r * a.ldqo + (h - 2 * kvh) * hd + 8 * c,
+                      make_uint4(pack_halves<kBf>(x[0], x[1]), pack_halves<kBf>(x[2], x[3]), pack_halves<kBf>(x[4], x[5]),
+                                 pack_halves<kBf>(x[6], x[7])));
+      continue;
+    }
+    if (place[t] < 0) continue;
+    // scale, zero and codes of the head
+    float lo = INFINITY, hi = -INFINITY;
+    bool bad = false;
+    if (on) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float n = rintf(__fsub_rn(__fmul_rn(x[e], inv), zero));
-        word |= static_cast<uint32_t>(fminf(fmaxf(n, 0.f), 15.f)) << (4 * e);
+        lo = fminf(lo, x[e]);
+        hi = fmaxf(hi, x[e]);
+        bad |= !(fabsf(x[e]) < INFINITY);
       }
-      uint32_t pair = static_cast<uint32_t>(__half_as_ushort(__float2half_rn(scale))) |
-                      (static_cast<uint32_t>(__half_as_ushort(zero16)) << 16);
-      if (bad) {  // an infinity, a NaN, or values beyond the scale's range
-        word = 0;
-        pair = 0x00007fffu;  // scale NaN, zero 0
-      }
-      const int head = is_v ? h - kvh : h;
-      const int off = place_pos[t] & (a.C.page_size - 1);
-      uint8_t* block = a.C.pages + place[t] + head * a.C.head_bytes;
-      const int codes = a.C.page_size * (hd >> 1);
-      if (on) *reinterpret_cast<uint32_t*>(block + (is_v ? codes : 0) + off * (hd >> 1) + 4 * c) = word;
-      if (c == 0)
-        *reinterpret_cast<uint32_t*>(block + 2 * codes + (is_v ? 4 * a.C.page_size : 0) + 4 * off) = pair;
     }
+#pragma unroll
+    for (int o = kLpr / 2; o > 0; o >>= 1) {
+      lo = fminf(lo, __shfl_xor_sync(gmask, lo, o));
+      hi = fmaxf(hi, __shfl_xor_sync(gmask, hi, o));
+    }
+    bad = (__ballot_sync(gmask, bad) & gmask) != 0;
+    const float big = fmaxf(fabsf(lo), fabsf(hi));
+    const float want = fmaxf(__fmul_rn(__fsub_rn(hi, lo), 1.0f / 15.0f), big * 0x1p-10f);
+    const float scale = fmaxf(__half2float(__float2half_rn(want)), 0x1p-24f);
+    bad |= !(scale < INFINITY);
+    const __half zero16 = __float2half_rn(__fdiv_rn(lo, scale));
+    const float zero = __half2float(zero16), inv = __frcp_rn(scale);
+    // code = round(x / scale - zero) clamped: 2^23 + n has n in its low bits, and its other bits add up to
+    // a constant over the word
+    uint32_t word = 0;
+#pragma unroll
+    for (int e = 7; e >= 0; --e) {
+      const float n = fminf(fmaxf(__fsub_rn(__fmul_rn(x[e], inv), zero), 0.f), 15.f);
+      word = word * 16u + __float_as_uint(__fadd_rn(n, 8388608.f));
+    }
+    word -= 0x4b000000u * 0x11111111u;
+    uint32_t pair = static_cast<uint32_t>(__half_as_ushort(__float2half_rn(scale))) |
+                    (static_cast<uint32_t>(__half_as_ushort(zero16)) << 16);
+    if (bad) {  // an infinity, a NaN, or values beyond the scale's range
+      word = 0;
+      pair = 0x00007fffu;  // scale NaN, zero 0
+    }
+    const int head = is_v ? h - kvh : h;
+    const int off = place_pos[t] & (a.C.page_size - 1);
+    uint8_t* block = a.C.pages + place[t] + head * a.C.head_bytes;
+    const int codes = a.C.page_size * (hd >> 1);
+    if (on) *reinterpret_cast<uint32_t*>(block + (is_v ? codes : 0) + off * (hd >> 1) + 4 * c) = word;
+    if (c == 0) *reinterpret_cast<uint32_t*>(block + 2 * codes + (is_v ? 4 * a.C.page_size : 0) + 4 * off) = pair;
   }
 }
 
@@ -350,6 +376,8 @@ __global__ void __launch_bounds__(kKvAppendThreads) kv_read_kernel(const KvReadA
   __shared__ int64_t sm_place;
   __shared__ int sm_off;
   const int tid = threadIdx.x, lane = tid & 31, r = blockIdx.x;
+  griddep_wait();
+  griddep_launch_dependents();
   if (tid < 32) {
     const KvRowPlace p = kv_row_place(a.B, r, lane);
     if (lane == 0) {

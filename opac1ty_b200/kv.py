@@ -25,25 +25,27 @@ import torch
 from . import _lib
 from .layer import _as_cuda_device
 
+_HALVES = {torch.float16: _lib.OPC_F16, torch.bfloat16: _lib.OPC_BF16}
 _DTYPES = {torch.float16: _lib.OPC_F16, torch.bfloat16: _lib.OPC_BF16, torch.float32: _lib.OPC_F32}
 
 
-class _On:
-    """Makes `index` the current device for a call when it is not already."""
+_get_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
 
-    __slots__ = ("want", "prev")
 
-    def __init__(self, index: int):
-        self.want = index
-
-    def __enter__(self):
-        self.prev = torch.cuda.current_device()
-        if self.prev != self.want:
-            torch.cuda.set_device(self.want)
-
-    def __exit__(self, *exc):
-        if self.prev != self.want:
-            torch.cuda.set_device(self.prev)
+def _call(fn, index: int, *args):
+    """fn(*args) with `index` the current device, which the library launches on."""
+    prev = _get_device()
+    if prev == index:
+        rc = fn(*args)
+    else:
+        torch.cuda.set_device(index)
+        try:
+            rc = fn(*args)
+        finally:
+            torch.cuda.set_device(prev)
+    if rc < 0:
+        raise _lib.OpcError(rc, _lib.last_error())
 
 
 _ws_lock = threading.Lock()
@@ -57,11 +59,13 @@ def _workspace(device: torch.device, stream: int, nbytes: int, kind: str) -> tor
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, stream, kind)
-    with _ws_lock:
-        ws = _workspaces.get(key)
-        if ws is None or ws.numel() < nbytes:
-            ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
-        return ws
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        with _ws_lock:
+            ws = _workspaces.get(key)
+            if ws is None or ws.numel() < nbytes:
+                ws = _workspaces[key] = torch.zeros(max(nbytes, 1 << 20), dtype=torch.uint8, device=device)
+    return ws
 
 
 class KVCache:
@@ -123,6 +127,7 @@ class KVBatch:
                               table_stride=max(page_table.stride(0), page_table.shape[1]) if n > 1
                               else page_table.shape[1], max_pages=page_table.shape[1])
         self._ref = ctypes.addressof(self.c)
+        self._need: Dict[Tuple[int, int, int, int], int] = {}  # workspace bytes by (device, heads, kv heads, head_dim)
 
 
 class Rope:
@@ -148,22 +153,21 @@ class Rope:
         self._ref = ctypes.addressof(self.c)
 
 
-def _rows(what: str, name: str, t: torch.Tensor, batch: KVBatch, heads: Optional[int], hd: int, dtype,
-          device) -> Tuple[int, int]:
-    """(leading dimension, heads) of rows t [n_tokens, heads, head_dim] or [n_tokens, heads * head_dim]."""
-    shape = t.shape
-    if t.dim() == 3:
+def _rows(what: str, name: str, t: torch.Tensor, n: int, heads: Optional[int], hd: int, dtype, device) -> Tuple[int, int]:
+    """(leading dimension, heads) of rows t [n, heads, head_dim] or [n, heads * head_dim]."""
+    shape, stride = t.shape, t.stride()
+    if len(shape) == 3:
         h = shape[1]
-        ok = shape[2] == hd and t.stride(2) == 1 and (h == 1 or t.stride(1) == hd)
+        ok = shape[2] == hd and stride[2] == 1 and (h == 1 or stride[1] == hd)
     else:
-        h = shape[1] // hd if t.dim() == 2 else 0
-        ok = t.dim() == 2 and shape[1] == h * hd and t.stride(1) == 1
-    if not ok or h < 1 or shape[0] != batch.n_tokens or (heads is not None and h != heads):
-        raise ValueError(f"{what}: {name} must be [{batch.n_tokens}, {heads if heads is not None else 'heads'}, {hd}] with "
-                         f"contiguous heads, got {tuple(shape)} with strides {t.stride()}")
-    if t.device != device or t.dtype != dtype or dtype not in (torch.float16, torch.bfloat16):
+        h = shape[1] // hd if len(shape) == 2 else 0
+        ok = len(shape) == 2 and shape[1] == h * hd and stride[1] == 1
+    if not ok or h < 1 or shape[0] != n or (heads is not None and h != heads):
+        raise ValueError(f"{what}: {name} must be [{n}, {heads if heads is not None else 'heads'}, {hd}] with "
+                         f"contiguous heads, got {tuple(shape)} with strides {stride}")
+    if t.device != device or t.dtype != dtype or dtype not in _HALVES:
         raise ValueError(f"{what}: {name} must be float16 or bfloat16 like the others on {device}, got {t.dtype} on {t.device}")
-    return (t.stride(0) if shape[0] > 1 else h * hd), h
+    return (stride[0] if n > 1 else h * hd), h
 
 
 def _same_device(what: str, cache: KVCache, batch: KVBatch):
@@ -177,24 +181,23 @@ def append(cache: KVCache, batch: KVBatch, k: torch.Tensor, v: torch.Tensor, q: 
     which may be q, or a new tensor)."""
     hd, dev = cache.head_dim, cache.device
     _same_device("append", cache, batch)
-    ldk, _ = _rows("append", "k", k, batch, cache.kv_heads, hd, k.dtype, dev)
-    ldv, _ = _rows("append", "v", v, batch, cache.kv_heads, hd, k.dtype, dev)
+    ldk, _ = _rows("append", "k", k, batch.n_tokens, cache.kv_heads, hd, k.dtype, dev)
+    ldv, _ = _rows("append", "v", v, batch.n_tokens, cache.kv_heads, hd, k.dtype, dev)
     ldq = ldo = heads = 0
     qp = op = None
     if q is not None:
-        ldq, heads = _rows("append", "q", q, batch, None, hd, k.dtype, dev)
+        ldq, heads = _rows("append", "q", q, batch.n_tokens, None, hd, k.dtype, dev)
         if q_out is None:
             q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        ldo, _ = _rows("append", "q_out", q_out, batch, heads, hd, k.dtype, dev)
+        ldo, _ = _rows("append", "q_out", q_out, batch.n_tokens, heads, hd, k.dtype, dev)
         qp, op = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("append: q_out given without q")
     if rope is not None and rope.device != dev:
         raise ValueError(f"append: the rope is on {rope.device}, the cache on {dev}")
-    with _On(dev.index):
-        _lib.check(_lib.load().opc_kv_append(cache._ref, batch._ref, heads, _DTYPES[k.dtype],
-                                             rope._ref if rope is not None else None, k.data_ptr(), ldk, v.data_ptr(),
-                                             ldv, qp, ldq, op, ldo, torch.cuda.current_stream(dev).cuda_stream))
+    _call(_lib.load().opc_kv_append, dev.index, cache._ref, batch._ref, heads, _DTYPES[k.dtype],
+          rope._ref if rope is not None else None, k.data_ptr(), ldk, v.data_ptr(), ldv, qp, ldq, op, ldo,
+          _raw_stream(dev.index))
     return q_out
 
 
@@ -205,18 +208,24 @@ def read(cache: KVCache, batch: KVBatch, dtype: torch.dtype = torch.float16, k: 
     dev = cache.device
     _same_device("read", cache, batch)
     shape = (batch.n_tokens, cache.kv_heads, cache.head_dim)
-    k = torch.empty(shape, dtype=dtype, device=dev) if k is None else k
-    v = torch.empty(shape, dtype=dtype, device=dev) if v is None else v
-    ldk, _ = _rows("read", "k", k, batch, cache.kv_heads, cache.head_dim, k.dtype, dev)
-    ldv, _ = _rows("read", "v", v, batch, cache.kv_heads, cache.head_dim, k.dtype, dev)
-    with _On(dev.index):
-        _lib.check(_lib.load().opc_kv_read(cache._ref, batch._ref, _DTYPES[k.dtype], k.data_ptr(), ldk, v.data_ptr(), ldv,
-                                           torch.cuda.current_stream(dev).cuda_stream))
+    if k is None and v is None:
+        k, v = torch.empty((2, *shape), dtype=dtype, device=dev)
+    elif k is None or v is None:
+        raise ValueError("read: k and v go together")
+    ldk, _ = _rows("read", "k", k, batch.n_tokens, cache.kv_heads, cache.head_dim, k.dtype, dev)
+    ldv, _ = _rows("read", "v", v, batch.n_tokens, cache.kv_heads, cache.head_dim, k.dtype, dev)
+    _call(_lib.load().opc_kv_read, dev.index, cache._ref, batch._ref, _DTYPES[k.dtype], k.data_ptr(), ldk, v.data_ptr(), ldv,
+          _raw_stream(dev.index))
     return k, v
 
 
 def attention_workspace_bytes(cache: KVCache, batch: KVBatch, heads: int) -> int:
-    return int(_lib.load().opc_kv_attention_workspace_bytes(cache._ref, batch._ref, int(heads), cache.device.index))
+    key = (cache.device.index, heads, cache.kv_heads, cache.head_dim)
+    need = batch._need.get(key)
+    if need is None:
+        need = batch._need[key] = int(_lib.load().opc_kv_attention_workspace_bytes(cache._ref, batch._ref, int(heads),
+                                                                                  cache.device.index))
+    return need
 
 
 def attention(cache: KVCache, batch: KVBatch, q: torch.Tensor, scale: Optional[float] = None,
@@ -227,19 +236,15 @@ def attention(cache: KVCache, batch: KVBatch, q: torch.Tensor, scale: Optional[f
     sequence are not written."""
     hd, dev = cache.head_dim, cache.device
     _same_device("attention", cache, batch)
-    ldq, heads = _rows("attention", "q", q, batch, None, hd, q.dtype, dev)
+    ldq, heads = _rows("attention", "q", q, batch.n_tokens, None, hd, q.dtype, dev)
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    ldo, _ = _rows("attention", "out", out, batch, heads, hd, q.dtype, dev)
+    ldo, _ = _rows("attention", "out", out, batch.n_tokens, heads, hd, q.dtype, dev)
     lse = torch.empty(batch.n_tokens, heads, dtype=torch.float32, device=dev) if return_lse else None
-    lib = _lib.load()
-    with _On(dev.index):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        need = lib.opc_kv_attention_workspace_bytes(cache._ref, batch._ref, heads, dev.index)
-        if workspace is None:
-            workspace = _workspace(dev, stream, need, "kv")
-        _lib.check(lib.opc_kv_attention(cache._ref, batch._ref, heads, _DTYPES[q.dtype],
-                                        hd ** -0.5 if scale is None else float(scale), q.data_ptr(), ldq,
-                                        out.data_ptr(), ldo, lse.data_ptr() if return_lse else None,
-                                        workspace.data_ptr(), workspace.numel(), stream))
+    stream = _raw_stream(dev.index)
+    if workspace is None:
+        workspace = _workspace(dev, stream, attention_workspace_bytes(cache, batch, heads), "kv")
+    _call(_lib.load().opc_kv_attention, dev.index, cache._ref, batch._ref, heads, _DTYPES[q.dtype],
+          hd ** -0.5 if scale is None else float(scale), q.data_ptr(), ldq, out.data_ptr(), ldo,
+          lse.data_ptr() if return_lse else None, workspace.data_ptr(), workspace.numel(), stream)
     return (out, lse) if return_lse else out

@@ -2,12 +2,13 @@
 
 from __future__ import annotations
 
+import functools
 from typing import NamedTuple, Optional
 
 import torch
 
 from . import _lib
-from .kv import _DTYPES, _On, _workspace
+from .kv import _DTYPES, _call, _raw_stream, _workspace
 
 
 class TokenLogprobs(NamedTuple):
@@ -17,6 +18,11 @@ class TokenLogprobs(NamedTuple):
     entropy: Optional[torch.Tensor]       # [rows] fp32
     top_ids: Optional[torch.Tensor]       # [rows, top_k] int32
     top_logprobs: Optional[torch.Tensor]  # [rows, top_k] fp32
+
+
+@functools.lru_cache(maxsize=256)
+def _need(rows: int, vocab: int, top_k: int, device: int) -> int:
+    return int(_lib.load().opc_token_logprobs_workspace_bytes(rows, vocab, top_k, device))
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top_k: int = 0,
@@ -41,14 +47,12 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     ids = torch.empty(rows, top_k, dtype=torch.int32, device=dev) if top_k >= 0 else None
     top = torch.empty(rows, top_k, dtype=torch.float32, device=dev) if top_k >= 0 else None
     lib = _lib.load()
-    with _On(dev.index):
-        stream = torch.cuda.current_stream(dev).cuda_stream
-        if workspace is None:
-            need = lib.opc_token_logprobs_workspace_bytes(rows, vocab, top_k, dev.index)
-            workspace = _workspace(dev, stream, need, "score")
-        _lib.check(lib.opc_token_logprobs(
-            logits.data_ptr(), logits.stride(0) if rows > 1 else vocab, _DTYPES[logits.dtype], rows, vocab,
-            targets.data_ptr() if targets is not None else None, logprob.data_ptr() if logprob is not None else None,
-            ent.data_ptr() if ent is not None else None, top_k, ids.data_ptr() if ids is not None else None,
-            top.data_ptr() if top is not None else None, workspace.data_ptr(), workspace.numel(), stream))
+    stream = _raw_stream(dev.index)
+    if workspace is None:
+        workspace = _workspace(dev, stream, _need(rows, vocab, top_k, dev.index), "score")
+    _call(lib.opc_token_logprobs, dev.index, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
+          _DTYPES[logits.dtype], rows, vocab, targets.data_ptr() if targets is not None else None,
+          logprob.data_ptr() if logprob is not None else None, ent.data_ptr() if ent is not None else None, top_k,
+          ids.data_ptr() if ids is not None else None, top.data_ptr() if top is not None else None,
+          workspace.data_ptr(), workspace.numel(), stream)
     return TokenLogprobs(logprob, ent, ids, top)
