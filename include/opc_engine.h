@@ -98,6 +98,11 @@ typedef struct {
 BFEngine* bf_engine_create(const char* path);
 /* Same, on `device` with `max_context` cache positions (0: the default above). */
 BFEngine* bf_engine_create_ex(const char* path, int32_t device, uint32_t max_context);
+/* Same, with the KV cache held in 4 bits (opc_kv_append, opc_kv_attention in opc_b200.h): pages of
+ * 64 positions, head_dim + 8 bytes per position, kv head and layer for keys and values together
+ * instead of 4 * head_dim -- 3.8 times less memory and attention traffic at head_dim 128.  Every
+ * call below works alike.  Fails for a head_dim that opc_kv_plan refuses. */
+BFEngine* bf_engine_create_kv4(const char* path, int32_t device, uint32_t max_context);
 void bf_engine_destroy(BFEngine* engine);
 const BFModelConfig* bf_engine_get_config(const BFEngine* engine);
 /* Message of the engine's last error, NULL if none (opacc1ty.h:90-93). */
@@ -122,6 +127,13 @@ int bf_engine_forward(BFEngine* engine, const int32_t* tokens, uint32_t seq_len,
 int bf_engine_prefill(BFEngine* engine, const int32_t* tokens, uint32_t seq_len);
 /* Append one token and write the next token's logits.  opacc1ty.h:154-171. */
 int bf_engine_forward_step(BFEngine* engine, int32_t token, float* logits_out, uint32_t vocab_size);
+/* Reset the cache, run all n tokens, and give for each but the last the model's view of the token
+ * that follows it: logprobs[i] = log p(tokens[i + 1] | tokens[0..i]), entropy[i] of that distribution
+ * (natural logarithms), and its top_k (at most 32) most probable tokens with their log probabilities,
+ * top_ids/top_logprobs [n - 1][top_k].  entropy may be NULL, the top arrays with top_k 0.  The cache
+ * holds all n tokens afterwards.  From the fp16 logits that forward() widens (opc_token_logprobs). */
+int bf_engine_score(BFEngine* engine, const int32_t* tokens, uint32_t n, float* logprobs, float* entropy,
+                    int32_t top_k, int32_t* top_ids, float* top_logprobs);
 void bf_engine_reset_kv_cache(BFEngine* engine);
 /* Bytes of the KV cache (allocated at create).  opacc1ty.h:178-181. */
 size_t bf_engine_kv_cache_size(const BFEngine* engine);

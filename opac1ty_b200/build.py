@@ -11,7 +11,7 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
 SOURCES = [CSRC / "opc_lib.cu", CSRC / "opc_engine.cu", CSRC / "opc_kv.cu", CSRC / "opc_score.cu"]
-DEPENDS = sorted(CSRC.glob("*.cu")) + sorted(CSRC.glob("*.cuh")) + sorted(INCLUDE.glob("*.h"))
+DEPENDS = sorted(p for pat in ("*.cu", "*.cuh", "*.h") for p in CSRC.glob(pat)) + sorted(INCLUDE.glob("*.h"))
 OUTPUT = PKG / "libopc_b200.so"
 
 NVCC_FLAGS = [

@@ -330,7 +330,9 @@ def _chain_phases_dataflow(st) -> dict:
 @click.option("--prompt", type=int, default=64, help="prompt tokens (prefill) before the timed steps")
 @click.option("--steps", type=int, default=32, help="timed decode steps")
 @click.option("--svs", type=click.Choice(["1", "8"]), default="1")
-def engine_bench(model, blocks, vocab, prompt, steps, svs):  # noqa: D401
+@click.option("--kv-bits", type=click.Choice(["16", "4"]), default="16", help="KV cache: fp16, or paged in 4 bits")
+@click.option("--context", type=int, default=0, help="cache positions (default: the model's, 4096 at most)")
+def engine_bench(model, blocks, vocab, prompt, steps, svs, kv_bits, context):  # noqa: D401
     """Time the engine API (bf_engine_*) on a synthetic Llama-shaped .bf2: prefill and decode steps
     with attention, norms and the lm_head (host-timed around each call, logits copied back)."""
     import os
@@ -349,9 +351,9 @@ def engine_bench(model, blocks, vocab, prompt, steps, svs):  # noqa: D401
         synthetic.write_llama_bf2(path, cfg, blocks, vocab, sub_vector_size=int(svs))
         t_write = time.time() - t0
         t0 = time.time()
-        with Engine(path) as eng:
+        with Engine(path, max_context=context, kv_bits=int(kv_bits)) as eng:
             t_load = time.time() - t0
-            toks = list(range(1, prompt + 1))
+            toks = [i % vocab for i in range(1, prompt + 1)]
             eng.prefill(toks[:-1])
             eng.forward_step(toks[-1])  # warm
             eng.reset()
@@ -365,11 +367,40 @@ def engine_bench(model, blocks, vocab, prompt, steps, svs):  # noqa: D401
                 eng.forward_step(200 + i)
             t_steps = (time.perf_counter() - t0) / steps
             st = eng.stats()
+            kv_bytes = eng.kv_cache_size
     click.echo(json.dumps({"gpu": get_cuda_device_info().name, "model": model, "svs": int(svs), "blocks": blocks,
-                           "vocab": vocab, "prompt_tokens": prompt, "prefill_ms": t_prefill * 1e3,
-                           "prefill_tok_s": prompt / t_prefill, "step_ms": t_steps * 1e3, "step_tok_s": 1.0 / t_steps,
+                           "vocab": vocab, "kv_bits": int(kv_bits), "kv_bytes": kv_bytes,
+                           "prompt_tokens": prompt, "prefill_ms": t_prefill * 1e3, "prefill_tok_s": prompt / t_prefill, "step_ms": t_steps * 1e3, "step_tok_s": 1.0 / t_steps,
                            "kernel_dispatches_total": st["n_kernel_dispatches"], "device_bytes": st["peak_memory_bytes"],
                            "write_s": round(t_write, 1), "load_s": round(t_load, 1)}))
+
+
+@cli.command()
+@click.argument("bf2_path", type=click.Path(exists=True))
+@click.option("--tokens", default=None, help="token ids, separated by commas or spaces")
+@click.option("--text", default=None, help="text, one token per byte (the engine's stub tokenizer)")
+@click.option("--top", type=int, default=0, help="list this many alternatives for every token")
+@click.option("--kv-bits", type=click.Choice(["16", "4"]), default="16", help="KV cache: fp16, or paged in 4 bits")
+@click.option("--device", type=int, default=0)
+def score(bf2_path, tokens, text, top, kv_bits, device):
+    """Log probability of every token of a text under a .bf2 model, and its perplexity (JSON)."""
+    from .engine import Engine
+
+    if (tokens is None) == (text is None):
+        raise click.UsageError("give either --tokens or --text")
+    try:
+        ids = [int(t) for t in re.split(r"[,\s]+", tokens.strip())] if tokens is not None else list(text.encode())
+    except ValueError:
+        raise click.UsageError("--tokens takes token ids, separated by commas or spaces")
+    if len(ids) < 2:
+        raise click.UsageError("at least two tokens are needed")
+    with Engine(bf2_path, device=device, max_context=len(ids), kv_bits=int(kv_bits)) as eng:
+        s = eng.score(ids, top_k=top)
+    out = {"tokens": len(ids), "kv_bits": int(kv_bits), "mean_logprob": float(s.logprob.mean()), "perplexity": s.perplexity,
+           "mean_entropy": float(s.entropy.mean()), "logprobs": [round(float(v), 5) for v in s.logprob]}
+    if top:
+        out["top"] = [[[int(i), round(float(v), 5)] for i, v in zip(a, b)] for a, b in zip(s.top_ids, s.top_logprobs)]
+    click.echo(json.dumps(out))
 
 
 @cli.command("gemm-bench")

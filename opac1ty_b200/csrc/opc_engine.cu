@@ -2,8 +2,9 @@
 // fused dequant library.  The reference declares the same calls (runtime/include/opacc1ty.h:69-212)
 // and implements them as stubs (runtime/src/inference.c:183-245, bf2_format.c:131-314); this file
 // loads a .bf2 model onto the GPU and runs it.  Projections go through the library's public C ABI
-// (opc_repack_layer, opc_gemv, opc_dequant); the small per-token operations (RMSNorm, rotary
-// embedding, attention over the KV cache, SiLU gating, residual adds) are the kernels below.
+// (opc_repack_layer, opc_gemv, opc_dequant), and so do the 4-bit cache (opc_kv_append,
+// opc_kv_attention) and the scores (opc_token_logprobs); the small per-token operations (RMSNorm, and
+// for the fp16 cache rotary embedding and attention, SiLU gating, residual adds) are the kernels below.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <fcntl.h>
@@ -46,6 +47,11 @@ constexpr int kNormThreads = 512;        // add_rmsnorm_kernel: one CTA per toke
 constexpr int kNormPer = 16;             // values per thread held in registers (rows up to 8192)
 constexpr int kRopeSplit = 4;            // rope_cache_kernel: CTAs per token
 constexpr int kMaxHeadDim = 256;
+constexpr int kKvPage = 64;              // 4-bit cache: positions per page
+constexpr uint32_t kScoreRows = 256;     // rows of logits held at once while scoring
+// The words copied to the device at the start of a chunk: the tokens, the first position, then the
+// description of the one-sequence batch that the 4-bit cache's calls read (q_start[2], kv_len[1]).
+constexpr uint32_t kTokPos = kChunk, kTokStart = kChunk + 1, kTokKvLen = kChunk + 3, kTokWords = kChunk + 4;
 
 // ------------------------------------------------------------------------------------------------
 // .bf2 file (opacc1ty/format/header.py:63-178, bf2.py:78-150): "BF2\0", u32 version, u32 flags,
@@ -569,6 +575,20 @@ struct BFEngine {
   bool graph_tried = false;
   uint32_t step_launches = 0;
   uint32_t direct_steps = 0;  // one-token steps launched directly (the first one sets up the kernels)
+  // 4-bit cache: one opc_kv_cache per layer over one allocation (kcache), pages in order
+  bool kv4 = false;
+  std::vector<opc_kv_cache> kv_layers;
+  int32_t* kv_table = nullptr;
+  int kv_pages = 0;              // per layer
+  opc_rope rope{};
+  void* kv_ws = nullptr;
+  size_t kv_ws_bytes = 0;
+  // scoring (allocated by the first bf_engine_score)
+  __half* score_logits = nullptr;
+  int32_t *score_targets = nullptr, *score_ids = nullptr;
+  float *score_lp = nullptr, *score_entropy = nullptr, *score_top = nullptr;
+  void* score_ws = nullptr;
+  size_t score_ws_bytes = 0;
   std::vector<void*> allocs;
   size_t dev_bytes = 0;
   std::vector<int32_t> history;   // tokens in the cache (repetition penalty)
@@ -833,6 +853,19 @@ const FileLayer* find(const Model& m, const std::string& name) {
   return it == m.layers.end() ? nullptr : &it->second;
 }
 
+// The chunk of n tokens as a batch of one sequence (4-bit cache); its lengths are in d_tokpos.
+opc_kv_batch kv_batch(const BFEngine* e, int n) {
+  opc_kv_batch b{};
+  b.n_seqs = 1;
+  b.n_tokens = b.max_q = n;
+  b.max_kv = static_cast<int32_t>(e->ctx);
+  b.q_start = e->d_tokpos + kTokStart;
+  b.kv_len = e->d_tokpos + kTokKvLen;
+  b.page_table = e->kv_table;
+  b.table_stride = b.max_pages = e->kv_pages;
+  return b;
+}
+
 int load_model(BFEngine* e, const char* path, uint32_t max_context) {
   MappedFile f;
   f.fd = open(path, O_RDONLY);
@@ -962,11 +995,38 @@ int load_model(BFEngine* e, const char* path, uint32_t max_context) {
   }
 
   // ---- KV cache and scratch
-  e->kv_bytes = 2ull * e->n_layers * e->kv_heads * static_cast<size_t>(e->ctx) * e->hd * 2;
   void* kv = nullptr;
-  if (dalloc(e, &kv, e->kv_bytes)) return -1;
-  e->kcache = static_cast<__half*>(kv);
-  e->vcache = e->kcache + e->kv_bytes / 4;
+  if (e->kv4) {
+    e->kv_pages = static_cast<int>((e->ctx + kKvPage - 1) / kKvPage);
+    opc_kv_cache one;
+    ENG_OPC(e, opc_kv_plan(e->kv_heads, e->hd, kKvPage, e->kv_pages, &one));
+    e->kv_bytes = static_cast<size_t>(e->n_layers) * one.total_bytes;
+    if (dalloc(e, &kv, e->kv_bytes)) return -1;
+    e->kcache = static_cast<__half*>(kv);
+    e->kv_layers.assign(e->n_layers, one);
+    for (int l = 0; l < e->n_layers; ++l) e->kv_layers[l].pages = static_cast<char*>(kv) + l * one.total_bytes;
+    std::vector<int32_t> table(e->kv_pages);
+    std::iota(table.begin(), table.end(), 0);
+    void* tb = nullptr;
+    if (dalloc(e, &tb, table.size() * sizeof(int32_t))) return -1;
+    e->kv_table = static_cast<int32_t*>(tb);
+    ENG_CUDA(e, cudaMemcpy(tb, table.data(), table.size() * sizeof(int32_t), cudaMemcpyHostToDevice));
+    std::vector<double> freq(e->hd / 2);
+    for (int i = 0; i < e->hd / 2; ++i) freq[i] = std::pow(static_cast<double>(theta), -2.0 * i / e->hd);
+    std::vector<uint64_t> turns(freq.size());
+    ENG_OPC(e, opc_rope_turns(freq.data(), static_cast<int32_t>(freq.size()), turns.data()));
+    void* tu = nullptr;
+    if (dalloc(e, &tu, turns.size() * sizeof(uint64_t))) return -1;
+    ENG_CUDA(e, cudaMemcpy(tu, turns.data(), turns.size() * sizeof(uint64_t), cudaMemcpyHostToDevice));
+    e->rope.rot_dim = e->hd;
+    e->rope.interleaved = 0;
+    e->rope.turns = static_cast<const uint64_t*>(tu);
+  } else {
+    e->kv_bytes = 2ull * e->n_layers * e->kv_heads * static_cast<size_t>(e->ctx) * e->hd * 2;
+    if (dalloc(e, &kv, e->kv_bytes)) return -1;
+    e->kcache = static_cast<__half*>(kv);
+    e->vcache = e->kcache + e->kv_bytes / 4;
+  }
   ENG_CUDA(e, cudaMemset(kv, 0, e->kv_bytes));
   e->ld_x = pad8(e->hidden);
   e->ld_q = pad8(qd);
@@ -1006,10 +1066,18 @@ int load_model(BFEngine* e, const char* path, uint32_t max_context) {
   if (dalloc(e, &lp, static_cast<size_t>(e->vocab) * 2)) return -1;
   e->logits16 = static_cast<__half*>(lp);
   ENG_CUDA(e, cudaMallocHost(reinterpret_cast<void**>(&e->host_logits), static_cast<size_t>(e->vocab) * 2));
-  ENG_CUDA(e, cudaMallocHost(reinterpret_cast<void**>(&e->h_tokpos), (kChunk + 1) * sizeof(int32_t)));
+  ENG_CUDA(e, cudaMallocHost(reinterpret_cast<void**>(&e->h_tokpos), kTokWords * sizeof(int32_t)));
   void* tp = nullptr;
-  if (dalloc(e, &tp, (kChunk + 1) * sizeof(int32_t))) return -1;
+  if (dalloc(e, &tp, kTokWords * sizeof(int32_t))) return -1;
   e->d_tokpos = static_cast<int32_t*>(tp);
+  if (e->kv4) {  // one attention workspace for every chunk size
+    for (int n = 1; n <= static_cast<int>(kChunk); ++n) {
+      const opc_kv_batch b = kv_batch(e, n);
+      e->kv_ws_bytes = std::max(e->kv_ws_bytes, opc_kv_attention_workspace_bytes(&e->kv_layers[0], &b, e->heads, e->device));
+    }
+    if (dalloc(e, &e->kv_ws, e->kv_ws_bytes)) return -1;
+    ENG_OPC(e, opc_workspace_init(e->kv_ws, e->kv_ws_bytes, e->stream));
+  }
 
   // one workspace for every projection and chunk size (calls are ordered on the engine's stream)
   std::vector<const DevLayer*> all;
@@ -1041,9 +1109,16 @@ cudaError_t launch_norm(cudaStream_t s, int rows, float* h, int hidden, const __
   return launch_pdl(k, dim3(rows), dim3(kNormThreads), s, h, hidden, y, ldy, row0, w, eps, out, ldo);
 }
 
-int enqueue_chunk(BFEngine* e, int n, bool want_logits, uint32_t* n_launches) {
+// What a chunk is to give: nothing, the last token's logits, or the scores of its first `score`
+// tokens against the targets already in score_targets.
+struct Want {
+  bool logits = false;
+  int score = 0, top_k = 0;
+};
+
+int enqueue_chunk(BFEngine* e, int n, const Want& want, uint32_t* n_launches) {
   cudaStream_t s = e->stream;
-  const int32_t* pos0 = e->d_tokpos + kChunk;
+  const int32_t* pos0 = e->d_tokpos + kTokPos;
   const int qd = e->heads * e->hd;
   uint32_t launches = 0;
   auto gemv = [&](const DevLayer& d, const __half* x, int ldx, __half* y, int ldy, int rows) -> int {
@@ -1060,7 +1135,7 @@ int enqueue_chunk(BFEngine* e, int n, bool want_logits, uint32_t* n_launches) {
     }
     return 0;
   };
-  ENG_CUDA(e, cudaMemcpyAsync(e->d_tokpos, e->h_tokpos, (kChunk + 1) * sizeof(int32_t), cudaMemcpyHostToDevice, s));
+  ENG_CUDA(e, cudaMemcpyAsync(e->d_tokpos, e->h_tokpos, kTokWords * sizeof(int32_t), cudaMemcpyHostToDevice, s));
   embed_kernel<<<n, 256, 0, s>>>(e->embed_table, e->hidden, e->d_tokpos, e->h);
   ++launches;
   const __half* res = nullptr;  // the previous block's down projection, still to be added into h
@@ -1068,8 +1143,8 @@ int enqueue_chunk(BFEngine* e, int n, bool want_logits, uint32_t* n_launches) {
   const unsigned silu_grid = static_cast<unsigned>(std::min<int64_t>((silu_n + 255) / 256, 4 * 148));
   for (int l = 0; l < e->n_layers; ++l) {
     const Block& B = e->blocks[l];
-    __half* kc = e->kcache + static_cast<size_t>(l) * e->kv_heads * e->ctx * e->hd;
-    __half* vc = e->vcache + static_cast<size_t>(l) * e->kv_heads * e->ctx * e->hd;
+    const size_t layer_at = static_cast<size_t>(l) * e->kv_heads * e->ctx * e->hd;  // (of the fp16 cache)
+    __half *kc = e->kv4 ? nullptr : e->kcache + layer_at, *vc = e->kv4 ? nullptr : e->vcache + layer_at;
     ENG_CUDA(e, launch_norm(s, n, e->h, e->hidden, res, e->ld_y, 0, B.ln_in, e->eps, e->xn, e->ld_x));
     __half *qb = e->q, *kb = e->k, *vb = e->v;
     int ldq = e->ld_q, ldkv = e->ld_kv;
@@ -1083,11 +1158,19 @@ int enqueue_chunk(BFEngine* e, int n, bool want_logits, uint32_t* n_launches) {
                gemv(B.v, e->xn, e->ld_x, e->v, e->ld_kv, n)) {
       return -1;
     }
-    ENG_CUDA(e, launch_pdl(rope_cache_kernel, dim3(n, kRopeSplit), dim3(256), s, qb, ldq, kb, vb, ldkv, e->heads,
-                           e->kv_heads, e->hd, pos0, e->cfg.rope_theta, kc, vc, static_cast<int>(e->ctx)));
-    ENG_CUDA(e, launch_pdl(attention_kernel, dim3(e->heads, n, attention_splits(n, e->heads)), dim3(kAttnThreads), s, qb, ldq, kc, vc,
-                           e->heads, e->kv_heads, e->hd, static_cast<int>(e->ctx), pos0, e->att, e->ld_q,
-                           e->att_part, e->att_count));
+    if (e->kv4) {
+      const opc_kv_batch batch = kv_batch(e, n);
+      const opc_kv_cache* cache = &e->kv_layers[l];
+      ENG_OPC(e, opc_kv_append(cache, &batch, e->heads, OPC_F16, &e->rope, kb, ldkv, vb, ldkv, qb, ldq, qb, ldq, s));
+      ENG_OPC(e, opc_kv_attention(cache, &batch, e->heads, OPC_F16, 1.0f / std::sqrt(static_cast<float>(e->hd)), qb, ldq, e->att,
+                                  e->ld_q, nullptr, e->kv_ws, e->kv_ws_bytes, s));
+    } else {
+      ENG_CUDA(e, launch_pdl(rope_cache_kernel, dim3(n, kRopeSplit), dim3(256), s, qb, ldq, kb, vb, ldkv, e->heads,
+                             e->kv_heads, e->hd, pos0, e->cfg.rope_theta, kc, vc, static_cast<int>(e->ctx)));
+      ENG_CUDA(e, launch_pdl(attention_kernel, dim3(e->heads, n, attention_splits(n, e->heads)), dim3(kAttnThreads), s, qb, ldq, kc, vc,
+                             e->heads, e->kv_heads, e->hd, static_cast<int>(e->ctx), pos0, e->att, e->ld_q,
+                             e->att_part, e->att_count));
+    }
     if (gemv(B.o, e->att, e->ld_q, e->y, e->ld_y, n)) return -1;
     ENG_CUDA(e, launch_norm(s, n, e->h, e->hidden, e->y, e->ld_y, 0, B.ln_post, e->eps, e->xn, e->ld_x));
     if (B.gu.present) {  // one GEMV for gate|up
@@ -1104,7 +1187,22 @@ int enqueue_chunk(BFEngine* e, int n, bool want_logits, uint32_t* n_launches) {
     launches += 5;  // two RMSNorms (each with the residual add before it), rotary + cache append, attention, SiLU
   }
 
-  if (want_logits) {  // the last residual add and the final norm, for the chunk's last token only
+  if (want.score) {  // the final norm of every scored token, then logits and scores kScoreRows at a time
+    ENG_CUDA(e, launch_norm(s, want.score, e->h, e->hidden, res, e->ld_y, 0, e->final_norm, e->eps, e->xn, e->ld_x));
+    ++launches;
+    const int ldl = pad8(e->vocab);
+    for (int r = 0; r < want.score; r += static_cast<int>(kScoreRows)) {
+      const int m = std::min(want.score - r, static_cast<int>(kScoreRows));
+      if (gemv(e->lm_from_embed ? e->embed : e->lm_head, e->xn + static_cast<size_t>(r) * e->ld_x, e->ld_x, e->score_logits, ldl, m))
+        return -1;
+      ++launches;
+      ENG_OPC(e, opc_token_logprobs(e->score_logits, ldl, OPC_F16, m, e->vocab, e->score_targets + r, e->score_lp + r,
+                                    e->score_entropy + r, want.top_k, e->score_ids + static_cast<size_t>(r) * want.top_k,
+                                    e->score_top + static_cast<size_t>(r) * want.top_k, e->score_ws, e->score_ws_bytes, s));
+      ++launches;
+    }
+  }
+  if (want.logits) {  // the last residual add and the final norm, for the chunk's last token only
     ENG_CUDA(e, launch_norm(s, 1, e->h, e->hidden, res, e->ld_y, n - 1, e->final_norm, e->eps, e->xn, e->ld_x));
     ++launches;
     if (gemv(e->lm_from_embed ? e->embed : e->lm_head, e->xn, e->ld_x, e->logits16, e->vocab, 1)) return -1;
@@ -1127,7 +1225,9 @@ void capture_step(BFEngine* e) {
   }
   const std::string saved = e->error;
   uint32_t launches = 0;
-  const int rc = enqueue_chunk(e, 1, true, &launches);
+  Want want;
+  want.logits = true;
+  const int rc = enqueue_chunk(e, 1, want, &launches);
   const cudaError_t ce = cudaStreamEndCapture(e->stream, &g);
   if (rc == 0 && ce == cudaSuccess && g && cudaGraphInstantiate(&e->step_exec, g, 0) == cudaSuccess) {
     e->step_launches = launches;
@@ -1139,17 +1239,24 @@ void capture_step(BFEngine* e) {
   cudaGetLastError();
 }
 
-int run_chunk(BFEngine* e, const int32_t* tokens, int n, float* logits) {
+int run_chunk(BFEngine* e, const int32_t* tokens, int n, float* logits, int score = 0, int top_k = 0) {
   cudaStream_t s = e->stream;
   for (int i = 0; i < n; ++i) e->h_tokpos[i] = tokens[i];
-  e->h_tokpos[kChunk] = static_cast<int32_t>(e->pos);
+  e->h_tokpos[kTokPos] = static_cast<int32_t>(e->pos);
+  e->h_tokpos[kTokStart] = 0;
+  e->h_tokpos[kTokStart + 1] = n;
+  e->h_tokpos[kTokKvLen] = static_cast<int32_t>(e->pos) + n;
   uint32_t launches = 0;
   if (n == 1 && logits && !e->graph_tried && e->direct_steps > 0) capture_step(e);
   if (n == 1 && logits && e->step_exec) {
     ENG_CUDA(e, cudaGraphLaunch(e->step_exec, s));
     launches = e->step_launches;
   } else {
-    if (enqueue_chunk(e, n, logits != nullptr, &launches)) return -1;
+    Want want;
+    want.logits = logits != nullptr;
+    want.score = score;
+    want.top_k = top_k;
+    if (enqueue_chunk(e, n, want, &launches)) return -1;
     if (n == 1 && logits) ++e->direct_steps;
   }
   ENG_CUDA(e, cudaStreamSynchronize(s));
@@ -1183,6 +1290,28 @@ int run_tokens(BFEngine* e, const int32_t* tokens, uint32_t n, float* logits) {
     if (run_chunk(e, tokens + i, c, (logits && i + c == n) ? logits : nullptr)) return -1;
   }
   e->stats.total_time_seconds += std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
+  return 0;
+}
+
+// The buffers of bf_engine_score, at its first call.
+int score_buffers(BFEngine* e) {
+  if (e->score_logits) return 0;
+  void *lg = nullptr, *tg = nullptr, *id = nullptr, *f = nullptr;
+  const int most = std::min(32, e->vocab);
+  if (dalloc(e, &lg, static_cast<size_t>(kScoreRows) * pad8(e->vocab) * 2) || dalloc(e, &tg, kChunk * sizeof(int32_t)) ||
+      dalloc(e, &id, static_cast<size_t>(kChunk) * 32 * sizeof(int32_t)) ||
+      dalloc(e, &f, static_cast<size_t>(kChunk) * 34 * sizeof(float)))
+    return -1;
+  for (uint32_t m = 1; m <= kScoreRows; ++m)
+    e->score_ws_bytes = std::max(e->score_ws_bytes, opc_token_logprobs_workspace_bytes(static_cast<int32_t>(m), e->vocab, most, e->device));
+  if (dalloc(e, &e->score_ws, e->score_ws_bytes)) return -1;
+  ENG_OPC(e, opc_workspace_init(e->score_ws, e->score_ws_bytes, e->stream));
+  e->score_targets = static_cast<int32_t*>(tg);
+  e->score_ids = static_cast<int32_t*>(id);
+  e->score_lp = static_cast<float*>(f);
+  e->score_entropy = e->score_lp + kChunk;
+  e->score_top = e->score_entropy + kChunk;
+  e->score_logits = static_cast<__half*>(lg);
   return 0;
 }
 
@@ -1255,11 +1384,12 @@ int32_t sample_token(const std::vector<float>& logits_in, const BFSamplingParams
 // ------------------------------------------------------------------------------------------------
 extern "C" {
 
-BFEngine* bf_engine_create_ex(const char* path, int32_t device, uint32_t max_context) {
+static BFEngine* create_engine(const char* path, int32_t device, uint32_t max_context, bool kv4) {
   if (!path) return nullptr;
   BFEngine* e = new (std::nothrow) BFEngine();
   if (!e) return nullptr;
   e->device = device;
+  e->kv4 = kv4;
   if (load_model(e, path, max_context) != 0) {
     // keep the message; release what was allocated (the handle stays, as in the reference)
     const std::string msg = e->error;
@@ -1276,6 +1406,13 @@ BFEngine* bf_engine_create_ex(const char* path, int32_t device, uint32_t max_con
     e->error = msg.empty() ? "load failed" : msg;
   }
   return e;
+}
+
+BFEngine* bf_engine_create_ex(const char* path, int32_t device, uint32_t max_context) {
+  return create_engine(path, device, max_context, false);
+}
+BFEngine* bf_engine_create_kv4(const char* path, int32_t device, uint32_t max_context) {
+  return create_engine(path, device, max_context, true);
 }
 
 BFEngine* bf_engine_create(const char* path) { return bf_engine_create_ex(path, 0, 0); }
@@ -1321,6 +1458,40 @@ int bf_engine_forward_step(BFEngine* e, int32_t token, float* logits_out, uint32
   if (vocab_size != e->cfg.vocab_size) return fail(e, "logits buffer holds %u values, the vocabulary %u", vocab_size, e->cfg.vocab_size);
   e->error.clear();
   return run_tokens(e, &token, 1, logits_out);
+}
+
+int bf_engine_score(BFEngine* e, const int32_t* tokens, uint32_t n, float* logprobs, float* entropy, int32_t top_k,
+                    int32_t* top_ids, float* top_logprobs) {
+  if (ready(e)) return -1;
+  if (!tokens || n == 0) return fail(e, "bf_engine_score: no tokens");
+  if (n > 1 && !logprobs) return fail(e, "bf_engine_score: NULL logprobs");
+  if (top_k < 0 || top_k > 32 || top_k > e->vocab) return fail(e, "bf_engine_score: top_k %d (at most 32 and the vocabulary of %d)", top_k, e->vocab);
+  if (top_k > 0 && (!top_ids || !top_logprobs)) return fail(e, "bf_engine_score: top_k %d without its arrays", top_k);
+  bf_engine_reset_kv_cache(e);
+  e->error.clear();
+  if (n > e->ctx) return fail(e, "context full: %u tokens exceed the %u-position cache", n, e->ctx);
+  for (uint32_t i = 0; i < n; ++i)
+    if (tokens[i] < 0 || tokens[i] >= e->vocab) return fail(e, "token id %d outside [0, %d)", tokens[i], e->vocab);
+  cudaSetDevice(e->device);
+  if (score_buffers(e)) return -1;
+  const auto t0 = std::chrono::steady_clock::now();
+  for (uint32_t i = 0; i < n; i += kChunk) {
+    const int c = static_cast<int>(std::min<uint32_t>(kChunk, n - i));
+    const int m = i + c < n ? c : c - 1;  // the last token has no successor
+    if (m > 0) ENG_CUDA(e, cudaMemcpyAsync(e->score_targets, tokens + i + 1, m * sizeof(int32_t), cudaMemcpyHostToDevice, e->stream));
+    if (run_chunk(e, tokens + i, c, nullptr, m, top_k)) return -1;
+    if (m > 0) {
+      ENG_CUDA(e, cudaMemcpy(logprobs + i, e->score_lp, m * sizeof(float), cudaMemcpyDeviceToHost));
+      if (entropy) ENG_CUDA(e, cudaMemcpy(entropy + i, e->score_entropy, m * sizeof(float), cudaMemcpyDeviceToHost));
+      if (top_k) {
+        const size_t at = static_cast<size_t>(i) * top_k, k = static_cast<size_t>(m) * top_k;
+        ENG_CUDA(e, cudaMemcpy(top_ids + at, e->score_ids, k * sizeof(int32_t), cudaMemcpyDeviceToHost));
+        ENG_CUDA(e, cudaMemcpy(top_logprobs + at, e->score_top, k * sizeof(float), cudaMemcpyDeviceToHost));
+      }
+    }
+  }
+  e->stats.total_time_seconds += std::chrono::duration<double>(std::chrono::steady_clock::now() - t0).count();
+  return 0;
 }
 
 int32_t bf_engine_generate_tokens(BFEngine* e, const int32_t* prompt, uint32_t prompt_len, uint32_t max_new_tokens,

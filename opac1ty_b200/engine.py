@@ -11,7 +11,7 @@ reference's C runtime, runtime/include/opacc1ty.h:69-212, implemented in
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Sequence
+from typing import NamedTuple, Optional, Sequence
 
 import numpy as np
 
@@ -61,6 +61,7 @@ _F32P = ctypes.POINTER(ctypes.c_float)
 PROTOTYPES = {
     "bf_engine_create": (_P, [ctypes.c_char_p]),
     "bf_engine_create_ex": (_P, [ctypes.c_char_p, ctypes.c_int32, ctypes.c_uint32]),
+    "bf_engine_create_kv4": (_P, [ctypes.c_char_p, ctypes.c_int32, ctypes.c_uint32]),
     "bf_engine_destroy": (None, [_P]),
     "bf_engine_get_config": (ctypes.POINTER(ModelConfig), [_P]),
     "bf_engine_get_error": (ctypes.c_char_p, [_P]),
@@ -71,6 +72,7 @@ PROTOTYPES = {
     "bf_engine_forward": (ctypes.c_int, [_P, _I32P, ctypes.c_uint32, _F32P, ctypes.c_uint32]),
     "bf_engine_prefill": (ctypes.c_int, [_P, _I32P, ctypes.c_uint32]),
     "bf_engine_forward_step": (ctypes.c_int, [_P, ctypes.c_int32, _F32P, ctypes.c_uint32]),
+    "bf_engine_score": (ctypes.c_int, [_P, _I32P, ctypes.c_uint32, _F32P, _F32P, ctypes.c_int32, _I32P, _F32P]),
     "bf_engine_reset_kv_cache": (None, [_P]),
     "bf_engine_kv_cache_size": (ctypes.c_size_t, [_P]),
     "bf_engine_position": (ctypes.c_uint32, [_P]),
@@ -110,12 +112,29 @@ def _i32(tokens: Sequence[int]) -> np.ndarray:
     return np.ascontiguousarray(np.asarray(tokens, dtype=np.int32).reshape(-1))
 
 
-class Engine:
-    """One loaded .bf2 model on one GPU (``bf_engine_create_ex``)."""
+class Score(NamedTuple):
+    """What the model thinks of each token but the first (``bf_engine_score``)."""
 
-    def __init__(self, path: str, device: int = 0, max_context: int = 0):
+    logprob: np.ndarray       # [n - 1] float32
+    entropy: np.ndarray       # [n - 1] float32
+    top_ids: np.ndarray       # [n - 1, top_k] int32
+    top_logprobs: np.ndarray  # [n - 1, top_k] float32
+
+    @property
+    def perplexity(self) -> float:
+        return float(np.exp(-self.logprob.astype(np.float64).mean())) if self.logprob.size else float("nan")
+
+
+class Engine:
+    """One loaded .bf2 model on one GPU (``bf_engine_create_ex``; ``kv_bits`` 4: ``bf_engine_create_kv4``)."""
+
+    def __init__(self, path: str, device: int = 0, max_context: int = 0, kv_bits: int = 16):
+        self._h = None
+        if kv_bits not in (4, 16):
+            raise ValueError(f"Engine: kv_bits must be 16 or 4, got {kv_bits}")
         self._L = lib()
-        self._h = self._L.bf_engine_create_ex(str(path).encode(), int(device), int(max_context))
+        create = self._L.bf_engine_create_kv4 if kv_bits == 4 else self._L.bf_engine_create_ex
+        self._h = create(str(path).encode(), int(device), int(max_context))
         if not self._h:
             raise EngineError("bf_engine_create returned NULL")
         err = self._L.bf_engine_get_error(self._h)
@@ -149,6 +168,18 @@ class Engine:
         self._check(self._L.bf_engine_forward_step(self._h, int(token), out.ctypes.data_as(_F32P), self.vocab_size),
                     "bf_engine_forward_step")
         return out
+
+    def score(self, tokens: Sequence[int], top_k: int = 0) -> Score:
+        """Log probability, entropy and the top_k alternatives of every token but the first, given the
+        ones before it (starts from an empty cache, which holds all of them afterwards)."""
+        t = _i32(tokens)
+        n = max(t.size - 1, 0)
+        k = max(int(top_k), 0)
+        s = Score(np.empty(n, np.float32), np.empty(n, np.float32), np.empty((n, k), np.int32), np.empty((n, k), np.float32))
+        self._check(self._L.bf_engine_score(self._h, t.ctypes.data_as(_I32P), t.size, s.logprob.ctypes.data_as(_F32P),
+                                            s.entropy.ctypes.data_as(_F32P), int(top_k), s.top_ids.ctypes.data_as(_I32P),
+                                            s.top_logprobs.ctypes.data_as(_F32P)), "bf_engine_score")
+        return s
 
     def generate_tokens(self, prompt: Sequence[int], max_new_tokens: int, temperature: float = 0.0,
                         top_p: float = 0.0, top_k: int = 0, repetition_penalty: float = 1.0, seed: int = 0) -> list:
