@@ -191,11 +191,15 @@ cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, int threads, int smem,
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     const std::pair<const void*, int> key(reinterpret_cast<const void*>(kern), dev);
-    std::lock_guard<std::mutex> lk(mu);
-    if (!done.count(key)) {
-      e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-      if (e != cudaSuccess) return e;
-      done.insert(key);
+    try {  // (no exception leaves a C entry)
+      std::lock_guard<std::mutex> lk(mu);
+      if (!done.count(key)) {
+        e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        done.insert(key);
+      }
+    } catch (...) {
+      return cudaErrorMemoryAllocation;
     }
   }
   cudaLaunchConfig_t cfg = {};

@@ -358,7 +358,7 @@ int fail(int code, const char* fmt, ...) {
 
 int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
 
-int current_device(Device* out) {
+int current_device(Device* out) try {
   int dev = 0;
   OPC_CUDA(cudaGetDevice(&dev), "cudaGetDevice");
   DeviceCache dc;
@@ -375,6 +375,8 @@ int current_device(Device* out) {
   out->max_smem_optin = dc.max_smem_optin;
   out->error_word = word;
   return OPC_OK;
+} catch (...) {  // (no exception leaves a C entry)
+  return fail(OPC_ERR_CUDA, "no memory for what is known of the device");
 }
 
 }  // namespace opc_host

@@ -207,3 +207,30 @@ def test_captured_graph_replays_on_new_logits(cuda_device):
         g.replay()
         torch.cuda.synchronize()
         check(x, t.tolist(), 4, r)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16, F32])
+@pytest.mark.parametrize("ld,off", [(50003, 0), (50001, 1), (50008, 3)])
+def test_few_long_rows_in_strided_logits(cuda_device, dtype, ld, off):
+    """Rows of 50001 with odd strides and starts, few enough to be divided over CTAs."""
+    flat = torch.randn(3 * ld + 8, generator=torch.Generator().manual_seed(ld)).mul(3).to(dtype).to(cuda_device)
+    x = flat.as_strided((3, 50001), (ld, 1), off)
+    t = [0, 50000, 777]
+    check(x, t, 32, token_logprobs(x, torch.tensor(t, dtype=torch.int32, device=cuda_device), top_k=32))
+
+
+def test_calls_on_two_streams_at_once(cuda_device):
+    xs = [torch.randn(2, 60000, generator=torch.Generator().manual_seed(i)).half().to(cuda_device) for i in range(2)]
+    t = torch.tensor([3, 4], dtype=torch.int32, device=cuda_device)
+    want = [token_logprobs(x, t, top_k=9) for x in xs]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], [[], []]
+    for _ in range(10):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(token_logprobs(xs[i], t, top_k=9))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for r in got[i]:
+            assert torch.equal(r.logprob, want[i].logprob) and torch.equal(r.top_ids, want[i].top_ids)
+            assert torch.equal(r.entropy, want[i].entropy) and torch.equal(r.top_logprobs, want[i].top_logprobs)
