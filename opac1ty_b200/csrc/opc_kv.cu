@@ -130,8 +130,8 @@ struct AttentionPlan {
   int step_nt;          // row tiles of the step kernel, 0: not launched
   int step_q;           // the step kernel takes sequences of at most this many rows
   int step_grid;
-  int pairs;            // row tile groups of the longest sequence in the prompt kernel, 0: not launched
-  int splits, tiles;    // CTAs per row tile group, key tiles of each
+  int64_t prompt_grid;  // 0: the prompt kernel is not launched
+  int prompt_ctas;      // CTAs that may share their items' keys
   size_t bytes;         // workspace: the counters, then the records (of one kernel after the other)
 };
 
@@ -149,17 +149,19 @@ AttentionPlan plan_attention(const opc_kv_cache& c, const opc_kv_batch& b, int g
     p.bytes += static_cast<size_t>(p.step_grid) * 2 * (p.step_q * group) * (c.head_dim + 4) * 4;
   }
   if (b.max_q > p.step_q) {
+    // At most this many tile pairs: the rows of all sequences, and one that is not full for each.
     const int64_t rows = static_cast<int64_t>(opc::kv_p_qt(c.head_dim)) * opc::kKvPM;
     const int64_t pairs = (static_cast<int64_t>(b.max_q) * group + rows - 1) / rows;
-    const int64_t items = std::max<int64_t>(1, pairs * c.kv_heads * std::max(b.n_seqs, 1));
-    const int64_t tiles = std::max<int64_t>(1, (static_cast<int64_t>(b.max_kv) + opc::kKvPN - 1) / opc::kKvPN);
-    // Fewer row tile groups than SMs are split over the keys, down to two tiles for each CTA.
-    const int64_t splits = std::max<int64_t>(1, std::min(sms / items, tiles / 2));
-    p.pairs = static_cast<int>(std::min<int64_t>(pairs, INT32_MAX / splits));
-    p.tiles = static_cast<int>((tiles + splits - 1) / splits);
-    p.splits = static_cast<int>((tiles + p.tiles - 1) / p.tiles);
-    if (p.splits > 1)
-      p.bytes = std::max(p.bytes, kCounterBytes + static_cast<size_t>(items) * p.splits * rows * (c.head_dim + 4) * 4);
+    const int64_t all = std::min(pairs * b.n_seqs, static_cast<int64_t>(b.n_tokens) * group / rows +
+                                                       std::min(b.n_seqs, b.n_tokens / (p.step_q + 1)));
+    p.prompt_grid = std::max<int64_t>(1, all * c.kv_heads);
+    // Fewer items than SMs share their keys, down to two tiles for each CTA.
+    p.prompt_ctas = 1;
+    if (b.max_kv > 3 * opc::kKvPN) {
+      p.prompt_ctas = std::min<int>(sms, kCounterBytes / 4);
+      p.prompt_grid = std::max<int64_t>(p.prompt_grid, p.prompt_ctas);
+      p.bytes = std::max(p.bytes, kCounterBytes + static_cast<size_t>(p.prompt_ctas) * rows * (c.head_dim + 4) * 4);
+    }
   }
   return p;
 }
@@ -362,12 +364,16 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
   if (static_cast<double>(batch->n_seqs) * cache->kv_heads * (batch->max_kv / opc::kKvStage + 2) > 4e9)
     return fail(OPC_ERR_INVALID, "%s: %d sequences of up to %d keys over %d kv heads are too many for one call", who,
                 batch->n_seqs, batch->max_kv, cache->kv_heads);
+  // (rows are counted in 32 bits)
+  if (static_cast<int64_t>(batch->n_tokens) * group > INT32_MAX - 1024)
+    return fail(OPC_ERR_INVALID, "%s: %d tokens of %d heads per kv head are too many for one call", who, batch->n_tokens, group);
   AttentionPlan p = plan_attention(*cache, *batch, group, dev.sm_count);
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.bytes)
     return fail(OPC_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", who, p.bytes, workspace_bytes);
   opc::KvAttnArgs a;
   a.C = geom_of(*cache);
   a.B = rows_of(*batch, *cache, dev.error_word);
+  a.B.max_q = std::min(a.B.max_q, batch->n_tokens);
   a.q = static_cast<const uint16_t*>(q);
   a.out = static_cast<uint16_t*>(out);
   a.lse = lse;
@@ -390,15 +396,16 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
     KV_CUDA(launch_pdl(kern, dim3(p.step_grid), opc::kKvStepThreads, opc::kv_step_smem(cache->head_dim, p.step_nt), s, a, sp),
             "opc_kv_attention launch (steps)");
   }
-  if (p.pairs) {
+  if (p.prompt_grid) {
+    if (p.prompt_grid > INT32_MAX)
+      return fail(OPC_ERR_INVALID, "%s: %d tokens of %d heads are too many for one call", who, batch->n_tokens, heads);
     a.lo_q = p.step_q + 1;
     a.hi_q = a.B.max_q;
     opc::KvPromptSplit sp;
-    sp.tiles = p.tiles;
-    sp.splits = p.splits;
+    sp.ctas = static_cast<uint32_t>(p.prompt_ctas);
     sp.count = static_cast<int32_t*>(workspace);
     sp.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCounterBytes);
-    KV_CUDA(launch_pdl(prompt_of(cache->head_dim), dim3(p.pairs * p.splits, cache->kv_heads, batch->n_seqs), opc::kKvPThreads,
+    KV_CUDA(launch_pdl(prompt_of(cache->head_dim), dim3(static_cast<unsigned>(p.prompt_grid)), opc::kKvPThreads,
                        opc::kv_p_smem(cache->head_dim), s, a, sp),
             "opc_kv_attention launch (prompts)");
   }

@@ -27,20 +27,31 @@ namespace opc {
 //                 The reference m of a row moves only when the sum of a half's weights says that one
 //                 times the tile's largest scale_v may pass 2^12: then the row's maximum is looked for,
 //                 O rescaled and the half evaluated again -- always in the first tile, hardly ever later.
-//   warps 16..19  thread = key: reads its codes (one tile ahead, in registers), writes K' and V' rows in
-//                 the 128-byte-swizzled layout -- the same bytes are K-major for K' (rows are the N
-//                 dimension) and MN-major for V' (rows are the K dimension)
-//   warp 20       issues the MMAs and commits them to the roles' barriers (21..23 idle)
-// The warpgroups trade registers: 80 a thread at the launch, then 88 for the softmax and the
+//   warps 16..19  thread = key: reads its key codes (one tile ahead, in registers) and writes the K' row
+//                 in the 128-byte-swizzled layout, and the scales
+//   warps 20..23  the same for V' -- the same layout is K-major for K' (rows are the N dimension) and
+//                 MN-major for V' (rows are the K dimension).  (Four warps for both: 347 us instead of 344
+//                 for three prompts of 1500 to 4097 tokens, 32 heads of 128.)
+//   warp 24       issues the MMAs and commits them to the roles' barriers (25..27 idle)
+// The warpgroups trade registers: 72 a thread at the launch, then 88 for the softmax, 56 for the
 // converters, 40 for the MMA warp; with one row tile (head_dim 192 and 256) two warpgroups less are
 // in the softmax and the converters take more.
 // The codes of a word come out in the order 0 4 1 5 2 6 3 7 (one mask per pair); q is staged in that
 // order too, and the output columns are put back in order by the epilogue.
-// Few CTAs are split over the keys: the partial results go to the workspace as records of the step
-// kernel's form, merged by the last CTA of a row tile pair.
+// An item is a tile pair of one sequence and kv head.  How many there are is known on the device only
+// (the host knows bounds, which a batch of a few prompts among many single tokens is far below), so each
+// CTA counts them from q_start (a grid of sequences times the longest one's tiles, most of it empty, took
+// 320 us instead of 161 for a prompt of 2000 among 100 single tokens); where they are fewer than the SMs,
+// several CTAs share an item's keys, evenly, and their partial results go to the workspace as records,
+// merged by the item's last CTA (one prompt of 2000 tokens, 256 items over 148 SMs: 79 -> 61 us by taking
+// the tiles with the most keys first).
+// Measured: 344 us for the three prompts, 735 TFLOP/s; 64 us for 512 tokens behind 3584, 505 TFLOP/s.  No
+// unit is full (tensor cores 37%, issue 58%, special functions 41%): leaving out the exponentials or the
+// products of Q K' changes nothing, so what bounds it is the latency of the chain scores - weights -
+// products in each of the four half tiles in flight, and about 8 us per CTA to fill and drain it.
 constexpr int kKvPM = 128, kKvPN = 128;            // rows per tile, keys per tile
-constexpr int kKvPThreads = 24 * 32;
-constexpr int kKvPConv = 16, kKvPMma = 20;         // first converter warp, the MMA warp
+constexpr int kKvPThreads = 28 * 32;
+constexpr int kKvPConv = 16, kKvPMma = 24;         // first converter warp, the MMA warp
 constexpr int kKvPScales = 4;                      // ring of the tiles' scales
 __host__ __device__ constexpr int kv_p_hdp(int hd) { return (hd + 63) / 64 * 64; }       // whole swizzle blocks
 __host__ __device__ constexpr int kv_p_qt(int hd) { return hd <= 128 ? 2 : 1; }          // row tiles per CTA
@@ -51,10 +62,9 @@ __host__ __device__ constexpr int kv_p_smem(int hd) {
 }
 
 struct KvPromptSplit {
-  int32_t tiles;      // key tiles per CTA
-  int32_t splits;
-  float* part;        // [items][splits][kQt * 128][head_dim + 4]
-  int32_t* count;     // [items]
+  uint32_t ctas;      // that may share their items' keys; 1: none do
+  float* part;        // [items][CTAs per item][kQt * 128][head_dim + 4]
+  int32_t* count;     // [items], zero between calls
 };
 
 // MMAs issued by one lane of a converged warp (`leader`, from elect.sync): outside a divergent branch
@@ -247,6 +257,10 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   __shared__ uint32_t sm_big, sm_tmem;
   __shared__ int sm_last;
+  __shared__ struct {
+    uint32_t item, first, rec;  // the item, its first record, this CTA's record
+    int splits, r0;
+  } sm_item;  // what the results need (in registers it would cost the loop between)
   __shared__ float2 sm_rows[kQt * kKvPM];  // (m, sum) of the rows
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = base, sK = sQ + kQt * kTile, sV = sK + kSt * kTile, sScale = sV + kSt * kTile;
@@ -276,27 +290,73 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   griddep_wait();
   griddep_launch_dependents();
   // ---------------------------------------------------------------- which rows and keys
-  // (later rows see more keys: the tiles of a sequence are taken from the last)
-  const int seq = blockIdx.z, kvh = blockIdx.y, split = blockIdx.x % sp.splits, pair_from_end = blockIdx.x / sp.splits;
-  const int r0 = __ldg(a.B.q_start + seq), q_all = __ldg(a.B.q_start + seq + 1) - r0, kv_all = __ldg(a.B.kv_len + seq);
-  const int q_len = min(q_all, a.B.max_q);
-  if (q_len < a.lo_q || q_len > a.hi_q) return;
+  // (by every warp for itself; the tile pairs of sequence s: none when the launch does not take it)
+  const int kvh_n = a.C.kv_heads;
+  int my_r0 = 0, my_q = 0, my_kv = 0;  // of sequence s0 + lane
+  const auto load_seqs = [&](int s0) {  // their tile pairs
+    const int s = s0 + lane;
+    if (s >= a.B.n_seqs) return 0;
+    my_r0 = __ldg(a.B.q_start + s);
+    my_q = __ldg(a.B.q_start + s + 1) - my_r0;
+    my_kv = __ldg(a.B.kv_len + s);
+    const int len = min(my_q, a.B.max_q);
+    return len < a.lo_q || len > a.hi_q ? 0 : (len * a.group + kQt * kKvPM - 1) / (kQt * kKvPM);
+  };
+  uint32_t items = 0;
+  for (int s0 = 32; s0 < a.B.n_seqs; s0 += 32) items += load_seqs(s0);
+  int n_pairs = load_seqs(0);
+  items = __reduce_add_sync(0xffffffffu, items + n_pairs) * kvh_n;
+  if (items == 0) return;
+  uint32_t most = 1, item = blockIdx.x, split = 0;  // most: CTAs that may share an item
+  if (2 * items <= sp.ctas) {
+    most = sp.ctas / items;
+    item = blockIdx.x / most;
+    split = blockIdx.x - item * most;
+  }
+  if (item >= items) return;
+  // The item's sequence; of a sequence the last tile pairs, which see the most keys, come first.
+  int src = 0, local = 0, s0 = 0;
+  for (int before = 0;;) {
+    int upto = n_pairs;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    const uint32_t here = __ballot_sync(0xffffffffu, static_cast<uint32_t>((before + upto) * kvh_n) > item);
+    if (here) {
+      src = __ffs(here) - 1;
+      local = static_cast<int>(item) - (before + __shfl_sync(0xffffffffu, upto - n_pairs, src)) * kvh_n;
+      break;
+    }
+    before += __shfl_sync(0xffffffffu, upto, 31);
+    s0 += 32;
+    if (s0 >= a.B.n_seqs) return;  // (starts that go up and down, so that the sum did not fit)
+    n_pairs = load_seqs(s0);
+  }
+  const int seq = s0 + src, pairs = __shfl_sync(0xffffffffu, n_pairs, src), r0 = __shfl_sync(0xffffffffu, my_r0, src);
+  const int q_all = __shfl_sync(0xffffffffu, my_q, src), kv_all = __shfl_sync(0xffffffffu, my_kv, src);
+  const int pair_from_end = local / kvh_n, kvh = local - pair_from_end * kvh_n, pair = pairs - 1 - pair_from_end;
+  const int q_len = min(q_all, a.B.max_q), R = q_len * a.group;
   if (r0 < 0 || r0 > a.B.n_tokens - q_len) {  // starts that lead outside q and out
     if (tid == 0) kv_bad_index(a.B);
     return;
   }
-  const int R = q_len * a.group, pairs = (R + kQt * kKvPM - 1) / (kQt * kKvPM);
-  const int pair = pairs - 1 - pair_from_end;
-  if (pair < 0) return;
-  if ((q_all > a.B.max_q || kv_all > a.B.max_kv) && pair_from_end == 0 && split == 0 && kvh == 0 && tid == 0) kv_bad_index(a.B);
+  if ((q_all > a.B.max_q || kv_all > a.B.max_kv) && local == 0 && split == 0 && tid == 0) kv_bad_index(a.B);
   const int n = max(0, min(kv_all, a.B.max_kv));
   const int row0 = pair * kQt * kKvPM, pos0 = kv_all - q_all;
   const int row_end = min(R, row0 + kQt * kKvPM);
   const int see = max(0, min(n, pos0 + (row_end - 1) / a.group + 1));      // keys that the last row sees
   const int tiles = (see + kKvPN - 1) / kKvPN;
-  const int splits = max(1, (tiles + sp.tiles - 1) / sp.tiles);            // CTAs that share this pair
+  int per = tiles, splits = 1;
+  if (most > 1 && tiles >= 4) {  // two key tiles a CTA at least
+    const int share = min(static_cast<int>(most), tiles / 2);
+    per = (tiles + share - 1) / share;
+    splits = (tiles + per - 1) / per;
+  }
   if (split >= splits) return;
-  const int t0 = split * sp.tiles, nt = min(tiles, t0 + sp.tiles) - t0;    // key tiles [t0, t0 + nt)
+  if (tid == 0) sm_item = {item, item * most, item * most + split, splits, r0};
+  const int t0 = split * per, nt = min(tiles, t0 + per) - t0;              // key tiles [t0, t0 + nt)
 
   if (warp == kKvPMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm_tmem)), "r"(512) : "memory");
@@ -308,7 +368,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   const bool softmax = warp < 8 * kQt, converter = warp >= kKvPConv && warp < kKvPMma;
   const int key = tid & 127;  // of the tile
   const int codes = a.C.page_size * (kHd / 2);
-  uint4 rk[kRaw], rv[kRaw];
+  const bool is_v = warp >= kKvPConv + 4;
+  uint4 raw[kRaw];
   uint32_t pk = 0, pv = 0;
   int64_t off = -1;  // the key's page in the tile to load next
   const auto find = [&](int kt) {
@@ -317,16 +378,14 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   };
   const auto load = [&](int kt) {
 #pragma unroll
-    for (int i = 0; i < kRaw; ++i) rk[i] = rv[i] = make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < kRaw; ++i) raw[i] = make_uint4(0, 0, 0, 0);
     pk = pv = 0;  // places past the end: scale and zero 0
     if (off >= 0) {
       const int in = ((t0 + kt) * kKvPN + key) & (a.C.page_size - 1);
       const uint8_t* block = a.C.pages + off + kvh * a.C.head_bytes;
 #pragma unroll
-      for (int i = 0; i < kRaw; ++i) {
-        rk[i] = __ldg(reinterpret_cast<const uint4*>(block + in * (kHd / 2) + 16 * i));
-        rv[i] = __ldg(reinterpret_cast<const uint4*>(block + codes + in * (kHd / 2) + 16 * i));
-      }
+      for (int i = 0; i < kRaw; ++i)
+        raw[i] = __ldg(reinterpret_cast<const uint4*>(block + (is_v ? codes : 0) + in * (kHd / 2) + 16 * i));
       pk = __ldg(reinterpret_cast<const uint32_t*>(block + 2 * codes + 4 * in));
       pv = __ldg(reinterpret_cast<const uint32_t*>(block + 2 * codes + 4 * (a.C.page_size + in)));
     }
@@ -386,11 +445,11 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   const uint32_t tS = tmem, tO = tmem + kQt * kKvPN;  // row tile t: S at + 128 t, O at + kHdp t
   bool ok = true;
 
-  // (every warpgroup trades before its role: 4 * 88 + 88 + 40 = 6 * 80, or with one row tile
-  // 2 * 88 + 2 * 24 + 168 + 40 below it)
+  // (every warpgroup trades before its role: 4 * 88 + 2 * 56 + 40 = 7 * 72, or with one row tile
+  // 2 * 96 + 2 * 24 + 2 * 112 + 40)
   if (softmax) {
     // ---------------------------------------------------------------- softmax
-    regs_up<88>();
+    regs_up<kQt == 2 ? 88 : 96>();
     const int t = warp >> 3, b = (warp >> 2) & 1, g = lane >> 2, q = lane & 3;
     const int lane0 = 32 * (warp & 3) + 16 * b;  // the warp's first row (TMEM lane) of the tile
     const uint32_t lanes = static_cast<uint32_t>(lane0) << 16;
@@ -491,11 +550,11 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     const uint32_t row_addr = tO + t * kHdp + (static_cast<uint32_t>(32 * (warp & 3)) << 16);
     const int row = row0 + tile_row;
     const bool live = row < R;
-    const bool single = splits == 1;
-    const int64_t item = (static_cast<int64_t>(seq) * gridDim.y + kvh) * (gridDim.x / sp.splits) + pair_from_end;
+    const int n_rec = *const_cast<volatile int*>(&sm_item.splits), first_token = *const_cast<volatile int*>(&sm_item.r0);
+    const bool single = n_rec == 1;
     // a record: the weighted sums [head_dim / 4][rows] x 4, then (m, sum) [rows]
     constexpr int kRows = kQt * kKvPM;
-    float* rec = sp.part + (item * sp.splits + split) * (kRows * (kHd + 4));
+    float* rec = sp.part + static_cast<int64_t>(sm_item.rec) * (kRows * (kHd + 4));
     const uint32_t out_s = sQ + t * kTile;  // the row tile's output, laid out like q, which is no longer needed
     const float inv = row_T == 0.f ? 0.f : 1.0f / row_T;  // a row that sees nothing: 0 (a NaN sum stays NaN)
 #pragma unroll 1
@@ -521,10 +580,10 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       }
     }
     const int tok = row / a.group, head = kvh * a.group + row - tok * a.group;
-    uint16_t* dst = a.out + static_cast<int64_t>(r0 + tok) * a.ldo + static_cast<int64_t>(head) * kHd;
+    uint16_t* dst = a.out + static_cast<int64_t>(first_token + tok) * a.ldo + static_cast<int64_t>(head) * kHd;
     if (single) {
       if (b == 0 && live && ok && a.lse)
-        a.lse[static_cast<int64_t>(r0 + tok) * a.heads + head] = row_T == 0.f ? -INFINITY : row_m * 0.6931471805599453f + logf(row_T);
+        a.lse[static_cast<int64_t>(first_token + tok) * a.heads + head] = row_T == 0.f ? -INFINITY : row_m * 0.6931471805599453f + logf(row_T);
       named_barrier(2 + t, 256);
       constexpr int kChunks = kHd / 8;
 #pragma unroll 2
@@ -542,25 +601,27 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       if (b == 0 && live) *reinterpret_cast<float2*>(rec + kRows * kHd + 2 * tile_row) = make_float2(row_m, row_T);
       named_barrier(4, 2 * kRows);
       if (tid == 0) {
-        const bool last = atom_add_acq_rel_gpu(sp.count + item, 1) == splits - 1;
-        if (last) sp.count[item] = 0;
+        const bool last = atom_add_acq_rel_gpu(sp.count + sm_item.item, 1) == n_rec - 1;
+        if (last) sp.count[sm_item.item] = 0;
         sm_last = last;
       }
       named_barrier(4, 2 * kRows);
       if (sm_last && live && ok) {  // merge, in order: thread = row and every other 16 dimensions
-        const float* part = sp.part + item * sp.splits * (kRows * (kHd + 4));
+        const float* part = sp.part + static_cast<int64_t>(sm_item.first) * (kRows * (kHd + 4));
         float M = -1e30f, S = 0.f;
-        for (int i = 0; i < splits; ++i) M = fmaxf(M, __ldcg(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tile_row));
-        for (int i = 0; i < splits; ++i) {
+#pragma unroll 4
+        for (int i = 0; i < n_rec; ++i) {
           const float2 w = __ldcg(reinterpret_cast<const float2*>(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tile_row));
-          S += ex2(w.x - M) * w.y;
+          const float up = fmaxf(M, w.x);
+          S = S * ex2(M - up) + w.y * ex2(w.x - up);
+          M = up;
         }
         const float scale = S == 0.f ? 0.f : 1.0f / S;
 #pragma unroll 1
         for (int d = 16 * b; d < kHd; d += 32) {
           float o[16] = {};
 #pragma unroll 2
-          for (int i = 0; i < splits; ++i) {
+          for (int i = 0; i < n_rec; ++i) {
             const float* src = part + i * (kRows * (kHd + 4));
             const float f = ex2(__ldcg(src + kRows * kHd + 2 * tile_row) - M);
 #pragma unroll
@@ -580,7 +641,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
           }
         }
         if (b == 0 && a.lse)
-          a.lse[static_cast<int64_t>(r0 + tok) * a.heads + head] = S == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(S);
+          a.lse[static_cast<int64_t>(first_token + tok) * a.heads + head] = S == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(S);
       }
     }
   } else if (warp < kKvPConv) {
@@ -588,14 +649,31 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   } else if (warp < kKvPMma) {
     // ---------------------------------------------------------------- keys: thread = key of the tile
     if constexpr (kQt == 2) {
-      regs_up<88>();
+      regs_down<56>();
     } else {
-      regs_up<168>();
+      regs_up<112>();
       load(0);
     }
     find(1);
-    const auto convert = [&](const uint4 (&raw)[kRaw], uint32_t pair, uint32_t tile) {
-      const __half2 zero = __half2half2(__ushort_as_half(static_cast<unsigned short>(pair >> 16)));
+    const float qf = a.scale * 1.4426950408889634f * pow2i(-q_power());  // factor of the scores (log2 units)
+    for (int kt = 0; kt < nt; ++kt) {
+      const int st = kt % kSt, ring = kt % kKvPScales;
+      if (kt >= kSt && !mbar_wait_bounded((is_v ? vempty_b : kempty_b) + 8 * st, ((kt / kSt) - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      if (!is_v) {
+        const float2 kf = unpack_half2(pk), vf = unpack_half2(pv);
+        // (in the order of the softmax's lanes: by half, then (key % 8) / 2, key / 8, key % 2)
+        const uint32_t at = sScale + ring * kKvPN * 8 + 4 * ((key & 64) + 16 * ((key >> 1) & 3) + 2 * ((key >> 3) & 7) + (key & 1));
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(kf.x * qf) : "memory");
+        asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 512), "f"(vf.x) : "memory");
+        const float size = fminf(fmaxf(fabsf(vf.x), 0.f), 65504.f);  // (a NaN has no size)
+        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size));
+        if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - kKvPConv)), "r"(top) : "memory");
+      }
+      const __half2 zero = __half2half2(__ushort_as_half(static_cast<unsigned short>((is_v ? pv : pk) >> 16)));
+      const uint32_t tile = (is_v ? sV : sK) + st * kTile;
 #pragma unroll
       for (int i = 0; i < kRaw; ++i) {
         const uint32_t w[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
@@ -605,38 +683,9 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
           sts128(tile + (c >> 3) * kBlock + sw128_off(key, c & 7), kv_codes_plus(w[j], zero));
         }
       }
-    };
-    const float qf = a.scale * 1.4426950408889634f * pow2i(-q_power());  // factor of the scores (log2 units)
-    for (int kt = 0; kt < nt; ++kt) {
-      const int st = kt % kSt, ring = kt % kKvPScales;
-      const uint32_t par = ((kt / kSt) - 1) & 1;
-      if (kt >= kSt && !mbar_wait_bounded(kempty_b + 8 * st, par)) {
-        ok = false;
-        break;
-      }
-      const float2 kf = unpack_half2(pk), vf = unpack_half2(pv);
-      // (in the order of the softmax's lanes: by half, then (key % 8) / 2, key / 8, key % 2)
-      const uint32_t at = sScale + ring * kKvPN * 8 + 4 * ((key & 64) + 16 * ((key >> 1) & 3) + 2 * ((key >> 3) & 7) + (key & 1));
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(kf.x * qf) : "memory");
-      asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 512), "f"(vf.x) : "memory");
-      const float size = fminf(fmaxf(fabsf(vf.x), 0.f), 65504.f);  // (a NaN has no size)
-      const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size));
-      if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - kKvPConv)), "r"(top) : "memory");
-#pragma unroll 1
-      for (int v = 0; v < 2; ++v) {  // K', then V' (one copy of the code)
-        if (v && kt >= kSt && !mbar_wait_bounded(vempty_b + 8 * st, par)) {
-          ok = false;
-          break;
-        }
-        convert(rk, pk, (v ? sV : sK) + st * kTile);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive((v ? vfull_b : kfull_b) + 8 * st);
-#pragma unroll
-        for (int i = 0; i < kRaw; ++i) rk[i] = rv[i];
-        pk = pv;
-      }
-      if (!ok) break;
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive((is_v ? vfull_b : kfull_b) + 8 * st);
       load(kt + 1);
       find(kt + 2);
     }
