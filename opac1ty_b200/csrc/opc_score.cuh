@@ -325,13 +325,11 @@ __global__ void __launch_bounds__(kScoreThreads, 5) score_kernel(const ScoreArgs
   all = sm_sums[0];
   for (int i = 1; i < kWarps; ++i) all = score_join(all, sm_sums[i]);
   if (kTop) {
-    if (warp == 0) {
-      uint32_t v = sm_top[0][lane];
 #pragma unroll 1
-      for (int w = 1; w < kWarps; ++w) v = score_merge32(v, sm_top[w][lane], lane);
-      sm_top[0][lane] = v;
+    for (int h = kWarps / 2; h > 0; h /= 2) {
+      if (warp < h) sm_top[warp][lane] = score_merge32(sm_top[warp][lane], sm_top[warp + h][lane], lane);
+      __syncthreads();
     }
-    __syncthreads();
     const int want = min(a.top_k, max(0, end - begin));
     // (where fewer shares hold something it is 0: everything is a candidate)
     const uint32_t bound = want > 0 ? sm_top[0][want - 1] : ~0u;
@@ -366,7 +364,9 @@ __global__ void __launch_bounds__(kScoreThreads, 5) score_kernel(const ScoreArgs
     });
     __syncthreads();
     const int n = sm_n;
-    if (n <= kScoreCand) {  // order them: sorted lists of 32 per warp, merged
+    if (n <= 32) {  // order them
+      if (warp == 0) mine = score_sort32(lane < n ? sm_cand[lane] : uint64_t{0}, lane);
+    } else if (n <= kScoreCand) {  // sorted lists of 32 per warp, merged
       for (int i = tid + n; i < kScoreCand; i += kScoreThreads) sm_cand[i] = 0;
       __syncthreads();
       uint64_t v = 0;
@@ -374,7 +374,7 @@ __global__ void __launch_bounds__(kScoreThreads, 5) score_kernel(const ScoreArgs
       sm_keys[warp][lane] = v;
       __syncthreads();
       if (warp == 0) {
-        for (int w = 1; w < kWarps; ++w) v = score_merge32(v, sm_keys[w][lane], lane);
+        for (int w = 1; w < min(kWarps, (n + 31) / 32); ++w) v = score_merge32(v, sm_keys[w][lane], lane);
         mine = v;
       }
     } else {  // too many (ties): the largest below the last one, top_k times
