@@ -128,12 +128,20 @@ __device__ __forceinline__ ScoreSums score_join(const ScoreSums& a, const ScoreS
   r.bad = fmaxf(a.bad, b.bad);
   return r;
 }
-__device__ __forceinline__ ScoreSums score_shfl(const ScoreSums& s, int o) {
+// The sums of a warp's lanes: the largest m first, so that each lane is scaled once.
+__device__ __forceinline__ ScoreSums score_join_warp(const ScoreSums& s) {
   ScoreSums r;
-  r.m = __shfl_xor_sync(0xffffffffu, s.m, o);
-  r.z = __shfl_xor_sync(0xffffffffu, s.z, o);
-  r.w = __shfl_xor_sync(0xffffffffu, s.w, o);
-  r.bad = __shfl_xor_sync(0xffffffffu, s.bad, o);
+  const uint32_t o = __reduce_max_sync(0xffffffffu, score_order(s.m));
+  r.m = __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o);
+  r.bad = __any_sync(0xffffffffu, s.bad != 0.f) ? 1.f : 0.f;
+  const float d = s.m == -INFINITY ? 0.f : (s.m - r.m) * 1.4426950408889634f, f = s.m == -INFINITY ? 0.f : exp2f(d);
+  r.z = f * s.z;
+  r.w = f > 0.f ? f * (s.w + d * s.z) : 0.f;
+#pragma unroll
+  for (int i = 16; i > 0; i >>= 1) {
+    r.z += __shfl_xor_sync(0xffffffffu, r.z, i);
+    r.w += __shfl_xor_sync(0xffffffffu, r.w, i);
+  }
   return r;
 }
 // 32 keys of a warp in descending order (bitonic).
@@ -313,8 +321,7 @@ __global__ void __launch_bounds__(kScoreThreads, 5) score_kernel(const ScoreArgs
   all.w = fmaf(all.w, exp2f(-c), -c * all.z);
   if (all.z != all.z || top == INFINITY) all.bad = 1.f;
   if (all.bad != 0.f) all.z = all.w = 0.f;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) all = score_join(all, score_shfl(all, o));
+  all = score_join_warp(all);
   if (lane == 0) sm_sums[warp] = all;
   uint64_t mine = 0;
   if (kTop) {
@@ -322,8 +329,7 @@ __global__ void __launch_bounds__(kScoreThreads, 5) score_kernel(const ScoreArgs
     sm_top[warp][lane] = score_sort32(any ? score_order(top) : 0u, lane);
   }
   __syncthreads();
-  all = sm_sums[0];
-  for (int i = 1; i < kWarps; ++i) all = score_join(all, sm_sums[i]);
+  if (warp == 0) all = score_join_warp(lane < kWarps ? sm_sums[lane] : ScoreSums{-INFINITY, 0.f, 0.f, 0.f});
   if (kTop) {
 #pragma unroll 1
     for (int h = kWarps / 2; h > 0; h /= 2) {
@@ -429,6 +435,11 @@ __global__ void __launch_bounds__(kScoreThreads, 5) score_kernel(const ScoreArgs
     for (int i = warp; i < a.split; i += kWarps) v = score_merge32(v, __ldcg(c + i * kScoreMaxTop + lane), lane);
     sm_keys[warp][lane] = v;
     __syncthreads();
+#pragma unroll 1
+    for (int h = kWarps / 2; h > 0; h /= 2) {
+      if (warp < h) sm_keys[warp][lane] = score_merge32(sm_keys[warp][lane], sm_keys[warp + h][lane], lane);
+      __syncthreads();
+    }
   }
   if (warp == 0) {
     ScoreSums sums = {-INFINITY, 0.f, 0.f, 0.f};
@@ -436,12 +447,8 @@ __global__ void __launch_bounds__(kScoreThreads, 5) score_kernel(const ScoreArgs
       const float4 p = __ldcg(a.part + r * a.split + i);
       sums = score_join(sums, ScoreSums{p.x, p.y, p.z, p.w});
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sums = score_join(sums, score_shfl(sums, o));
-    uint64_t v = 0;
-    if (kTop)
-      for (int w = 0; w < kWarps; ++w) v = score_merge32(v, sm_keys[w][lane], lane);
-    score_write<kType>(a, r, row, sums, v, lane);
+    sums = score_join_warp(sums);
+    score_write<kType>(a, r, row, sums, kTop ? sm_keys[0][lane] : 0, lane);
   }
 }
 
