@@ -43,7 +43,7 @@ struct KvAttnArgs {
 //             grow, while the results of long contexts are small differences of them and the zeros'
 //             share, and the tensor cores cut what they add: so the share goes into the sums every
 //             kKvFold stages (131071 keys: results off by 4.2e-4 of their norm without,
-//             3.2e-4 with, 2.8e-4 being the roundings of the weights and of the result; 1.5% of the time).
+//             3.1e-4 with, 2.8e-4 being the roundings of the weights and of the result; 2% of the time).
 //   maximum   m and e move only when a score passes m + 8 or a scale 2^(e+5) (one vote per tile):
 //             weights stay below 2^13, and the common tile has no shuffles and no rescaling.
 //
@@ -62,7 +62,7 @@ constexpr int kKvStageShift = 7;
 constexpr int kKvStepWarps = 4;               // consumers
 constexpr int kKvStepThreads = (kKvStepWarps + 1) * 32;
 constexpr int kKvMinStages = 2;               // stages per CTA below which fewer CTAs take part
-constexpr int kKvFold = 8;                    // stages between two foldings of the zeros' share
+constexpr int kKvFold = 4;                    // stages between two foldings of the zeros' share
 constexpr int kKvItemCost = 3;                // what an item costs beside its stages, in stages
 __host__ __device__ constexpr int kv_stage_bytes(int hd) { return kKvStage * (hd + 8); }
 // CTAs per SM: bounded by the accumulators' registers and the shared memory of a record.
@@ -127,6 +127,12 @@ __device__ __forceinline__ uint32_t lds16(uint32_t addr) {
   return v;
 }
 
+// The logarithm of a row's sum T of weights at maximum M (log2 units): ln 2 in two parts, so that the
+// product with M adds no rounding.
+__device__ __forceinline__ float kv_lse(float M, float T) {
+  return T == 0.f ? -INFINITY : fmaf(M, 0.693147182f, fmaf(M, -1.90465421e-9f, logf(T)));
+}
+
 // Write 4 dimensions d.. of the result of row `row` (query token row / group, head row % group of
 // the kv head): the weighted sums o over the sum T of weights at maximum M (log2 units).
 __device__ __forceinline__ void kv_finish_row(const KvAttnArgs& a, int r0, int kvh, int row, int d, const float4& o, float M,
@@ -145,7 +151,7 @@ __device__ __forceinline__ void kv_finish_row(const KvAttnArgs& a, int r0, int k
     dst[3] = static_cast<uint16_t>(hi >> 16);
   }
   if (d == 0 && a.lse)
-    a.lse[static_cast<int64_t>(r0 + i) * a.heads + head] = T == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(T);
+    a.lse[static_cast<int64_t>(r0 + i) * a.heads + head] = kv_lse(M, T);
 }
 
 // Merge the records of an item that `n` CTAs share, the first of them `c_first`, in order (record 1

@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     uint16_t* dst = a.out + static_cast<int64_t>(first_token + tok) * a.ldo + static_cast<int64_t>(head) * kHd;
     if (single) {
       if (b == 0 && live && ok && a.lse)
-        a.lse[static_cast<int64_t>(first_token + tok) * a.heads + head] = row_T == 0.f ? -INFINITY : row_m * 0.6931471805599453f + logf(row_T);
+        a.lse[static_cast<int64_t>(first_token + tok) * a.heads + head] = kv_lse(row_m, row_T);
       named_barrier(2 + t, 256);
       constexpr int kChunks = kHd / 8;
 #pragma unroll 2
@@ -641,7 +641,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
           }
         }
         if (b == 0 && a.lse)
-          a.lse[static_cast<int64_t>(first_token + tok) * a.heads + head] = S == 0.f ? -INFINITY : M * 0.6931471805599453f + logf(S);
+          a.lse[static_cast<int64_t>(first_token + tok) * a.heads + head] = kv_lse(M, S);
       }
     }
   } else if (warp < kKvPConv) {
