@@ -11,10 +11,14 @@ namespace opc {
 // tiles of 128; a CTA takes kQt tiles against the keys they see, 128 at a time:
 //
 //   S = Q K'^T     (in halves of 64 keys, so that the next half's scores are there while one is evaluated)
-//                  K' = code + zero in fp16: exact for |zero| < 8, one rounding otherwise.  The key's
-//                  scale multiplies its column of S in fp32, so nothing of a key is rounded.
+//                  K' = code - 8, exact in fp16; what is left of the zeros, (zero + 8) sum q, is added by
+//                  one more product in tf32, with both factors in parts of 11 bits (sum q three, zero + 8
+//                  two).  The key's scale multiplies its column of S in fp32: nothing of a key is rounded.
+//                  (K' = code + zero in fp16 would take 345 us instead of 358 for the prompts below, but
+//                  round the keys' largest elements: log sums off by 1e-6 of their value instead of 4e-8.)
 //   P = exp2(S * scale_k - m) * scale_v, rounded once to fp16, written over S in tensor memory
-//   O += P V'      V' = code + zero in fp16, as above
+//   O += P V'      V' = code + zero in fp16: exact where no value is larger than |zero|, else one rounding
+//                  (2^-11 of the value, as for P and the result)
 //
 // 4 * 128 * 128 * head_dim operations per tile pair, against 128 * 128 exponentials, which the
 // special-function units take as long for as the tensor cores for the products at head_dim 128: two
@@ -30,8 +34,7 @@ namespace opc {
 //   warps 16..19  thread = key: reads its key codes (one tile ahead, in registers) and writes the K' row
 //                 in the 128-byte-swizzled layout, and the scales
 //   warps 20..23  the same for V' -- the same layout is K-major for K' (rows are the N dimension) and
-//                 MN-major for V' (rows are the K dimension).  (Four warps for both: 347 us instead of 344
-//                 for three prompts of 1500 to 4097 tokens, 32 heads of 128.)
+//                 MN-major for V' (rows are the K dimension).  (Four warps for both took 1% longer.)
 //   warp 24       issues the MMAs and commits them to the roles' barriers (25..27 idle)
 // The warpgroups trade registers: 72 a thread at the launch, then 88 for the softmax, 56 for the
 // converters, 40 for the MMA warp; with one row tile (head_dim 192 and 256) two warpgroups less are
@@ -41,24 +44,25 @@ namespace opc {
 // An item is a tile pair of one sequence and kv head.  How many there are is known on the device only
 // (the host knows bounds, which a batch of a few prompts among many single tokens is far below), so each
 // CTA counts them from q_start (a grid of sequences times the longest one's tiles, most of it empty, took
-// 320 us instead of 161 for a prompt of 2000 among 100 single tokens); where they are fewer than the SMs,
+// 320 us instead of 165 for a prompt of 2000 among 100 single tokens); where they are fewer than the SMs,
 // several CTAs share an item's keys, evenly, and their partial results go to the workspace as records,
-// merged by the item's last CTA (one prompt of 2000 tokens, 256 items over 148 SMs: 79 -> 61 us by taking
+// merged by the item's last CTA (one prompt of 2000 tokens, 256 items over 148 SMs: 79 -> 65 us by taking
 // the tiles with the most keys first).
-// Measured: 344 us for the three prompts, 735 TFLOP/s; 64 us for 512 tokens behind 3584, 505 TFLOP/s.  No
-// unit is full (tensor cores 37%, issue 58%, special functions 41%): leaving out the exponentials or the
-// products of Q K' changes nothing, so what bounds it is the latency of the chain scores - weights -
+// Measured, 32 heads of 128 over 8: 358 us for three prompts of 1500 to 4097 tokens, 706 TFLOP/s; 66 us for
+// 512 tokens behind 3584, 488 TFLOP/s.  No unit is full (tensor cores 38%, issue 60%, special functions
+// 40%): leaving out the exponentials or most of the products of Q K' changes nothing, so what bounds it is the latency of the chain scores - weights -
 // products in each of the four half tiles in flight, and about 8 us per CTA to fill and drain it.
 constexpr int kKvPM = 128, kKvPN = 128;            // rows per tile, keys per tile
 constexpr int kKvPThreads = 28 * 32;
 constexpr int kKvPConv = 16, kKvPMma = 24;         // first converter warp, the MMA warp
+constexpr int kKvPZero = 128 * 32;                 // bytes of a tile's factors of the tf32 product
 constexpr int kKvPScales = 4;                      // ring of the tiles' scales
 __host__ __device__ constexpr int kv_p_hdp(int hd) { return (hd + 63) / 64 * 64; }       // whole swizzle blocks
 __host__ __device__ constexpr int kv_p_qt(int hd) { return hd <= 128 ? 2 : 1; }          // row tiles per CTA
 __host__ __device__ constexpr int kv_p_st(int hd) { return hd <= 128 ? 2 : 1; }          // K' and V' stages
 __host__ __device__ constexpr int kv_p_tile(int hd) { return 128 * kv_p_hdp(hd) * 2; }   // bytes of Q, K', V' tiles
 __host__ __device__ constexpr int kv_p_smem(int hd) {
-  return 1024 + (kv_p_qt(hd) + 2 * kv_p_st(hd)) * kv_p_tile(hd) + kKvPScales * (kKvPN * 8 + 16) + 256;
+  return 1024 + (kv_p_qt(hd) + 2 * kv_p_st(hd)) * kv_p_tile(hd) + (kv_p_qt(hd) + kv_p_st(hd)) * kKvPZero + kKvPScales * (kKvPN * 8 + 16) + 256;
 }
 
 struct KvPromptSplit {
@@ -82,6 +86,20 @@ __device__ __forceinline__ void umma_f16_by(uint32_t leader, uint32_t tmem_d, ui
       "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum), "r"(leader)
       : "memory");
 }
+// tf32, 8 along K: tiles of 128 rows of 32 bytes without swizzle, in blocks of 8 rows x 16 bytes (the two of
+// a row 128 bytes apart, the next 8 rows 256).
+__device__ __forceinline__ void umma_tf32_by(uint32_t leader, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n .reg .pred p, l;\n setp.ne.b32 l, %5, 0;\n setp.ne.b32 p, %4, 0;\n"
+      " @l tcgen05.mma.cta_group::1.kind::tf32 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum), "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ uint64_t kv_desc_rows32(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (8ull << 16) | (16ull << 32) | (1ull << 46);
+}
+__device__ __forceinline__ uint32_t kv_rows32_off(int row) { return static_cast<uint32_t>((row >> 3) * 256 + (row & 7) * 16); }
+__device__ __forceinline__ float high11(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 // The same with A in tensor memory, fp16 packed in pairs along K.
 __device__ __forceinline__ void umma_f16_ts_by(uint32_t leader, uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
                                                uint32_t accum) {
@@ -122,6 +140,10 @@ __device__ __forceinline__ uint64_t kv_desc_mn(uint32_t saddr) {
 }
 __host__ __device__ constexpr uint32_t kv_idesc(int n, bool b_mn) {
   return (1u << 4) | (b_mn ? 1u << 16 : 0u) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kKvPM >> 4) << 24);
+}
+
+__host__ __device__ constexpr uint32_t kv_idesc_tf32(int n) {
+  return (1u << 4) | (2u << 7) | (2u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(kKvPM >> 4) << 24);
 }
 
 // The 16-row fragment shapes: of 8 fp32 columns lane (g, q) = (lane / 4, lane % 4) holds (row g, columns
@@ -222,6 +244,21 @@ __device__ __forceinline__ void kv_row_max(uint32_t s_addr, uint32_t sk, const i
   }
 }
 
+// Eight codes of a word minus 8, as four pairs of fp16 in the order 04 15 26 37.
+__device__ __forceinline__ uint4 kv_codes_minus8(uint32_t w) {
+  const __half2 big = __float2half2_rn(-1032.f), small = __float2half2_rn(-72.f), sixteenth = __float2half2_rn(0.0625f);
+  uint32_t r[4];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const uint32_t u = w >> (8 * h);
+    const uint32_t a = (u & 0x000f000fu) | 0x64006400u, b = (u & 0x00f000f0u) | 0x64006400u;  // 1024 + c, 1024 + 16 c
+    const __half2 x = __hadd2(*reinterpret_cast<const __half2*>(&a), big);
+    const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&b), sixteenth, small);
+    r[2 * h] = *reinterpret_cast<const uint32_t*>(&x);
+    r[2 * h + 1] = *reinterpret_cast<const uint32_t*>(&y);
+  }
+  return make_uint4(r[0], r[1], r[2], r[3]);
+}
 // Eight codes of a word plus the zero, as four pairs of fp16 in the order 04 15 26 37.
 __device__ __forceinline__ uint4 kv_codes_plus(uint32_t w, __half2 zero) {
   const __half2 big = __float2half2_rn(-1024.f), small = __float2half2_rn(-64.f), sixteenth = __float2half2_rn(0.0625f);
@@ -263,12 +300,13 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   } sm_item;  // what the results need (in registers it would cost the loop between)
   __shared__ float2 sm_rows[kQt * kKvPM];  // (m, sum) of the rows
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  const uint32_t sQ = base, sK = sQ + kQt * kTile, sV = sK + kSt * kTile, sScale = sV + kSt * kTile;
+  const uint32_t sQ = base, sK = sQ + kQt * kTile, sV = sK + kSt * kTile, sQz = sV + kSt * kTile;
+  const uint32_t sKz = sQz + kQt * kKvPZero, sScale = sKz + kSt * kKvPZero;
   const uint32_t sTop = sScale + kKvPScales * kKvPN * 8;  // [ring][4] largest scale_v of the warps' keys
   const uint32_t bars = sTop + kKvPScales * 16;
   const uint32_t kfull_b = bars, kempty_b = bars + 16, vfull_b = bars + 32, vempty_b = bars + 48;
   // (per row tile t and half h of a key tile: [t][h], one phase per key tile each)
-  const uint32_t sfull_b = bars + 64, pfull_b = bars + 96, odone_b = bars + 128, drain_b = bars + 160;
+  const uint32_t sfull_b = bars + 64, pfull_b = bars + 96, odone_b = bars + 128, drain_b = bars + 160, qsum_b = bars + 168;
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
   if (tid == 0) {
@@ -284,6 +322,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       }
     }
     mbar_init(drain_b, 1);
+    mbar_init(qsum_b, 4 * kQt);
     fence_mbar_init();
     sm_big = 0;
   }
@@ -455,6 +494,23 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     const uint32_t lanes = static_cast<uint32_t>(lane0) << 16;
     const uint32_t s_addr = tS + t * kKvPN + lanes, o_addr = tO + t * kHdp + lanes;
     const int first_row = row0 + t * kKvPM + lane0;
+    if (b == 0) {  // thread = row: the sum of its q, as staged
+      const int in = tid & 127;
+      float x = 0.f;
+#pragma unroll 4
+      for (int c = 0; c < kHd / 8; ++c) {
+        const uint4 w = lds128(sQ + t * kTile + (c >> 3) * kBlock + sw128_off(in, c & 7));
+        const float2 e0 = unpack_half2(w.x), e1 = unpack_half2(w.y), e2 = unpack_half2(w.z), e3 = unpack_half2(w.w);
+        x += ((e0.x + e0.y) + (e1.x + e1.y)) + ((e2.x + e2.y) + (e3.x + e3.y));
+      }
+      const float x1 = high11(x), x2 = high11(x - x1), x3 = x - x1 - x2;
+      const uint32_t at = sQz + t * kKvPZero + kv_rows32_off(in);
+      sts128(at, make_uint4(__float_as_uint(x1), __float_as_uint(x1), __float_as_uint(x2), __float_as_uint(x2)));
+      sts128(at + 128, make_uint4(__float_as_uint(x3), 0, 0, 0));
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(qsum_b);
+    }
     float m[2], T[2];   // of rows g and g + 8
     int lim[2];         // keys below it are seen by the row
     bool fresh[2];      // no key seen yet, but one will be: m means nothing
@@ -669,10 +725,14 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(at), "f"(kf.x * qf) : "memory");
         asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 512), "f"(vf.x) : "memory");
         const float size = fminf(fmaxf(fabsf(vf.x), 0.f), 65504.f);  // (a NaN has no size)
+        const float z = kf.y + 8.f, z1 = high11(z), z2 = z - z1;
+        const uint32_t z_at = sKz + st * kKvPZero + kv_rows32_off(key);
+        sts128(z_at, make_uint4(__float_as_uint(z1), __float_as_uint(z2), __float_as_uint(z1), __float_as_uint(z2)));
+        sts128(z_at + 128, make_uint4(__float_as_uint(z1), 0, 0, 0));
         const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size));
         if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - kKvPConv)), "r"(top) : "memory");
       }
-      const __half2 zero = __half2half2(__ushort_as_half(static_cast<unsigned short>((is_v ? pv : pk) >> 16)));
+      const __half2 zero = __half2half2(__ushort_as_half(static_cast<unsigned short>(pv >> 16)));
       const uint32_t tile = (is_v ? sV : sK) + st * kTile;
 #pragma unroll
       for (int i = 0; i < kRaw; ++i) {
@@ -680,7 +740,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const int c = 4 * i + j;  // 8 dimensions
-          sts128(tile + (c >> 3) * kBlock + sw128_off(key, c & 7), kv_codes_plus(w[j], zero));
+          sts128(tile + (c >> 3) * kBlock + sw128_off(key, c & 7), is_v ? kv_codes_plus(w[j], zero) : kv_codes_minus8(w[j]));
         }
       }
       fence_proxy_async_smem();
@@ -704,6 +764,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
           umma_f16_by(leader, tS + t * kKvPN + 64 * h, qd + ((k >> 2) * kB + (k & 3) * 2), kd + ((k >> 2) * kB + (k & 3) * 2),
                    kv_idesc(kKvPN / 2, false), k > 0);
         }
+        umma_tf32_by(leader, tS + t * kKvPN + 64 * h, kv_desc_rows32(sQz + t * kKvPZero), kv_desc_rows32(sKz + st * kKvPZero) + 128 * h,
+                     kv_idesc_tf32(kKvPN / 2), 1);
         umma_commit_by(leader, sfull_b + 16 * t + 8 * h);
         if (t == kQt - 1 && h == 1) umma_commit_by(leader, kempty_b + 8 * st);
       };
@@ -712,7 +774,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         tc_fence_after();
         return ok;
       };
-      if (nt > 0 && wait(kfull_b, 0))
+      if (nt > 0 && wait(qsum_b, 0) && wait(kfull_b, 0))
         for (int i = 0; i < 2 * kQt; ++i) scores(i % kQt, 0, i / kQt);
       for (int kt = 0; kt < nt && ok; ++kt) {
         const int st = kt % kSt;
