@@ -139,9 +139,15 @@ constexpr size_t kCounterBytes = 4096;  // one per CTA of a launch
 
 AttentionPlan plan_attention(const opc_kv_cache& c, const opc_kv_batch& b, int group, int sms) {
   AttentionPlan p{};
-  // Row tiles of 8 (query token, head) pairs: two where the accumulators leave registers for them.
+  // Row tiles of 8 (query token, head) pairs: two where the accumulators leave registers for them.  (Heads
+  // of 128, four rows of four heads over 4000 keys: 20 us in the step kernel, 35 in the prompt kernel;
+  // 16 such sequences 39 and 96.)
   const int most = c.head_dim <= 128 ? 16 : 8;
   p.step_q = std::min(std::max(b.max_q, 0), most / group);
+  // Where a sequence of few rows would leave rows of the batch to nobody, as with one sequence, the prompt
+  // kernel takes what there is (five rows of four heads over 4000 keys: 47 us after a step kernel that
+  // finds nothing to do, 36 without).
+  if (b.max_q > p.step_q && b.n_tokens > (b.n_seqs - 1LL) * b.max_q + p.step_q) p.step_q = 0;
   p.bytes = kCounterBytes;
   if (p.step_q > 0) {
     p.step_nt = p.step_q * group > 8 ? 2 : 1;
@@ -295,8 +301,9 @@ int opc_kv_append(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t 
                    (!q || (aligned16(q) && aligned16(q_out) && ldq % 8 == 0 && ldqo % 8 == 0));
   const int lpr = lanes_per_head(hd), groups = opc::kKvAppendThreads / lpr, all = 2 * kvh + a.heads;
   const bool bf = dtype == OPC_BF16;
-  // few rows: a CTA per row and `groups` heads; many: four rows per CTA, which share its set-up
-  const bool few = batch->n_tokens < 4 * dev.sm_count;
+  // few rows: a CTA per row and `groups` heads; many: four rows per CTA, which share its set-up (32/8 heads
+  // of 128: 96 rows 3.7 and 9.5 us, 600 rows 8.9 and 11.0, 1200 rows 14.5 and 13.8, 5000 rows 51 and 36)
+  const bool few = batch->n_tokens < 6 * dev.sm_count;
   const int tok = few ? 1 : 4;
   const dim3 grid((batch->n_tokens + tok - 1) / tok, few ? (all + groups - 1) / groups : 1);
   auto kern = few ? append_for<1>(lpr, bf, vec) : append_for<4>(lpr, bf, vec);

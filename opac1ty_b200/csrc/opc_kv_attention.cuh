@@ -56,6 +56,11 @@ struct KvAttnArgs {
 // memory at the end of the item.  An item that is a whole sequence and head is written out; else
 // its record (m, sum, weighted sums) goes to the workspace -- a CTA has at most two -- and the last
 // CTA of that sequence and head to arrive merges the records in order.
+//
+// Measured: 64 sequences of up to 8192 keys, 64/8 heads of 128: 76 us, 3.9 TB/s; one of 131071 keys, 32/8
+// heads: 41 us, 3.5 TB/s; one of 4000 keys: 12 us, latency (lengths, pages, keys, records, one after the
+// other).  What bounds the large ones is the instructions that spread codes into operands (logic units 48%,
+// issue 50% with three CTAs per SM, the registers' limit), not memory.
 // ------------------------------------------------------------------------------------------------
 constexpr int kKvStage = 128;                 // keys per stage, 32 for each consumer
 constexpr int kKvStageShift = 7;

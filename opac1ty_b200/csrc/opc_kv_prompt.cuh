@@ -14,7 +14,7 @@ namespace opc {
 //                  K' = code - 8, exact in fp16; what is left of the zeros, (zero + 8) sum q, is added by
 //                  one more product in tf32, with both factors in parts of 11 bits (sum q three, zero + 8
 //                  two).  The key's scale multiplies its column of S in fp32: nothing of a key is rounded.
-//                  (K' = code + zero in fp16 would take 345 us instead of 358 for the prompts below, but
+//                  (K' = code + zero in fp16 would take 345 us instead of 357 for the prompts below, but
 //                  round the keys' largest elements: log sums off by 1e-6 of their value instead of 4e-8.)
 //   P = exp2(S * scale_k - m) * scale_v, rounded once to fp16, written over S in tensor memory
 //   O += P V'      V' = code + zero in fp16: exact where no value is larger than |zero|, else one rounding
@@ -48,8 +48,8 @@ namespace opc {
 // several CTAs share an item's keys, evenly, and their partial results go to the workspace as records,
 // merged by the item's last CTA (one prompt of 2000 tokens, 256 items over 148 SMs: 79 -> 65 us by taking
 // the tiles with the most keys first).
-// Measured, 32 heads of 128 over 8: 358 us for three prompts of 1500 to 4097 tokens, 706 TFLOP/s; 66 us for
-// 512 tokens behind 3584, 488 TFLOP/s.  No unit is full (tensor cores 38%, issue 60%, special functions
+// Measured, 32 heads of 128 over 8: 357 us for three prompts of 1500 to 4097 tokens, 710 TFLOP/s; 63 us for
+// 512 tokens behind 3584, 509 TFLOP/s.  No unit is full (tensor cores 38%, issue 60%, special functions
 // 40%): leaving out the exponentials or most of the products of Q K' changes nothing, so what bounds it is the latency of the chain scores - weights -
 // products in each of the four half tiles in flight, and about 8 us per CTA to fill and drain it.
 constexpr int kKvPM = 128, kKvPN = 128;            // rows per tile, keys per tile

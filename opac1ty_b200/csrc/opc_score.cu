@@ -30,7 +30,8 @@ struct ScorePlan {
 
 ScorePlan plan_score(int32_t rows, int32_t vocab, int sms) {
   // One CTA per row, unless the rows leave SMs idle: then up to two CTAs per SM, with no fewer than two
-  // groups of 8 logits for each thread.
+  // groups of 8 logits for each thread (128256 logits: one row 9.6 us instead of 20.3, 100 rows 18.7
+  // instead of 20.8; 17 rows of 32000 9.5 and 9.1).
   ScorePlan p{1, vocab, kCounterBytes};
   if (rows > 0 && rows <= opc::kScoreMaxRows) {
     const int most = std::min<int>(opc::kScoreMaxSplit, vocab / (opc::kScoreThreads * 16));

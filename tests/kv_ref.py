@@ -16,6 +16,7 @@ class Setup:
         rng = np.random.default_rng(seed)
         self.q_lens, self.kv_lens = list(q_lens), list(kv_lens)
         self.kv_heads, self.hd, self.page = kv_heads, hd, page
+        self.rounded = False  # the batch's bounds send sequences of few rows to the form for many
         used = [-(-max(n, 0) // page) for n in kv_lens]
         self.n_pages = sum(used) + spare_pages
         order = rng.permutation(self.n_pages)
@@ -122,7 +123,7 @@ def attention64(su: Setup, pages_np, q, scale, table_ok=None):
             continue
         # many rows per kv head (more than the 16, or with large heads 8, of the form for steps): code +
         # zero goes to the tensor cores rounded to fp16, which moves the scores and values by this
-        rounded = su.q_lens[s] * G > (16 if hd <= 128 else 8)
+        rounded = su.q_lens[s] * G > (16 if hd <= 128 else 8) or su.rounded
         idx = np.arange(pos + 1)
         pg, off = su.table[s, idx // su.page], idx % su.page
         for h in range(H):

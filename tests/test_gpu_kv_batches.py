@@ -123,3 +123,15 @@ def test_a_step_captured_from_append_to_log_probabilities(cuda_device):
         assert torch.equal(again[1], out) and torch.equal(su.cache.pages, pages)
         assert torch.equal(again[3].logprob, res.logprob) and torch.equal(again[3].top_ids, res.top_ids)
     assert device_error(cuda_device) == 0
+
+
+@pytest.mark.parametrize("hd,heads", [(64, 4), (128, 16), (256, 2)])
+@pytest.mark.parametrize("q_len", [0, 1, 2, 20])
+def test_a_padded_batch_of_one_sequence(cuda_device, hd, heads, q_len):
+    """Bounds for 40 rows, as a captured graph has them, and fewer in use: the form is chosen by the bounds."""
+    rng = np.random.default_rng(hd + q_len)
+    su = Setup(cuda_device, [q_len], [700], 1, hd, 32, pad_rows=40 - q_len)
+    su.batch = kv.KVBatch(su.batch.q_start, su.batch.kv_len, su.batch.page_table, n_tokens=40, max_q=40, max_kv=1000)
+    su.rounded = True
+    q, out, lse = run_attention(su, rng, heads, F16, cuda_device)
+    assert device_error(cuda_device) == 0
