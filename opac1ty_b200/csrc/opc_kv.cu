@@ -90,8 +90,8 @@ opc::KvRows rows_of(const opc_kv_batch& b, const opc_kv_cache& c, int* err) {
   r.n_seqs = b.n_seqs;
   r.n_tokens = b.n_tokens;
   r.max_q = b.max_q;
-  // (page counts are kept below 2^31 positions, so positions and their sums stay in 32 bits)
-  r.max_pages = static_cast<int32_t>(std::min<int64_t>(b.max_pages, INT32_MAX / c.page_size));
+  // (page counts are kept below 2^31 positions, so positions and their sums with tiles stay in 32 bits)
+  r.max_pages = static_cast<int32_t>(std::min<int64_t>(b.max_pages, (INT32_MAX - 1024) / c.page_size));
   r.max_kv = std::min(b.max_kv, r.max_pages * c.page_size);
   r.err = err;
   return r;

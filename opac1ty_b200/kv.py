@@ -68,6 +68,12 @@ def _workspace(device: torch.device, stream: int, nbytes: int, kind: str) -> tor
     return ws
 
 
+def _check_workspace(what: str, ws: torch.Tensor, device: torch.device):
+    if ws.device != device or ws.dtype != torch.uint8 or not ws.is_contiguous():
+        raise ValueError(f"{what}: the workspace must be contiguous uint8 values on {device}, got {ws.dtype} "
+                         f"{tuple(ws.shape)} on {ws.device}")
+
+
 class KVCache:
     """n_pages pages of page_size tokens for kv_heads heads of head_dim, 4 bits a value
     (``opc_kv_plan``).  ``pages``: an existing uint8 tensor of ``total_bytes`` bytes to use."""
@@ -113,6 +119,8 @@ class KVBatch:
         n = kv_len.numel()
         if q_start.numel() != n + 1 or page_table.shape[0] != n:
             raise ValueError(f"KVBatch: {q_start.numel()} starts and {page_table.shape[0]} table rows for {n} sequences")
+        if n > 1 and page_table.numel() and page_table.stride(0) < page_table.shape[1]:
+            raise ValueError(f"KVBatch: the rows of page_table overlap (strides {page_table.stride()}); give each sequence its own")
         if n_tokens is None:
             n_tokens = int(q_start[-1])
         if max_q is None:
@@ -232,8 +240,9 @@ def attention(cache: KVCache, batch: KVBatch, q: torch.Tensor, scale: Optional[f
               out: Optional[torch.Tensor] = None, return_lse: bool = False,
               workspace: Optional[torch.Tensor] = None):
     """Causal attention of the rows q [n_tokens, heads, head_dim] over the cache: out, or (out, lse)
-    with lse [n_tokens, heads] fp32.  ``scale``: 1/sqrt(head_dim) by default.  Rows that belong to no
-    sequence are not written."""
+    with lse [n_tokens, heads] fp32.  ``scale``: 1/sqrt(head_dim) by default.  ``workspace``: zeroed
+    uint8 memory of ``attention_workspace_bytes`` that no other call in flight uses (one per stream
+    by default).  Rows that belong to no sequence are not written."""
     hd, dev = cache.head_dim, cache.device
     _same_device("attention", cache, batch)
     ldq, heads = _rows("attention", "q", q, batch.n_tokens, None, hd, q.dtype, dev)
@@ -244,6 +253,8 @@ def attention(cache: KVCache, batch: KVBatch, q: torch.Tensor, scale: Optional[f
     stream = _raw_stream(dev.index)
     if workspace is None:
         workspace = _workspace(dev, stream, attention_workspace_bytes(cache, batch, heads), "kv")
+    else:
+        _check_workspace("attention", workspace, dev)
     _call(_lib.load().opc_kv_attention, dev.index, cache._ref, batch._ref, heads, _DTYPES[q.dtype],
           hd ** -0.5 if scale is None else float(scale), q.data_ptr(), ldq, out.data_ptr(), ldo,
           lse.data_ptr() if return_lse else None, workspace.data_ptr(), workspace.numel(), stream)

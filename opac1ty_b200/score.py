@@ -8,7 +8,7 @@ from typing import NamedTuple, Optional
 import torch
 
 from . import _lib
-from .kv import _DTYPES, _call, _raw_stream, _workspace
+from .kv import _DTYPES, _call, _check_workspace, _raw_stream, _workspace
 
 
 class TokenLogprobs(NamedTuple):
@@ -50,6 +50,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     stream = _raw_stream(dev.index)
     if workspace is None:
         workspace = _workspace(dev, stream, _need(rows, vocab, top_k, dev.index), "score")
+    else:
+        _check_workspace("token_logprobs", workspace, dev)
     _call(lib.opc_token_logprobs, dev.index, logits.data_ptr(), logits.stride(0) if rows > 1 else vocab,
           _DTYPES[logits.dtype], rows, vocab, targets.data_ptr() if targets is not None else None,
           logprob.data_ptr() if logprob is not None else None, ent.data_ptr() if ent is not None else None, top_k,

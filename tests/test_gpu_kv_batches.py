@@ -135,3 +135,29 @@ def test_a_padded_batch_of_one_sequence(cuda_device, hd, heads, q_len):
     su.rounded = True
     q, out, lse = run_attention(su, rng, heads, F16, cuda_device)
     assert device_error(cuda_device) == 0
+
+
+def test_refusals_of_workspaces_and_tables(cuda_device):
+    """A workspace elsewhere and a table whose rows overlap are refused before anything is launched."""
+    su = Setup(cuda_device, [1, 1], [10, 20], 1, 64, 16)
+    q = torch.zeros(2, 2, 64, dtype=F16, device=cuda_device)
+    need = kv.attention_workspace_bytes(su.cache, su.batch, 2)
+    for ws in (torch.zeros(need, dtype=torch.uint8), torch.zeros(need, dtype=torch.float32, device=cuda_device),
+               torch.zeros(2 * need, dtype=torch.uint8, device=cuda_device)[::2]):
+        with pytest.raises(ValueError, match="workspace"):
+            kv.attention(su.cache, su.batch, q, workspace=ws)
+        with pytest.raises(ValueError, match="workspace"):
+            token_logprobs(q[:, 0], workspace=ws)
+    with pytest.raises(ValueError, match="overlap"):
+        kv.KVBatch(su.batch.q_start, su.batch.kv_len, su.batch.page_table[:1].expand(2, -1))
+
+
+def test_attention_in_place_of_its_queries(cuda_device):
+    """out may be q: every CTA of an item has read its rows before the item's result is written."""
+    rng = np.random.default_rng(31)
+    su = Setup(cuda_device, [1, 60, 2], [4000, 2000, 300], 2, 128, 64)
+    q, out, lse = run_attention(su, rng, 8, F16, cuda_device)
+    for _ in range(3):
+        x = q.clone()
+        kv.attention(su.cache, su.batch, x, out=x)
+        assert torch.equal(x, out)
