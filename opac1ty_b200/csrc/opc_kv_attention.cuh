@@ -42,8 +42,9 @@ struct KvAttnArgs {
 //             the values themselves (code + zero), not on the all-positive codes.  Their sums only
 //             grow, while the results of long contexts are small differences of them and the zeros'
 //             share, and the tensor cores cut what they add: so the share goes into the sums every
-//             kKvFold stages (131071 keys: results off by 4.2e-4 of their norm without,
-//             3.1e-4 with, 2.8e-4 being the roundings of the weights and of the result; 2% of the time).
+//             kKvFold stages, with half of the next stages' expected share in advance, so that they
+//             run through 0 and what is cut cancels (131071 keys: results off by 4.2e-4 of their norm
+//             without, 3.1e-4 with, 2.8e-4 being the roundings of the weights and of the result).
 //   maximum   m and e move only when a score passes m + 8 or a scale 2^(e+5) (one vote per tile):
 //             weights stay below 2^13, and the common tile has no shuffles and no rescaling.
 //
@@ -67,7 +68,7 @@ constexpr int kKvStageShift = 7;
 constexpr int kKvStepWarps = 4;               // consumers
 constexpr int kKvStepThreads = (kKvStepWarps + 1) * 32;
 constexpr int kKvMinStages = 2;               // stages per CTA below which fewer CTAs take part
-constexpr int kKvFold = 4;                    // stages between two foldings of the zeros' share
+constexpr int kKvFold = 8;                    // stages between two foldings of the zeros' share
 constexpr int kKvItemCost = 3;                // what an item costs beside its stages, in stages
 __host__ __device__ constexpr int kv_stage_bytes(int hd) { return kKvStage * (hd + 8); }
 // CTAs per SM: bounded by the accumulators' registers and the shared memory of a record.
@@ -567,7 +568,7 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
   // keys below this need no mask: every live row sees them
   const int plain_end = min(k1, it.seq_end - it.hidden);
 
-  float acc[kNT][kMt][4], az[kNT][2], sum[kNT][2], m[kNT][2];
+  float acc[kNT][kMt][4], az[kNT][2], ahead[kNT][2], sum[kNT][2], m[kNT][2];
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
 #pragma unroll
@@ -576,7 +577,7 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
       for (int c = 0; c < 4; ++c) acc[t][i][c] = 0.f;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      az[t][c] = sum[t][c] = 0.f;
+      az[t][c] = ahead[t][c] = sum[t][c] = 0.f;
       m[t][c] = -1e30f;
     }
   }
@@ -679,6 +680,7 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
             m[t][c] = mn;
             sum[t][c] *= corr;
             az[t][c] *= corr * drop;
+            ahead[t][c] *= corr * drop;
 #pragma unroll
             for (int i = 0; i < kMt; ++i) {
               acc[t][i][c] *= corr * drop;
@@ -750,7 +752,10 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
             float z = az[t][c];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) z += __shfl_xor_sync(0xffffffffu, z, o);
-            az[t][c] = 0.f;
+            const float half = 0.5f * (z + ahead[t][c]);  // of these stages' share, now for the next ones'
+            ahead[t][c] = half;
+            az[t][c] = g == 0 ? -half : 0.f;
+            z += half;
 #pragma unroll
             for (int i = 0; i < kMt; ++i) {
               acc[t][i][c] += z * 0x1p-24f;
