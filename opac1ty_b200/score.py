@@ -43,7 +43,9 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
             targets = targets.clamp(-1, 2**31 - 1).to(torch.int32)
         targets = targets.contiguous()
     logprob = torch.empty(rows, dtype=torch.float32, device=dev) if targets is not None else None
-    ent = torch.empty(rows, dtype=torch.float32, device=dev) if entropy else None
+    ent = None
+    if entropy:
+        ent = torch.empty_like(logprob) if logprob is not None else torch.empty(rows, dtype=torch.float32, device=dev)
     ids = torch.empty(rows, top_k, dtype=torch.int32, device=dev) if top_k >= 0 else None
     top = torch.empty(rows, top_k, dtype=torch.float32, device=dev) if top_k >= 0 else None
     lib = _lib.load()
