@@ -32,7 +32,8 @@ namespace opc {
 //                 times the tile's largest scale_v may pass 2^12: then the row's maximum is looked for,
 //                 O rescaled and the half evaluated again -- always in the first tile, hardly ever later.
 //   warps 16..19  thread = key: reads its key codes (one tile ahead, in registers) and writes the K' row
-//                 in the 128-byte-swizzled layout, and the scales
+//                 in the 128-byte-swizzled layout, the scales, and a bit for each key of a missing page (the
+//                 softmax takes its masked path in such a tile: the bits keep them out of maximum and sum)
 //   warps 20..23  the same for V' -- the same layout is K-major for K' (rows are the N dimension) and
 //                 MN-major for V' (rows are the K dimension).  (Four warps for both took 1% longer.)
 //   warp 24       issues the MMAs and commits them to the roles' barriers (25..27 idle)
@@ -62,7 +63,7 @@ __host__ __device__ constexpr int kv_p_qt(int hd) { return hd <= 128 ? 2 : 1; } 
 __host__ __device__ constexpr int kv_p_st(int hd) { return hd <= 128 ? 2 : 1; }          // K' and V' stages
 __host__ __device__ constexpr int kv_p_tile(int hd) { return 128 * kv_p_hdp(hd) * 2; }   // bytes of Q, K', V' tiles
 __host__ __device__ constexpr int kv_p_smem(int hd) {
-  return 1024 + (kv_p_qt(hd) + 2 * kv_p_st(hd)) * kv_p_tile(hd) + (kv_p_qt(hd) + kv_p_st(hd)) * kKvPZero + kKvPScales * (kKvPN * 8 + 16) + 256;
+  return 1024 + (kv_p_qt(hd) + 2 * kv_p_st(hd)) * kv_p_tile(hd) + (kv_p_qt(hd) + kv_p_st(hd)) * kKvPZero + kKvPScales * (kKvPN * 8 + 32) + 256;
 }
 
 struct KvPromptSplit {
@@ -176,10 +177,10 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 // The weights of 16 rows (lane (g, q): rows g and g + 8) for 64 keys: pk the fp16 pairs
 // exp2(S * scale_k - m) * scale_v; the lane's share of the rows' sums of the weights without scale_v.
 // sk, sv: shared-memory addresses of the scales of the lane's 16 keys (8i + 2q, 8i + 2q + 1).  kMask: a
-// row sees its first `seen` keys only.
+// row sees its first `seen` keys only, without those whose bits are set in the two words at sg.
 template <bool kMask>
-__device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_t sv, const float* m, const int* seen, int q, uint32_t* pk,
-                                           float* add) {
+__device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_t sv, const float* m, const int* seen, uint32_t sg, int q,
+                                           uint32_t* pk, float* add) {
   const uint64_t minus[2] = {pack2(-m[0], -m[0]), pack2(-m[1], -m[1])};
   uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -187,6 +188,7 @@ __device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_
     uint32_t v[16];
     tmem_ld_rows32(s_addr + 32 * c, v);
     const uint4 k4[2] = {lds128(sk + 32 * c), lds128(sk + 32 * c + 16)}, v4[2] = {lds128(sv + 32 * c), lds128(sv + 32 * c + 16)};
+    const uint32_t out = kMask ? lds32(sg + 4 * c) >> (2 * q) : 0;  // bits 8j, 8j + 1: the lane's keys
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -198,15 +200,15 @@ __device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_
       for (int a = 0; a < 2; ++a) {
         float2 y = unpack2(fma2(pack2(__uint_as_float(v[4 * j + 2 * a]), __uint_as_float(v[4 * j + 2 * a + 1])), ks, minus[a]));
         if (kMask) {
-          if (col >= seen[a]) y.x = -INFINITY;
-          if (col + 1 >= seen[a]) y.y = -INFINITY;
+          if (col >= seen[a] || (out >> (8 * j) & 1u)) y.x = -INFINITY;
+          if (col + 1 >= seen[a] || (out >> (8 * j) & 2u)) y.y = -INFINITY;
         }
         const uint64_t p = pack2(ex2(y.x), ex2(y.y));
         sum[a] = add2(sum[a], p);
         float2 w = unpack2(mul2(p, vs));
         if (kMask) {  // (a hidden key's scale may be NaN)
-          if (col >= seen[a]) w.x = 0.f;
-          if (col + 1 >= seen[a]) w.y = 0.f;
+          if (col >= seen[a] || (out >> (8 * j) & 1u)) w.x = 0.f;
+          if (col + 1 >= seen[a] || (out >> (8 * j) & 2u)) w.y = 0.f;
         }
         pk[8 * c + 2 * j + a] = pack_halves<false>(w.x, w.y);
       }
@@ -219,12 +221,13 @@ __device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_
   }
 }
 // The largest S * scale_k of the two rows over the 64 keys (whole rows: all four lanes get it).
-__device__ __forceinline__ void kv_row_max(uint32_t s_addr, uint32_t sk, const int* seen, int q, float* mx) {
+__device__ __forceinline__ void kv_row_max(uint32_t s_addr, uint32_t sk, const int* seen, uint32_t sg, int q, float* mx) {
   mx[0] = mx[1] = -INFINITY;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     uint32_t v[16];
     tmem_ld_rows32(s_addr + 32 * c, v);
+    const uint32_t out = lds32(sg + 4 * c) >> (2 * q);
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -232,8 +235,8 @@ __device__ __forceinline__ void kv_row_max(uint32_t s_addr, uint32_t sk, const i
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const int col = 32 * c + 8 * j + 2 * q;
-        if (col < seen[a]) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a]) * __uint_as_float(k.x));
-        if (col + 1 < seen[a]) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a + 1]) * __uint_as_float(k.y));
+        if (col < seen[a] && !(out >> (8 * j) & 1u)) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a]) * __uint_as_float(k.x));
+        if (col + 1 < seen[a] && !(out >> (8 * j) & 2u)) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a + 1]) * __uint_as_float(k.y));
       }
     }
   }
@@ -303,7 +306,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   const uint32_t sQ = base, sK = sQ + kQt * kTile, sV = sK + kSt * kTile, sQz = sV + kSt * kTile;
   const uint32_t sKz = sQz + kQt * kKvPZero, sScale = sKz + kSt * kKvPZero;
   const uint32_t sTop = sScale + kKvPScales * kKvPN * 8;  // [ring][4] largest scale_v of the warps' keys
-  const uint32_t bars = sTop + kKvPScales * 16;
+  const uint32_t sGone = sTop + kKvPScales * 16;          // [ring] 128 bits: the keys that are past the end or of a missing page
+  const uint32_t bars = sGone + kKvPScales * 16;
   const uint32_t kfull_b = bars, kempty_b = bars + 16, vfull_b = bars + 32, vempty_b = bars + 48;
   // (per row tile t and half h of a key tile: [t][h], one phase per key tile each)
   const uint32_t sfull_b = bars + 64, pfull_b = bars + 96, odone_b = bars + 128, drain_b = bars + 160, qsum_b = bars + 168;
@@ -410,7 +414,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   const bool is_v = warp >= kKvPConv + 4;
   uint4 raw[kRaw];
   uint32_t pk = 0, pv = 0;
-  int64_t off = -1;  // the key's page in the tile to load next
+  bool there = false;  // whether raw, pk and pv are a key's
+  int64_t off = -1;    // the key's page in the tile to load next
   const auto find = [&](int kt) {
     const int pos = (t0 + kt) * kKvPN + key;
     off = kt < nt && pos < n ? kv_page_offset(a.C, a.B, seq, pos >> a.C.page_shift) : -1;
@@ -418,8 +423,9 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   const auto load = [&](int kt) {
 #pragma unroll
     for (int i = 0; i < kRaw; ++i) raw[i] = make_uint4(0, 0, 0, 0);
-    pk = pv = 0;  // places past the end: scale and zero 0
-    if (off >= 0) {
+    pk = pv = 0;  // places past the end and of missing pages: scale and zero 0
+    there = off >= 0;
+    if (there) {
       const int in = ((t0 + kt) * kKvPN + key) & (a.C.page_size - 1);
       const uint8_t* block = a.C.pages + off + kvh * a.C.head_bytes;
 #pragma unroll
@@ -535,13 +541,19 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
           break;
         }
         tc_fence_after();
-        // log2 of the largest scale_v of the tile, rounded up (NaN scales are left out; all zero: 2^-30)
+        // log2 of the largest scale_v of the tile, rounded up (NaN scales are left out; all zero: 2^-30); bit 31
+        // of a word says that some of its keys are gone
         const uint4 tops = lds128(sTop + ring * 16);
-        const uint32_t top = max(max(tops.x, tops.y), max(tops.z, tops.w));
+        uint32_t top = max(max(tops.x, tops.y), max(tops.z, tops.w));
+        const bool plain_half = whole && !(top >> 31);
+        if (top >> 31) {
+          constexpr uint32_t kSize = 0x7fffffffu;
+          top = max(max(tops.x & kSize, tops.y & kSize), max(tops.z & kSize, tops.w & kSize));
+        }
         const float ev = static_cast<float>(max(-30, static_cast<int>(top >> 23) - 126));
         uint32_t pk[16];
         float add[2];
-        const uint32_t addr = s_addr + 64 * h, sk = sc + 256 * h + 64 * q, sv = sk + 512;
+        const uint32_t addr = s_addr + 64 * h, sk = sc + 256 * h + 64 * q, sv = sk + 512, sg = sGone + ring * 16 + 8 * h;
         const int seen[2] = {lim[0] - kb - 64 * h, lim[1] - kb - 64 * h};
         // A row moves m when its weights' sum (the lane's share) says that one times scale_v may pass 2^12,
         // or when it has seen no key yet.
@@ -550,7 +562,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         for (;;) {
           if (moved) {
             float mx[2], corr[2];
-            kv_row_max(addr, sk, seen, q, mx);
+            kv_row_max(addr, sk, seen, sg, q, mx);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const bool first = fresh[r] && mx[r] > -INFINITY;
@@ -574,8 +586,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
               }
             }
           }
-          if (whole) kv_weights<false>(addr, sk, sv, m, seen, q, pk, add);
-          else kv_weights<true>(addr, sk, sv, m, seen, q, pk, add);
+          if (plain_half) kv_weights<false>(addr, sk, sv, m, seen, sg, q, pk, add);
+          else kv_weights<true>(addr, sk, sv, m, seen, sg, q, pk, add);
           if (moved || !__any_sync(0xffffffffu, fmaxf(add[0], add[1]) > ex2(12.f - ev))) break;
           moved = true;
         }
@@ -729,8 +741,12 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         const uint32_t z_at = sKz + st * kKvPZero + kv_rows32_off(key);
         sts128(z_at, make_uint4(__float_as_uint(z1), __float_as_uint(z2), __float_as_uint(z1), __float_as_uint(z2)));
         sts128(z_at + 128, make_uint4(__float_as_uint(z1), 0, 0, 0));
-        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size));
-        if (lane == 0) asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - kKvPConv)), "r"(top) : "memory");
+        const uint32_t gone = __ballot_sync(0xffffffffu, !there);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size)) | (gone ? 0x80000000u : 0u);
+        if (lane == 0) {
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - kKvPConv)), "r"(top) : "memory");
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(sGone + ring * 16 + 4 * (warp - kKvPConv)), "r"(gone) : "memory");
+        }
       }
       const __half2 zero = __half2half2(__ushort_as_half(static_cast<unsigned short>(pv >> 16)));
       const uint32_t tile = (is_v ? sV : sK) + st * kTile;
