@@ -33,7 +33,7 @@ namespace opc {
 //                 O rescaled and the half evaluated again -- always in the first tile, hardly ever later.
 //   warps 16..19  thread = key: reads its key codes (one tile ahead, in registers) and writes the K' row
 //                 in the 128-byte-swizzled layout, the scales, and a bit for each key of a missing page (the
-//                 softmax takes its masked path in such a tile: the bits keep them out of maximum and sum)
+//                 softmax then keeps them out of maximum and sum)
 //   warps 20..23  the same for V' -- the same layout is K-major for K' (rows are the N dimension) and
 //                 MN-major for V' (rows are the K dimension).  (Four warps for both took 1% longer.)
 //   warp 24       issues the MMAs and commits them to the roles' barriers (25..27 idle)
@@ -176,19 +176,26 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 
 // The weights of 16 rows (lane (g, q): rows g and g + 8) for 64 keys: pk the fp16 pairs
 // exp2(S * scale_k - m) * scale_v; the lane's share of the rows' sums of the weights without scale_v.
-// sk, sv: shared-memory addresses of the scales of the lane's 16 keys (8i + 2q, 8i + 2q + 1).  kMask: a
-// row sees its first `seen` keys only, without those whose bits are set in the two words at sg.
-template <bool kMask>
-__device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_t sv, const float* m, const int* seen, uint32_t sg, int q,
-                                           uint32_t* pk, float* add) {
+// sk, sv: shared-memory addresses of the scales of the lane's 16 keys (8i + 2q, 8i + 2q + 1).  kMode 1: a
+// row sees its first `seen` keys only.  2: and of those none whose bit is set in the two words at sg; its
+// scores are multiplied by its factor, at sf (row g + 8: sf + 64), and rounded as in kv_row_max, so that a
+// maximum of any size meets itself.
+template <int kMode>
+__device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_t sv, const float* m, const int* seen, uint32_t sg,
+                                           uint32_t sf, int q, uint32_t* pk, float* add) {
   const uint64_t minus[2] = {pack2(-m[0], -m[0]), pack2(-m[1], -m[1])};
+  float factor[2] = {1.f, 1.f};
+  if (kMode == 2) {
+    factor[0] = __uint_as_float(lds32(sf));
+    factor[1] = __uint_as_float(lds32(sf + 64));
+  }
   uint64_t sum[2] = {0, 0};
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     uint32_t v[16];
     tmem_ld_rows32(s_addr + 32 * c, v);
     const uint4 k4[2] = {lds128(sk + 32 * c), lds128(sk + 32 * c + 16)}, v4[2] = {lds128(sv + 32 * c), lds128(sv + 32 * c + 16)};
-    const uint32_t out = kMask ? lds32(sg + 4 * c) >> (2 * q) : 0;  // bits 8j, 8j + 1: the lane's keys
+    const uint32_t out = kMode == 2 ? lds32(sg + 4 * c) >> (2 * q) : 0;  // bits 8j, 8j + 1: the lane's keys
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -198,15 +205,23 @@ __device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_
       const uint64_t vs = pack2(__uint_as_float((j & 1) ? vv.z : vv.x), __uint_as_float((j & 1) ? vv.w : vv.y));
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
-        float2 y = unpack2(fma2(pack2(__uint_as_float(v[4 * j + 2 * a]), __uint_as_float(v[4 * j + 2 * a + 1])), ks, minus[a]));
-        if (kMask) {
+        const float s0 = __uint_as_float(v[4 * j + 2 * a]), s1 = __uint_as_float(v[4 * j + 2 * a + 1]);
+        float2 y;
+        if (kMode == 2) {
+          const float2 k = unpack2(ks);
+          y.x = __fsub_rn(__fmul_rn(s0, k.x * factor[a]), m[a]);
+          y.y = __fsub_rn(__fmul_rn(s1, k.y * factor[a]), m[a]);
+        } else {
+          y = unpack2(fma2(pack2(s0, s1), ks, minus[a]));
+        }
+        if (kMode) {
           if (col >= seen[a] || (out >> (8 * j) & 1u)) y.x = -INFINITY;
           if (col + 1 >= seen[a] || (out >> (8 * j) & 2u)) y.y = -INFINITY;
         }
         const uint64_t p = pack2(ex2(y.x), ex2(y.y));
         sum[a] = add2(sum[a], p);
         float2 w = unpack2(mul2(p, vs));
-        if (kMask) {  // (a hidden key's scale may be NaN)
+        if (kMode) {  // (a hidden key's scale may be NaN)
           if (col >= seen[a] || (out >> (8 * j) & 1u)) w.x = 0.f;
           if (col + 1 >= seen[a] || (out >> (8 * j) & 2u)) w.y = 0.f;
         }
@@ -220,14 +235,20 @@ __device__ __forceinline__ void kv_weights(uint32_t s_addr, uint32_t sk, uint32_
     add[a] = x.x + x.y;
   }
 }
-// The largest S * scale_k of the two rows over the 64 keys (whole rows: all four lanes get it).
-__device__ __forceinline__ void kv_row_max(uint32_t s_addr, uint32_t sk, const int* seen, uint32_t sg, int q, float* mx) {
+// The largest S * scale_k (kAny: * factor, as in kv_weights) of the two rows over the 64 keys (whole rows: all four lanes get it).
+template <bool kAny>
+__device__ __forceinline__ void kv_row_max(uint32_t s_addr, uint32_t sk, const int* seen, uint32_t sg, uint32_t sf, int q, float* mx) {
   mx[0] = mx[1] = -INFINITY;
+  float f[2] = {1.f, 1.f};
+  if (kAny) {
+    f[0] = __uint_as_float(lds32(sf));
+    f[1] = __uint_as_float(lds32(sf + 64));
+  }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     uint32_t v[16];
     tmem_ld_rows32(s_addr + 32 * c, v);
-    const uint32_t out = lds32(sg + 4 * c) >> (2 * q);
+    const uint32_t out = kAny ? lds32(sg + 4 * c) >> (2 * q) : 0;
     tmem_wait_ld();
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -235,8 +256,8 @@ __device__ __forceinline__ void kv_row_max(uint32_t s_addr, uint32_t sk, const i
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const int col = 32 * c + 8 * j + 2 * q;
-        if (col < seen[a] && !(out >> (8 * j) & 1u)) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a]) * __uint_as_float(k.x));
-        if (col + 1 < seen[a] && !(out >> (8 * j) & 2u)) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a + 1]) * __uint_as_float(k.y));
+        if (col < seen[a] && !(out >> (8 * j) & 1u)) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a]) * (__uint_as_float(k.x) * f[a]));
+        if (col + 1 < seen[a] && !(out >> (8 * j) & 2u)) mx[a] = fmaxf(mx[a], __uint_as_float(v[4 * j + 2 * a + 1]) * (__uint_as_float(k.y) * f[a]));
       }
     }
   }
@@ -295,18 +316,19 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   constexpr int kBlock = 16384;                 // bytes of 128 rows x 64 columns
   constexpr int kRaw = kHd / 32;                // 16-byte pieces of a key's codes
   extern __shared__ __align__(1024) unsigned char smem_raw[];
-  __shared__ uint32_t sm_big, sm_tmem;
+  __shared__ uint32_t sm_tmem, sm_top, sm_low;
+  __shared__ int sm_power, sm_uneven;  // of q as staged (below)
   __shared__ int sm_last;
   __shared__ struct {
     uint32_t item, first, rec;  // the item, its first record, this CTA's record
     int splits, r0;
   } sm_item;  // what the results need (in registers it would cost the loop between)
-  __shared__ float2 sm_rows[kQt * kKvPM];  // (m, sum) of the rows
+  __shared__ float2 sm_rows[kQt * kKvPM];  // of the rows: (largest |q|, factor of the scores), then (m, sum)
   const uint32_t base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = base, sK = sQ + kQt * kTile, sV = sK + kSt * kTile, sQz = sV + kSt * kTile;
   const uint32_t sKz = sQz + kQt * kKvPZero, sScale = sKz + kSt * kKvPZero;
   const uint32_t sTop = sScale + kKvPScales * kKvPN * 8;  // [ring][4] largest scale_v of the warps' keys
-  const uint32_t sGone = sTop + kKvPScales * 16;          // [ring] 128 bits: the keys that are past the end or of a missing page
+  const uint32_t sGone = sTop + kKvPScales * 16;          // [ring] 128 bits: the keys of missing pages
   const uint32_t bars = sGone + kKvPScales * 16;
   const uint32_t kfull_b = bars, kempty_b = bars + 16, vfull_b = bars + 32, vempty_b = bars + 48;
   // (per row tile t and half h of a key tile: [t][h], one phase per key tile each)
@@ -328,7 +350,9 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     mbar_init(drain_b, 1);
     mbar_init(qsum_b, 4 * kQt);
     fence_mbar_init();
-    sm_big = 0;
+    sm_power = sm_uneven = 0;
+    sm_top = 0;
+    sm_low = 0x7f800000u;
   }
   griddep_wait();
   griddep_launch_dependents();
@@ -405,6 +429,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm_tmem)), "r"(512) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
+  if (tid < kQt * kKvPM) sm_rows[tid] = make_float2(0.f, 1.f);
   __syncthreads();
 
   // ---------------------------------------------------------------- the converters' first loads
@@ -414,7 +439,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   const bool is_v = warp >= kKvPConv + 4;
   uint4 raw[kRaw];
   uint32_t pk = 0, pv = 0;
-  bool there = false;  // whether raw, pk and pv are a key's
+  bool gone = false;   // whether the key in raw, pk and pv is of a missing page
   int64_t off = -1;    // the key's page in the tile to load next
   const auto find = [&](int kt) {
     const int pos = (t0 + kt) * kKvPN + key;
@@ -424,8 +449,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
 #pragma unroll
     for (int i = 0; i < kRaw; ++i) raw[i] = make_uint4(0, 0, 0, 0);
     pk = pv = 0;  // places past the end and of missing pages: scale and zero 0
-    there = off >= 0;
-    if (there) {
+    gone = off < 0 && (t0 + kt) * kKvPN + key < n;
+    if (off >= 0) {
       const int in = ((t0 + kt) * kKvPN + key) & (a.C.page_size - 1);
       const uint8_t* block = a.C.pages + off + kvh * a.C.head_bytes;
 #pragma unroll
@@ -438,11 +463,13 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   if (converter) find(0);
 
   // ---------------------------------------------------------------- q, by all threads
-  // the power of two that q is multiplied by (bf16: fp16 has less range; one for the whole tile pair, that
-  // puts its largest near 2^14)
-  const auto q_power = [&]() {
-    const float top = __uint_as_float(*const_cast<volatile uint32_t*>(&sm_big));
-    return a.bf16 ? max(-99, min(99, top > 0.f ? 14 - ((__float_as_int(top) >> 23) - 127) : 0)) : 0;
+  // bf16 q goes in multiplied by a power of two that puts its largest near 2^14 (fp16 has less range): one
+  // for the whole tile pair, which the keys' scales take back, where every row's largest reaches 2^-12 of the
+  // pair's (what is rounded then lies 2^-27 below its row's largest, less than the sums in fp32 round).  Else
+  // each row has its own, and its scores are multiplied by its factor (kMode 2).  Rows with an infinity or
+  // NaN stay out of the choice: they give NaN with any factor.
+  const auto power_of = [](uint32_t big) {
+    return big ? max(-99, min(99, 14 - (static_cast<int>(big >> 23) - 127))) : 0;
   };
   {
     constexpr int kChunks = kHd / 8, kAll = kQt * kKvPM * kChunks, kMine = (kAll + kKvPThreads - 1) / kKvPThreads;
@@ -455,20 +482,59 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       if (x < kAll && row < R) v[i] = a.vec ? ld_row8<true>(src) : ld_row8<false>(src);
     }
     if (a.bf16) {
-      float big = 0.f;
+      uint32_t top = 0, low = 0x7f800000u;  // of finite chunks of 8; of chunks that are not 0
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        float x[8];
+        float x[8], big = 0.f;
         unpack_halves<true>(v[i], x);
 #pragma unroll
         for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+        const uint32_t b = __float_as_uint(big);
+        if (b < 0x7f800000u) top = max(top, b);
+        if (b) low = min(low, b);
       }
-      big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
-      if (lane == 0) atomicMax(&sm_big, __float_as_uint(big));
+      top = __reduce_max_sync(0xffffffffu, top);
+      low = __reduce_min_sync(0xffffffffu, low);
+      if (lane == 0) {
+        atomicMax(&sm_top, top);
+        atomicMin(&sm_low, low);
+      }
       __syncthreads();
-      const float up = pow2i(q_power());
+      top = *const_cast<volatile uint32_t*>(&sm_top);
+      bool uneven = *const_cast<volatile uint32_t*>(&sm_low) + (12u << 23) < top;
+      if (uneven) {  // some chunk is that small: is a whole row?
+        // (a row's chunks are kChunks lanes in a row: those of an aligned span of them meet in registers)
+        constexpr int kSpan = kChunks % 32 == 0 ? 32 : kChunks % 16 == 0 ? 16 : kChunks % 8 == 0 ? 8 : 4;
+        static_assert(kChunks % kSpan == 0 && kAll % 32 == 0, "a span of lanes is of one row");
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) {
+          float x[8], big = 0.f;
+          unpack_halves<true>(v[i], x);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
+#pragma unroll
+          for (int o = 1; o < kSpan; o <<= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+          const int at = i * kKvPThreads + tid;
+          if (at < kAll && (lane & (kSpan - 1)) == 0) atomicMax(reinterpret_cast<uint32_t*>(&sm_rows[at / kChunks].x), __float_as_uint(big));
+        }
+        __syncthreads();
+        low = 0x7f800000u;
+#pragma unroll
+        for (int i = 0; i < kQt * kKvPM; i += 32) {
+          const uint32_t big = __float_as_uint(sm_rows[i + lane].x);
+          if (big) low = min(low, big);
+        }
+        uneven = __reduce_min_sync(0xffffffffu, low) + (12u << 23) < top;
+      }
+      if (tid == 0) {
+        sm_power = uneven ? 0 : power_of(top);
+        sm_uneven = uneven;
+      }
+      if (uneven && tid < kQt * kKvPM) sm_rows[tid].y = pow2i(-power_of(__float_as_uint(sm_rows[tid].x)));
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
+        const int at = i * kKvPThreads + tid;
+        const float up = pow2i(power_of(uneven && at < kAll ? __float_as_uint(sm_rows[at / kChunks].x) : top));
         float x[8];
         unpack_halves<true>(v[i], x);
         v[i] = make_uint4(pack_halves<false>(x[0] * up, x[1] * up), pack_halves<false>(x[2] * up, x[3] * up),
@@ -529,6 +595,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     }
     // tiles below need no mask (rows that do not exist see nothing; the first row sees the fewest)
     const int plain = first_row + 15 < R ? max(0, min(n, pos0 + first_row / a.group + 1)) : 0;
+    bool any = sm_uneven != 0;  // everything in kMode 2
+    const uint32_t factors = smem_u32(&sm_rows[t * kKvPM + lane0 + g].y);  // of row g; of g + 8 64 bytes on
     for (int kt = 0; kt < nt; ++kt) {
       const int kb = (t0 + kt) * kKvPN, ring = kt % kKvPScales;
       const uint32_t sc = sScale + ring * kKvPN * 8;
@@ -545,8 +613,9 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         // of a word says that some of its keys are gone
         const uint4 tops = lds128(sTop + ring * 16);
         uint32_t top = max(max(tops.x, tops.y), max(tops.z, tops.w));
-        const bool plain_half = whole && !(top >> 31);
+        bool full = any;
         if (top >> 31) {
+          full = true;
           constexpr uint32_t kSize = 0x7fffffffu;
           top = max(max(tops.x & kSize, tops.y & kSize), max(tops.z & kSize, tops.w & kSize));
         }
@@ -562,16 +631,20 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         for (;;) {
           if (moved) {
             float mx[2], corr[2];
-            kv_row_max(addr, sk, seen, sg, q, mx);
+            if (full) kv_row_max<true>(addr, sk, seen, sg, factors, q, mx);
+            else kv_row_max<false>(addr, sk, seen, sg, factors, q, mx);
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const bool first = fresh[r] && mx[r] > -INFINITY;
-              const float up = first || mx[r] + ev > m[r] ? mx[r] + ev - m[r] : 0.f;
-              corr[r] = first ? 1.f : ex2(-up);
-              m[r] += up;
+              const float to = first || mx[r] + ev > m[r] ? mx[r] + ev : m[r];
+              corr[r] = first ? 1.f : ex2(m[r] - to);
+              m[r] = to;
               T[r] *= corr[r];
               fresh[r] = fresh[r] && !first;
             }
+            // scores so large that products which are not rounded may differ from the maximum by more than the
+            // weights' range
+            if (__any_sync(0xffffffffu, fmaxf(fabsf(m[0]), fabsf(m[1])) > 1e6f)) full = any = true;
             if (kt + h > 0) {  // O holds the halves before
               if (!mbar_wait_bounded(odone_b + 16 * t + 8 * (1 - h), (kt + h - 1) & 1)) ok = false;
               tc_fence_after();
@@ -586,8 +659,9 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
               }
             }
           }
-          if (plain_half) kv_weights<false>(addr, sk, sv, m, seen, sg, q, pk, add);
-          else kv_weights<true>(addr, sk, sv, m, seen, sg, q, pk, add);
+          if (full) kv_weights<2>(addr, sk, sv, m, seen, sg, factors, q, pk, add);
+          else if (whole) kv_weights<0>(addr, sk, sv, m, seen, sg, factors, q, pk, add);
+          else kv_weights<1>(addr, sk, sv, m, seen, sg, factors, q, pk, add);
           if (moved || !__any_sync(0xffffffffu, fmaxf(add[0], add[1]) > ex2(12.f - ev))) break;
           moved = true;
         }
@@ -723,7 +797,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       load(0);
     }
     find(1);
-    const float qf = a.scale * 1.4426950408889634f * pow2i(-q_power());  // factor of the scores (log2 units)
+    const float qf = a.scale * 1.4426950408889634f * pow2i(-sm_power);  // factor of the scores (log2 units)
     for (int kt = 0; kt < nt; ++kt) {
       const int st = kt % kSt, ring = kt % kKvPScales;
       if (kt >= kSt && !mbar_wait_bounded((is_v ? vempty_b : kempty_b) + 8 * st, ((kt / kSt) - 1) & 1)) {
@@ -741,11 +815,11 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         const uint32_t z_at = sKz + st * kKvPZero + kv_rows32_off(key);
         sts128(z_at, make_uint4(__float_as_uint(z1), __float_as_uint(z2), __float_as_uint(z1), __float_as_uint(z2)));
         sts128(z_at + 128, make_uint4(__float_as_uint(z1), 0, 0, 0));
-        const uint32_t gone = __ballot_sync(0xffffffffu, !there);
-        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size)) | (gone ? 0x80000000u : 0u);
+        const uint32_t out = __ballot_sync(0xffffffffu, gone);
+        const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(size)) | (out ? 0x80000000u : 0u);
         if (lane == 0) {
           asm volatile("st.shared.u32 [%0], %1;" ::"r"(sTop + ring * 16 + 4 * (warp - kKvPConv)), "r"(top) : "memory");
-          asm volatile("st.shared.u32 [%0], %1;" ::"r"(sGone + ring * 16 + 4 * (warp - kKvPConv)), "r"(gone) : "memory");
+          asm volatile("st.shared.u32 [%0], %1;" ::"r"(sGone + ring * 16 + 4 * (warp - kKvPConv)), "r"(out) : "memory");
         }
       }
       const __half2 zero = __half2half2(__ushort_as_half(static_cast<unsigned short>(pv >> 16)));
