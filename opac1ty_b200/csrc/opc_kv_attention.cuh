@@ -33,7 +33,7 @@ struct KvAttnArgs {
 //   scores    A = 16 keys x 16 dimensions of codes, B = 16 dimensions x 8 rows of q; then
 //             score = scale_k * (q . code + zero_k * sum q), the sums in fp32.  q is multiplied by a
 //             power of two per row (its largest value near 2^14), and by 1/16 where it meets the
-//             2^-20 codes, so fp16 and bf16 queries enter exactly.
+//             2^-20 codes, so fp16 and bf16 queries enter exactly down to 2^-39 of their row's largest.
 //   values    A = 16 dimensions x 16 keys (the codes of two keys interleaved by byte permutes),
 //             B = 16 keys x 8 rows of weights: the score tile's accumulators are already the
 //             transposed fragments that movmatrix turns into B.  A weight carries its key's scale,
@@ -245,39 +245,34 @@ struct KvItem {
 
 // The rows of q as B fragments in an item's slot, from the elements each lane holds (row g of each
 // row tile, dimensions q*kHd/4 + 8d + 0..7): multiplication s of code word d meets codes (2s, 2s + 4)
-// in the first register, (2s + 1, 2s + 5), which are 16 times larger, in the second.  fp16 queries go
-// in as they are (a sixteenth of one below 2^-10 is rounded, by 2^-25 at most); bf16 ones, whose
-// range is wider, are first multiplied by the power of two that puts the row's largest near 2^14.
+// in the first register, (2s + 1, 2s + 5), which are 16 times larger, in the second and so have to go in
+// by the sixteenth.  A row is first multiplied by the power of two that puts its largest near 2^14 (fp16
+// ones only upwards): what is rounded then, of elements below 2^-10, lies 2^-39 below the row's largest.
 // Behind the fragments, per row: the factor of its scores (log2 units) and the sum of its elements.
 template <int kHd, int kNT, bool kBf>
 __device__ __forceinline__ void kv_stage_q(const uint4 (&raw)[kNT][kHd / 32], uint32_t slot_s, float scale, int lane) {
   const __half2 sixteenth = __float2half2_rn(0.0625f);
 #pragma unroll
   for (int t = 0; t < kNT; ++t) {
-    int e2 = 0;
-    if (kBf) {
-      float big = 0.f;
+    float big = 0.f;
 #pragma unroll
-      for (int d = 0; d < kHd / 32; ++d) {
-        float x[8];
-        unpack_halves<kBf>(raw[t][d], x);
+    for (int d = 0; d < kHd / 32; ++d) {
+      float x[8];
+      unpack_halves<kBf>(raw[t][d], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
-      }
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
-      big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-      // |e2| is kept below 100 (a query beyond fp32's reach overflows)
-      e2 = max(-99, min(99, big > 0.f ? 14 - ((__float_as_int(big) >> 23) - 127) : 0));
+      for (int e = 0; e < 8; ++e) big = fmaxf(big, fabsf(x[e]));
     }
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
+    big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
+    // |e2| is kept below 100 (a query beyond fp32's reach overflows)
+    const int e2 = max(kBf ? -99 : 0, min(99, big > 0.f ? 14 - ((__float_as_int(big) >> 23) - 127) : 0));
+    const float up = pow2i(e2);
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int d = 0; d < kHd / 32; ++d) {
       uint32_t w[4] = {raw[t][d].x, raw[t][d].y, raw[t][d].z, raw[t][d].w};
-      if (kBf) {
-        const float up = pow2i(e2);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[i] = pack_halves<false>(half_lo<true>(w[i]) * up, half_hi<true>(w[i]) * up);
-      }
+      for (int i = 0; i < 4; ++i) w[i] = pack_halves<false>(half_lo<kBf>(w[i]) * up, half_hi<kBf>(w[i]) * up);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const float2 f = unpack_half2(w[i]);

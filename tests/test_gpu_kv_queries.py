@@ -50,3 +50,16 @@ def test_rows_beside_odd_bf16_queries(cuda_device, hd, page, heads, kv_heads, q_
         q[2, 1] = 0.0
         q[last, heads - 1] *= 2.0 ** -20
     run(su, cuda_device, q, pages)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,heads,kv_heads", [(128, 8, 2), (64, 3, 1), (256, 4, 1)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 2, 1], [1, 2, 3, 300]), ([40], [40])])
+@pytest.mark.parametrize("small", [2.0 ** -12, 2.0 ** -14, 2.0 ** -18])
+def test_tiny_queries_and_a_large_scale(cuda_device, hd, heads, kv_heads, q_lens, kv_lens, dtype, small):
+    # Scores of ordinary size from queries near fp16's smallest; rows that see one key show a score as
+    # their log sum.
+    rng = np.random.default_rng(hd + int(1 / small))
+    su = Setup(cuda_device, q_lens, kv_lens, kv_heads, hd, 32)
+    q = (rows(rng, su.rows, heads, hd, torch.float32, cuda_device) * small).to(dtype)
+    run(su, cuda_device, q, filled_pages(rng, su.n_pages, kv_heads, 32, hd), scale=hd ** -0.5 / small)
