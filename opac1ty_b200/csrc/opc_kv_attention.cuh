@@ -69,6 +69,7 @@ constexpr int kKvStepWarps = 4;               // consumers
 constexpr int kKvStepThreads = (kKvStepWarps + 1) * 32;
 constexpr int kKvMinStages = 2;               // stages per CTA below which fewer CTAs take part
 constexpr int kKvFold = 8;                    // stages between two foldings of the zeros' share
+constexpr float kKvNone = -3.402823466e38f;   // the maximum of no keys: below every finite score
 constexpr int kKvItemCost = 3;                // what an item costs beside its stages, in stages
 __host__ __device__ constexpr int kv_stage_bytes(int hd) { return kKvStage * (hd + 8); }
 // CTAs per SM: bounded by the accumulators' registers and the shared memory of a record.
@@ -193,7 +194,7 @@ __device__ __forceinline__ void kv_merge_records(const KvAttnArgs& a, const KvSp
 #pragma unroll 1
     for (int i = tid; i < R * kQ; i += kThreads) {
       const int row = i / kQ, d = 4 * (i - row * kQ);
-      float M = -1e30f, T = 0.f;
+      float M = kKvNone, T = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       const float* src = smem + row * kRec;
 #pragma unroll 4
@@ -573,7 +574,7 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       az[t][c] = ahead[t][c] = sum[t][c] = 0.f;
-      m[t][c] = -1e30f;
+      m[t][c] = kKvNone;
     }
   }
   int ve = -30;             // the weights carry scale_v * 2^-ve
@@ -806,7 +807,7 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
   constexpr int kQ = kHd / 4;  // float4 columns of a row
   for (int i = tid; i < R * kQ; i += kKvStepWarps * 32) {
     const int row = i / kQ, d = 4 * (i - row * kQ);
-    float M = -1e30f, T = 0.f;
+    float M = kKvNone, T = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     float mw[kKvStepWarps];
 #pragma unroll

@@ -684,7 +684,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     for (int r = 0; r < 2; ++r) {
       T[r] += __shfl_xor_sync(0xffffffffu, T[r], 1);
       T[r] += __shfl_xor_sync(0xffffffffu, T[r], 2);
-      if (q == 0) sm_rows[t * kKvPM + lane0 + 8 * r + g] = make_float2(lim[r] > 0 && !fresh[r] ? m[r] : -1e30f, T[r]);
+      if (q == 0) sm_rows[t * kKvPM + lane0 + 8 * r + g] = make_float2(lim[r] > 0 && !fresh[r] ? m[r] : kKvNone, T[r]);
     }
     named_barrier(2 + t, 256);
     const int in = tid & 127, tile_row = t * kKvPM + in;
@@ -750,7 +750,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
       named_barrier(4, 2 * kRows);
       if (sm_last && live && ok) {  // merge, in order: thread = row and every other 16 dimensions
         const float* part = sp.part + static_cast<int64_t>(sm_item.first) * (kRows * (kHd + 4));
-        float M = -1e30f, S = 0.f;
+        float M = kKvNone, S = 0.f;
 #pragma unroll 4
         for (int i = 0; i < n_rec; ++i) {
           const float2 w = __ldcg(reinterpret_cast<const float2*>(part + i * (kRows * (kHd + 4)) + kRows * kHd + 2 * tile_row));

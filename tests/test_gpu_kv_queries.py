@@ -63,3 +63,15 @@ def test_tiny_queries_and_a_large_scale(cuda_device, hd, heads, kv_heads, q_lens
     su = Setup(cuda_device, q_lens, kv_lens, kv_heads, hd, 32)
     q = (rows(rng, su.rows, heads, hd, torch.float32, cuda_device) * small).to(dtype)
     run(su, cuda_device, q, filled_pages(rng, su.n_pages, kv_heads, 32, hd), scale=hd ** -0.5 / small)
+
+
+@pytest.mark.parametrize("dtype", [F16, BF16])
+@pytest.mark.parametrize("hd,heads,kv_heads", [(128, 8, 2), (64, 3, 1), (256, 4, 1)])
+@pytest.mark.parametrize("q_lens,kv_lens", [([1, 1, 2, 1], [1, 2, 300, 4000]), ([40], [40]), ([40], [1500])])
+@pytest.mark.parametrize("scale", [1e6, 1e31])
+def test_scores_far_below_zero(cuda_device, hd, heads, kv_heads, q_lens, kv_lens, dtype, scale):
+    # every score of a row is hugely negative, and the largest of them takes all of the weight
+    rng = np.random.default_rng(hd + sum(kv_lens))
+    su = Setup(cuda_device, q_lens, kv_lens, kv_heads, hd, 32)
+    q = rows(rng, su.rows, heads, hd, dtype, cuda_device, mean=-0.5)
+    run(su, cuda_device, q, filled_pages(rng, su.n_pages, kv_heads, 32, hd, mean=1.0), scale=scale)
