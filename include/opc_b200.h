@@ -434,11 +434,16 @@ int opc_kv_read(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t dt
  *   out[r][h] = sum_j softmax_j(scale * q[r][h] . k[j][h / (heads/kv_heads)]) v[j][...]
  * over the positions j <= the row's own, with k and v as the cache holds them.  lse (may be NULL):
  * [n_tokens][heads] fp32, the natural logarithm of the softmax's sum.  A row that sees no key
- * gives out 0 and lse -infinity.  dtype (of q and out) OPC_F16 or OPC_BF16.  Statistics and sums in
- * fp32; deterministic.  The workspace (opc_kv_attention_workspace_bytes; 0 for a refused request)
- * is zero-filled once before first use (opc_workspace_init), is not to be shared with opc_gemv, and
- * serves any calls that are ordered on one stream; calls that may overlap, replays of two graphs
- * among them, need one each. */
+ * gives out 0 and lse -infinity.  dtype (of q and out) OPC_F16 or OPC_BF16.  Scores, statistics and
+ * sums are in fp32; the products with the values take fp16 factors: a weight is rounded by 2^-11 of
+ * itself or 2^-30 of the row's largest (as shares of scale_v, the largest of the keys so far), and
+ * where a sequence has many rows (q_len * heads/kv_heads above 16, or above 8 for head_dim 192 and
+ * 256; where all sequences may, also below) code + zero of a value by 2^-11 of itself.  lse has
+ * neither.  Deterministic.
+ * The workspace (opc_kv_attention_workspace_bytes; 0 for a refused request) is zero-filled once
+ * before first use (opc_workspace_init), is not to be shared with opc_gemv, and serves any calls
+ * that are ordered on one stream; calls that may overlap, replays of two graphs among them, need
+ * one each. */
 size_t opc_kv_attention_workspace_bytes(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads,
                                         int32_t device);
 int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads, int32_t dtype, float scale,

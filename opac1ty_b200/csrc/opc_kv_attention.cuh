@@ -45,8 +45,11 @@ struct KvAttnArgs {
 //             kKvFold stages, with half of the next stages' expected share in advance, so that they
 //             run through 0 and what is cut cancels (131071 keys: results off by 4.2e-4 of their norm
 //             without, 3.1e-4 with, 2.8e-4 being the roundings of the weights and of the result).
-//   maximum   m and e move only when a score passes m + 8 or a scale 2^(e+5) (one vote per tile):
-//             weights stay below 2^13, and the common tile has no shuffles and no rescaling.
+//   maximum   m and e move only when a score passes m + 7 or a scale 2^(e+8), 8 times the largest so far
+//             (one vote per tile): the common tile has no shuffles and no rescaling.  At a move 2^(e+5) lies
+//             above the largest scale, so that weights stay below 2^15 and a row's largest is near 2^5
+//             (kKvLift): what fp16 cannot hold, 2^-25, is 2^-30 of it (at 2^0 a key with nearly all of the
+//             weight and a value near 0 takes n * 2^-25 of the others' mean value away).
 //
 // The work -- for every sequence and kv head the stages of 128 keys -- is one line that the CTAs
 // (persistent, two or three per SM) cut into equal contiguous ranges, whatever the sequences'
@@ -69,6 +72,7 @@ constexpr int kKvStepWarps = 4;               // consumers
 constexpr int kKvStepThreads = (kKvStepWarps + 1) * 32;
 constexpr int kKvMinStages = 2;               // stages per CTA below which fewer CTAs take part
 constexpr int kKvFold = 8;                    // stages between two foldings of the zeros' share
+constexpr int kKvLift = 5;                    // log2 of a row's largest weight in fp16 when its reference is set
 constexpr float kKvNone = -3.402823466e38f;   // the maximum of no keys: below every finite score
 constexpr int kKvItemCost = 3;                // what an item costs beside its stages, in stages
 __host__ __device__ constexpr int kv_stage_bytes(int hd) { return kKvStage * (hd + 8); }
@@ -655,13 +659,13 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
               top[t][c] = fmaxf(top[t][c], x);
             }
         }
-      bool move = vmax * vinv > 32.f;
+      bool move = vmax * vinv > 256.f;
 #pragma unroll
-      for (int t = 0; t < kNT; ++t) move |= top[t][0] > m[t][0] + 8.f || top[t][1] > m[t][1] + 8.f;
+      for (int t = 0; t < kNT; ++t) move |= top[t][0] > m[t][0] + 7.f || top[t][1] > m[t][1] + 7.f;
       if (__any_sync(0xffffffffu, move)) {
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, o));
-        const int e = max(ve, min(17, (__float_as_int(vmax) >> 23) - 126));  // 2^e above every scale so far
+        const int e = max(ve, min(17, (__float_as_int(vmax) >> 23) - 126) - kKvLift);  // 2^(e + kKvLift) above every scale so far
         const float drop = pow2i(max(-126, ve - e));
         ve = e;
         vinv = pow2i(-e);

@@ -29,8 +29,9 @@ namespace opc {
 //                 from shared memory (with thread = row every thread would read all of them), and four
 //                 warps per SM sub-partition hide each other's latencies (two took twice as long).
 //                 The reference m of a row moves only when the sum of a half's weights says that one
-//                 times the tile's largest scale_v may pass 2^12: then the row's maximum is looked for,
-//                 O rescaled and the half evaluated again -- always in the first tile, hardly ever later.
+//                 times the tile's largest scale_v may pass 2^15: then the row's maximum is looked for,
+//                 O rescaled and the half evaluated again, its largest weight times that scale at 2^5
+//                 (kKvLift) -- always in the first tile, hardly ever later.
 //   warps 16..19  thread = key: reads its key codes (one tile ahead, in registers) and writes the K' row
 //                 in the 128-byte-swizzled layout, the scales, and a bit for each key of a missing page (the
 //                 softmax then keeps them out of maximum and sum)
@@ -624,7 +625,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
         float add[2];
         const uint32_t addr = s_addr + 64 * h, sk = sc + 256 * h + 64 * q, sv = sk + 512, sg = sGone + ring * 16 + 8 * h;
         const int seen[2] = {lim[0] - kb - 64 * h, lim[1] - kb - 64 * h};
-        // A row moves m when its weights' sum (the lane's share) says that one times scale_v may pass 2^12,
+        // A row moves m when its weights' sum (the lane's share) says that one times scale_v may pass 2^15,
         // or when it has seen no key yet.
         bool moved = __any_sync(0xffffffffu, (fresh[0] && seen[0] > 0) || (fresh[1] && seen[1] > 0));
 #pragma unroll 1
@@ -636,7 +637,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
 #pragma unroll
             for (int r = 0; r < 2; ++r) {
               const bool first = fresh[r] && mx[r] > -INFINITY;
-              const float to = first || mx[r] + ev > m[r] ? mx[r] + ev : m[r];
+              const float at = mx[r] + (ev - kKvLift), to = first || at > m[r] ? at : m[r];
               corr[r] = first ? 1.f : ex2(m[r] - to);
               m[r] = to;
               T[r] *= corr[r];
@@ -662,7 +663,7 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
           if (full) kv_weights<2>(addr, sk, sv, m, seen, sg, factors, q, pk, add);
           else if (whole) kv_weights<0>(addr, sk, sv, m, seen, sg, factors, q, pk, add);
           else kv_weights<1>(addr, sk, sv, m, seen, sg, factors, q, pk, add);
-          if (moved || !__any_sync(0xffffffffu, fmaxf(add[0], add[1]) > ex2(12.f - ev))) break;
+          if (moved || !__any_sync(0xffffffffu, fmaxf(add[0], add[1]) > ex2(15.f - ev))) break;
           moved = true;
         }
         T[0] += add[0];

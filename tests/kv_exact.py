@@ -8,7 +8,7 @@ import numpy as np
 
 from kv_ref import nibbles, parts
 
-LIFT = 0  # the weights' reference lies 2^LIFT above fp16's 1 (in steps of the row's largest weight)
+LIFT = 5  # the reference of a row's weights: the largest is 2^LIFT in fp16 when it is set
 
 
 def heads_of(pages, page, hd):
