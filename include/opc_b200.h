@@ -442,8 +442,8 @@ int opc_kv_read(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t dt
  * neither.  Deterministic.
  * The workspace (opc_kv_attention_workspace_bytes; 0 for a refused request) is zero-filled once
  * before first use (opc_workspace_init), is not to be shared with opc_gemv, and serves any calls
- * that are ordered on one stream; calls that may overlap, replays of two graphs among them, need
- * one each. */
+ * that are ordered on one stream, after device error 1 too; calls that may overlap, replays of two
+ * graphs among them, need one each. */
 size_t opc_kv_attention_workspace_bytes(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads,
                                         int32_t device);
 int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t heads, int32_t dtype, float scale,

@@ -245,7 +245,7 @@ struct KvItem {
   int32_t seq_end;    // keys the sequence holds (the last row's limit)
   int32_t hidden;     // seq_end - (position of row 0 + 1): row i sees keys below seq_end - hidden + i
   int32_t r0, rows, kvh;
-  int32_t c_first, contributors, record;
+  int32_t contributors, record;
 };
 
 // The rows of q as B fragments in an item's slot, from the elements each lane holds (row g of each
@@ -314,7 +314,8 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ int sm_last[2];
   __shared__ volatile int sm_failed;
-  __shared__ KvShared sm_shared[2];
+  __shared__ KvShared sm_shared[2];  // of the CTA's items those that it shares with others
+  __shared__ volatile int sm_n_shared;
   float* rec = reinterpret_cast<float*>(smem + kS * kStageBytes);  // [warp][row][kHd + 4]
   unsigned char* slots = smem + kS * kStageBytes + kv_rec_bytes(kHd, kNT);
   const uint32_t ring = smem_u32(smem), bars = smem_u32(slots) + 2 * kSlotBytes;
@@ -385,7 +386,7 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
       w_end = place_of(c + 1);
     }
     // the first sequence of the range: base = places before sequence s0 + i
-    int s0 = 0, i = 0, n_items = 0;
+    int s0 = 0, i = 0, n_items = 0, n_shared = 0;
     uint32_t base = 0;
     if (w < w_end) {
       for (;; s0 += 32) {
@@ -396,7 +397,7 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
       }
     }
     int st_all = 0;  // stages issued
-    while (w < w_end && ok) {
+    while (w < w_end) {
       const uint32_t st = __shfl_sync(0xffffffffu, my_st, i), cost = st ? st + kKvItemCost : 0;
       if (base + cost * kvh_n <= w) {  // the next sequence
         base += cost * kvh_n;
@@ -416,6 +417,13 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
       const int k0 = static_cast<int>(begin - pair0) * kKvStage, n_st = static_cast<int>(end - begin);
       const int k1 = min(n, k0 + n_st * kKvStage);
       const int is = n_items & 1, R = q_len * a.group;
+      const int c_first = cta_of(pair0), contributors = cta_of(pair1 - 1) - c_first + 1;
+      if (contributors > 1) {  // (two at most: the items that the range's ends cut)
+        if (lane == 0) sm_shared[n_shared] = {r0, head, c_first, contributors, R};
+        ++n_shared;
+      }
+      w = end;
+      if (!ok) continue;  // (a wait gave up: only what the CTA shares is still of interest)
       uint4 raw[kNT][kHd / 32];
 #pragma unroll
       for (int t = 0; t < kNT; ++t) {
@@ -475,13 +483,13 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
       };
       const int first = min(n_st, st_all == 0 ? kS : 1);
       for (int t = 0; t < first && ok; ++t) issue(t);
-      if (!ok) break;
+      if (!ok) continue;
       // The item's slot: the description, and q as fragments (once per item here instead of once per
       // consumer; the consumers read them back for every 32 keys, which costs them less than holding
       // them in registers).
       if (n_items >= 2 && !mbar_wait_bounded(free_b + 8 * is, ((n_items >> 1) - 1) & 1)) {
         ok = false;
-        break;
+        continue;
       }
       if (lane == 0) {
         KvItem it;
@@ -493,9 +501,8 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
         it.r0 = r0;
         it.rows = R;
         it.kvh = head;
-        it.c_first = cta_of(pair0);
-        it.contributors = cta_of(pair1 - 1) - it.c_first + 1;
-        it.record = 2 * c + (static_cast<int>(c) == it.c_first);
+        it.contributors = contributors;
+        it.record = 2 * c + (static_cast<int>(c) == c_first);
         *reinterpret_cast<KvItem*>(slots + is * kSlotBytes + kItemAt) = it;
       }
       const uint32_t slot_s = smem_u32(slots) + is * kSlotBytes;
@@ -505,7 +512,6 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
       if (lane == 0) mbar_arrive(item_b + 8 * is);
       ++n_items;
       for (int t = first; t < n_st && ok; ++t) issue(t);
-      w = end;
     }
     // no more items
     const int is = n_items & 1;
@@ -516,7 +522,11 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
     }
     // every copy has landed before the CTA can end, whatever its consumers did
     for (int t = max(0, st_all - kS); t < st_all; ++t) ok = mbar_wait_bounded(full_b + 8 * (t % kS), (t / kS) & 1) && ok;
-    if (!ok && lane == 0) atomicCAS(a.B.err, 0, kDevErrTmaTimeout);
+    if (lane == 0) {
+      if (!ok) atomicCAS(a.B.err, 0, kDevErrTmaTimeout);
+      sm_n_shared = n_shared;
+    }
+    named_barrier(2, kKvStepThreads);
     return;
   }
 
@@ -803,8 +813,8 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
     }
   }
   named_barrier(1, kKvStepWarps * 32);
-  const int r0 = it.r0, kvh = it.kvh, c_first = it.c_first, contributors = it.contributors;
-  const bool single = contributors == 1;
+  const int r0 = it.r0, kvh = it.kvh;
+  const bool single = it.contributors == 1;
   float* part = sp.part + static_cast<int64_t>(it.record) * sp.rows * kRec;
   __syncwarp();
   if (lane == 0) mbar_arrive(free_b + 8 * (item & 1));
@@ -837,16 +847,16 @@ kv_attention_step_kernel(const KvAttnArgs a, const KvSplit sp) {
       if (d == 0) *reinterpret_cast<float2*>(part + row * kRec + kHd) = make_float2(M, T);
     }
   }
-  if (!single) {
-    if (tid == 0) sm_shared[n_shared] = {r0, kvh, c_first, contributors, R};
-    ++n_shared;
-  }
+  n_shared += !single;
   }
   // Merges come after the loop: in it their registers would push the tile's to local memory
   // (attention over 131071 keys 44 -> 68 us).
-  named_barrier(1, kKvStepWarps * 32);  // sm_shared and sm_failed are final; rec may be overwritten
-  if (sm_failed) {
-    if (tid == 0) atomicCAS(a.B.err, 0, kDevErrTmaTimeout);
+  named_barrier(2, kKvStepThreads);  // sm_shared and sm_failed are final; rec may be overwritten
+  if (sm_failed) {  // arrive for every shared item all the same: the counts go back to zero for the calls to come
+    if (tid == 0) {
+      atomicCAS(a.B.err, 0, kDevErrTmaTimeout);
+      for (int i = n_arrived; i < sm_n_shared; ++i) kv_arrive(sp, sm_shared[i], &sm_last[i]);
+    }
     return;
   }
   if (tid == 0 && n_arrived < n_shared) kv_arrive(sp, sm_shared[n_arrived], &sm_last[n_arrived]);
