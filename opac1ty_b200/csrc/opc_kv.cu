@@ -137,17 +137,34 @@ struct AttentionPlan {
 
 constexpr size_t kCounterBytes = 4096;  // one per CTA of a launch
 
-AttentionPlan plan_attention(const opc_kv_cache& c, const opc_kv_batch& b, int group, int sms) {
-  AttentionPlan p{};
+// The step kernel takes sequences of at most this many rows.
+int step_rows(const opc_kv_cache& c, const opc_kv_batch& b, int group) {
   // Row tiles of 8 (query token, head) pairs: two where the accumulators leave registers for them.  (Heads
   // of 128, four rows of four heads over 4000 keys: 20 us in the step kernel, 35 in the prompt kernel;
   // 16 such sequences 39 and 96.)
   const int most = c.head_dim <= 128 ? 16 : 8;
-  p.step_q = std::min(std::max(b.max_q, 0), most / group);
+  const int q = std::min(std::max(b.max_q, 0), most / group);
   // Where a sequence of few rows would leave rows of the batch to nobody, as with one sequence, the prompt
   // kernel takes what there is (five rows of four heads over 4000 keys: 47 us after a step kernel that
   // finds nothing to do, 36 without).
-  if (b.max_q > p.step_q && b.n_tokens > (b.n_seqs - 1LL) * b.max_q + p.step_q) p.step_q = 0;
+  return b.max_q > q && b.n_tokens > (b.n_seqs - 1LL) * b.max_q + q ? 0 : q;
+}
+
+// At most this many tile pairs, over all kv heads, are the prompt kernel's: the rows of all sequences, and one
+// that is not full for each.
+int64_t prompt_items(const opc_kv_cache& c, const opc_kv_batch& b, int group) {
+  const int step_q = step_rows(c, b, group);
+  if (b.max_q <= step_q) return 0;
+  const int64_t rows = static_cast<int64_t>(opc::kv_p_qt(c.head_dim)) * opc::kKvPM;
+  const int64_t pairs = (static_cast<int64_t>(b.max_q) * group + rows - 1) / rows;
+  const int64_t all = std::min(pairs * b.n_seqs, static_cast<int64_t>(b.n_tokens) * group / rows +
+                                                     std::min(b.n_seqs, b.n_tokens / (step_q + 1)));
+  return std::max<int64_t>(1, all * c.kv_heads);
+}
+
+AttentionPlan plan_attention(const opc_kv_cache& c, const opc_kv_batch& b, int group, int sms) {
+  AttentionPlan p{};
+  p.step_q = step_rows(c, b, group);
   p.bytes = kCounterBytes;
   if (p.step_q > 0) {
     p.step_nt = p.step_q * group > 8 ? 2 : 1;
@@ -155,12 +172,8 @@ AttentionPlan plan_attention(const opc_kv_cache& c, const opc_kv_batch& b, int g
     p.bytes += static_cast<size_t>(p.step_grid) * 2 * (p.step_q * group) * (c.head_dim + 4) * 4;
   }
   if (b.max_q > p.step_q) {
-    // At most this many tile pairs: the rows of all sequences, and one that is not full for each.
     const int64_t rows = static_cast<int64_t>(opc::kv_p_qt(c.head_dim)) * opc::kKvPM;
-    const int64_t pairs = (static_cast<int64_t>(b.max_q) * group + rows - 1) / rows;
-    const int64_t all = std::min(pairs * b.n_seqs, static_cast<int64_t>(b.n_tokens) * group / rows +
-                                                       std::min(b.n_seqs, b.n_tokens / (p.step_q + 1)));
-    p.prompt_grid = std::max<int64_t>(1, all * c.kv_heads);
+    p.prompt_grid = prompt_items(c, b, group);
     // Fewer items than SMs share their keys, down to two tiles for each CTA.
     p.prompt_ctas = 1;
     if (b.max_kv > 3 * opc::kKvPN) {
@@ -364,22 +377,26 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
   const int64_t cols = static_cast<int64_t>(heads) * cache->head_dim;
   KV_CHECK(check_matrix(who, "q", q, ldq, cols));
   KV_CHECK(check_matrix(who, "out", out, ldo, cols));
+  const int group = heads / cache->kv_heads;
+  const opc::KvRows rows = rows_of(*batch, *cache, nullptr);
+  // (the step kernel counts its work in 32 bits: stages of keys, and what an item costs beside them)
+  const int64_t stages = std::max(1, (rows.max_kv + opc::kKvStage - 1) / opc::kKvStage) + opc::kKvItemCost;
+  if (static_cast<double>(batch->n_seqs) * cache->kv_heads * stages > UINT32_MAX)
+    return fail(OPC_ERR_INVALID, "%s: %d sequences of up to %d keys over %d kv heads are too many for one call", who,
+                batch->n_seqs, rows.max_kv, cache->kv_heads);
+  // (rows are counted in 32 bits, tiles of them in a grid)
+  if (static_cast<int64_t>(batch->n_tokens) * group > INT32_MAX - 1024 || prompt_items(*cache, *batch, group) > INT32_MAX)
+    return fail(OPC_ERR_INVALID, "%s: %d tokens of %d heads over %d kv heads are too many for one call", who, batch->n_tokens, heads,
+                cache->kv_heads);
   opc_host::Device dev;
   KV_CHECK(opc_host::current_device(&dev));
-  const int group = heads / cache->kv_heads;
-  // (the work of a call is counted in 32 bits, in stages of 128 keys)
-  if (static_cast<double>(batch->n_seqs) * cache->kv_heads * (batch->max_kv / opc::kKvStage + 2) > 4e9)
-    return fail(OPC_ERR_INVALID, "%s: %d sequences of up to %d keys over %d kv heads are too many for one call", who,
-                batch->n_seqs, batch->max_kv, cache->kv_heads);
-  // (rows are counted in 32 bits)
-  if (static_cast<int64_t>(batch->n_tokens) * group > INT32_MAX - 1024)
-    return fail(OPC_ERR_INVALID, "%s: %d tokens of %d heads per kv head are too many for one call", who, batch->n_tokens, group);
   AttentionPlan p = plan_attention(*cache, *batch, group, dev.sm_count);
   if (!workspace || !aligned16(workspace) || workspace_bytes < p.bytes)
     return fail(OPC_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", who, p.bytes, workspace_bytes);
   opc::KvAttnArgs a;
   a.C = geom_of(*cache);
-  a.B = rows_of(*batch, *cache, dev.error_word);
+  a.B = rows;
+  a.B.err = dev.error_word;
   a.B.max_q = std::min(a.B.max_q, batch->n_tokens);
   a.q = static_cast<const uint16_t*>(q);
   a.out = static_cast<uint16_t*>(out);
@@ -404,8 +421,6 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
             "opc_kv_attention launch (steps)");
   }
   if (p.prompt_grid) {
-    if (p.prompt_grid > INT32_MAX)
-      return fail(OPC_ERR_INVALID, "%s: %d tokens of %d heads are too many for one call", who, batch->n_tokens, heads);
     a.lo_q = p.step_q + 1;
     a.hi_q = a.B.max_q;
     opc::KvPromptSplit sp;

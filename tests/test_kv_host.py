@@ -158,3 +158,27 @@ def test_workspace_sizes_of_refused_requests_are_zero():
     assert lib.opc_kv_attention_workspace_bytes(None, None, 4, 0) == 0
     assert lib.opc_kv_attention_workspace_bytes(ctypes.byref(cache()), ctypes.byref(batch()), 3, 0) == 0
     assert lib.opc_token_logprobs_workspace_bytes(3, 100, 33, 0) == 0
+
+
+def call_attention_of(kv_heads, head_dim=64, heads=None, max_kv=100, **kw):
+    _, c = plan(kv_heads, head_dim, 16, 3)
+    c.pages = P
+    heads = kv_heads if heads is None else heads
+    ld = heads * head_dim
+    return _lib.load().opc_kv_attention(ctypes.byref(c), ctypes.byref(batch(max_kv=max_kv, max_pages=1 << 20, table_stride=1 << 20, **kw)),
+                                        heads, 0, 1.0, P, ld, P, ld, None, P, 1 << 20, None)
+
+
+@pytest.mark.parametrize("n_seqs,kv_heads,max_kv", [(65535, 20000, 100), (65535, 16385, 1), (1, 65535, 128 * 65535), (65535, 1, 2**31 - 1)])
+def test_attention_refuses_more_work_than_it_counts(n_seqs, kv_heads, max_kv):
+    # places of the line of work: (stages of 128 keys, one at least, + 3) for every sequence and kv head
+    assert n_seqs * kv_heads * (max(1, -(-min(max_kv, 1 << 24) // 128)) + 3) > 2**32 - 1
+    assert call_attention_of(kv_heads, max_kv=max_kv, n_seqs=n_seqs, n_tokens=n_seqs, max_q=1) == INVALID
+    assert "too many for one call" in _lib.last_error()
+
+
+@pytest.mark.parametrize("n_seqs,kv_heads,n_tokens,max_q", [(1, 65535, 1 << 24, 1 << 24), (2, 65535, 1 << 24, (1 << 24) - 1)])
+def test_attention_refuses_more_tiles_than_a_grid_has(n_seqs, kv_heads, n_tokens, max_q):
+    # tiles of 256 rows, for every kv head: before anything is launched, for the sequences of few rows too
+    assert call_attention_of(kv_heads, n_seqs=n_seqs, n_tokens=n_tokens, max_q=max_q) == INVALID
+    assert "too many for one call" in _lib.last_error()
