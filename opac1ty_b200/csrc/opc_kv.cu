@@ -29,14 +29,19 @@ using opc_host::fail;
 
 bool head_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 96 || hd == 128 || hd == 192 || hd == 256; }
 bool page_size_ok(int p) { return p == 16 || p == 32 || p == 64 || p == 128 || p == 256; }
+// Bytes of a cache; false where 64 bits do not hold them.
+bool cache_bytes(int32_t n_pages, int32_t kv_heads, int64_t head_bytes, int64_t* total) {
+  return !__builtin_mul_overflow(kv_heads * head_bytes, static_cast<int64_t>(n_pages), total);
+}
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 // The checks of a cache and a batch that every call makes.
 int check_cache(const char* who, const opc_kv_cache* c) {
   if (!c) return fail(OPC_ERR_INVALID, "%s: cache is NULL", who);
+  int64_t total = 0;
   if (c->kv_heads < 1 || c->kv_heads > 65535 || !head_dim_ok(c->head_dim) || !page_size_ok(c->page_size) || c->n_pages < 1 ||
       c->head_bytes != static_cast<int64_t>(c->page_size) * (c->head_dim + 8) ||
-      c->total_bytes != c->n_pages * (c->kv_heads * c->head_bytes))
+      !cache_bytes(c->n_pages, c->kv_heads, c->head_bytes, &total) || c->total_bytes != total)
     return fail(OPC_ERR_INVALID, "%s: the cache is not one that opc_kv_plan filled (kv_heads %d, head_dim %d, page_size %d, n_pages %d)",
                 who, c->kv_heads, c->head_dim, c->page_size, c->n_pages);
   if (!c->pages || !aligned16(c->pages)) return fail(OPC_ERR_INVALID, "%s: cache.pages must be a 16-byte aligned device pointer", who);
@@ -246,12 +251,16 @@ int opc_kv_plan(int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t n
     return fail(OPC_ERR_INVALID, "opc_kv_plan: kv_heads %d, n_pages %d", kv_heads, n_pages);
   if (!head_dim_ok(head_dim)) return fail(OPC_ERR_UNSUPPORTED, "opc_kv_plan: head_dim %d (32, 64, 96, 128, 192 and 256 are supported)", head_dim);
   if (!page_size_ok(page_size)) return fail(OPC_ERR_UNSUPPORTED, "opc_kv_plan: page_size %d (16, 32, 64, 128 and 256 are supported)", page_size);
+  const int64_t head_bytes = static_cast<int64_t>(page_size) * (head_dim + 8);
+  int64_t total = 0;
+  if (!cache_bytes(n_pages, kv_heads, head_bytes, &total))
+    return fail(OPC_ERR_INVALID, "opc_kv_plan: %d pages of %d kv heads are more than 2^63 bytes", n_pages, kv_heads);
   cache->kv_heads = kv_heads;
   cache->head_dim = head_dim;
   cache->page_size = page_size;
   cache->n_pages = n_pages;
-  cache->head_bytes = static_cast<int64_t>(page_size) * (head_dim + 8);
-  cache->total_bytes = n_pages * (kv_heads * cache->head_bytes);
+  cache->head_bytes = head_bytes;
+  cache->total_bytes = total;
   cache->pages = nullptr;
   return OPC_OK;
 }

@@ -182,3 +182,14 @@ def test_attention_refuses_more_tiles_than_a_grid_has(n_seqs, kv_heads, n_tokens
     # tiles of 256 rows, for every kv head: before anything is launched, for the sequences of few rows too
     assert call_attention_of(kv_heads, n_seqs=n_seqs, n_tokens=n_tokens, max_q=max_q) == INVALID
     assert "too many for one call" in _lib.last_error()
+
+
+def test_plan_refuses_sizes_past_64_bits():
+    assert plan(65535, 256, 256, 2**31 - 1)[0] == INVALID
+    assert "opc_kv_plan" in _lib.last_error()
+    rc, c = plan(63000, 256, 256, 2**31 - 1)  # below 2^63 bytes
+    assert rc == _lib.OPC_OK and c.total_bytes == (2**31 - 1) * 63000 * 256 * 264
+    # a cache of such sizes that was filled by hand
+    big = cache(kv_heads=65535, head_dim=256, page_size=256, n_pages=2**31 - 1, head_bytes=256 * 264)
+    big.total_bytes = ((2**31 - 1) * 65535 * 256 * 264 + 2**63) % 2**64 - 2**63  # what 64 bits make of it
+    assert call_append(c=big) == INVALID and "opc_kv_append" in _lib.last_error()
