@@ -29,8 +29,14 @@ _HALVES = {torch.float16: _lib.OPC_F16, torch.bfloat16: _lib.OPC_BF16}
 _DTYPES = {torch.float16: _lib.OPC_F16, torch.bfloat16: _lib.OPC_BF16, torch.float32: _lib.OPC_F32}
 
 
-_get_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+def _public_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the current device, and the handle of a device's current stream: torch's own names where it has them
+# (the public calls, which take their place elsewhere, wrap them in checks and objects)
+_get_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
 
 def _call(fn, index: int, *args):
