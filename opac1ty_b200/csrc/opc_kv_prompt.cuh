@@ -356,7 +356,6 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
     sm_low = 0x7f800000u;
   }
   griddep_wait();
-  griddep_launch_dependents();
   // ---------------------------------------------------------------- which rows and keys
   // (by every warp for itself; the tile pairs of sequence s: none when the launch does not take it)
   const int kvh_n = a.C.kv_heads;
@@ -432,6 +431,9 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   }
   if (tid < kQt * kKvPM) sm_rows[tid] = make_float2(0.f, 1.f);
   __syncthreads();
+  // (after the allocation: a kernel that allocates tensor memory before it waits for this one could otherwise
+  // take, on this SM, the columns that this CTA goes on to ask for, and neither would end)
+  griddep_launch_dependents();
 
   // ---------------------------------------------------------------- the converters' first loads
   const bool softmax = warp < 8 * kQt, converter = warp >= kKvPConv && warp < kKvPMma;

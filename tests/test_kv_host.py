@@ -193,3 +193,14 @@ def test_plan_refuses_sizes_past_64_bits():
     big = cache(kv_heads=65535, head_dim=256, page_size=256, n_pages=2**31 - 1, head_bytes=256 * 264)
     big.total_bytes = ((2**31 - 1) * 65535 * 256 * 264 + 2**63) % 2**64 - 2**63  # what 64 bits make of it
     assert call_append(c=big) == INVALID and "opc_kv_append" in _lib.last_error()
+
+
+def test_tensor_memory_is_allocated_before_dependents_may_start():
+    """A dependent kernel may take tensor memory before it waits; a CTA that asked for its own only then could
+    wait for a kernel that waits for it.  Such a hang is not for a GPU: the order is read in the source."""
+    from opac1ty_b200.build import CSRC
+
+    for name in ("opc_kv_prompt.cuh", "opc_gemm.cuh"):
+        text = (CSRC / name).read_text()
+        alloc, at = text.index('"tcgen05.alloc'), text.find("griddep_launch_dependents();")
+        assert at < 0 or alloc < at, name
