@@ -361,12 +361,13 @@ int opc_coo_scatter(int32_t M, const int32_t* row_ptr, const int32_t* cols, cons
  *   key pairs    [page_size]              fp16 scale (low half), fp16 zero (high half)
  *   value pairs  [page_size]
  * A stored value stands for scale * (code + zero).  opc_kv_append stores a head x as
- *   scale = max(fp16(max((max x - min x) / 15, max |x| / 1024)), 2^-24)
+ *   scale = max(fp16(max((max x - min x) * fifteenth, max |x| / 1024)), 2^-24)
  *   zero  = fp16(min x / scale)
- *   code  = clamp(round(x / scale - zero), 0, 15)        (round to even, in fp32)
- * -- the max |x| / 1024 term keeps |zero| <= 1024, so the pair's own rounding stays below half a
- * step for heads whose values lie far from 0.  A head with an infinity or NaN (or beyond the
- * range of an fp16 scale) is stored with a NaN scale, zero and codes 0: what attends to it is NaN.
+ *   code  = clamp(round(x * (1 / scale) - zero), 0, 15)
+ * every operation rounded to fp32 by itself (to even), fifteenth = 1/15 in fp32.  The max |x| / 1024
+ * term keeps |zero| <= 1024, so the pair's own rounding stays below half a step for heads whose
+ * values lie far from 0.  A head with an infinity or NaN (or beyond the range of an fp16 scale) is
+ * stored with a NaN scale, zero and codes 0: what attends to it is NaN.
  * --------------------------------------------------------------------------------------------- */
 enum { OPC_F16 = 0, OPC_BF16 = 1, OPC_F32 = 2 };  /* element types */
 
@@ -386,9 +387,9 @@ typedef struct opc_kv_cache {
  * not stored and attend to nothing.  Table entries past a sequence's last page are not read.
  * max_q and max_kv bound the sequences' q_len and kv_len on the host (they size the grids; the
  * lengths themselves are read on the device, so a captured graph replays with new ones): keys
- * beyond max_kv or beyond the table are not read, and a row that would be stored there, a page
- * outside [0, n_pages) and a q_len above max_q raise device error 2 (opc_take_device_error) and
- * are skipped. */
+ * beyond max_kv, beyond the table or in a page outside [0, n_pages) take no part, a row that would
+ * be stored there is not, and the attention leaves out a sequence's rows from max_q on (append and
+ * read take them); each raises device error 2 (opc_take_device_error). */
 typedef struct opc_kv_batch {
   int32_t n_seqs, n_tokens;       /* sequences; rows in q, k, v and out */
   int32_t max_q, max_kv;
@@ -460,7 +461,8 @@ int opc_kv_attention(const opc_kv_cache* cache, const opc_kv_batch* batch, int32
  * most vocab.  Logits of -infinity are tokens of probability 0.  A row of nothing else gives
  * logprob and top_logprobs -infinity and entropy 0; a row with a NaN or +infinity gives NaN for
  * all of them (its ids are ordered with NaN below everything).  A target >= vocab gives NaN and
- * device error 2.  Sums in fp32; deterministic.  The workspace
+ * device error 2.  Sums in fp32; deterministic.  Rows in which fewer than top_k logits lie above a
+ * value that thousands share (a mask) are read top_k times instead of once.  The workspace
  * (opc_token_logprobs_workspace_bytes) follows opc_kv_attention's rules. */
 size_t opc_token_logprobs_workspace_bytes(int32_t rows, int32_t vocab, int32_t top_k, int32_t device);
 int opc_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int32_t rows, int32_t vocab,

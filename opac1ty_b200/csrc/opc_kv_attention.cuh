@@ -44,7 +44,7 @@ struct KvAttnArgs {
 //             share, and the tensor cores cut what they add: so the share goes into the sums every
 //             kKvFold stages, with half of the next stages' expected share in advance, so that they
 //             run through 0 and what is cut cancels (131071 keys: results off by 4.2e-4 of their norm
-//             without, 3.1e-4 with, 2.8e-4 being the roundings of the weights and of the result).
+//             without, 3.0e-4 with, 2.8e-4 being the roundings of the weights and of the result).
 //   maximum   m and e move only when a score passes m + 7 or a scale 2^(e+8), 8 times the largest so far
 //             (one vote per tile): the common tile has no shuffles and no rescaling.  At a move 2^(e+5) lies
 //             above the largest scale, so that weights stay below 2^15 and a row's largest is near 2^5
@@ -61,10 +61,11 @@ struct KvAttnArgs {
 // its record (m, sum, weighted sums) goes to the workspace -- a CTA has at most two -- and the last
 // CTA of that sequence and head to arrive merges the records in order.
 //
-// Measured: 64 sequences of up to 8192 keys, 64/8 heads of 128: 76 us, 3.9 TB/s; one of 131071 keys, 32/8
-// heads: 41 us, 3.5 TB/s; one of 4000 keys: 12 us, latency (lengths, pages, keys, records, one after the
-// other).  What bounds the large ones is the instructions that spread codes into operands (logic units 48%,
-// issue 50% with three CTAs per SM, the registers' limit), not memory.
+// Measured: 64 sequences of up to 8192 keys, 64/8 heads of 128: 74 us, 4.0 TB/s; one of 131071 keys, 32/8
+// heads: 40 us, 3.6 TB/s; one of 4000 keys: 11 us, latency (lengths, pages, keys, records, one after the
+// other).  Nothing is full in the large ones (logic units 48%, issue 49%, memory 60% of what a copy reaches):
+// with three CTAs per SM, the registers' limit, a scheduler has three consumer warps to hide the chain of a
+// tile's loads, products, exponentials and products behind.
 // ------------------------------------------------------------------------------------------------
 constexpr int kKvStage = 128;                 // keys per stage, 32 for each consumer
 constexpr int kKvStageShift = 7;
@@ -76,7 +77,8 @@ constexpr int kKvLift = 5;                    // log2 of a row's largest weight 
 constexpr float kKvNone = -3.402823466e38f;   // the maximum of no keys: below every finite score
 constexpr int kKvItemCost = 3;                // what an item costs beside its stages, in stages
 __host__ __device__ constexpr int kv_stage_bytes(int hd) { return kKvStage * (hd + 8); }
-// CTAs per SM: bounded by the accumulators' registers and the shared memory of a record.
+// CTAs per SM: bounded by the accumulators' registers and the shared memory of a record.  (Heads of 128 with
+// two row tiles keep 32 bytes of a thread in local memory: four rows of four heads over 4000 keys 20 us.)
 __host__ __device__ constexpr int kv_step_ctas(int hd, int nt) { return hd <= 128 && nt == 1 ? 3 : 2; }
 __host__ __device__ constexpr int kv_rec_bytes(int hd, int nt) { return kKvStepWarps * 8 * nt * (hd + 4) * 4; }
 __host__ __device__ constexpr int kv_slot_bytes(int hd, int nt) { return 8 * nt * (hd * 2 + 8) + 64; }  // q, its factors, description

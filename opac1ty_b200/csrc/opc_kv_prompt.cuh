@@ -14,8 +14,8 @@ namespace opc {
 //                  K' = code - 8, exact in fp16; what is left of the zeros, (zero + 8) sum q, is added by
 //                  one more product in tf32, with both factors in parts of 11 bits (sum q three, zero + 8
 //                  two).  The key's scale multiplies its column of S in fp32: nothing of a key is rounded.
-//                  (K' = code + zero in fp16 would take 345 us instead of 357 for the prompts below, but
-//                  round the keys' largest elements: log sums off by 1e-6 of their value instead of 4e-8.)
+//                  (K' = code + zero in fp16 would save 3% of the prompts below, but round the keys' largest
+//                  elements: log sums off by 1e-6 of their value instead of 4e-8.)
 //   P = exp2(S * scale_k - m) * scale_v, rounded once to fp16, written over S in tensor memory
 //   O += P V'      V' = code + zero in fp16: exact where no value is larger than |zero|, else one rounding
 //                  (2^-11 of the value, as for P and the result)
@@ -45,15 +45,16 @@ namespace opc {
 // order too, and the output columns are put back in order by the epilogue.
 // An item is a tile pair of one sequence and kv head.  How many there are is known on the device only
 // (the host knows bounds, which a batch of a few prompts among many single tokens is far below), so each
-// CTA counts them from q_start (a grid of sequences times the longest one's tiles, most of it empty, took
-// 320 us instead of 165 for a prompt of 2000 among 100 single tokens); where they are fewer than the SMs,
+// CTA counts them from q_start (a grid of sequences times the longest one's tiles, most of it empty, would
+// take twice as long for a prompt of 2000 among 100 single tokens, 161 us); where they are fewer than the SMs,
 // several CTAs share an item's keys, evenly, and their partial results go to the workspace as records,
-// merged by the item's last CTA (one prompt of 2000 tokens, 256 items over 148 SMs: 79 -> 65 us by taking
-// the tiles with the most keys first).
-// Measured, 32 heads of 128 over 8: 357 us for three prompts of 1500 to 4097 tokens, 710 TFLOP/s; 63 us for
-// 512 tokens behind 3584, 509 TFLOP/s.  No unit is full (tensor cores 38%, issue 60%, special functions
-// 40%): leaving out the exponentials or most of the products of Q K' changes nothing, so what bounds it is the latency of the chain scores - weights -
-// products in each of the four half tiles in flight, and about 8 us per CTA to fill and drain it.
+// merged by the item's last CTA.  The tiles with the most keys come first (one prompt of 2000 tokens, 256
+// items over 148 SMs, 57 us: a fifth less than in order).
+// Measured, 32 heads of 128 over 8, fp16: 359 us for three prompts of 1500 to 4097 tokens, 705 TFLOP/s; 59 us
+// for 512 tokens behind 3584, 547 TFLOP/s; bf16 371 and 60 us, with the look at q's rows in every CTA.  No unit is
+// full (tensor cores 37%, issue 59%, special functions 37%): leaving out the exponentials or most of the products
+// of Q K' changes nothing, so what bounds it is the latency of the chain scores - weights - products in each of
+// the four half tiles in flight, and about 8 us per CTA to fill and drain it.
 constexpr int kKvPM = 128, kKvPN = 128;            // rows per tile, keys per tile
 constexpr int kKvPThreads = 28 * 32;
 constexpr int kKvPConv = 16, kKvPMma = 24;         // first converter warp, the MMA warp

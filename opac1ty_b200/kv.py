@@ -10,7 +10,8 @@ Rows are packed: rows ``q_start[s] .. q_start[s+1]`` of q, k and v are the last 
 which holds ``kv_len[s]`` tokens once they are in.  The layout of a page, the quantization and the
 treatment of rows that belong nowhere are in ``include/opc_b200.h``.  The lengths and the page table
 are read on the device: a captured graph replays with what they hold then.  Every computation is a
-call into ``libopc_b200.so``.
+call into ``libopc_b200.so``.  There is no backward pass: results carry no gradient, whatever their
+inputs ask for.
 """
 
 from __future__ import annotations
@@ -60,8 +61,9 @@ _workspaces: Dict[Tuple[int, int, str], torch.Tensor] = {}
 
 def _workspace(device: torch.device, stream: int, nbytes: int, kind: str) -> torch.Tensor:
     """A zeroed workspace for one device and stream.  Calls under graph capture get one of their
-    own from the graph's memory (cleared by every replay), so graphs captured on one stream may be
-    replayed side by side."""
+    own from the graph's memory, so graphs captured on one stream may be replayed side by side; every
+    replay clears it (0.8 us for a token of one sequence, 6 to 7 us for chunks and prompts: a workspace
+    given by the caller saves that)."""
     if torch.cuda.is_current_stream_capturing():
         return torch.zeros(nbytes, dtype=torch.uint8, device=device)
     key = (device.index, stream, kind)

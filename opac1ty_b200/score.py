@@ -27,9 +27,10 @@ def _need(rows: int, vocab: int, top_k: int, device: int) -> int:
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top_k: int = 0,
                    entropy: bool = True, workspace: Optional[torch.Tensor] = None) -> TokenLogprobs:
-    """For every row of logits [rows, vocab] (float16, bfloat16 or float32, any row stride): the log
+    """For every row of logits [rows, vocab] (float16, bfloat16 or float32, any row stride from vocab on): the log
     probability of its target (int32 or int64 [rows]; negative: none, 0), the entropy, and the top_k
-    (at most 32) most probable tokens with their log probabilities, equal logits by the lower id."""
+    (at most 32) most probable tokens with their log probabilities, equal logits by the lower id.
+    There is no backward pass: the results carry no gradient."""
     if logits.dim() != 2 or not logits.is_cuda or logits.dtype not in _DTYPES or (logits.numel() and logits.stride(1) != 1):
         raise ValueError(f"token_logprobs: logits must be float16, bfloat16 or float32 [rows, vocab] on a CUDA device with "
                          f"unit stride, got {logits.dtype} {tuple(logits.shape)} on {logits.device}")
