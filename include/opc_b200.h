@@ -437,10 +437,11 @@ int opc_kv_read(const opc_kv_cache* cache, const opc_kv_batch* batch, int32_t dt
  * [n_tokens][heads] fp32, the natural logarithm of the softmax's sum.  A row that sees no key
  * gives out 0 and lse -infinity.  dtype (of q and out) OPC_F16 or OPC_BF16.  Scores, statistics and
  * sums are in fp32; the products with the values take fp16 factors: a weight is rounded by 2^-11 of
- * itself or 2^-30 of the row's largest (as shares of scale_v, the largest of the keys so far), and
- * where a sequence has many rows (q_len * heads/kv_heads above 16, or above 8 for head_dim 192 and
- * 256; where all sequences may, also below) code + zero of a value by 2^-11 of itself.  lse has
- * neither.  Deterministic.
+ * itself or 2^-30 of the row's largest (as shares of the largest scale of a value in the row's tiles
+ * of 128 positions so far, its last one whole).  Where a sequence has many rows (q_len *
+ * heads/kv_heads above 16, or above 8 for head_dim 192 and 256; where all sequences may, also below)
+ * code + zero of a value is rounded by 2^-11 of itself, elsewhere the sums cut up to 2^-10 code steps
+ * of the largest weight of 16 keys.  lse has none of these.  Deterministic.
  * The workspace (opc_kv_attention_workspace_bytes; 0 for a refused request) is zero-filled once
  * before first use (opc_workspace_init), is not to be shared with opc_gemv, and serves any calls
  * that are ordered on one stream, after device error 1 too; calls that may overlap, replays of two

@@ -39,7 +39,9 @@ struct KvAttnArgs {
 //             transposed fragments that movmatrix turns into B.  A weight carries its key's scale,
 //             p = exp2(x - m) * scale_v * 2^-e, and is rounded once to fp16; the zeros' share
 //             sum p * zero_v is summed in fp32 from the rounded weights, so the rounding acts on
-//             the values themselves (code + zero), not on the all-positive codes.  Their sums only
+//             the values themselves (code + zero), not on the all-positive codes.  (What lies 2^-24
+//             below the largest product, for which a code counts as 2^-14, is cut: up to 2^-10 code
+//             steps of the largest weight of 16 keys.)  Their sums only
 //             grow, while the results of long contexts are small differences of them and the zeros'
 //             share, and the tensor cores cut what they add: so the share goes into the sums every
 //             kKvFold stages, with half of the next stages' expected share in advance, so that they

@@ -37,13 +37,18 @@ class Exact:
             idx = np.arange(max(pos + 1, 0))
             pg, off = su.table[s, idx // su.page], idx % su.page
             there = (pg >= 0) & (pg < su.n_pages)
-            pg, off = pg[there], off[there]
+            idx, pg, off = idx[there], pg[there], off[there]
+            # per kv head and tile of 128 keys: the largest scale of a value up to its end
+            far = np.arange(max(min(su.kv_lens[s], (pos // 128 + 1) * 128), 0))
+            tiles = su.table[s, far // su.page]
+            held = (tiles >= 0) & (tiles < su.n_pages)
             for h in range(H):
                 if pg.size == 0:
                     self.out[r, h], self.tol[r, h] = 0.0, 0.0
                     self.lse[r, h], self.tol_lse[r, h] = -np.inf, 0.0
                     continue
                 at = (pg, h // G, off)
+                largest = np.abs(vs[tiles[held], h // G, far[held] % su.page]).max()
                 k = ks[at] * (kc[at] + kz[at])
                 cz = vc[at] + vz[at]
                 v = vs[at] * cz
@@ -66,10 +71,17 @@ class Exact:
                 moved = np.minimum(np.expm1(min(2 * d, 700.0)) * mag,
                                    2 * sc.size * np.exp(np.clip(2 * d - gap, -700.0, 700.0)) * np.abs(v).max(0))
                 # A weight rounded to fp16: 2^-11 of it and 2^-18 from the exponential and the sums, or half a step of
-                # fp16's smallest, 2^-25, at a reference that is 2^LIFT and at most twice the largest scale.
-                small = sc.size * 2.0 ** (-25 - LIFT) * 2 * np.abs(vs[at]).max() * np.abs(cz).max(0) / T
+                # fp16's smallest, 2^-25, at a reference that is 2^LIFT and at most twice the largest scale of the keys
+                # so far, whole tiles of 128 (what a row does not see of them included).
+                small = sc.size * 2.0 ** (-25 - LIFT) * 2 * largest * np.abs(cz).max(0) / T
+                # Products of 16 keys at a time: codes enter as code * 2^-24, fp16 numbers of exponent 2^-14, and what
+                # lies 2^-24 below the largest exponent of a product is cut, for 16 products and the sum: 17 * 2^-24 *
+                # 2^-14, in code steps 2^-10, of the largest weight (times its scale) among them.
+                ws = np.zeros(-(-(pos + 1) // 16) * 16)
+                ws[idx] = w * np.abs(vs[at][:, 0])
+                cut = 17 * 2.0 ** -14 * ws.reshape(-1, 16).max(1).sum()
                 sums = 2.0 ** -23 * (sc.size / 16 + 8) * (w @ (np.abs(vs[at]) * (16 + np.abs(vz[at]))))
-                tol = moved + (2.0 ** -11 + 2.0 ** -18) * mag + small + sums
+                tol = moved + (2.0 ** -11 + 2.0 ** -18) * mag + small + cut + sums
                 if form_many:  # code + zero rounded to fp16
                     tol += w @ np.abs(vs[at] * (cz.astype(np.float16) - cz))
                 self.out[r, h] = out
