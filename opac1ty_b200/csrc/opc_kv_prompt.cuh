@@ -433,7 +433,8 @@ __global__ void __launch_bounds__(kKvPThreads, 1) kv_attention_prompt_kernel(con
   if (tid < kQt * kKvPM) sm_rows[tid] = make_float2(0.f, 1.f);
   __syncthreads();
   // (after the allocation: a kernel that allocates tensor memory before it waits for this one could otherwise
-  // take, on this SM, the columns that this CTA goes on to ask for, and neither would end)
+  // take, on this SM, the columns that this CTA goes on to ask for, and neither would end; that this CTA's
+  // registers leave hardly any room for another is not what this should rest on)
   griddep_launch_dependents();
 
   // ---------------------------------------------------------------- the converters' first loads
