@@ -470,6 +470,58 @@ int opc_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int32_t ro
                        const int32_t* targets, float* logprob, float* entropy, int32_t top_k, int32_t* top_ids,
                        float* top_logprobs, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------------------------------------
+ * Products in 8-bit integers: tokens and weights held as codes with one scale a row (tokens: a scale
+ * each; weights: a scale for each output channel), the operators that bring tokens into that form,
+ * and the matrix product of the two.
+ *
+ * A row v of n values is held as
+ *   a     = max |v|
+ *   scale = a / 127                (fp32)
+ *   code  = round(v * 127 / a)     (to even; -127 .. 127)
+ * and stands for scale * code.  A row with a < 2^-100 counts as zeros (scale 0, codes 0).  A row with
+ * an infinity or NaN has a NaN scale and codes 0: everything made of it is NaN.  v is formed in fp32
+ * from the inputs, and so is the quotient v * 127 / a, rounded to the nearest fp32 before it is rounded
+ * to a whole number (for 16-bit inputs taken as they are, codes are exact, halves included).
+ * --------------------------------------------------------------------------------------------- */
+typedef struct opc_i8_rows {
+  int32_t rows, n;                /* n 1 .. 131071 (no sum of products of two rows leaves 32 bits) */
+  int64_t ld;                     /* bytes from a row to the next: a multiple of 16, at least n */
+  int8_t* codes;                  /* device, 16-byte aligned: [rows][ld]; bytes from n on are neither read nor written */
+  float* scales;                  /* device [rows] */
+} opc_i8_rows;
+
+/* The three calls that make such rows write out->codes and out->scales and, when `values` is given,
+ * what the codes stand for (scale * code rounded to v_dtype) at values + r * ldv.  dtypes OPC_F16,
+ * OPC_BF16, OPC_F32; leading dimensions in elements.  One launch each; no workspace.
+ *
+ * opc_i8_quantize      v = x                      activations, or a layer's weights (row = channel)
+ * opc_i8_silu_mul      v = g / (1 + exp(-g)) * u
+ * opc_i8_add_rmsnorm   t = h + y (y may be NULL), written to h_out rounded to h's type (h_out may be
+ *                      h itself, or NULL); v = t * weight (NULL: ones), and the scale is also divided by
+ *                      sqrt(mean t^2 + eps), t as formed, before its rounding: the codes of the
+ *                      normalized row.  y has h's type, or h is OPC_F32.  eps from 1e-12 on.  (The
+ *                      limits of a zero row above are those of t * weight.)  Sums in fp32, a row whose
+ *                      squares leave fp32 included; deterministic. */
+int opc_i8_quantize(const void* x, int64_t ldx, int32_t dtype, const opc_i8_rows* out, void* values, int64_t ldv,
+                    int32_t v_dtype, void* stream);
+int opc_i8_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, int32_t dtype, const opc_i8_rows* out,
+                    void* values, int64_t ldv, int32_t v_dtype, void* stream);
+int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* y, int64_t ldy, int32_t y_dtype,
+                       const void* weight, int32_t w_dtype, float eps, void* h_out, int64_t ldho, const opc_i8_rows* out,
+                       void* values, int64_t ldv, int32_t v_dtype, void* stream);
+
+/* y[t][r] = x.scales[t] * w.scales[r] * sum_k x.codes[t][k] * w.codes[r][k] + bias[r]
+ * for the rows t of x (tokens) and r of w (channels), x.n == w.n; bias (bias_dtype, [w.rows]) may be
+ * NULL.  Codes may be any 8-bit integers, -128 too.  The sum is exact; it is rounded to fp32, multiplied
+ * by the two scales in the order given, the bias is added in fp32, and the result rounded to y_dtype.
+ * Deterministic.  The workspace (opc_i8_gemm_workspace_bytes) is zero-filled once before first use
+ * (opc_workspace_init), is not to be shared with other entry points, and serves any calls that are
+ * ordered on one stream; calls that may overlap, replays of two graphs among them, need one each. */
+size_t opc_i8_gemm_workspace_bytes(int32_t rows, int32_t M, int32_t K, int32_t device);
+int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, int32_t bias_dtype, void* y, int64_t ldy,
+                int32_t y_dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 /* XXH64 (seed `seed`) of a HOST buffer: the checksum that the .bf2 layout places after the last
  * layer (opacc1ty/format/header.py:26; the reference documents it but never writes it).  Files
  * written with it set bit 0 of the file header's flags.  A format helper, not a kernel. */

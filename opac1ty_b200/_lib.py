@@ -138,6 +138,16 @@ class Rope(ctypes.Structure):
     ]
 
 
+class I8Rows(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int32),
+        ("n", ctypes.c_int32),
+        ("ld", ctypes.c_int64),
+        ("codes", ctypes.c_void_p),
+        ("scales", ctypes.c_void_p),
+    ]
+
+
 # Exported symbols and their prototypes: (restype, argtypes).  Kept in the order of the header.
 _c = ctypes
 PROTOTYPES = {
@@ -224,6 +234,26 @@ PROTOTYPES = {
         _c.c_int,
         [_c.c_void_p, _c.c_int64, _c.c_int32, _c.c_int32, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_void_p,
          _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_size_t, _c.c_void_p],
+    ),
+    "opc_i8_quantize": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_int64, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int32, _c.c_void_p],
+    ),
+    "opc_i8_silu_mul": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int32, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int32,
+         _c.c_void_p],
+    ),
+    "opc_i8_add_rmsnorm": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_int64, _c.c_int32, _c.c_void_p, _c.c_int64, _c.c_int32, _c.c_void_p, _c.c_int32, _c.c_float,
+         _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_int32, _c.c_void_p],
+    ),
+    "opc_i8_gemm_workspace_bytes": (_c.c_size_t, [_c.c_int32, _c.c_int32, _c.c_int32, _c.c_int32]),
+    "opc_i8_gemm": (
+        _c.c_int,
+        [_c.c_void_p, _c.c_void_p, _c.c_void_p, _c.c_int32, _c.c_void_p, _c.c_int64, _c.c_int32, _c.c_void_p, _c.c_size_t,
+         _c.c_void_p],
     ),
     "opc_take_device_error": (_c.c_int, [_c.c_int32, _c.POINTER(_c.c_int32)]),
 }

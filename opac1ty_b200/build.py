@@ -10,7 +10,7 @@ from pathlib import Path
 PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 INCLUDE = PKG.parent / "include"
-SOURCES = [CSRC / "opc_lib.cu", CSRC / "opc_engine.cu", CSRC / "opc_kv.cu", CSRC / "opc_score.cu"]
+SOURCES = [CSRC / "opc_lib.cu", CSRC / "opc_engine.cu", CSRC / "opc_kv.cu", CSRC / "opc_score.cu", CSRC / "opc_i8.cu"]
 DEPENDS = sorted(p for pat in ("*.cu", "*.cuh", "*.h") for p in CSRC.glob(pat)) + sorted(INCLUDE.glob("*.h"))
 OUTPUT = PKG / "libopc_b200.so"
 

@@ -1,0 +1,202 @@
+// opc_i8.cu -- C ABI of the 8-bit products (opc_i8_*, include/opc_b200.h).
+#define OPC_WITHOUT_ERROR_WORD
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+
+#include "../../include/opc_b200.h"
+#include "opc_i8_gemm.cuh"
+#include "opc_i8_rows.cuh"
+#include "opc_internal.h"
+
+using opc_host::cuda_fail;
+using opc_host::fail;
+
+namespace {
+
+constexpr int kMaxWidth = 131071;  // 128 * 128 * 131071 < 2^31: no sum of products leaves 32 bits
+
+int bytes_of(int32_t dtype) { return dtype == OPC_F32 ? 4 : 2; }
+bool is_type(int32_t dtype) { return dtype == OPC_F16 || dtype == OPC_BF16 || dtype == OPC_F32; }
+
+// A matrix of `rows` rows of n values at p with leading dimension ld: present and aligned to its elements.
+int check_matrix(const char* who, const char* name, const void* p, int64_t ld, int32_t dtype, int32_t n) {
+  if (!is_type(dtype)) return fail(OPC_ERR_UNSUPPORTED, "%s: element type %d of %s", who, dtype, name);
+  if (!p || (reinterpret_cast<uintptr_t>(p) & (bytes_of(dtype) - 1u)))
+    return fail(OPC_ERR_INVALID, "%s: %s is NULL or not aligned to its elements", who, name);
+  if (ld < n) return fail(OPC_ERR_INVALID, "%s: leading dimension %lld of %s below %d", who, static_cast<long long>(ld), name, n);
+  return OPC_OK;
+}
+
+int check_codes(const char* who, const char* name, const opc_i8_rows* m) {
+  if (!m) return fail(OPC_ERR_INVALID, "%s: %s is NULL", who, name);
+  if (m->rows < 0 || m->n < 1 || m->n > kMaxWidth)
+    return fail(OPC_ERR_INVALID, "%s: %s is %d x %d (rows of 1 to %d values)", who, name, m->rows, m->n, kMaxWidth);
+  if (m->rows == 0) return OPC_OK;
+  if (!m->codes || (reinterpret_cast<uintptr_t>(m->codes) & 15u) || m->ld < m->n || (m->ld & 15))
+    return fail(OPC_ERR_INVALID, "%s: the codes of %s must start on 16 bytes in rows of a multiple of 16 bytes from %d on, got a leading dimension of %lld",
+                who, name, m->n, static_cast<long long>(m->ld));
+  if (!m->scales || (reinterpret_cast<uintptr_t>(m->scales) & 3u))
+    return fail(OPC_ERR_INVALID, "%s: the scales of %s are NULL or not aligned", who, name);
+  return OPC_OK;
+}
+
+bool vec_ok(const void* p, int64_t ld, int32_t dtype) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * bytes_of(dtype)) % 16 == 0;
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y, int threads, void* stream, Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(grid_x, grid_y);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr[1];  // the launch overlaps the end of the kernel before, which the kernel waits for
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+
+// One warp per row up to 1024 values; beyond, one CTA per row with 16 values a thread (32 from 16384
+// values on), and rows of more than 32768 values, which no CTA's registers hold, are read twice.
+template <int kOp, int kTX, int kTU>
+cudaError_t launch_rows(const opc::I8RowsArgs& a, void* stream) {
+  const int groups = (a.n + 7) / 8;
+  if (groups <= 128) {
+    const int per = (groups + 31) / 32;
+    auto k = per == 1 ? opc::i8_rows_kernel<kOp, kTX, kTU, 1, true>
+             : per == 2 ? opc::i8_rows_kernel<kOp, kTX, kTU, 2, true> : opc::i8_rows_kernel<kOp, kTX, kTU, 4, true>;
+    return launch(k, (a.rows + 3) / 4, 1, 128, stream, a);
+  }
+  const int per = groups <= 2048 ? 2 : groups <= 4096 ? 4 : 0;
+  const int threads = per ? ((groups + per - 1) / per + 31) / 32 * 32 : 1024;
+  auto k = per == 2 ? opc::i8_rows_kernel<kOp, kTX, kTU, 2, false>
+           : per == 4 ? opc::i8_rows_kernel<kOp, kTX, kTU, 4, false> : opc::i8_rows_kernel<kOp, kTX, kTU, 0, false>;
+  return launch(k, a.rows, 1, threads, stream, a);
+}
+
+template <int kOp, int kTU>
+cudaError_t launch_rows_x(int32_t x_type, const opc::I8RowsArgs& a, void* stream) {
+  if (x_type == OPC_F16) return launch_rows<kOp, opc::kI8F16, kTU == 4 ? opc::kI8F16 : kTU>(a, stream);
+  if (x_type == OPC_BF16) return launch_rows<kOp, opc::kI8BF16, kTU == 4 ? opc::kI8BF16 : kTU>(a, stream);
+  return launch_rows<kOp, opc::kI8F32, kTU == 4 ? opc::kI8F32 : kTU>(a, stream);
+}
+constexpr int kSame = 4;  // launch_rows_x: the second operand has the first one's type
+
+// What the three quantizing calls share: the output's checks and arguments.
+int start_rows(const char* who, const opc_i8_rows* out, void* values, int64_t ldv, int32_t v_dtype, opc::I8RowsArgs* a) {
+  const int rc = check_codes(who, "the output", out);
+  if (rc != OPC_OK || out->rows == 0) return rc;
+  if (values) {
+    const int rv = check_matrix(who, "values", values, ldv, v_dtype, out->n);
+    if (rv != OPC_OK) return rv;
+  }
+  *a = {};
+  a->rows = out->rows;
+  a->n = out->n;
+  a->codes = out->codes;
+  a->ldc = out->ld;
+  a->scales = out->scales;
+  a->values = values;
+  a->ldv = ldv;
+  a->v_type = v_dtype;
+  a->vec_v = values && vec_ok(values, ldv, v_dtype);
+  return OPC_OK;
+}
+
+int end_rows(const char* who, cudaError_t e) { return e == cudaSuccess ? OPC_OK : cuda_fail(e, who); }
+
+}  // namespace
+
+extern "C" {
+
+int opc_i8_quantize(const void* x, int64_t ldx, int32_t dtype, const opc_i8_rows* out, void* values, int64_t ldv,
+                    int32_t v_dtype, void* stream) {
+  const char* who = "opc_i8_quantize";
+  opc::I8RowsArgs a;
+  int rc = start_rows(who, out, values, ldv, v_dtype, &a);
+  if (rc != OPC_OK || out->rows == 0) return rc;
+  if ((rc = check_matrix(who, "x", x, ldx, dtype, out->n)) != OPC_OK) return rc;
+  a.x = x;
+  a.ldx = ldx;
+  a.vec_x = vec_ok(x, ldx, dtype);
+  return end_rows(who, launch_rows_x<opc::kI8Quant, opc::kI8None>(dtype, a, stream));
+}
+
+int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* y, int64_t ldy, int32_t y_dtype,
+                       const void* weight, int32_t w_dtype, float eps, void* h_out, int64_t ldho, const opc_i8_rows* out,
+                       void* values, int64_t ldv, int32_t v_dtype, void* stream) {
+  const char* who = "opc_i8_add_rmsnorm";
+  opc::I8RowsArgs a;
+  int rc = start_rows(who, out, values, ldv, v_dtype, &a);
+  if (rc != OPC_OK || out->rows == 0) return rc;
+  const int32_t n = out->n;
+  if ((rc = check_matrix(who, "h", h, ldh, h_dtype, n)) != OPC_OK) return rc;
+  if (y && (rc = check_matrix(who, "y", y, ldy, y_dtype, n)) != OPC_OK) return rc;
+  if (y && y_dtype != h_dtype && h_dtype != OPC_F32)
+    return fail(OPC_ERR_UNSUPPORTED, "%s: y of type %d beside h of type %d (the same, or h of type %d)", who, y_dtype, h_dtype, OPC_F32);
+  if (weight && (rc = check_matrix(who, "weight", weight, n, w_dtype, n)) != OPC_OK) return rc;
+  if (h_out && (rc = check_matrix(who, "h_out", h_out, ldho, h_dtype, n)) != OPC_OK) return rc;
+  if (!(eps >= 1e-12f) || !std::isfinite(eps)) return fail(OPC_ERR_INVALID, "%s: eps %g (1e-12 or more)", who, static_cast<double>(eps));
+  a.x = h;
+  a.ldx = ldh;
+  a.vec_x = vec_ok(h, ldh, h_dtype);
+  a.u = y;
+  a.ldu = ldy;
+  a.vec_u = y && vec_ok(y, ldy, y_dtype);
+  a.w = weight;
+  a.w_type = w_dtype;
+  a.vec_w = weight && vec_ok(weight, 8, w_dtype);
+  a.h_out = h_out;
+  a.ldh = ldho;
+  a.vec_h = h_out && vec_ok(h_out, ldho, h_dtype);
+  a.eps = eps;
+  cudaError_t e;
+  if (!y) e = launch_rows_x<opc::kI8Norm, opc::kI8None>(h_dtype, a, stream);
+  else if (y_dtype == h_dtype) e = launch_rows_x<opc::kI8Norm, kSame>(h_dtype, a, stream);
+  else if (y_dtype == OPC_F16) e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8F16>(a, stream);
+  else e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8BF16>(a, stream);
+  return end_rows(who, e);
+}
+
+int opc_i8_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, int32_t dtype, const opc_i8_rows* out,
+                    void* values, int64_t ldv, int32_t v_dtype, void* stream) {
+  const char* who = "opc_i8_silu_mul";
+  opc::I8RowsArgs a;
+  int rc = start_rows(who, out, values, ldv, v_dtype, &a);
+  if (rc != OPC_OK || out->rows == 0) return rc;
+  if ((rc = check_matrix(who, "gate", gate, ldg, dtype, out->n)) != OPC_OK) return rc;
+  if ((rc = check_matrix(who, "up", up, ldu, dtype, out->n)) != OPC_OK) return rc;
+  a.x = gate;
+  a.ldx = ldg;
+  a.vec_x = vec_ok(gate, ldg, dtype);
+  a.u = up;
+  a.ldu = ldu;
+  a.vec_u = vec_ok(up, ldu, dtype);
+  return end_rows(who, launch_rows_x<opc::kI8Silu, kSame>(dtype, a, stream));
+}
+
+size_t opc_i8_gemm_workspace_bytes(int32_t rows, int32_t M, int32_t K, int32_t device) {
+  (void)device;
+  return rows >= 0 && M >= 1 && K >= 1 && K <= kMaxWidth ? 16 : 0;
+}
+
+int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, int32_t bias_dtype, void* y, int64_t ldy,
+                int32_t y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "opc_i8_gemm";
+  int rc = check_codes(who, "x", x);
+  if (rc != OPC_OK || (rc = check_codes(who, "w", w)) != OPC_OK) return rc;
+  if (x->n != w->n) return fail(OPC_ERR_INVALID, "%s: x has rows of %d values, w of %d", who, x->n, w->n);
+  if (w->rows < 1) return fail(OPC_ERR_INVALID, "%s: w has no rows", who);
+  if (x->rows == 0) return OPC_OK;
+  if ((rc = check_matrix(who, "y", y, ldy, y_dtype, w->rows)) != OPC_OK) return rc;
+  if (bias && (rc = check_matrix(who, "bias", bias, w->rows, bias_dtype, w->rows)) != OPC_OK) return rc;
+  if (!workspace || workspace_bytes < 16) return fail(OPC_ERR_WORKSPACE, "%s: a workspace of 16 bytes is needed, got %zu", who, workspace_bytes);
+  opc::I8GemmArgs a = {x->codes, w->codes, x->scales, w->scales, bias, y, x->ld, w->ld, ldy, x->rows, w->rows, x->n, bias_dtype, y_dtype};
+  return end_rows(who, launch(opc::i8_gemm_simple, (w->rows + 63) / 64, (x->rows + 63) / 64, 256, stream, a));
+}
+
+}  // extern "C"
