@@ -3,6 +3,8 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
+#include <climits>
 #include <cmath>
 
 #include "../../include/opc_b200.h"
@@ -47,10 +49,11 @@ bool vec_ok(const void* p, int64_t ld, int32_t dtype) {
 }
 
 template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y, int threads, void* stream, Args... args) {
+cudaError_t launch_smem(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y, int threads, size_t smem, void* stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(grid_x, grid_y);
   cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];  // the launch overlaps the end of the kernel before, which the kernel waits for
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -58,6 +61,10 @@ cudaError_t launch(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y, int
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, args...);
+}
+template <typename... KArgs, typename... Args>
+cudaError_t launch(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y, int threads, void* stream, const Args&... args) {
+  return launch_smem(kern, grid_x, grid_y, threads, 0, stream, args...);
 }
 
 // One warp per row up to 1024 values; beyond, one CTA per row with 16 values a thread (32 from 16384
@@ -105,6 +112,86 @@ int start_rows(const char* who, const opc_i8_rows* out, void* values, int64_t ld
   a->v_type = v_dtype;
   a->vec_v = values && vec_ok(values, ldv, v_dtype);
   return OPC_OK;
+}
+
+// ---- the product's plan
+constexpr size_t kCountBytes = 16384;  // arrival counts, at the front of the workspace: 256 cut tiles at most
+
+struct GemmPlan {
+  opc::I8Deal deal;
+  int pairs;
+  size_t bytes;  // of workspace; 0: refused
+};
+
+GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, int sms) {
+  GemmPlan p = {};
+  p.bytes = kCountBytes;
+  if (rows <= opc::kI8GemvRows) return p;
+  opc::I8Deal& d = p.deal;
+  p.pairs = std::min(std::max(sms / 2, 1), 256);
+  d.nk = (K + opc::kI8Block - 1) / opc::kI8Block;
+  const int64_t m_tiles = (static_cast<int64_t>(M) + 255) / 256;
+  // Clocks of one stage: 2 a token for the MMAs, or the loads of 16 KB + 64 bytes a token at 64 a clock.
+  auto clocks = [](int n) { return std::max(2 * n, 256 + n); };
+  int64_t best = 0;
+  for (int n = 256; n >= 32; n -= 32) {
+    const int64_t t = (static_cast<int64_t>(rows) + n - 1) / n * clocks(n);
+    if (!best || t < best) {
+      best = t;
+      d.tile_n = n;
+    }
+  }
+  const int64_t n_tiles = (static_cast<int64_t>(rows) + d.tile_n - 1) / d.tile_n, tiles = m_tiles * n_tiles;
+  if (tiles > INT32_MAX / 2) {
+    p.bytes = 0;
+    return p;
+  }
+  d.m_tiles = static_cast<int32_t>(m_tiles);
+  d.n_tiles = static_cast<int32_t>(n_tiles);
+  d.full = static_cast<int32_t>(tiles / p.pairs * p.pairs);
+  d.rest = static_cast<int32_t>(tiles) - d.full;
+  // The rest along K: each pair does fewer stages, and a cut tile's sums go through L2 once more for
+  // every pair that shares it (512 bytes a token for each CTA, some 40 a clock, after about 2000 to start).
+  d.sharers = d.rest;
+  const int64_t stages = static_cast<int64_t>(d.rest) * d.nk;
+  int64_t least = 0;
+  for (int s = d.rest; d.rest && s <= std::min<int64_t>(p.pairs, stages); ++s) {
+    const int share = (s + d.rest - 1) / d.rest + (s % d.rest ? 1 : 0);  // most pairs at a tile
+    const int64_t t = (stages + s - 1) / s * clocks(d.tile_n) + (s > d.rest ? 2000 + static_cast<int64_t>(share) * d.tile_n * 13 : 0);
+    if (!least || t < least) {
+      least = t;
+      d.sharers = s;
+    }
+  }
+  if (!d.full) p.pairs = d.sharers;  // (no more CTAs than have work)
+  if (d.sharers > d.rest) p.bytes += static_cast<size_t>(d.sharers) * 4 * 128 * d.tile_n * sizeof(int32_t);
+  return p;
+}
+
+// Rows of codes as a tensor of bytes, in boxes of 128 bytes x box rows, zeros beyond its edges.
+int map_codes(const char* who, const opc_i8_rows* m, int box, CUtensorMap* map) {
+  auto encode = opc_host::tensor_map_encoder();
+  if (!encode) return fail(OPC_ERR_CUDA, "%s: cuTensorMapEncodeTiled unavailable", who);
+  const cuuint64_t dim[2] = {static_cast<cuuint64_t>(m->n), static_cast<cuuint64_t>(m->rows)};
+  const cuuint64_t stride[1] = {static_cast<cuuint64_t>(m->ld)};
+  const cuuint32_t boxes[2] = {opc::kI8Block, static_cast<cuuint32_t>(box)}, step[2] = {1, 1};
+  const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, m->codes, dim, stride, boxes, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? OPC_OK : fail(OPC_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", who, static_cast<int>(r));
+}
+
+// The most dynamic shared memory for kernel `k` (number `which`), once per device.
+template <typename K>
+cudaError_t allow_smem(K k, int which) {
+  static std::atomic<uint64_t> done[3];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+  if (done[which].load(std::memory_order_acquire) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+  if (e == cudaSuccess) done[which].fetch_or(bit, std::memory_order_release);
+  return e;
 }
 
 int end_rows(const char* who, cudaError_t e) { return e == cudaSuccess ? OPC_OK : cuda_fail(e, who); }
@@ -180,8 +267,13 @@ int opc_i8_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, 
 }
 
 size_t opc_i8_gemm_workspace_bytes(int32_t rows, int32_t M, int32_t K, int32_t device) {
-  (void)device;
-  return rows >= 0 && M >= 1 && K >= 1 && K <= kMaxWidth ? 16 : 0;
+  if (rows < 0 || M < 1 || K < 1 || K > kMaxWidth) return 0;
+  int sms = 0;
+  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
+    cudaGetLastError();
+    return 0;
+  }
+  return plan_gemm(rows, M, K, sms).bytes;
 }
 
 int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, int32_t bias_dtype, void* y, int64_t ldy,
@@ -194,9 +286,31 @@ int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, in
   if (x->rows == 0) return OPC_OK;
   if ((rc = check_matrix(who, "y", y, ldy, y_dtype, w->rows)) != OPC_OK) return rc;
   if (bias && (rc = check_matrix(who, "bias", bias, w->rows, bias_dtype, w->rows)) != OPC_OK) return rc;
-  if (!workspace || workspace_bytes < 16) return fail(OPC_ERR_WORKSPACE, "%s: a workspace of 16 bytes is needed, got %zu", who, workspace_bytes);
-  opc::I8GemmArgs a = {x->codes, w->codes, x->scales, w->scales, bias, y, x->ld, w->ld, ldy, x->rows, w->rows, x->n, bias_dtype, y_dtype};
-  return end_rows(who, launch(opc::i8_gemm_simple, (w->rows + 63) / 64, (x->rows + 63) / 64, 256, stream, a));
+  opc_host::Device dev;
+  if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
+  const GemmPlan p = plan_gemm(x->rows, w->rows, x->n, dev.sm_count);
+  if (!p.bytes) return fail(OPC_ERR_UNSUPPORTED, "%s: %d tokens times %d channels are too many tiles for one call", who, x->rows, w->rows);
+  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < p.bytes)
+    return fail(OPC_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", who, p.bytes, workspace_bytes);
+  opc::I8GemmArgs a;
+  a.o = {x->scales, w->scales, bias, y, ldy, x->rows, w->rows, bias_dtype, y_dtype};
+  if (x->rows <= opc::kI8GemvRows) {
+    auto k = y_dtype == OPC_F16 ? opc::i8_gemv_kernel<opc::kI8F16>
+             : y_dtype == OPC_BF16 ? opc::i8_gemv_kernel<opc::kI8BF16> : opc::i8_gemv_kernel<opc::kI8F32>;
+    return end_rows(who, launch(k, (w->rows + 15) / 16, 1, opc::kI8GemvWarps * 32, stream, x->codes, x->ld, w->codes, w->ld, x->n, a.o));
+  }
+  a.d = p.deal;
+  a.count = static_cast<int32_t*>(workspace);
+  a.part = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + kCountBytes);
+  a.err = dev.error_word;
+  CUtensorMap tw, tx;
+  if ((rc = map_codes(who, w, 128, &tw)) != OPC_OK || (rc = map_codes(who, x, p.deal.tile_n / 2, &tx)) != OPC_OK) return rc;
+  auto k = y_dtype == OPC_F16 ? opc::i8_gemm_kernel<opc::kI8F16>
+           : y_dtype == OPC_BF16 ? opc::i8_gemm_kernel<opc::kI8BF16> : opc::i8_gemm_kernel<opc::kI8F32>;
+  const size_t smem = 1024 + static_cast<size_t>(opc::i8_stages(p.deal.tile_n)) * opc::i8_stage_bytes(p.deal.tile_n) + 512;
+  const cudaError_t e = allow_smem(k, y_dtype);
+  if (e != cudaSuccess) return cuda_fail(e, "opc_i8_gemm: shared memory");
+  return end_rows(who, launch_smem(k, 2 * p.pairs, 1, opc::kI8Threads, smem, stream, tw, tx, a));
 }
 
 }  // extern "C"

@@ -2,6 +2,7 @@
 // the calling thread, device properties and the device error word (all defined in opc_lib.cu).
 #pragma once
 
+#include <cudaTypedefs.h>
 #include <cuda_runtime.h>
 
 namespace opc_host {
@@ -17,5 +18,8 @@ struct Device {
 };
 // Properties of the current device (looked up once per device).
 __attribute__((visibility("hidden"))) int current_device(Device* out);
+
+// cuTensorMapEncodeTiled (NULL where the driver has none).
+__attribute__((visibility("hidden"))) PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
 }  // namespace opc_host

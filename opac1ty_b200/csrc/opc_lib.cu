@@ -357,6 +357,7 @@ int fail(int code, const char* fmt, ...) {
 }
 
 int cuda_fail(cudaError_t e, const char* what) { return ::cuda_fail(e, what); }
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() { return ::tensor_map_encoder(); }
 
 int current_device(Device* out) try {
   int dev = 0;
