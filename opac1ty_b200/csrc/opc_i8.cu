@@ -129,7 +129,6 @@ GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, int sms) {
   if (rows <= opc::kI8GemvRows) return p;
   opc::I8Deal& d = p.deal;
   p.pairs = std::min(std::max(sms / 2, 1), 256);
-  d.nk = (K + opc::kI8Block - 1) / opc::kI8Block;
   const int64_t m_tiles = (static_cast<int64_t>(M) + 255) / 256;
   // Clocks of one stage: 2 a token for the MMAs, or the loads of 16 KB + 64 bytes a token at 64 a clock.
   auto clocks = [](int n) { return std::max(2 * n, 256 + n); };
@@ -141,6 +140,10 @@ GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, int sms) {
       d.tile_n = n;
     }
   }
+  // Few tokens: two blocks a stage, since the barriers of a stage outlast its small MMAs (24 tokens,
+  // 14336 -> 4096: 18.7 -> 17.1 us; 4 blocks no better).
+  d.sub = d.tile_n <= 64 ? 2 : 1;
+  d.nk = (K + opc::kI8Block * d.sub - 1) / (opc::kI8Block * d.sub);
   const int64_t n_tiles = (static_cast<int64_t>(rows) + d.tile_n - 1) / d.tile_n, tiles = m_tiles * n_tiles;
   if (tiles > INT32_MAX / 2) {
     p.bytes = 0;
@@ -157,7 +160,7 @@ GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, int sms) {
   int64_t least = 0;
   for (int s = d.rest; d.rest && s <= std::min<int64_t>(p.pairs, stages); ++s) {
     const int share = (s + d.rest - 1) / d.rest + (s % d.rest ? 1 : 0);  // most pairs at a tile
-    const int64_t t = (stages + s - 1) / s * clocks(d.tile_n) + (s > d.rest ? 2000 + static_cast<int64_t>(share) * d.tile_n * 13 : 0);
+    const int64_t t = (stages + s - 1) / s * clocks(d.tile_n) * d.sub + (s > d.rest ? 2000 + static_cast<int64_t>(share) * d.tile_n * 13 : 0);
     if (!least || t < least) {
       least = t;
       d.sharers = s;
@@ -307,7 +310,7 @@ int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, in
   if ((rc = map_codes(who, w, 128, &tw)) != OPC_OK || (rc = map_codes(who, x, p.deal.tile_n / 2, &tx)) != OPC_OK) return rc;
   auto k = y_dtype == OPC_F16 ? opc::i8_gemm_kernel<opc::kI8F16>
            : y_dtype == OPC_BF16 ? opc::i8_gemm_kernel<opc::kI8BF16> : opc::i8_gemm_kernel<opc::kI8F32>;
-  const size_t smem = 1024 + static_cast<size_t>(opc::i8_stages(p.deal.tile_n)) * opc::i8_stage_bytes(p.deal.tile_n) + 512;
+  const size_t smem = 1024 + static_cast<size_t>(opc::i8_stages(p.deal.tile_n, p.deal.sub)) * p.deal.sub * opc::i8_block_bytes(p.deal.tile_n) + 512;
   const cudaError_t e = allow_smem(k, y_dtype);
   if (e != cudaSuccess) return cuda_fail(e, "opc_i8_gemm: shared memory");
   return end_rows(who, launch_smem(k, 2 * p.pairs, 1, opc::kI8Threads, smem, stream, tw, tx, a));

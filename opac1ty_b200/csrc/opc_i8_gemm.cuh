@@ -12,7 +12,7 @@
 //                 that what they read stays in L2), then share the rest out along K in equal ranges.
 //                 Tiles cut by a range are summed through the workspace by whoever comes last.
 //                   warp 0     TMA
-//                   warp 1     tensor memory; in the pair's first CTA one lane issues the MMAs
+//                   warp 1     tensor memory; in the pair's first CTA it issues the MMAs
 //                   warps 2-9  epilogue: two warps per TMEM lane quarter, half of the columns each;
 //                              it reads one accumulator while the MMAs fill the other
 // i8_gemv_kernel  up to 8 tokens: mma.sync fragments straight from global memory; bound by the reading
@@ -34,9 +34,10 @@ constexpr int kI8Group = 8;                   // channel tiles taken together
 constexpr int kI8MaxStages = 12;
 constexpr int kI8SmemBudget = 227 * 1024 - 1024 - 512;  // less alignment slack and barriers
 
-__host__ __device__ constexpr int i8_stage_bytes(int n) { return kI8ABytes + n * (kI8Block / 2); }
-__host__ __device__ constexpr int i8_stages(int n) {
-  return kI8SmemBudget / i8_stage_bytes(n) > kI8MaxStages ? kI8MaxStages : kI8SmemBudget / i8_stage_bytes(n);
+// A stage holds `sub` blocks of 128 values of K: the channels' block, then half of the tokens'.
+__host__ __device__ constexpr int i8_block_bytes(int n) { return kI8ABytes + n * (kI8Block / 2); }
+__host__ __device__ constexpr int i8_stages(int n, int sub) {
+  return kI8SmemBudget / (sub * i8_block_bytes(n)) > kI8MaxStages ? kI8MaxStages : kI8SmemBudget / (sub * i8_block_bytes(n));
 }
 
 struct I8Out {
@@ -51,6 +52,7 @@ struct I8Out {
 struct I8Deal {
   int32_t tile_n;              // tokens of a tile
   int32_t m_tiles, n_tiles;    // tiles of 256 channels, of tile_n tokens
+  int32_t sub;                 // blocks of 128 values of K in a stage
   int32_t nk;                  // stages of a tile
   int32_t full;                // tiles taken whole, in turn (a multiple of the pairs)
   int32_t rest;                // tiles after them, cut along K into `sharers` equal ranges
@@ -76,11 +78,12 @@ __device__ __forceinline__ void i8_store1(void* p, int64_t i, float v) {
   else if constexpr (kY == kI8BF16) static_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
   else static_cast<float*>(p)[i] = v;
 }
-// The one way from a sum to a result: fp32 operations in this order, no fused ones.
-__device__ __forceinline__ float i8_result(int32_t sum, float sx, float sw, float bias, bool with_bias) {
-  const float v = __fmul_rn(__fmul_rn(static_cast<float>(sum), sx), sw);
-  return with_bias ? __fadd_rn(v, bias) : v;
+// The one way from a sum to a result: fp32 operations in this order, no fused ones.  Without a bias it
+// is -0, which changes nothing.
+__device__ __forceinline__ float i8_result(int32_t sum, float sx, float sw, float bias) {
+  return __fadd_rn(__fmul_rn(__fmul_rn(static_cast<float>(sum), sx), sw), bias);
 }
+__device__ __forceinline__ float i8_bias(const I8Out& o, int32_t r) { return o.bias ? i8_load1(o.bias_type, o.bias, r) : -0.f; }
 
 // ------------------------------------------------------------------------------------------------
 // Pairs of CTAs
@@ -102,24 +105,36 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The asynchronous operations are issued by one lane (`leader`) of a converged warp: outside a divergent
+// branch their operands can stay in uniform registers.
 // A TMA load into this CTA's shared memory that completes on a barrier of either CTA of the pair.
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t leader, uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
   asm volatile(
-      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
-      "l"(map), "r"(x), "r"(y), "r"(bar)
+      "{\n .reg .pred l;\n setp.ne.b32 l, %5, 0;\n"
+      " @l cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n}\n" ::"r"(dst),
+      "l"(map), "r"(x), "r"(y), "r"(bar), "r"(leader)
       : "memory");
 }
-__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+__device__ __forceinline__ void mbar_expect_tx_by(uint32_t leader, uint32_t bar, uint32_t bytes) {
   asm volatile(
-      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum)
+      "{\n .reg .pred l;\n setp.ne.b32 l, %2, 0;\n @l mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n}\n" ::"r"(bar), "r"(bytes),
+      "r"(leader)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t leader, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
+  asm volatile(
+      "{\n .reg .pred p, l;\n setp.ne.b32 l, %5, 0;\n setp.ne.b32 p, %4, 0;\n"
+      " @l tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem_d),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accum), "r"(leader)
       : "memory");
 }
 // Arrives at the barrier of both CTAs once the MMAs issued so far are done.
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-               "h"(static_cast<uint16_t>(3))
-               : "memory");
+__device__ __forceinline__ void umma_commit_pair(uint32_t leader, uint32_t bar) {
+  asm volatile(
+      "{\n .reg .pred l;\n setp.ne.b32 l, %2, 0;\n"
+      " @l tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(bar),
+      "h"(static_cast<uint16_t>(3)), "r"(leader)
+      : "memory");
 }
 // kind::i8, A and B signed, D 32-bit integers, both K-major, 256 channels x n tokens.
 __device__ __forceinline__ uint32_t i8_idesc(int n) {
@@ -186,8 +201,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
   const int kN = a.d.tile_n;
-  const int stages = i8_stages(kN);
-  const uint32_t stage_bytes = i8_stage_bytes(kN);
+  const int sub = a.d.sub, stages = i8_stages(kN, sub);
+  const uint32_t block_bytes = i8_block_bytes(kN), stage_bytes = sub * block_bytes;
   const uint32_t bars = base + stages * stage_bytes;
   const uint32_t full_b = bars, empty_b = full_b + 8 * kI8MaxStages, accf_b = empty_b + 8 * kI8MaxStages, acce_b = accf_b + 16,
                  drain_b = acce_b + 16, tmem_slot = drain_b + 8;
@@ -227,65 +242,80 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
-    if (lane == 0) {
-      const uint32_t full0 = map_to_rank(full_b, 0);  // the first CTA's MMA lane waits for both CTAs' loads
-      int g = 0;
-      while (ok && walk.step()) {
-        int32_t mi, ni;
-        walk.place(&mi, &ni);
-        const int32_t r0 = mi * 256 + static_cast<int32_t>(rank) * 128, t0 = ni * kN + static_cast<int32_t>(rank) * (kN / 2);
-        for (int k = walk.k0; k < walk.k1; ++k, ++g) {
-          const int st = g % stages;
-          if (g >= stages && !mbar_wait_bounded(empty_b + 8 * st, ((g / stages) - 1) & 1)) {
-            ok = false;
-            break;
-          }
-          if (rank == 0) mbar_expect_tx(full_b + 8 * st, 2 * stage_bytes);
-          const uint32_t at = base + st * stage_bytes;
-          tma_load_2d_pair(at, &tw, k * kI8Block, r0, full0 + 8 * st);
-          tma_load_2d_pair(at + kI8ABytes, &tx, k * kI8Block, t0, full0 + 8 * st);
+    const uint32_t leader = elect_leader();
+    const uint32_t full0 = map_to_rank(full_b, 0);  // the first CTA's MMA warp waits for both CTAs' loads
+    int g = 0, st = 0;
+    uint32_t par = 1;  // of the stage's use before (the first round waits for nothing)
+    while (ok && walk.step()) {
+      int32_t mi, ni;
+      walk.place(&mi, &ni);
+      const int32_t r0 = mi * 256 + static_cast<int32_t>(rank) * 128, t0 = ni * kN + static_cast<int32_t>(rank) * (kN / 2);
+      for (int k = walk.k0; k < walk.k1; ++k, ++g) {
+        if (g >= stages) {
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty_b + 8 * st, par));
+          if (!ok) break;
+        }
+        if (rank == 0) mbar_expect_tx_by(leader, full_b + 8 * st, 2 * stage_bytes);
+        uint32_t at = base + st * stage_bytes;
+        int32_t x = k * sub * kI8Block;
+        for (int j = 0; j < sub; ++j, at += block_bytes, x += kI8Block) {
+          tma_load_2d_pair(leader, at, &tw, x, r0, full0 + 8 * st);
+          tma_load_2d_pair(leader, at + kI8ABytes, &tx, x, t0, full0 + 8 * st);
+        }
+        if (++st == stages) {
+          st = 0;
+          par ^= 1;
         }
       }
-      // what is under way to this CTA's shared memory arrives before it ends: the loads (which the first
-      // CTA's barriers count, for both) where a role gave up, and the last signals of the MMAs
-      for (int st = 0; st < stages && st < g; ++st) {
-        const uint32_t par = ((g - 1 - ((g - 1 - st) % stages)) / stages) & 1;  // of the stage's last use
-        if (rank == 0) mbar_wait_bounded(full_b + 8 * st, par);
-        if (ok && !mbar_wait_bounded(empty_b + 8 * st, par)) ok = false;
-      }
+    }
+    // what is under way to this CTA's shared memory arrives before it ends: the loads (which the first
+    // CTA's barriers count, for both) where a role gave up, and the last signals of the MMAs
+    for (int i = 0; i < stages && i < g; ++i) {
+      const uint32_t last = ((g - 1 - ((g - 1 - i) % stages)) / stages) & 1;  // parity of the stage's last use
+      if (rank == 0) mbar_wait_bounded(full_b + 8 * i, last);
+      if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(empty_b + 8 * i, last));
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- MMAs
-    if (rank == 0 && lane == 0) {
+    if (rank == 0) {
+      const uint32_t leader = elect_leader();
       const uint32_t idesc = i8_idesc(kN);
-      int g = 0, tl = 0;
+      int st = 0, tl = 0;
+      uint32_t par = 0;
       while (ok && walk.step()) {
         const int b = tl & 1;
-        if (tl >= 2 && !mbar_wait_bounded(acce_b + 8 * b, ((tl >> 1) - 1) & 1)) {
-          ok = false;
-          break;
+        if (tl >= 2) {
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(acce_b + 8 * b, ((tl >> 1) - 1) & 1));
+          if (!ok) break;
         }
         tc_fence_after();
         const uint32_t acc = tmem + static_cast<uint32_t>(b * (cols / 2));
-        for (int k = walk.k0; k < walk.k1; ++k, ++g) {
-          const int st = g % stages;
-          if (!mbar_wait_bounded(full_b + 8 * st, (g / stages) & 1)) {
-            ok = false;
-            break;
-          }
+        uint32_t more = 0;  // the tile's first MMA clears the accumulator
+        for (int k = walk.k0; k < walk.k1; ++k) {
+          ok = __all_sync(0xffffffffu, mbar_wait_bounded(full_b + 8 * st, par));
+          if (!ok) break;
           tc_fence_after();
-          const uint64_t ad = umma_desc_sw128(base + st * stage_bytes), bd = umma_desc_sw128(base + st * stage_bytes + kI8ABytes);
+          uint32_t at = base + st * stage_bytes;
+          for (int j = 0; j < sub; ++j, at += block_bytes) {
+            const uint64_t ad = umma_desc_sw128(at), bd = umma_desc_sw128(at + kI8ABytes);
 #pragma unroll
-          for (int kk = 0; kk < kI8Block / 32; ++kk)  // 32 bytes further in the swizzled rows
-            umma_i8_pair(acc, ad + 2 * kk, bd + 2 * kk, idesc, (k > walk.k0 || kk > 0) ? 1u : 0u);
-          umma_commit_pair(empty_b + 8 * st);
+            for (int kk = 0; kk < kI8Block / 32; ++kk) {  // 32 bytes further in the swizzled rows
+              umma_i8_pair(leader, acc, ad + 2 * kk, bd + 2 * kk, idesc, more);
+              more = 1;
+            }
+          }
+          umma_commit_pair(leader, empty_b + 8 * st);
+          if (++st == stages) {
+            st = 0;
+            par ^= 1;
+          }
         }
         if (!ok) break;
-        umma_commit_pair(accf_b + 8 * b);
+        umma_commit_pair(leader, accf_b + 8 * b);
         ++tl;
       }
       // no MMA of this pair is in flight past this point
-      asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_b) : "memory");
+      if (leader) asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(drain_b) : "memory");
       mbar_wait_bounded(drain_b, 0);
     }
   } else {
@@ -303,8 +333,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
       const bool live = r < a.o.M, cut = walk.cut();
       const int b = tl & 1;
       const uint32_t acc = lanes + static_cast<uint32_t>(b * (cols / 2));
+      // before the wait: what the results take from memory (lane l has the scales of columns l, l + 32, ...)
+      float sx[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int c = c0 + 32 * j + lane;
+        sx[j] = c < c1 && t0 + c < a.o.rows ? a.o.sx[t0 + c] : 0.f;
+      }
       const float sw = live ? a.o.sw[r] : 0.f;
-      const float bias = live && a.o.bias ? i8_load1(a.o.bias_type, a.o.bias, r) : 0.f;
+      const float bias = live ? i8_bias(a.o, r) : 0.f;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(accf_b + 8 * b, (tl >> 1) & 1));
       tc_fence_after();
       int32_t first = 0, last = 0;
@@ -337,26 +374,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
           uint32_t v[16];
           tmem_ld16(acc + c, v);
           if (cut)
-            for (int p = first; p <= last; ++p) {
-              if (p == pair) continue;
-              const int32_t* other = a.part + (static_cast<int64_t>(walk.slot(p)) * 2 + rank) * (128 * kN);
+            for (int p0 = first; p0 <= last; p0 += 4) {  // four pairs' loads in flight
+              uint4 q[4][4];
 #pragma unroll
-              for (int i = 0; i < 16; i += 4) {
-                const uint4 q = __ldcg(reinterpret_cast<const uint4*>(other + ((c + i) / 4 * 128 + row) * 4));
-                v[i] += q.x;
-                v[i + 1] += q.y;
-                v[i + 2] += q.z;
-                v[i + 3] += q.w;
+              for (int j = 0; j < 4; ++j) {
+                const int p = p0 + j;
+                const bool other = p <= last && p != pair;
+                const int32_t* from = a.part + (static_cast<int64_t>(walk.slot(other ? p : pair)) * 2 + rank) * (128 * kN);
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  q[j][i] = other ? ld_cg_v4(from + ((c / 4 + i) * 128 + row) * 4) : make_uint4(0, 0, 0, 0);
               }
-            }
-          const int32_t t = t0 + c;
-          const float sx = t + (lane & 15) < a.o.rows ? a.o.sx[t + (lane & 15)] : 0.f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float s = __shfl_sync(0xffffffffu, sx, i);
-            if (live && t + i < a.o.rows)
-              i8_store1<kY>(a.o.y, static_cast<int64_t>(t + i) * a.o.ldy + r,
-                            i8_result(static_cast<int32_t>(v[i]), s, sw, bias, a.o.bias != nullptr));
+              for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  v[4 * i] += q[j][i].x;
+                  v[4 * i + 1] += q[j][i].y;
+                  v[4 * i + 2] += q[j][i].z;
+                  v[4 * i + 3] += q[j][i].w;
+                }
+            }
+          const int j = (c - c0) >> 4;
+          const float sc = __shfl_sync(0xffffffffu, j < 4 ? (j < 2 ? sx[0] : sx[1]) : (j < 6 ? sx[2] : sx[3]), (lane & 15) + 16 * (j & 1));
+          float f[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) f[i] = i8_result(static_cast<int32_t>(v[i]), __shfl_sync(0xffffffffu, sc, i), sw, bias);
+          const int32_t left = a.o.rows - (t0 + c);
+          const int64_t at = static_cast<int64_t>(t0 + c) * a.o.ldy + r;
+          if (live && left >= 16) {  // (without a branch per value, so that their chains overlap)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) i8_store1<kY>(a.o.y, at + i * a.o.ldy, f[i]);
+          } else if (live) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (i < left) i8_store1<kY>(a.o.y, at + i * a.o.ldy, f[i]);
           }
         }
       }
@@ -455,7 +507,7 @@ __global__ void __launch_bounds__(kI8GemvWarps * 32) i8_gemv_kernel(const int8_t
 #pragma unroll
     for (int i = 0; i < kI8GemvWarps; ++i) s += sums[i][threadIdx.x];
     i8_store1<kY>(o.y, static_cast<int64_t>(t) * o.ldy + r,
-                  i8_result(s, o.sx[t], o.sw[r], o.bias ? i8_load1(o.bias_type, o.bias, r) : 0.f, o.bias != nullptr));
+                  i8_result(s, o.sx[t], o.sw[r], i8_bias(o, r)));
   }
 }
 

@@ -77,11 +77,6 @@ struct KvPromptSplit {
 // MMAs issued by one lane of a converged warp (`leader`, from elect.sync): outside a divergent branch
 // their operands can be formed in uniform registers, which brought a key tile's 48 instructions and
 // their barriers from ~6300 cycles to what the tensor cores take.
-__device__ __forceinline__ uint32_t elect_leader() {
-  uint32_t p;
-  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(p));
-  return p;
-}
 __device__ __forceinline__ void umma_f16_by(uint32_t leader, uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accum) {
   asm volatile(
       "{\n .reg .pred p, l;\n setp.ne.b32 l, %5, 0;\n setp.ne.b32 p, %4, 0;\n"

@@ -16,8 +16,9 @@ def clocks(n):
 
 def plan(rows, m, k, sms):
     pairs = min(max(sms // 2, 1), 256)
-    nk = -(-k // 128)
     tile_n = min(range(256, 31, -32), key=lambda n: -(-rows // n) * clocks(n))
+    sub = 2 if tile_n <= 64 else 1
+    nk = -(-k // (128 * sub))
     m_tiles, n_tiles = -(-m // 256), -(-rows // tile_n)
     tiles = m_tiles * n_tiles
     full = tiles // pairs * pairs
@@ -25,7 +26,7 @@ def plan(rows, m, k, sms):
     stages, least, sharers = rest * nk, 0, rest
     for s in range(rest, min(pairs, stages) + 1) if rest else ():
         share = -(-s // rest) + (1 if s % rest else 0)
-        t = -(-stages // s) * clocks(tile_n) + (2000 + share * tile_n * 13 if s > rest else 0)
+        t = -(-stages // s) * clocks(tile_n) * sub + (2000 + share * tile_n * 13 if s > rest else 0)
         if not least or t < least:
             least, sharers = t, s
     if not full:
