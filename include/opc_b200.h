@@ -481,8 +481,9 @@ int opc_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int32_t ro
  *   code  = round(v * 127 / a)     (to even; -127 .. 127)
  * and stands for scale * code.  A row with a < 2^-100 counts as zeros (scale 0, codes 0).  A row with
  * an infinity or NaN has a NaN scale and codes 0: everything made of it is NaN.  v is formed in fp32
- * from the inputs, and so is the quotient v * 127 / a, rounded to the nearest fp32 before it is rounded
- * to a whole number (for 16-bit inputs taken as they are, codes are exact, halves included).
+ * from the inputs (silu's exponential to |g| 2^-23 of itself), and so is v * 127 / a before it is rounded
+ * to a whole number.  Where nothing was added or gated, that quotient is the nearest fp32: codes of 16-bit
+ * inputs taken as they are are exact, halves included.
  * --------------------------------------------------------------------------------------------- */
 typedef struct opc_i8_rows {
   int32_t rows, n;                /* n 1 .. 131071 (no sum of products of two rows leaves 32 bits) */

@@ -6,6 +6,7 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
+#include <cstdlib>
 
 #include "../../include/opc_b200.h"
 #include "opc_i8_gemm.cuh"
@@ -166,6 +167,7 @@ GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, int sms) {
       d.sharers = s;
     }
   }
+  if (getenv("I8_SHARE") && d.rest) { int v = atoi(getenv("I8_SHARE")); if (v) d.sharers = (int)std::min<int64_t>(std::min<int64_t>((int64_t)v * d.rest, p.pairs), stages); }
   if (!d.full) p.pairs = d.sharers;  // (no more CTAs than have work)
   if (d.sharers > d.rest) p.bytes += static_cast<size_t>(d.sharers) * 4 * 128 * d.tile_n * sizeof(int32_t);
   return p;

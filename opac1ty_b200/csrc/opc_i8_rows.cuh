@@ -7,8 +7,9 @@
 //
 // The norm's factor is the same for a whole row, so the codes do not depend on it: the sum of
 // squares and the largest magnitude come out of ONE reduction, and every value is read once and kept
-// in registers between the reduction and the rounding.  Memory bound; see opc_i8.cu for how rows are
-// dealt to threads.
+// in registers between the reduction and the rounding.  Bound by memory for large calls, which takes
+// few enough instructions per value that it stays so: pairs of values in packed fp32 operations, one
+// maximum of three per two values (see opc_i8.cu for how rows are dealt to threads and what it measured).
 #pragma once
 
 #include <cuda_bf16.h>
@@ -24,7 +25,6 @@ enum : int { kI8Quant = 0, kI8Norm = 1, kI8Silu = 2 };
 enum : int { kI8F16 = 0, kI8BF16 = 1, kI8F32 = 2, kI8None = 3 };  // element types (OPC_F16, ...)
 
 constexpr float kI8Least = 7.888609052210118e-31f;  // 2^-100: rows below it are zeros
-constexpr int kI8MaxPer = 4;                         // most groups of 8 values a thread keeps in registers
 
 struct I8RowsArgs {
   const void* x;      // quantize: x; norm: h; silu: gate
@@ -36,76 +36,142 @@ struct I8RowsArgs {
   void* values;       // what the codes stand for (or NULL), element type v_type
   int64_t ldx, ldu, ldh, ldc, ldv;
   int32_t rows, n, w_type, v_type;
-  // groups of 8 values that may be moved 16 bytes at a time (else one value at a time)
-  int32_t vec_x, vec_u, vec_w, vec_h, vec_v, vec_c;
+  // whether groups of 8 values may be moved 16 bytes at a time (else one value at a time)
+  int32_t vec_x, vec_u, vec_w, vec_h, vec_v;
   float eps;
 };
 
-// 8 values at p (element type kT) as fp32; with !vec, or fewer than 8 left, one at a time, zeros after them.
+// Two fp32 values, one instruction for both.
+using I8Pair = unsigned long long;
+__device__ __forceinline__ I8Pair i8_pair(float a, float b) {
+  I8Pair p;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(a), "f"(b));
+  return p;
+}
+__device__ __forceinline__ float2 i8_both(I8Pair p) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(p));
+  return f;
+}
+__device__ __forceinline__ I8Pair i8_mul2(I8Pair a, I8Pair b) {
+  I8Pair d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ I8Pair i8_add2(I8Pair a, I8Pair b) {
+  I8Pair d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ I8Pair i8_fma2(I8Pair a, I8Pair b, I8Pair c) {
+  I8Pair d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+// max(|a|, |b|, |c|), NaN if one of them is.
+__device__ __forceinline__ float i8_max3(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+// 8 values as they lie in memory.
 template <int kT>
-__device__ __forceinline__ void i8_load8(const void* base, int64_t at, int left, bool vec, float (&v)[8]) {
+struct I8Raw {
+  uint4 a, b;  // (b: the second half of 32-bit values)
+};
+
+// With !vec, or fewer than 8 left, one at a time, zeros after them.
+template <int kT>
+__device__ __forceinline__ void i8_load8(const void* base, int64_t at, int left, bool vec, I8Raw<kT>& r) {
   if constexpr (kT == kI8F32) {
-    const float* p = static_cast<const float*>(base) + at;
+    const uint32_t* p = static_cast<const uint32_t*>(base) + at;
     if (vec && left >= 8) {
-      const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      r.a = *reinterpret_cast<const uint4*>(p);
+      r.b = *reinterpret_cast<const uint4*>(p + 4);
     } else {
+      uint32_t v[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0.f;
+      for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0u;
+      r.a = make_uint4(v[0], v[1], v[2], v[3]);
+      r.b = make_uint4(v[4], v[5], v[6], v[7]);
     }
   } else {
     const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-    uint32_t h[4];
     if (vec && left >= 8) {
-      const uint4 a = *reinterpret_cast<const uint4*>(p);
-      h[0] = a.x; h[1] = a.y; h[2] = a.z; h[3] = a.w;
+      r.a = *reinterpret_cast<const uint4*>(p);
     } else {
+      uint32_t h[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         h[i] = (2 * i < left ? p[2 * i] : 0u) | (2 * i + 1 < left ? static_cast<uint32_t>(p[2 * i + 1]) << 16 : 0u);
+      r.a = make_uint4(h[0], h[1], h[2], h[3]);
     }
+  }
+}
+template <int kT>
+__device__ __forceinline__ void i8_open8(const I8Raw<kT>& r, I8Pair (&v)[4]) {
+  const uint32_t a[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
+  if constexpr (kT == kI8F32) {
+    const uint32_t b[4] = {r.b.x, r.b.y, r.b.z, r.b.w};
+    v[0] = i8_pair(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    v[1] = i8_pair(__uint_as_float(a[2]), __uint_as_float(a[3]));
+    v[2] = i8_pair(__uint_as_float(b[0]), __uint_as_float(b[1]));
+    v[3] = i8_pair(__uint_as_float(b[2]), __uint_as_float(b[3]));
+  } else {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if constexpr (kT == kI8BF16) {  // a bf16 is the upper half of an fp32
-        v[2 * i] = __uint_as_float(h[i] << 16);
-        v[2 * i + 1] = __uint_as_float(h[i] & 0xffff0000u);
+        v[i] = i8_pair(__uint_as_float(a[i] << 16), __uint_as_float(a[i] & 0xffff0000u));
       } else {
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
-        v[2 * i] = f.x;
-        v[2 * i + 1] = f.y;
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
+        v[i] = i8_pair(f.x, f.y);
       }
     }
   }
 }
-__device__ __forceinline__ void i8_load8_of(int type, const void* base, int64_t at, int left, bool vec, float (&v)[8]) {
-  if (type == kI8F16) i8_load8<kI8F16>(base, at, left, vec, v);
-  else if (type == kI8BF16) i8_load8<kI8BF16>(base, at, left, vec, v);
-  else i8_load8<kI8F32>(base, at, left, vec, v);
+__device__ __forceinline__ void i8_load8_of(int type, const void* base, int64_t at, int left, bool vec, I8Pair (&v)[4]) {
+  if (type == kI8F16) {
+    I8Raw<kI8F16> r;
+    i8_load8(base, at, left, vec, r);
+    i8_open8(r, v);
+  } else if (type == kI8BF16) {
+    I8Raw<kI8BF16> r;
+    i8_load8(base, at, left, vec, r);
+    i8_open8(r, v);
+  } else {
+    I8Raw<kI8F32> r;
+    i8_load8(base, at, left, vec, r);
+    i8_open8(r, v);
+  }
 }
 
 template <int kT>
-__device__ __forceinline__ void i8_store8(void* base, int64_t at, int left, bool vec, const float (&v)[8]) {
+__device__ __forceinline__ void i8_store8(void* base, int64_t at, int left, bool vec, const I8Pair (&v)[4]) {
   if constexpr (kT == kI8F32) {
     float* p = static_cast<float*>(base) + at;
     if (vec && left >= 8) {
-      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
+      const float2 a = i8_both(v[0]), b = i8_both(v[1]), c = i8_both(v[2]), d = i8_both(v[3]);
+      *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
+      *reinterpret_cast<float4*>(p + 4) = make_float4(c.x, c.y, d.x, d.y);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) p[i] = v[i];
+      for (int i = 0; i < 8; ++i) {
+        const float2 f = i8_both(v[i >> 1]);
+        if (i < left) p[i] = (i & 1) ? f.y : f.x;
+      }
     }
   } else {
     uint16_t* p = static_cast<uint16_t*>(base) + at;
     uint32_t h[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      const float2 f = i8_both(v[i]);
       if constexpr (kT == kI8BF16) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+        const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
         h[i] = *reinterpret_cast<const uint32_t*>(&b);
       } else {
-        const __half2 b = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+        const __half2 b = __floats2half2_rn(f.x, f.y);
         h[i] = *reinterpret_cast<const uint32_t*>(&b);
       }
     }
@@ -118,21 +184,24 @@ __device__ __forceinline__ void i8_store8(void* base, int64_t at, int left, bool
     }
   }
 }
-__device__ __forceinline__ void i8_store8_of(int type, void* base, int64_t at, int left, bool vec, const float (&v)[8]) {
+__device__ __forceinline__ void i8_store8_of(int type, void* base, int64_t at, int left, bool vec, const I8Pair (&v)[4]) {
   if (type == kI8F16) i8_store8<kI8F16>(base, at, left, vec, v);
   else if (type == kI8BF16) i8_store8<kI8BF16>(base, at, left, vec, v);
   else i8_store8<kI8F32>(base, at, left, vec, v);
 }
 
-// What a row's reduction carries: max |v| as bits (a NaN's are above infinity's, so it is kept), the
-// sum of t^2, and the same of t * 2^-80, which holds where the first one leaves the range of fp32.
+// What a row's reduction carries: max |v| (NaN if a value is), and for the norm two sums of squares,
+// of t and of t * 2^-80; the second holds where the first leaves the range of fp32.
 struct I8Stat {
-  uint32_t big;
-  float ss, small;
+  float big;
+  I8Pair ss, small;  // sums of even and odd places
+};
+struct I8Row {
+  float big, ss, small;
 };
 
-__device__ __forceinline__ void i8_warp_reduce(I8Stat& s, bool norm) {
-  s.big = __reduce_max_sync(0xffffffffu, s.big);
+__device__ __forceinline__ void i8_warp_reduce(I8Row& s, bool norm) {
+  s.big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(s.big)));  // (not negative; a NaN's bits are the largest)
   if (norm) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) {
@@ -141,45 +210,55 @@ __device__ __forceinline__ void i8_warp_reduce(I8Stat& s, bool norm) {
     }
   }
 }
-// Over the CTA; every thread gets the result.  Sums in one order, whatever the timing.
-__device__ __forceinline__ void i8_block_reduce(I8Stat& s, bool norm) {
-  __shared__ uint32_t part_big[32];
-  __shared__ float part_ss[32], part_small[32];
-  i8_warp_reduce(s, norm);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-  if (lane == 0) {
-    part_big[warp] = s.big;
-    if (norm) {
-      part_ss[warp] = s.ss;
-      part_small[warp] = s.small;
-    }
-  }
-  __syncthreads();
-  s.big = lane < warps ? part_big[lane] : 0u;
+// Over the row's threads; every one gets the result.  Sums in one order, whatever the timing.
+template <bool kWarpRow>
+__device__ __forceinline__ I8Row i8_reduce(const I8Stat& p, bool norm) {
+  I8Row s;
+  s.big = p.big;
   if (norm) {
-    s.ss = lane < warps ? part_ss[lane] : 0.f;
-    s.small = lane < warps ? part_small[lane] : 0.f;
+    const float2 a = i8_both(p.ss), b = i8_both(p.small);
+    s.ss = a.x + a.y;
+    s.small = b.x + b.y;
   }
   i8_warp_reduce(s, norm);
+  if constexpr (!kWarpRow) {
+    __shared__ float part_big[32], part_ss[32], part_small[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    if (lane == 0) {
+      part_big[warp] = s.big;
+      if (norm) {
+        part_ss[warp] = s.ss;
+        part_small[warp] = s.small;
+      }
+    }
+    __syncthreads();
+    s.big = lane < warps ? part_big[lane] : 0.f;
+    if (norm) {
+      s.ss = lane < warps ? part_ss[lane] : 0.f;
+      s.small = lane < warps ? part_small[lane] : 0.f;
+    }
+    i8_warp_reduce(s, norm);
+  }
+  return s;
 }
 
-// What the codes are made with: code = round((v * c) / a) with c = 127 and a the largest magnitude, or
-// both times 2^-32 where v * 127 could leave fp32; inv = 1 / a.  `live` is false for rows of zeros and
-// rows that hold an infinity or NaN, whose codes are 0 whatever v is.
+// What the codes are made with.  `exact`: code = round((v * c) / a) with c = 127 and a the largest
+// magnitude, or both times 2^-32 where v * 127 could leave fp32; inv = 1 / a.  Else round(v * mul).
+// `live` is false for rows of zeros and rows that hold an infinity or NaN, whose codes are 0 whatever v is.
 struct I8Scale {
-  float scale, c, a, inv;
+  float scale, mul, c, a, inv;
   bool live;
 };
-__device__ __forceinline__ I8Scale i8_scale_of(const I8Stat& s, bool norm, int n, float eps) {
+__device__ __forceinline__ I8Scale i8_scale_of(const I8Row& s, bool norm, int n, float eps) {
   I8Scale r;
-  const float big = __uint_as_float(s.big);
-  const bool bad = s.big >= 0x7f800000u;
-  r.live = !bad && big >= kI8Least;
-  const bool huge = s.big >= 0x70000000u;  // 2^97
+  const bool bad = !(s.big < __uint_as_float(0x7f800000u));
+  r.live = !bad && s.big >= kI8Least;
+  const bool huge = s.big >= 0x1p97f;
   r.c = huge ? 127.0f * 0x1p-32f : 127.0f;
-  r.a = huge ? big * 0x1p-32f : big;
+  r.a = huge ? s.big * 0x1p-32f : s.big;
   r.inv = 1.0f / r.a;
-  r.scale = bad ? __uint_as_float(0x7fffffffu) : r.live ? big / 127.0f : 0.f;
+  r.mul = 127.0f / s.big;
+  r.scale = bad ? __uint_as_float(0x7fffffffu) : r.live ? s.big / 127.0f : 0.f;
   if (norm && r.live) {
     const float len = static_cast<float>(n);
     // a finite row whose squares leave fp32: sqrt(mean (t 2^-80)^2) 2^80 (eps is nothing beside it)
@@ -189,23 +268,33 @@ __device__ __forceinline__ I8Scale i8_scale_of(const I8Stat& s, bool norm, int n
   return r;
 }
 
-// Codes (and values) of 8 values.  The quotient is corrected once by its remainder, so it is the
-// nearest fp32: a half that 16-bit inputs often meet is a half and goes to even (with v * (127 / a)
-// every half of a row goes the way that 127 / a was rounded).  Adding 1.5 * 2^23 rounds it to a whole
-// number; the lowest byte is the code.
-__device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, int left, const float (&v)[8], const I8Scale& s) {
+// Codes (and values) of 8 values.  Adding 1.5 * 2^23 rounds to a whole number, to even, whose lowest
+// byte is the code.  Exact: the quotient is corrected once by its remainder, so it is the nearest fp32,
+// and a half that 16-bit inputs often meet is a half and goes to even (with v * (127 / a) every half of
+// a row goes the way that 127 / a was rounded); where v itself is a rounded result there are none.
+template <bool kExact>
+__device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, int left, const I8Pair (&v)[4], const I8Scale& s) {
   constexpr float kMagic = 12582912.0f;
-  float f[8];
+  const I8Pair magic = i8_pair(kMagic, kMagic);
+  I8Pair f[4];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const float t = v[e] * s.c, q0 = t * s.inv;
-    f[e] = s.live ? __fadd_rn(fmaf(fmaf(-q0, s.a, t), s.inv, q0), kMagic) : kMagic;
+  for (int e = 0; e < 4; ++e) {
+    if (!s.live) {  // (the same for the whole row)
+      f[e] = magic;
+    } else if constexpr (kExact) {
+      const I8Pair inv = i8_pair(s.inv, s.inv), t = i8_mul2(v[e], i8_pair(s.c, s.c)), q = i8_mul2(t, inv);
+      f[e] = i8_add2(i8_fma2(i8_fma2(q, i8_pair(-s.a, -s.a), t), inv, q), magic);
+    } else {
+      f[e] = i8_fma2(v[e], i8_pair(s.mul, s.mul), magic);
+    }
   }
   uint32_t q[2];
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
-    q[e] = __byte_perm(__byte_perm(__float_as_uint(f[4 * e]), __float_as_uint(f[4 * e + 1]), 0x0040),
-                       __byte_perm(__float_as_uint(f[4 * e + 2]), __float_as_uint(f[4 * e + 3]), 0x0040), 0x5410);
+  for (int e = 0; e < 2; ++e) {
+    const float2 lo = i8_both(f[2 * e]), hi = i8_both(f[2 * e + 1]);
+    q[e] = __byte_perm(__byte_perm(__float_as_uint(lo.x), __float_as_uint(lo.y), 0x0040),
+                       __byte_perm(__float_as_uint(hi.x), __float_as_uint(hi.y), 0x0040), 0x5410);
+  }
   int8_t* c = a.codes + static_cast<int64_t>(row) * a.ldc + i;
   if (left >= 8) {
     *reinterpret_cast<uint2*>(c) = make_uint2(q[0], q[1]);  // (codes start on 16 bytes, rows too)
@@ -215,50 +304,67 @@ __device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, i
       if (e < left) c[e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
   }
   if (a.values) {
-    float o[8];
+    I8Pair o[4];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o[e] = (f[e] - kMagic) * s.scale;
+    for (int e = 0; e < 4; ++e) o[e] = i8_mul2(i8_add2(f[e], i8_pair(-kMagic, -kMagic)), i8_pair(s.scale, s.scale));
     i8_store8_of(a.v_type, a.values, static_cast<int64_t>(row) * a.ldv + i, left, a.vec_v, o);
   }
 }
 
-// The 8 values from i on of a row before its scale, their part of the statistics, and (norm) h_out.
+// silu(g) * u.  exp(-g) = 2^(-g log2 e): the rounded exponent is off by |g| 2^-24 at most, which next to
+// the row's largest value is nothing where |g| is large; 1 / (1 + it) to one step of fp32.
+__device__ __forceinline__ float i8_silu_mul(float g, float u) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
+  return g * r * u;
+}
+
+// 8 values of a row before its scale from what was loaded, their part of the statistics, and (norm) h_out.
 template <int kOp, int kTX, int kTU>
-__device__ __forceinline__ void i8_make8(const I8RowsArgs& a, int row, int i, float (&v)[8], I8Stat& s, bool write_h) {
+__device__ __forceinline__ void i8_make8(const I8RowsArgs& a, int row, int i, const I8Raw<kTX>& rx, const I8Raw<kTU>& ru, I8Pair (&v)[4],
+                                         I8Stat& s, bool write_h) {
   const int left = a.n - i;
-  i8_load8<kTX>(a.x, static_cast<int64_t>(row) * a.ldx + i, left, a.vec_x, v);
+  i8_open8(rx, v);
   if constexpr (kTU != kI8None) {
-    float u[8];
-    i8_load8<kTU>(a.u, static_cast<int64_t>(row) * a.ldu + i, left, a.vec_u, u);
+    I8Pair u[4];
+    i8_open8(ru, u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      if constexpr (kOp == kI8Silu) v[e] = __fdividef(v[e], 1.0f + expf(-v[e])) * u[e];
-      else v[e] += u[e];
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (kOp == kI8Silu) {
+        const float2 g = i8_both(v[e]), f = i8_both(u[e]);
+        v[e] = i8_pair(i8_silu_mul(g.x, f.x), i8_silu_mul(g.y, f.y));
+      } else {
+        v[e] = i8_add2(v[e], u[e]);
+      }
     }
   }
   if constexpr (kOp == kI8Norm) {
     if (write_h && a.h_out) i8_store8<kTX>(a.h_out, static_cast<int64_t>(row) * a.ldh + i, left, a.vec_h, v);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      s.ss = fmaf(v[e], v[e], s.ss);
-      const float t = v[e] * 0x1p-80f;
-      s.small = fmaf(t, t, s.small);
+    for (int e = 0; e < 4; ++e) {
+      s.ss = i8_fma2(v[e], v[e], s.ss);
+      const I8Pair t = i8_mul2(v[e], i8_pair(0x1p-80f, 0x1p-80f));
+      s.small = i8_fma2(t, t, s.small);
     }
     if (a.w) {
-      float w[8];
+      I8Pair w[4];
       i8_load8_of(a.w_type, a.w, i, left, a.vec_w, w);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] *= w[e];
+      for (int e = 0; e < 4; ++e) v[e] = i8_mul2(v[e], w[e]);
     }
   }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) s.big = max(s.big, __float_as_uint(v[e]) & 0x7fffffffu);
+  for (int e = 0; e < 4; ++e) {
+    const float2 f = i8_both(v[e]);
+    s.big = i8_max3(s.big, f.x, f.y);
+  }
 }
 
 // One row per CTA (kWarpRow: per warp), kPer groups of 8 values per thread in registers; kPer 0: rows
 // of any length, read once for the statistics and once more for the codes.
 template <int kOp, int kTX, int kTU, int kPer, bool kWarpRow>
-__global__ void i8_rows_kernel(const I8RowsArgs a) {
+__global__ void __launch_bounds__(kWarpRow ? 128 : 1024) i8_rows_kernel(const I8RowsArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   const int threads = kWarpRow ? 32 : blockDim.x;
@@ -266,33 +372,57 @@ __global__ void i8_rows_kernel(const I8RowsArgs a) {
   const int row = kWarpRow ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   if (kWarpRow && row >= a.rows) return;
   constexpr bool kNorm = kOp == kI8Norm;
-  I8Stat s{0u, 0.f, 0.f};
+  constexpr bool kExact = kOp != kI8Silu && kTU == kI8None;
+  const int64_t at_x = static_cast<int64_t>(row) * a.ldx, at_u = static_cast<int64_t>(row) * a.ldu;
+  I8Stat s{0.f, 0ull, 0ull};
   if constexpr (kPer > 0) {
-    float v[kPer][8];
+    // groups whose loads are all under way before the first is used (two of 64 registers would not stay in them)
+    constexpr int kBatch = kPer < 2 || (kPer == 4 && kTX == kI8F32 && kTU == kI8F32) ? 1 : 2;
+    I8Pair v[kPer][4];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int i = 8 * (t + j * threads);
-      if (i < a.n) i8_make8<kOp, kTX, kTU>(a, row, i, v[j], s, true);
+    for (int j0 = 0; j0 < kPer; j0 += kBatch) {
+      I8Raw<kTX> rx[kBatch];
+      I8Raw<kTU> ru[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = 8 * (t + (j0 + j) * threads);
+        if (i < a.n) {
+          i8_load8(a.x, at_x + i, a.n - i, a.vec_x, rx[j]);
+          if constexpr (kTU != kI8None) i8_load8(a.u, at_u + i, a.n - i, a.vec_u, ru[j]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = 8 * (t + (j0 + j) * threads);
+        if (i < a.n) i8_make8<kOp, kTX, kTU>(a, row, i, rx[j], ru[j], v[j0 + j], s, true);
+      }
     }
-    if (kWarpRow) i8_warp_reduce(s, kNorm);
-    else i8_block_reduce(s, kNorm);
-    const I8Scale sc = i8_scale_of(s, kNorm, a.n, a.eps);
+    const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), kNorm, a.n, a.eps);
     if (t == 0) a.scales[row] = sc.scale;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
       const int i = 8 * (t + j * threads);
-      if (i < a.n) i8_write8(a, row, i, a.n - i, v[j], sc);
+      if (i < a.n) i8_write8<kExact>(a, row, i, a.n - i, v[j], sc);
     }
   } else {
-    float v[8];
-    for (int i = 8 * t; i < a.n; i += 8 * threads) i8_make8<kOp, kTX, kTU>(a, row, i, v, s, false);
-    i8_block_reduce(s, kNorm);
-    const I8Scale sc = i8_scale_of(s, kNorm, a.n, a.eps);
+    I8Raw<kTX> rx;
+    I8Raw<kTU> ru;
+    I8Pair v[4];
+    auto load = [&](int i) {
+      i8_load8(a.x, at_x + i, a.n - i, a.vec_x, rx);
+      if constexpr (kTU != kI8None) i8_load8(a.u, at_u + i, a.n - i, a.vec_u, ru);
+    };
+    for (int i = 8 * t; i < a.n; i += 8 * threads) {
+      load(i);
+      i8_make8<kOp, kTX, kTU>(a, row, i, rx, ru, v, s, false);
+    }
+    const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), kNorm, a.n, a.eps);
     if (t == 0) a.scales[row] = sc.scale;
-    I8Stat none{0u, 0.f, 0.f};
+    I8Stat none{0.f, 0ull, 0ull};
     for (int i = 8 * t; i < a.n; i += 8 * threads) {  // (h_out may be h: each thread reads a place before it writes it)
-      i8_make8<kOp, kTX, kTU>(a, row, i, v, none, true);
-      i8_write8(a, row, i, a.n - i, v, sc);
+      load(i);
+      i8_make8<kOp, kTX, kTU>(a, row, i, rx, ru, v, none, true);
+      i8_write8<kExact>(a, row, i, a.n - i, v, sc);
     }
   }
 }

@@ -31,6 +31,8 @@ class Int8Rows:
     """Rows in 8 bits: ``codes`` int8 [rows, n], each row starting on 16 bytes, and ``scales`` fp32
     [rows].  ``values``: what they stand for, where the call that made them was asked for it."""
 
+    __slots__ = ("_codes", "_scales", "_held", "values", "rows", "n", "index", "c", "_ref")
+
     def __init__(self, codes: torch.Tensor, scales: torch.Tensor, values: Optional[torch.Tensor] = None):
         if codes.dim() != 2 or codes.dtype != torch.int8 or not codes.is_cuda:
             raise ValueError(f"Int8Rows: codes must be int8 [rows, n] on a CUDA device, got {codes.dtype} "
@@ -45,31 +47,52 @@ class Int8Rows:
         ld = codes.stride(0) if rows > 1 else -(-n // 16) * 16
         if (n > 1 and codes.stride(1) != 1) or ld < n or ld % 16 or (rows and codes.data_ptr() % 16):
             raise ValueError(f"Int8Rows: rows of codes must start on 16 bytes and not overlap, got strides {codes.stride()}")
-        self._set(codes, scales, values, rows, n, ld)
-
-    def _set(self, codes, scales, values, rows, n, ld):
-        self.codes, self.scales, self.values = codes, scales, values
-        self.rows, self.n, self.device = rows, n, codes.device
+        self._codes, self._scales, self._held, self.values = codes, scales, None, values
+        self.rows, self.n, self.index = rows, n, codes.get_device()
         self.c = _lib.I8Rows(rows, n, ld, codes.data_ptr(), scales.data_ptr())
         self._ref = ctypes.addressof(self.c)
 
     @classmethod
     def _new(cls, like: torch.Tensor, rows: int, n: int, values: Optional[torch.dtype]) -> "Int8Rows":
-        """Memory for rows of n values on like's device."""
+        """Memory for rows of n values on like's device: codes and then scales in one piece (a tensor costs
+        more to make than the quantization of a token)."""
         if n < 1 or n > MAX_WIDTH:
             raise ValueError(f"rows of {n} values (1 to {MAX_WIDTH})")
-        if values is not None and values not in _DTYPES:
-            raise ValueError(f"values must be float16, bfloat16 or float32, got {values}")
-        ld = -(-n // 16) * 16
-        codes = like.new_empty((rows, ld), dtype=torch.int8)
         self = cls.__new__(cls)
-        self._set(codes if ld == n else codes[:, :n], like.new_empty(rows, dtype=torch.float32),
-                  None if values is None else like.new_empty((rows, n), dtype=values), rows, n, ld)
+        if values is None:
+            self.values = None
+        elif values not in _DTYPES:
+            raise ValueError(f"values must be float16, bfloat16 or float32, got {values}")
+        elif like.shape[1] == n:  # (rows are like's everywhere)
+            self.values = torch.empty_like(like, dtype=values, memory_format=torch.contiguous_format)
+        else:
+            self.values = like.new_empty((rows, n), dtype=values)
+        ld = -(-n // 16) * 16
+        held = like.new_empty(rows * (ld // 4 + 1), dtype=torch.float32)
+        self._codes = self._scales = None
+        self._held, self.rows, self.n, self.index = held, rows, n, like.get_device()
+        at = held.data_ptr()
+        self.c = _lib.I8Rows(rows, n, ld, at, at + rows * ld)
+        self._ref = ctypes.addressof(self.c)
         return self
 
-    def _values_args(self) -> Tuple[Optional[int], int, int]:
-        v = self.values
-        return (None, 0, 0) if v is None else (v.data_ptr(), self.n, _DTYPES[v.dtype])
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            ld = self.c.ld
+            codes = self._held[:self.rows * (ld // 4)].view(torch.int8).view(self.rows, ld)
+            self._codes = codes if ld == self.n else codes[:, :self.n]
+        return self._codes
+
+    @property
+    def scales(self) -> torch.Tensor:
+        if self._scales is None:
+            self._scales = self._held.narrow(0, self.rows * (self.c.ld // 4), self.rows)
+        return self._scales
+
+    @property
+    def device(self) -> torch.device:
+        return (self._held if self._codes is None else self._codes).device
 
     def device_bytes(self) -> int:
         return int(self.rows * (self.c.ld + 4))
@@ -103,27 +126,34 @@ class Int8Weight(Int8Rows):
         return cls.quantize(L.dequantize(dl))
 
 
-def _matrix(what: str, name: str, t: torch.Tensor, rows: Optional[int] = None, n: Optional[int] = None) -> int:
-    """Leading dimension of a matrix t, checked."""
-    if t.dim() != 2 or not t.is_cuda or t.dtype not in _DTYPES or (t.shape[1] > 1 and t.numel() and t.stride(1) != 1):
+def _matrix(what: str, name: str, t: torch.Tensor, rows: Optional[int] = None, n: int = 0, index: int = 0) -> int:
+    """Leading dimension of a matrix t; with ``rows``, it is [rows, n] on device ``index``."""
+    shape, strides, at = t.shape, t.stride(), t.get_device()
+    if len(shape) != 2 or at < 0 or t.dtype not in _DTYPES or (strides[1] != 1 and shape[1] > 1 and shape[0]):
         raise ValueError(f"{what}: {name} must be float16, bfloat16 or float32 [rows, n] on a CUDA device with unit stride, got "
-                         f"{t.dtype} {tuple(t.shape)} with strides {t.stride()} on {t.device}")
-    if (rows is not None and t.shape[0] != rows) or (n is not None and t.shape[1] != n):
-        raise ValueError(f"{what}: {name} must be [{rows}, {n}], got {tuple(t.shape)}")
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+                         f"{t.dtype} {tuple(shape)} with strides {strides} on {t.device}")
+    if rows is not None:
+        if shape[0] != rows or shape[1] != n:
+            raise ValueError(f"{what}: {name} must be [{rows}, {n}], got {tuple(shape)}")
+        if at != index:
+            raise ValueError(f"{what}: {name} is on {t.device}, the others on cuda:{index}")
+    return strides[0] if shape[0] > 1 else shape[1]
 
 
-def _like(what: str, name: str, t: torch.Tensor, other: torch.Tensor):
-    if t.device != other.device:
-        raise ValueError(f"{what}: {name} is on {t.device}, the others on {other.device}")
+def _vector(what: str, name: str, t: torch.Tensor, n: int, index: int):
+    if t.dtype not in _DTYPES or t.shape != (n,) or (n > 1 and t.stride(0) != 1) or t.get_device() != index:
+        raise ValueError(f"{what}: {name} must be contiguous float16, bfloat16 or float32 [{n}] on cuda:{index}, got {t.dtype} "
+                         f"{tuple(t.shape)} on {t.device}")
 
 
 def quantize(x: torch.Tensor, values: Optional[torch.dtype] = None) -> Int8Rows:
     """The rows of x [rows, n] in 8 bits.  ``values``: also give what they stand for, in that type."""
     ld = _matrix("quantize", "x", x)
-    out = Int8Rows._new(x, x.shape[0], x.shape[1], values)
-    _call(_lib.load().opc_i8_quantize, x.device.index, x.data_ptr(), ld, _DTYPES[x.dtype], out._ref, *out._values_args(),
-          _raw_stream(x.device.index))
+    rows, n = x.shape
+    out = Int8Rows._new(x, rows, n, values)
+    index, v = out.index, out.values
+    _call(_lib.load().opc_i8_quantize, index, x.data_ptr(), ld, _DTYPES[x.dtype], out._ref,
+          None if v is None else v.data_ptr(), n, 0 if v is None else _DTYPES[values], _raw_stream(index))
     return out
 
 
@@ -131,21 +161,21 @@ def silu_mul(gate: torch.Tensor, up: Optional[torch.Tensor] = None, values: Opti
     """The rows of silu(gate) * up in 8 bits; without ``up``, gate holds both side by side, gate first."""
     ldg = _matrix("silu_mul", "gate", gate)
     rows, n = gate.shape
-    size = gate.element_size()
+    gate_ptr = gate.data_ptr()
     if up is None:
         if n % 2:
             raise ValueError(f"silu_mul: gate and up side by side need an even width, got {n}")
         n //= 2
-        up_ptr, ldu = gate.data_ptr() + n * size, ldg
+        up_ptr, ldu = gate_ptr + n * gate.element_size(), ldg
     else:
-        ldu = _matrix("silu_mul", "up", up, rows, n)
-        _like("silu_mul", "up", up, gate)
+        ldu = _matrix("silu_mul", "up", up, rows, n, gate.get_device())
         if up.dtype != gate.dtype:
             raise ValueError(f"silu_mul: gate is {gate.dtype}, up {up.dtype}")
         up_ptr = up.data_ptr()
     out = Int8Rows._new(gate, rows, n, values)
-    _call(_lib.load().opc_i8_silu_mul, gate.device.index, gate.data_ptr(), ldg, up_ptr, ldu, _DTYPES[gate.dtype], out._ref,
-          *out._values_args(), _raw_stream(gate.device.index))
+    index, v = out.index, out.values
+    _call(_lib.load().opc_i8_silu_mul, index, gate_ptr, ldg, up_ptr, ldu, _DTYPES[gate.dtype], out._ref,
+          None if v is None else v.data_ptr(), n, 0 if v is None else _DTYPES[values], _raw_stream(index))
     return out
 
 
@@ -154,34 +184,33 @@ def add_rmsnorm(h: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Optio
     """(h + y, the rows of its root-mean-square norm times ``weight`` in 8 bits).  y has h's type, or
     any beside an h of float32.  The sum goes to ``h_out`` (which may be h) or a new tensor; without y
     the first result is h itself (or h copied into ``h_out``)."""
-    rows, n = h.shape if h.dim() == 2 else (0, 0)
     ldh = _matrix("add_rmsnorm", "h", h)
-    ldy = 0
+    rows, n = h.shape
+    index, h_type = h.get_device(), _DTYPES[h.dtype]
+    y_ptr = w_ptr = o_ptr = None
+    ldy = y_type = w_type = ldo = 0
     if y is not None:
-        ldy = _matrix("add_rmsnorm", "y", y, rows, n)
-        _like("add_rmsnorm", "y", y, h)
-        if y.dtype != h.dtype and h.dtype != torch.float32:
+        ldy = _matrix("add_rmsnorm", "y", y, rows, n, index)
+        y_ptr, y_type = y.data_ptr(), _DTYPES[y.dtype]
+        if y_type != h_type and h_type != _lib.OPC_F32:
             raise ValueError(f"add_rmsnorm: y is {y.dtype} beside an h of {h.dtype}")
         if h_out is None:
             h_out = torch.empty_like(h, memory_format=torch.contiguous_format)
-    ldo = 0
-    if h_out is not None:
-        ldo = _matrix("add_rmsnorm", "h_out", h_out, rows, n)
-        _like("add_rmsnorm", "h_out", h_out, h)
+            o_ptr, ldo = h_out.data_ptr(), n
+    if h_out is not None and o_ptr is None:
+        ldo = _matrix("add_rmsnorm", "h_out", h_out, rows, n, index)
         if h_out.dtype != h.dtype:
             raise ValueError(f"add_rmsnorm: h_out is {h_out.dtype}, h {h.dtype}")
         if rows > 1 and ldo < n:
             raise ValueError(f"add_rmsnorm: the rows of h_out overlap (strides {h_out.stride()})")
+        o_ptr = h_out.data_ptr()
     if weight is not None:
-        if weight.dtype not in _DTYPES or tuple(weight.shape) != (n,) or (n > 1 and weight.stride(0) != 1):
-            raise ValueError(f"add_rmsnorm: weight must be contiguous float16, bfloat16 or float32 [{n}], got {weight.dtype} "
-                             f"{tuple(weight.shape)}")
-        _like("add_rmsnorm", "weight", weight, h)
+        _vector("add_rmsnorm", "weight", weight, n, index)
+        w_ptr, w_type = weight.data_ptr(), _DTYPES[weight.dtype]
     out = Int8Rows._new(h, rows, n, values)
-    _call(_lib.load().opc_i8_add_rmsnorm, h.device.index, h.data_ptr(), ldh, _DTYPES[h.dtype],
-          y.data_ptr() if y is not None else None, ldy, _DTYPES[y.dtype] if y is not None else 0,
-          weight.data_ptr() if weight is not None else None, _DTYPES[weight.dtype] if weight is not None else 0, float(eps),
-          h_out.data_ptr() if h_out is not None else None, ldo, out._ref, *out._values_args(), _raw_stream(h.device.index))
+    v = out.values
+    _call(_lib.load().opc_i8_add_rmsnorm, index, h.data_ptr(), ldh, h_type, y_ptr, ldy, y_type, w_ptr, w_type, eps, o_ptr, ldo,
+          out._ref, None if v is None else v.data_ptr(), n, 0 if v is None else _DTYPES[values], _raw_stream(index))
     return (h if h_out is None else h_out), out
 
 
@@ -195,27 +224,28 @@ def linear(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = None,
     """x times weight transposed, with both scales (and a bias [channels]): [rows, channels] in
     ``dtype``, or in ``out`` and its type.  ``workspace``: zeroed uint8 memory of
     ``linear_workspace_bytes`` that no other call in flight uses (one per stream by default)."""
-    dev, rows, m = x.device, x.rows, weight.rows
-    if weight.n != x.n or weight.device != dev:
-        raise ValueError(f"linear: x has rows of {x.n} on {dev}, the weight of {weight.n} on {weight.device}")
+    index, rows, m = x.index, x.rows, weight.rows
+    if weight.n != x.n or weight.index != index:
+        raise ValueError(f"linear: x has rows of {x.n} on cuda:{index}, the weight of {weight.n} on cuda:{weight.index}")
     if out is None:
         if dtype not in _DTYPES:
             raise ValueError(f"linear: results are float16, bfloat16 or float32, not {dtype}")
-        out = x.scales.new_empty((rows, m), dtype=dtype)
+        out = weight._scales.new_empty((rows, m), dtype=dtype)
         ldy = m
     else:
-        ldy = _matrix("linear", "out", out, rows, m)
-        if out.device != dev or (rows > 1 and ldy < m):
-            raise ValueError(f"linear: out must be on {dev} in rows that do not overlap, got strides {out.stride()} on {out.device}")
-    if bias is not None and (bias.dtype not in _DTYPES or tuple(bias.shape) != (m,) or (m > 1 and bias.stride(0) != 1) or bias.device != dev):
-        raise ValueError(f"linear: bias must be contiguous float16, bfloat16 or float32 [{m}] on {dev}, got {bias.dtype} "
-                         f"{tuple(bias.shape)} on {bias.device}")
-    stream = _raw_stream(dev.index)
+        ldy = _matrix("linear", "out", out, rows, m, index)
+        if rows > 1 and ldy < m:
+            raise ValueError(f"linear: the rows of out overlap (strides {out.stride()})")
+        dtype = out.dtype
+    b_ptr, b_type = None, 0
+    if bias is not None:
+        _vector("linear", "bias", bias, m, index)
+        b_ptr, b_type = bias.data_ptr(), _DTYPES[bias.dtype]
+    stream = _raw_stream(index)
     if workspace is None:
-        workspace = _workspace(dev, stream, linear_workspace_bytes(rows, m, x.n, dev.index), "i8")
+        workspace = _workspace(weight._scales.device, stream, linear_workspace_bytes(rows, m, x.n, index), "i8")
     else:
-        _check_workspace("linear", workspace, dev)
-    _call(_lib.load().opc_i8_gemm, dev.index, x._ref, weight._ref, bias.data_ptr() if bias is not None else None,
-          _DTYPES[bias.dtype] if bias is not None else 0, out.data_ptr(), ldy, _DTYPES[out.dtype], workspace.data_ptr(),
-          workspace.numel(), stream)
+        _check_workspace("linear", workspace, weight.device)
+    _call(_lib.load().opc_i8_gemm, index, x._ref, weight._ref, b_ptr, b_type, out.data_ptr(), ldy, _DTYPES[dtype],
+          workspace.data_ptr(), workspace.numel(), stream)
     return out

@@ -13,9 +13,11 @@ pytestmark = pytest.mark.gpu
 
 WIDTHS = [1, 7, 8, 9, 255, 256, 257, 600, 1000, 1024, 1025, 2047, 4096, 5003, 8192, 14336, 16384, 16385, 28672, 32768,
           32769, 131071]
-# relative errors of v, from the roundings that make it.  silu: the exponential to 2 steps of fp32 (its
-# documented bound; a step is 2 E), 1 + it and the product one rounding each, the quotient 2 steps
-E_SILU = (4 + 1 + 1 + 4) * E
+# relative errors of v, from the roundings that make it.  silu(g): the exponent g log2 e by a rounding and
+# half of one of the constant, so its power by |g| 1.5 E, the power of two by 2 steps of fp32 (a step is
+# 2 E), 1 + it by a rounding, the reciprocal by a step, two products.  Gates in the tests stay below 20
+# (or are so far out that the power is 0 or infinite)
+E_SILU = (20 * 1.5 + 4 + 1 + 2 + 2) * E
 E_SUM = E           # h + y
 E_NORM = E_SUM + E  # times the weight
 
@@ -62,7 +64,7 @@ def test_quantize(cuda_device, n, dtype):
 @pytest.mark.parametrize("n", WIDTHS)
 @pytest.mark.parametrize("dtype", [F16, BF16, F32])
 def test_silu_mul(cuda_device, n, dtype):
-    gu = values(3, 2 * n, n, dtype, cuda_device, spread=False) * 3
+    gu = (values(3, 2 * n, n, dtype, cuda_device, spread=False) * 3).clamp(-20, 20)
     g, u = f64(gu[:, :n]), f64(gu[:, n:])
     v = g / (1 + np.exp(-g)) * u
     check_rows(int8.silu_mul(gu, values=F16), v, E_SILU, 0.0)
