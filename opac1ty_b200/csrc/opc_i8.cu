@@ -68,10 +68,13 @@ cudaError_t launch(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y, int
   return launch_smem(kern, grid_x, grid_y, threads, 0, stream, args...);
 }
 
-// One warp per row up to 1024 values; beyond, one CTA per row with 16 values a thread (32 from 16384
-// values on), and rows of more than 32768 values, which no CTA's registers hold, are read twice.
+// One warp per row up to 1024 values; beyond, one CTA per row with 16 values a thread, or 8 where there
+// are few rows and a row up to 8192 values (96 x 8192 bf16 norms 3.4 -> 3.2 us, 512 x 4096 fp32 ones 6.1 ->
+// 5.8 us; but 28672 x 4096 quantized 97 -> 111 us), 32 from 16384 values on (shorter rows lose by it:
+// 4097 x 14336 gated 62 -> 83 us).  Rows of more than 32768 values, which no CTA's registers hold, are
+// read twice.
 template <int kOp, int kTX, int kTU>
-cudaError_t launch_rows(const opc::I8RowsArgs& a, void* stream) {
+cudaError_t launch_rows(const opc::I8RowsArgs& a, int sms, void* stream) {
   const int groups = (a.n + 7) / 8;
   if (groups <= 128) {
     const int per = (groups + 31) / 32;
@@ -79,18 +82,19 @@ cudaError_t launch_rows(const opc::I8RowsArgs& a, void* stream) {
              : per == 2 ? opc::i8_rows_kernel<kOp, kTX, kTU, 2, true> : opc::i8_rows_kernel<kOp, kTX, kTU, 4, true>;
     return launch(k, (a.rows + 3) / 4, 1, 128, stream, a);
   }
-  const int per = groups <= 2048 ? 2 : groups <= 4096 ? 4 : 0;
+  const int per = groups <= 1024 && a.rows <= 4 * sms ? 1 : groups <= 2048 ? 2 : groups <= 4096 ? 4 : 0;
   const int threads = per ? ((groups + per - 1) / per + 31) / 32 * 32 : 1024;
-  auto k = per == 2 ? opc::i8_rows_kernel<kOp, kTX, kTU, 2, false>
+  auto k = per == 1 ? opc::i8_rows_kernel<kOp, kTX, kTU, 1, false>
+           : per == 2 ? opc::i8_rows_kernel<kOp, kTX, kTU, 2, false>
            : per == 4 ? opc::i8_rows_kernel<kOp, kTX, kTU, 4, false> : opc::i8_rows_kernel<kOp, kTX, kTU, 0, false>;
   return launch(k, a.rows, 1, threads, stream, a);
 }
 
 template <int kOp, int kTU>
-cudaError_t launch_rows_x(int32_t x_type, const opc::I8RowsArgs& a, void* stream) {
-  if (x_type == OPC_F16) return launch_rows<kOp, opc::kI8F16, kTU == 4 ? opc::kI8F16 : kTU>(a, stream);
-  if (x_type == OPC_BF16) return launch_rows<kOp, opc::kI8BF16, kTU == 4 ? opc::kI8BF16 : kTU>(a, stream);
-  return launch_rows<kOp, opc::kI8F32, kTU == 4 ? opc::kI8F32 : kTU>(a, stream);
+cudaError_t launch_rows_x(int32_t x_type, const opc::I8RowsArgs& a, int sms, void* stream) {
+  if (x_type == OPC_F16) return launch_rows<kOp, opc::kI8F16, kTU == 4 ? opc::kI8F16 : kTU>(a, sms, stream);
+  if (x_type == OPC_BF16) return launch_rows<kOp, opc::kI8BF16, kTU == 4 ? opc::kI8BF16 : kTU>(a, sms, stream);
+  return launch_rows<kOp, opc::kI8F32, kTU == 4 ? opc::kI8F32 : kTU>(a, sms, stream);
 }
 constexpr int kSame = 4;  // launch_rows_x: the second operand has the first one's type
 
@@ -167,7 +171,6 @@ GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, int sms) {
       d.sharers = s;
     }
   }
-  if (getenv("I8_SHARE") && d.rest) { int v = atoi(getenv("I8_SHARE")); if (v) d.sharers = (int)std::min<int64_t>(std::min<int64_t>((int64_t)v * d.rest, p.pairs), stages); }
   if (!d.full) p.pairs = d.sharers;  // (no more CTAs than have work)
   if (d.sharers > d.rest) p.bytes += static_cast<size_t>(d.sharers) * 4 * 128 * d.tile_n * sizeof(int32_t);
   return p;
@@ -215,7 +218,9 @@ int opc_i8_quantize(const void* x, int64_t ldx, int32_t dtype, const opc_i8_rows
   a.x = x;
   a.ldx = ldx;
   a.vec_x = vec_ok(x, ldx, dtype);
-  return end_rows(who, launch_rows_x<opc::kI8Quant, opc::kI8None>(dtype, a, stream));
+  opc_host::Device dev;
+  if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
+  return end_rows(who, launch_rows_x<opc::kI8Quant, opc::kI8None>(dtype, a, dev.sm_count, stream));
 }
 
 int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* y, int64_t ldy, int32_t y_dtype,
@@ -246,11 +251,14 @@ int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* 
   a.ldh = ldho;
   a.vec_h = h_out && vec_ok(h_out, ldho, h_dtype);
   a.eps = eps;
+  a.inv_n = 1.0f / static_cast<float>(n);
+  opc_host::Device dev;
+  if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
   cudaError_t e;
-  if (!y) e = launch_rows_x<opc::kI8Norm, opc::kI8None>(h_dtype, a, stream);
-  else if (y_dtype == h_dtype) e = launch_rows_x<opc::kI8Norm, kSame>(h_dtype, a, stream);
-  else if (y_dtype == OPC_F16) e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8F16>(a, stream);
-  else e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8BF16>(a, stream);
+  if (!y) e = launch_rows_x<opc::kI8Norm, opc::kI8None>(h_dtype, a, dev.sm_count, stream);
+  else if (y_dtype == h_dtype) e = launch_rows_x<opc::kI8Norm, kSame>(h_dtype, a, dev.sm_count, stream);
+  else if (y_dtype == OPC_F16) e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8F16>(a, dev.sm_count, stream);
+  else e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8BF16>(a, dev.sm_count, stream);
   return end_rows(who, e);
 }
 
@@ -268,7 +276,9 @@ int opc_i8_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, 
   a.u = up;
   a.ldu = ldu;
   a.vec_u = vec_ok(up, ldu, dtype);
-  return end_rows(who, launch_rows_x<opc::kI8Silu, kSame>(dtype, a, stream));
+  opc_host::Device dev;
+  if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
+  return end_rows(who, launch_rows_x<opc::kI8Silu, kSame>(dtype, a, dev.sm_count, stream));
 }
 
 size_t opc_i8_gemm_workspace_bytes(int32_t rows, int32_t M, int32_t K, int32_t device) {

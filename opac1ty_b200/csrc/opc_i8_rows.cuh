@@ -9,7 +9,9 @@
 // squares and the largest magnitude come out of ONE reduction, and every value is read once and kept
 // in registers between the reduction and the rounding.  Bound by memory for large calls, which takes
 // few enough instructions per value that it stays so: pairs of values in packed fp32 operations, one
-// maximum of three per two values (see opc_i8.cu for how rows are dealt to threads and what it measured).
+// maximum of three per two values (device time with L2 flushed by the inputs: 8191 x 4096 fp32 + fp16 norms
+// with values 66 us, 6.6 TB/s; 4097 x 14336 fp16 gated with values 62 us, 6.6 TB/s; 28672 x 4096 fp16
+// quantized with values 97 us, 6.1 TB/s).  opc_i8.cu has how rows are dealt to threads.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -38,7 +40,7 @@ struct I8RowsArgs {
   int32_t rows, n, w_type, v_type;
   // whether groups of 8 values may be moved 16 bytes at a time (else one value at a time)
   int32_t vec_x, vec_u, vec_w, vec_h, vec_v;
-  float eps;
+  float eps, inv_n;   // norm: 1 / n
 };
 
 // Two fp32 values, one instruction for both.
@@ -245,26 +247,36 @@ __device__ __forceinline__ I8Row i8_reduce(const I8Stat& p, bool norm) {
 // What the codes are made with.  `exact`: code = round((v * c) / a) with c = 127 and a the largest
 // magnitude, or both times 2^-32 where v * 127 could leave fp32; inv = 1 / a.  Else round(v * mul).
 // `live` is false for rows of zeros and rows that hold an infinity or NaN, whose codes are 0 whatever v is.
+// Every thread forms them, so they cost as much as several values do: reciprocals to a step or two of
+// fp32 and their products instead of divisions (4097 x 14336 gated 77 -> 47 us).
 struct I8Scale {
   float scale, mul, c, a, inv;
   bool live;
 };
-__device__ __forceinline__ I8Scale i8_scale_of(const I8Row& s, bool norm, int n, float eps) {
+__device__ __forceinline__ float i8_recip(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ I8Scale i8_scale_of(const I8Row& s, const I8RowsArgs& a, bool norm) {
   I8Scale r;
   const bool bad = !(s.big < __uint_as_float(0x7f800000u));
   r.live = !bad && s.big >= kI8Least;
   const bool huge = s.big >= 0x1p97f;
   r.c = huge ? 127.0f * 0x1p-32f : 127.0f;
   r.a = huge ? s.big * 0x1p-32f : s.big;
-  r.inv = 1.0f / r.a;
-  r.mul = 127.0f / s.big;
-  r.scale = bad ? __uint_as_float(0x7fffffffu) : r.live ? s.big / 127.0f : 0.f;
-  if (norm && r.live) {
-    const float len = static_cast<float>(n);
-    // a finite row whose squares leave fp32: sqrt(mean (t 2^-80)^2) 2^80 (eps is nothing beside it)
-    const float rms = s.ss < __uint_as_float(0x7f800000u) ? sqrtf(s.ss / len + eps) : sqrtf(s.small / len) * 0x1p80f;
-    r.scale = r.scale / rms;
+  r.inv = i8_recip(r.a);
+  r.mul = r.c * r.inv;
+  const float q = s.big * (1.0f / 127.0f);
+  r.scale = fmaf(fmaf(-q, 127.0f, s.big), 1.0f / 127.0f, q);  // big / 127, the nearest fp32
+  if (norm) {
+    // a finite row whose squares leave fp32: mean (t 2^-80)^2 (eps is nothing beside it)
+    const bool far = !(s.ss < __uint_as_float(0x7f800000u));
+    float root;
+    asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(far ? s.small * a.inv_n : fmaf(s.ss, a.inv_n, a.eps)));
+    r.scale *= far ? root * 0x1p-80f : root;
   }
+  r.scale = bad ? __uint_as_float(0x7fffffffu) : r.live ? r.scale : 0.f;
   return r;
 }
 
@@ -272,14 +284,14 @@ __device__ __forceinline__ I8Scale i8_scale_of(const I8Row& s, bool norm, int n,
 // byte is the code.  Exact: the quotient is corrected once by its remainder, so it is the nearest fp32,
 // and a half that 16-bit inputs often meet is a half and goes to even (with v * (127 / a) every half of
 // a row goes the way that 127 / a was rounded); where v itself is a rounded result there are none.
-template <bool kExact>
+template <bool kLive, bool kExact>
 __device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, int left, const I8Pair (&v)[4], const I8Scale& s) {
   constexpr float kMagic = 12582912.0f;
   const I8Pair magic = i8_pair(kMagic, kMagic);
   I8Pair f[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    if (!s.live) {  // (the same for the whole row)
+    if constexpr (!kLive) {
       f[e] = magic;
     } else if constexpr (kExact) {
       const I8Pair inv = i8_pair(s.inv, s.inv), t = i8_mul2(v[e], i8_pair(s.c, s.c)), q = i8_mul2(t, inv);
@@ -314,10 +326,9 @@ __device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, i
 // silu(g) * u.  exp(-g) = 2^(-g log2 e): the rounded exponent is off by |g| 2^-24 at most, which next to
 // the row's largest value is nothing where |g| is large; 1 / (1 + it) to one step of fp32.
 __device__ __forceinline__ float i8_silu_mul(float g, float u) {
-  float e, r;
+  float e;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-  return g * r * u;
+  return g * i8_recip(1.0f + e) * u;
 }
 
 // 8 values of a row before its scale from what was loaded, their part of the statistics, and (norm) h_out.
@@ -397,12 +408,17 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024) i8_rows_kernel(const I8
         if (i < a.n) i8_make8<kOp, kTX, kTU>(a, row, i, rx[j], ru[j], v[j0 + j], s, true);
       }
     }
-    const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), kNorm, a.n, a.eps);
+    const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), a, kNorm);
     if (t == 0) a.scales[row] = sc.scale;
+    if (sc.live) {
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-      const int i = 8 * (t + j * threads);
-      if (i < a.n) i8_write8<kExact>(a, row, i, a.n - i, v[j], sc);
+      for (int j = 0; j < kPer; ++j) {
+        const int i = 8 * (t + j * threads);
+        if (i < a.n) i8_write8<true, kExact>(a, row, i, a.n - i, v[j], sc);
+      }
+    } else {
+#pragma unroll 1
+      for (int i = 8 * t; i < a.n; i += 8 * threads) i8_write8<false, kExact>(a, row, i, a.n - i, v[0], sc);
     }
   } else {
     I8Raw<kTX> rx;
@@ -416,13 +432,14 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024) i8_rows_kernel(const I8
       load(i);
       i8_make8<kOp, kTX, kTU>(a, row, i, rx, ru, v, s, false);
     }
-    const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), kNorm, a.n, a.eps);
+    const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), a, kNorm);
     if (t == 0) a.scales[row] = sc.scale;
     I8Stat none{0.f, 0ull, 0ull};
     for (int i = 8 * t; i < a.n; i += 8 * threads) {  // (h_out may be h: each thread reads a place before it writes it)
       load(i);
       i8_make8<kOp, kTX, kTU>(a, row, i, rx, ru, v, none, true);
-      i8_write8<kExact>(a, row, i, a.n - i, v, sc);
+      if (sc.live) i8_write8<true, kExact>(a, row, i, a.n - i, v, sc);
+      else i8_write8<false, kExact>(a, row, i, a.n - i, v, sc);
     }
   }
 }
