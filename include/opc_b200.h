@@ -516,12 +516,9 @@ int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* 
  * for the rows t of x (tokens) and r of w (channels), x.n == w.n; bias (bias_dtype, [w.rows]) may be
  * NULL.  Codes may be any 8-bit integers, -128 too.  The sum is exact; it is rounded to fp32, multiplied
  * by the two scales in the order given, the bias is added in fp32, and the result rounded to y_dtype.
- * Deterministic.  The workspace (opc_i8_gemm_workspace_bytes) is zero-filled once before first use
- * (opc_workspace_init), is not to be shared with other entry points, and serves any calls that are
- * ordered on one stream; calls that may overlap, replays of two graphs among them, need one each. */
-size_t opc_i8_gemm_workspace_bytes(int32_t rows, int32_t M, int32_t K, int32_t device);
+ * Deterministic; no workspace. */
 int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, int32_t bias_dtype, void* y, int64_t ldy,
-                int32_t y_dtype, void* workspace, size_t workspace_bytes, void* stream);
+                int32_t y_dtype, void* stream);
 
 /* XXH64 (seed `seed`) of a HOST buffer: the checksum that the .bf2 layout places after the last
  * layer (opacc1ty/format/header.py:26; the reference documents it but never writes it).  Files

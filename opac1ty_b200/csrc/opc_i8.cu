@@ -6,7 +6,6 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
-#include <cstdlib>
 
 #include "../../include/opc_b200.h"
 #include "opc_i8_gemm.cuh"
@@ -120,59 +119,43 @@ int start_rows(const char* who, const opc_i8_rows* out, void* values, int64_t ld
 }
 
 // ---- the product's plan
-constexpr size_t kCountBytes = 16384;  // arrival counts, at the front of the workspace: 256 cut tiles at most
-
 struct GemmPlan {
   opc::I8Deal deal;
-  int pairs;
-  size_t bytes;  // of workspace; 0: refused
+  int ctas;  // 0: too many tiles
 };
 
-GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, int sms) {
+// clusters[s]: how many clusters of s pairs run at once.  The choice is by a model of the time in clocks,
+// fitted to 5 widths and 3 splits of 14 products (in the comments: what was measured, at 1.9 GHz).
+GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, const int (&clusters)[5]) {
   GemmPlan p = {};
-  p.bytes = kCountBytes;
-  if (rows <= opc::kI8GemvRows) return p;
-  opc::I8Deal& d = p.deal;
-  p.pairs = std::min(std::max(sms / 2, 1), 256);
   const int64_t m_tiles = (static_cast<int64_t>(M) + 255) / 256;
-  // Clocks of one stage: 2 a token for the MMAs, or the loads of 16 KB + 64 bytes a token at 64 a clock.
-  auto clocks = [](int n) { return std::max(2 * n, 256 + n); };
   int64_t best = 0;
   for (int n = 256; n >= 32; n -= 32) {
-    const int64_t t = (static_cast<int64_t>(rows) + n - 1) / n * clocks(n);
-    if (!best || t < best) {
-      best = t;
-      d.tile_n = n;
+    // Narrow tiles: two blocks a stage, since the barriers of a stage outlast its small MMAs (96 tokens,
+    // 14336 -> 4096: 25.1 -> 21.5 us; 512 tokens, 4096 -> 6144 with tiles of 128: 18.5 -> 17.3; four blocks,
+    // or two in wide tiles, no better).
+    const int sub = n <= 128 ? 2 : 1;
+    const int nk = (K + opc::kI8Block * sub - 1) / (opc::kI8Block * sub);
+    const int64_t n_tiles = (static_cast<int64_t>(rows) + n - 1) / n, tiles = m_tiles * n_tiles;
+    if (tiles > INT32_MAX / 2) continue;
+    for (int split = 1; split <= 4; ++split) {
+      if (split > 1 && (tiles > clusters[split] || nk < 2 * split)) continue;
+      const int64_t rounds = (tiles + clusters[1] - 1) / clusters[1];
+      const int64_t busy = 2 * split * std::min<int64_t>(tiles, clusters[1]);  // CTAs
+      // One block: its MMAs at 2 clocks a token, its loads at 75 bytes a clock into an SM (57 when every SM
+      // loads), the weights' part of them at 3580 a clock from memory.
+      const int64_t rate = 75 - 18 * busy / (2 * clusters[1]);
+      const int64_t block = std::max<int64_t>(std::max<int64_t>(2 * n + 12, (16384 + 64 * n) / rate),
+                                              16384 * busy / (3580 * std::min<int64_t>(n_tiles, 8)));
+      // Then the results of a tile, and for a split tile the exchange of sums (1.2 us for 32 tokens, 2.4 for 256).
+      const int64_t t = rounds * ((nk + split - 1) / split) * sub * block + 19 * n / split + (split > 1 ? 2200 + 10 * n : 0);
+      if (!best || t < best) {
+        best = t;
+        p.deal = {n, static_cast<int32_t>(m_tiles), static_cast<int32_t>(n_tiles), sub, nk, split};
+        p.ctas = static_cast<int>(2 * split * (split > 1 ? tiles : std::min<int64_t>(tiles, clusters[1])));
+      }
     }
   }
-  // Few tokens: two blocks a stage, since the barriers of a stage outlast its small MMAs (24 tokens,
-  // 14336 -> 4096: 18.7 -> 17.1 us; 4 blocks no better).
-  d.sub = d.tile_n <= 64 ? 2 : 1;
-  d.nk = (K + opc::kI8Block * d.sub - 1) / (opc::kI8Block * d.sub);
-  const int64_t n_tiles = (static_cast<int64_t>(rows) + d.tile_n - 1) / d.tile_n, tiles = m_tiles * n_tiles;
-  if (tiles > INT32_MAX / 2) {
-    p.bytes = 0;
-    return p;
-  }
-  d.m_tiles = static_cast<int32_t>(m_tiles);
-  d.n_tiles = static_cast<int32_t>(n_tiles);
-  d.full = static_cast<int32_t>(tiles / p.pairs * p.pairs);
-  d.rest = static_cast<int32_t>(tiles) - d.full;
-  // The rest along K: each pair does fewer stages, and a cut tile's sums go through L2 once more for
-  // every pair that shares it (512 bytes a token for each CTA, some 40 a clock, after about 2000 to start).
-  d.sharers = d.rest;
-  const int64_t stages = static_cast<int64_t>(d.rest) * d.nk;
-  int64_t least = 0;
-  for (int s = d.rest; d.rest && s <= std::min<int64_t>(p.pairs, stages); ++s) {
-    const int share = (s + d.rest - 1) / d.rest + (s % d.rest ? 1 : 0);  // most pairs at a tile
-    const int64_t t = (stages + s - 1) / s * clocks(d.tile_n) * d.sub + (s > d.rest ? 2000 + static_cast<int64_t>(share) * d.tile_n * 13 : 0);
-    if (!least || t < least) {
-      least = t;
-      d.sharers = s;
-    }
-  }
-  if (!d.full) p.pairs = d.sharers;  // (no more CTAs than have work)
-  if (d.sharers > d.rest) p.bytes += static_cast<size_t>(d.sharers) * 4 * 128 * d.tile_n * sizeof(int32_t);
   return p;
 }
 
@@ -188,18 +171,64 @@ int map_codes(const char* who, const opc_i8_rows* m, int box, CUtensorMap* map) 
   return r == CUDA_SUCCESS ? OPC_OK : fail(OPC_ERR_CUDA, "%s: cuTensorMapEncodeTiled failed (%d)", who, static_cast<int>(r));
 }
 
-// The most dynamic shared memory for kernel `k` (number `which`), once per device.
+void gemm_config(int ctas, int split, cudaLaunchConfig_t* cfg, cudaLaunchAttribute (&attr)[2]) {
+  cfg->gridDim = dim3(ctas);
+  cfg->blockDim = dim3(opc::kI8Threads);
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 2 * split;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg->attrs = attr;
+  cfg->numAttrs = 2;
+}
+
+// Once per device and kernel (number `which`): its shared memory, and how many clusters of 1 to 4 pairs
+// run at once (0: none).
 template <typename K>
-cudaError_t allow_smem(K k, int which) {
-  static std::atomic<uint64_t> done[3];
+cudaError_t gemm_setup(K k, int which, int (*clusters)[5]) {
+  static std::atomic<uint32_t> known[64][3];  // 7 bits for each, and bit 31
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  const uint64_t bit = dev < 64 ? 1ull << dev : 0;
-  if (done[which].load(std::memory_order_acquire) & bit) return cudaSuccess;
-  e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
-  if (e == cudaSuccess) done[which].fetch_or(bit, std::memory_order_release);
-  return e;
+  uint32_t v = dev < 64 ? known[dev][which].load(std::memory_order_acquire) : 0u;
+  if (!v) {
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) return e;
+    v = 1u << 31;
+    for (int split = 1, at = 0; split <= 4; ++split, at += 7) {
+      cudaLaunchConfig_t cfg = {};
+      cudaLaunchAttribute attr[2];
+      gemm_config(2 * split, split, &cfg, attr);
+      cfg.dynamicSmemBytes = 227 * 1024;
+      int n = 0;
+      if ((e = cudaOccupancyMaxActiveClusters(&n, k, &cfg)) != cudaSuccess) return e;
+      v |= static_cast<uint32_t>(std::max(0, std::min(n, 127))) << at;
+    }
+    if (dev < 64) known[dev][which].store(v, std::memory_order_release);
+  }
+  for (int split = 1; split <= 4; ++split) (*clusters)[split] = static_cast<int>((v >> (7 * (split - 1))) & 127u);
+  (*clusters)[1] = std::max(1, (*clusters)[1]);
+  return cudaSuccess;
+}
+
+// ---- few tokens
+struct GemvKernel {
+  void (*kernel)(const int8_t*, int64_t, const int8_t*, int64_t, int32_t, opc::I8Out);
+  int threads;
+};
+// 16 warps share K, or 8 where it is short (1024 -> 32768: 10.7 -> 8.3 us); each has one step of 128 values
+// under way at a time, or two where there are few CTAs with long rows (14336 -> 4096: 13.4 -> 13.1 us,
+// 4096 -> 4096 5.7 -> 5.2; but 4096 -> 28672 20.5 -> 22.9).
+template <int kY, int kTok>
+GemvKernel gemv_kernel_t(int32_t M, int32_t K, int sms) {
+  if (K < 2048) return {opc::i8_gemv_kernel<kY, kTok, 8, 1>, 256};
+  if (K >= 4096 && (M + 15) / 16 <= 2 * sms) return {opc::i8_gemv_kernel<kY, kTok, 16, 2>, 512};
+  return {opc::i8_gemv_kernel<kY, kTok, 16, 1>, 512};
+}
+template <int kY>
+GemvKernel gemv_kernel(int32_t rows, int32_t M, int32_t K, int sms) {
+  return rows <= 8 ? gemv_kernel_t<kY, 1>(M, K, sms) : gemv_kernel_t<kY, 2>(M, K, sms);
 }
 
 int end_rows(const char* who, cudaError_t e) { return e == cudaSuccess ? OPC_OK : cuda_fail(e, who); }
@@ -281,18 +310,8 @@ int opc_i8_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, 
   return end_rows(who, launch_rows_x<opc::kI8Silu, kSame>(dtype, a, dev.sm_count, stream));
 }
 
-size_t opc_i8_gemm_workspace_bytes(int32_t rows, int32_t M, int32_t K, int32_t device) {
-  if (rows < 0 || M < 1 || K < 1 || K > kMaxWidth) return 0;
-  int sms = 0;
-  if (cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device) != cudaSuccess) {
-    cudaGetLastError();
-    return 0;
-  }
-  return plan_gemm(rows, M, K, sms).bytes;
-}
-
 int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, int32_t bias_dtype, void* y, int64_t ldy,
-                int32_t y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+                int32_t y_dtype, void* stream) {
   const char* who = "opc_i8_gemm";
   int rc = check_codes(who, "x", x);
   if (rc != OPC_OK || (rc = check_codes(who, "w", w)) != OPC_OK) return rc;
@@ -303,29 +322,31 @@ int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, in
   if (bias && (rc = check_matrix(who, "bias", bias, w->rows, bias_dtype, w->rows)) != OPC_OK) return rc;
   opc_host::Device dev;
   if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
-  const GemmPlan p = plan_gemm(x->rows, w->rows, x->n, dev.sm_count);
-  if (!p.bytes) return fail(OPC_ERR_UNSUPPORTED, "%s: %d tokens times %d channels are too many tiles for one call", who, x->rows, w->rows);
-  if (!workspace || (reinterpret_cast<uintptr_t>(workspace) & 15u) || workspace_bytes < p.bytes)
-    return fail(OPC_ERR_WORKSPACE, "%s: a 16-byte aligned workspace of %zu bytes is needed, got %zu", who, p.bytes, workspace_bytes);
-  opc::I8GemmArgs a;
-  a.o = {x->scales, w->scales, bias, y, ldy, x->rows, w->rows, bias_dtype, y_dtype};
-  if (x->rows <= opc::kI8GemvRows) {
-    auto k = y_dtype == OPC_F16 ? opc::i8_gemv_kernel<opc::kI8F16>
-             : y_dtype == OPC_BF16 ? opc::i8_gemv_kernel<opc::kI8BF16> : opc::i8_gemv_kernel<opc::kI8F32>;
-    return end_rows(who, launch(k, (w->rows + 15) / 16, 1, opc::kI8GemvWarps * 32, stream, x->codes, x->ld, w->codes, w->ld, x->n, a.o));
+  const opc::I8Out o = {x->scales, w->scales, bias, y, ldy, x->rows, w->rows, bias_dtype, y_dtype};
+  // Few tokens by mma.sync; beyond 8, which it reads twice as often, only where the weights are few (16 tokens,
+  // 4096 -> 4096: 6.7 us instead of 9.0; 4096 -> 28672: 31.7 instead of 22.6).
+  if (x->rows <= 8 || (x->rows <= 16 && static_cast<int64_t>(w->rows) * w->n <= 1 << 24)) {
+    const GemvKernel g = y_dtype == OPC_F16 ? gemv_kernel<opc::kI8F16>(x->rows, w->rows, x->n, dev.sm_count)
+                         : y_dtype == OPC_BF16 ? gemv_kernel<opc::kI8BF16>(x->rows, w->rows, x->n, dev.sm_count)
+                                               : gemv_kernel<opc::kI8F32>(x->rows, w->rows, x->n, dev.sm_count);
+    return end_rows(who, launch(g.kernel, (w->rows + 15) / 16, 1, g.threads, stream, x->codes, x->ld, w->codes, w->ld, x->n, o));
   }
-  a.d = p.deal;
-  a.count = static_cast<int32_t*>(workspace);
-  a.part = reinterpret_cast<int32_t*>(static_cast<char*>(workspace) + kCountBytes);
-  a.err = dev.error_word;
-  CUtensorMap tw, tx;
-  if ((rc = map_codes(who, w, 128, &tw)) != OPC_OK || (rc = map_codes(who, x, p.deal.tile_n / 2, &tx)) != OPC_OK) return rc;
   auto k = y_dtype == OPC_F16 ? opc::i8_gemm_kernel<opc::kI8F16>
            : y_dtype == OPC_BF16 ? opc::i8_gemm_kernel<opc::kI8BF16> : opc::i8_gemm_kernel<opc::kI8F32>;
-  const size_t smem = 1024 + static_cast<size_t>(opc::i8_stages(p.deal.tile_n, p.deal.sub)) * p.deal.sub * opc::i8_block_bytes(p.deal.tile_n) + 512;
-  const cudaError_t e = allow_smem(k, y_dtype);
-  if (e != cudaSuccess) return cuda_fail(e, "opc_i8_gemm: shared memory");
-  return end_rows(who, launch_smem(k, 2 * p.pairs, 1, opc::kI8Threads, smem, stream, tw, tx, a));
+  int clusters[5];
+  cudaError_t e = gemm_setup(k, y_dtype, &clusters);
+  if (e != cudaSuccess) return cuda_fail(e, "opc_i8_gemm: setting up");
+  const GemmPlan p = plan_gemm(x->rows, w->rows, x->n, clusters);
+  if (!p.ctas) return fail(OPC_ERR_UNSUPPORTED, "%s: %d tokens times %d channels are too many tiles for one call", who, x->rows, w->rows);
+  opc::I8GemmArgs a = {o, p.deal, dev.error_word};
+  CUtensorMap tw, tx;
+  if ((rc = map_codes(who, w, 128, &tw)) != OPC_OK || (rc = map_codes(who, x, p.deal.tile_n / 2, &tx)) != OPC_OK) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  gemm_config(p.ctas, p.deal.split, &cfg, attr);
+  cfg.dynamicSmemBytes = 1024 + static_cast<size_t>(opc::i8_stages(p.deal.tile_n, p.deal.sub)) * p.deal.sub * opc::i8_block_bytes(p.deal.tile_n) + 512;
+  cfg.stream = static_cast<cudaStream_t>(stream);
+  return end_rows(who, cudaLaunchKernelEx(&cfg, k, tw, tx, a));
 }
 
 }  // extern "C"

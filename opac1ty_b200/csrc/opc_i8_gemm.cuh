@@ -8,15 +8,14 @@
 //                 by TMA (128-byte swizzle); the hardware reads both halves, so a CTA's shared memory
 //                 takes 8 KB instead of 12 KB per 128 x 256 x 32 step -- alone, a CTA would need
 //                 96 bytes a clock from L2 and as many from shared memory.
-//                 Persistent: pairs take whole tiles in turn (a group of 8 channel tiles at a time, so
-//                 that what they read stays in L2), then share the rest out along K in equal ranges.
-//                 Tiles cut by a range are summed through the workspace by whoever comes last.
+//                 Persistent: pairs take tiles in turn, 8 channel tiles at a time, so that what they
+//                 read stays in L2.  Where there are few tiles, a cluster of 2 to 4 pairs shares one
+//                 along K and adds its sums through distributed shared memory.
 //                   warp 0     TMA
-//                   warp 1     tensor memory; in the pair's first CTA it issues the MMAs
+//                   warp 1     tensor memory; in a pair's first CTA it issues the MMAs
 //                   warps 2-9  epilogue: two warps per TMEM lane quarter, half of the columns each;
 //                              it reads one accumulator while the MMAs fill the other
-// i8_gemv_kernel  up to 8 tokens: mma.sync fragments straight from global memory; bound by the reading
-//                 of W.  16 channels per CTA, K dealt to its warps 128 bytes at a time.
+// i8_gemv_kernel  few tokens: mma.sync fragments straight from global memory; bound by the reading of W.
 #pragma once
 
 #include <cuda.h>
@@ -54,16 +53,12 @@ struct I8Deal {
   int32_t m_tiles, n_tiles;    // tiles of 256 channels, of tile_n tokens
   int32_t sub;                 // blocks of 128 values of K in a stage
   int32_t nk;                  // stages of a tile
-  int32_t full;                // tiles taken whole, in turn (a multiple of the pairs)
-  int32_t rest;                // tiles after them, cut along K into `sharers` equal ranges
-  int32_t sharers;             // rest .. pairs (== rest: none is cut); a range lies in at most 2 tiles
+  int32_t split;               // 1: a pair does whole tiles in turn; 2 .. 4: so many pairs (a cluster) do one
 };
 
 struct I8GemmArgs {
   I8Out o;
   I8Deal d;
-  int32_t* count;              // [rest][2 CTAs][epilogue warps] arrivals at cut tiles; 0 between calls
-  int32_t* part;               // [sharers][2][2 CTAs][tile_n / 4][128][4] sums of cut tiles
   int* err;
 };
 
@@ -107,6 +102,11 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
 }
 // The asynchronous operations are issued by one lane (`leader`) of a converged warp: outside a divergent
 // branch their operands can stay in uniform registers.
+__device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
 // A TMA load into this CTA's shared memory that completes on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t leader, uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
   asm volatile(
@@ -129,11 +129,11 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t leader, uint32_t tmem_d, u
       : "memory");
 }
 // Arrives at the barrier of both CTAs once the MMAs issued so far are done.
-__device__ __forceinline__ void umma_commit_pair(uint32_t leader, uint32_t bar) {
+__device__ __forceinline__ void umma_commit_pair(uint32_t leader, uint32_t bar, uint32_t first) {
   asm volatile(
       "{\n .reg .pred l;\n setp.ne.b32 l, %2, 0;\n"
       " @l tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n}\n" ::"r"(bar),
-      "h"(static_cast<uint16_t>(3)), "r"(leader)
+      "h"(static_cast<uint16_t>(3u << first)), "r"(leader)
       : "memory");
 }
 // kind::i8, A and B signed, D 32-bit integers, both K-major, 256 channels x n tokens.
@@ -141,34 +141,21 @@ __device__ __forceinline__ uint32_t i8_idesc(int n) {
   return (2u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(256 >> 4) << 24);
 }
 
-// One pair's work, item by item: a tile, and the stages of it that are the pair's.
+// One pair's work: tile after tile, and the stages of each that are the pair's.
 struct I8Walk {
   const I8Deal& d;
-  int32_t pair, pairs, next;   // next whole tile
-  int64_t u, u1;               // the pair's range of the rest, in stages
-  int32_t tile, k0, k1;
-  __device__ I8Walk(const I8Deal& deal, int32_t p, int32_t n) : d(deal), pair(p), pairs(n), next(p), tile(0), k0(0), k1(0) {
-    const int64_t all = static_cast<int64_t>(d.rest) * d.nk;
-    u = p < d.sharers ? all * p / d.sharers : 0;
-    u1 = p < d.sharers ? all * (p + 1) / d.sharers : 0;
+  int32_t next, step_, tile, k0, k1;
+  // `unit`: the pair, or with split > 1 the cluster, of `units`; `part`: the pair's place in its cluster
+  __device__ I8Walk(const I8Deal& deal, int32_t unit, int32_t units, int32_t part) : d(deal), next(unit), step_(units), tile(0) {
+    k0 = d.nk * part / d.split;
+    k1 = d.nk * (part + 1) / d.split;
   }
   __device__ bool step() {
-    if (next < d.full) {
-      tile = next;
-      next += pairs;
-      k0 = 0;
-      k1 = d.nk;
-      return true;
-    }
-    if (u >= u1) return false;
-    const int32_t j = static_cast<int32_t>(u / d.nk);
-    tile = d.full + j;
-    k0 = static_cast<int32_t>(u - static_cast<int64_t>(j) * d.nk);
-    k1 = static_cast<int32_t>(min(static_cast<int64_t>(d.nk), k0 + (u1 - u)));
-    u += k1 - k0;
+    if (next >= d.m_tiles * d.n_tiles) return false;
+    tile = next;
+    next += step_;
     return true;
   }
-  __device__ bool cut() const { return k0 > 0 || k1 < d.nk; }
   // Channel and token tile: groups of kI8Group channel tiles, channels first.
   __device__ void place(int32_t* mi, int32_t* ni) const {
     const int32_t per = kI8Group * d.n_tiles, g = tile / per, in = tile - g * per;
@@ -176,26 +163,27 @@ struct I8Walk {
     *mi = g * kI8Group + in % width;
     *ni = in / width;
   }
-  // Who shares the cut tile `tile`: the pairs first .. last.
-  __device__ int32_t owner(int64_t unit) const {
-    return static_cast<int32_t>(((unit + 1) * d.sharers - 1) / (static_cast<int64_t>(d.rest) * d.nk));
-  }
-  __device__ void sharers(int32_t* first, int32_t* last) const {
-    const int64_t a = static_cast<int64_t>(tile - d.full) * d.nk;
-    *first = owner(a);
-    *last = owner(a + d.nk - 1);
-  }
-  // Where pair p keeps its part of `tile`: of the two places, the second if its range began in the tile before.
-  __device__ int32_t slot(int32_t p) const {
-    const int64_t begin = static_cast<int64_t>(d.rest) * d.nk * p / d.sharers;
-    return 2 * p + (begin / d.nk != tile - d.full ? 1 : 0);
-  }
 };
+
+// kNum results of one channel, for tokens t, t + 1, ... of which `left` exist.
+template <int kY, int kNum>
+__device__ __forceinline__ void i8_store_column(const I8Out& o, const float (&f)[kNum], int32_t t, int32_t r, int32_t left) {
+  const int64_t at = static_cast<int64_t>(t) * o.ldy + r;
+  if (left >= kNum) {  // (without a branch per value, so that their chains overlap)
+#pragma unroll
+    for (int i = 0; i < kNum; ++i) i8_store1<kY>(o.y, at + i * o.ldy, f[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < kNum; ++i)
+      if (i < left) i8_store1<kY>(o.y, at + i * o.ldy, f[i]);
+  }
+}
 
 // tw: w [M][K], box 128 bytes x 128 channels; tx: x [rows][K], box 128 bytes x tile_n / 2 tokens; both
 // with the 128-byte swizzle, zeros beyond the edges.
+// Clusters of 2 * split CTAs.
 template <int kY>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
+__global__ void __launch_bounds__(kI8Threads, 1)
     i8_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const I8GemmArgs a) {
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -210,8 +198,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
 
   const int warp = __shfl_sync(0xffffffffu, static_cast<int>(threadIdx.x >> 5), 0);
   const int lane = threadIdx.x & 31;
-  const uint32_t rank = cluster_rank();
-  const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  const uint32_t in_cluster = cluster_rank(), first = in_cluster & ~1u, rank = in_cluster & 1u;  // `first`: the pair's first CTA
+  const int split = a.d.split;
   const int cols = kN <= 16 ? 32 : kN <= 32 ? 64 : kN <= 64 ? 128 : kN <= 128 ? 256 : 512;  // two accumulators
 
   if (threadIdx.x == 0) {
@@ -238,12 +226,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
   griddep_launch_dependents();  // every CTA that has come this far holds its tensor memory
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot_ptr);
   bool ok = true;
-  I8Walk walk(a.d, pair, pairs);
+  const int quarter = warp & 3, half = (warp - 2) >> 2;  // epilogue warps: TMEM lanes, and which half of the columns
+  const int row = 32 * quarter + lane;                   // channel of the CTA's 128 = TMEM lane
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
+  I8Walk walk(a.d, static_cast<int>(blockIdx.x) / (2 * split), static_cast<int>(gridDim.x) / (2 * split), static_cast<int>(first >> 1));
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
     const uint32_t leader = elect_leader();
-    const uint32_t full0 = map_to_rank(full_b, 0);  // the first CTA's MMA warp waits for both CTAs' loads
+    const uint32_t full0 = map_to_rank(full_b, first);  // the first CTA's MMA warp waits for both CTAs' loads
     int g = 0, st = 0;
     uint32_t par = 1;  // of the stage's use before (the first round waits for nothing)
     while (ok && walk.step()) {
@@ -304,14 +295,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
               more = 1;
             }
           }
-          umma_commit_pair(leader, empty_b + 8 * st);
+          umma_commit_pair(leader, empty_b + 8 * st, first);
           if (++st == stages) {
             st = 0;
             par ^= 1;
           }
         }
         if (!ok) break;
-        umma_commit_pair(leader, accf_b + 8 * b);
+        umma_commit_pair(leader, accf_b + 8 * b, first);
         ++tl;
       }
       // no MMA of this pair is in flight past this point
@@ -320,17 +311,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
     }
   } else {
     // ---------------------------------------------------------------- epilogue
-    const int e = warp - 2, quarter = warp & 3, half = e >> 2;
-    const int row = 32 * quarter + lane;  // channel of the CTA's 128 = TMEM lane
-    const uint32_t lanes = tmem + (static_cast<uint32_t>(32 * quarter) << 16);
-    const uint32_t acce0 = map_to_rank(acce_b, 0);
+    const uint32_t acce0 = map_to_rank(acce_b, first);
     const int c0 = half * (kN / 2), c1 = c0 + kN / 2;  // this warp's columns, 16 at a time
     int tl = 0;
     while (walk.step()) {
       int32_t mi, ni;
       walk.place(&mi, &ni);
       const int32_t r = mi * 256 + static_cast<int32_t>(rank) * 128 + row, t0 = ni * kN;
-      const bool live = r < a.o.M, cut = walk.cut();
+      const bool live = r < a.o.M;
       const int b = tl & 1;
       const uint32_t acc = lanes + static_cast<uint32_t>(b * (cols / 2));
       // before the wait: what the results take from memory (lane l has the scales of columns l, l + 32, ...)
@@ -344,71 +332,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
       const float bias = live ? i8_bias(a.o, r) : 0.f;
       if (ok) ok = __all_sync(0xffffffffu, mbar_wait_bounded(accf_b + 8 * b, (tl >> 1) & 1));
       tc_fence_after();
-      int32_t first = 0, last = 0;
-      bool finish = ok;
-      if (cut) {
-        walk.sharers(&first, &last);
-        int32_t* mine = a.part + (static_cast<int64_t>(walk.slot(pair)) * 2 + rank) * (128 * kN);
-        if (ok)
-          for (int c = c0; c < c1; c += 16) {
-            uint32_t v[16];
-            tmem_ld16(acc + c, v);
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              *reinterpret_cast<uint4*>(mine + ((c + i) / 4 * 128 + row) * 4) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
-          }
-        __syncwarp();  // the lanes' stores are ordered before lane 0's release
-        // (a warp that gave up arrives too, so that the counts are 0 for the next call)
-        int32_t* n = a.count + (static_cast<int64_t>(walk.tile - a.d.full) * 2 + rank) * kI8Epi + e;
-        int old = 0;
-        if (lane == 0) {
-          old = atom_add_acq_rel_gpu(n, 1);
-          if (old == last - first) *n = 0;
-        }
-        old = __shfl_sync(0xffffffffu, old, 0);
-        __syncwarp();
-        finish = ok && old == last - first;
-      }
-      if (finish) {
+      if (ok) {
         for (int c = c0; c < c1; c += 16) {
           uint32_t v[16];
           tmem_ld16(acc + c, v);
-          if (cut)
-            for (int p0 = first; p0 <= last; p0 += 4) {  // four pairs' loads in flight
-              uint4 q[4][4];
+          if (split > 1) {  // (every MMA of the pair has ended: the stages are free)
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int p = p0 + j;
-                const bool other = p <= last && p != pair;
-                const int32_t* from = a.part + (static_cast<int64_t>(walk.slot(other ? p : pair)) * 2 + rank) * (128 * kN);
+            for (int i = 0; i < 4; ++i)
+              sts128(base + ((c / 4 + i) * 128 + row) * 16, make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+          } else {
+            const int j = (c - c0) >> 4;
+            const float sc = __shfl_sync(0xffffffffu, j < 4 ? (j < 2 ? sx[0] : sx[1]) : (j < 6 ? sx[2] : sx[3]), (lane & 15) + 16 * (j & 1));
+            float f[16];
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                  q[j][i] = other ? ld_cg_v4(from + ((c / 4 + i) * 128 + row) * 4) : make_uint4(0, 0, 0, 0);
-              }
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  v[4 * i] += q[j][i].x;
-                  v[4 * i + 1] += q[j][i].y;
-                  v[4 * i + 2] += q[j][i].z;
-                  v[4 * i + 3] += q[j][i].w;
-                }
-            }
-          const int j = (c - c0) >> 4;
-          const float sc = __shfl_sync(0xffffffffu, j < 4 ? (j < 2 ? sx[0] : sx[1]) : (j < 6 ? sx[2] : sx[3]), (lane & 15) + 16 * (j & 1));
-          float f[16];
-#pragma unroll
-          for (int i = 0; i < 16; ++i) f[i] = i8_result(static_cast<int32_t>(v[i]), __shfl_sync(0xffffffffu, sc, i), sw, bias);
-          const int32_t left = a.o.rows - (t0 + c);
-          const int64_t at = static_cast<int64_t>(t0 + c) * a.o.ldy + r;
-          if (live && left >= 16) {  // (without a branch per value, so that their chains overlap)
-#pragma unroll
-            for (int i = 0; i < 16; ++i) i8_store1<kY>(a.o.y, at + i * a.o.ldy, f[i]);
-          } else if (live) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (i < left) i8_store1<kY>(a.o.y, at + i * a.o.ldy, f[i]);
+            for (int i = 0; i < 16; ++i) f[i] = i8_result(static_cast<int32_t>(v[i]), __shfl_sync(0xffffffffu, sc, i), sw, bias);
+            if (live) i8_store_column<kY>(a.o, f, t0 + c, r, a.o.rows - (t0 + c));
           }
         }
       }
@@ -421,7 +359,49 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
   if (!ok && lane == 0) atomicCAS(a.err, 0, kDevErrTmaTimeout);
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // neither CTA ends while the other may still signal its barriers or read its memory
+  cluster_sync();  // (split: every pair's sums lie in shared memory)
+  if (split > 1) {
+    if (warp >= 2) {
+      // The pair's share of the columns, 8 at a time for each warp, from all pairs of the cluster.
+      int32_t mi, ni;
+      walk.place(&mi, &ni);
+      const int32_t r = mi * 256 + static_cast<int32_t>(rank) * 128 + row, t0 = ni * kN;
+      const bool live = r < a.o.M;
+      const float sw = live ? a.o.sw[r] : 0.f;
+      const float bias = live ? i8_bias(a.o, r) : 0.f;
+#pragma unroll 2
+      for (int c = 8 * (static_cast<int>(first) + half); c < kN; c += 16 * split) {
+        const int32_t t = t0 + c;
+        const float sx = t + (lane & 7) < a.o.rows ? a.o.sx[t + (lane & 7)] : 0.f;
+        uint4 q[4][2];
+#pragma unroll
+        for (int p = 0; p < 4; ++p)  // (all under way before the first is used)
+          if (p < split) {
+            const uint32_t from = map_to_rank(base, 2 * p + rank) + ((c / 4) * 128 + row) * 16;
+            q[p][0] = ld_cluster_v4(from);
+            q[p][1] = ld_cluster_v4(from + 128 * 16);
+          }
+        uint32_t v[8] = {q[0][0].x, q[0][0].y, q[0][0].z, q[0][0].w, q[0][1].x, q[0][1].y, q[0][1].z, q[0][1].w};
+#pragma unroll
+        for (int p = 1; p < 4; ++p)
+          if (p < split) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              v[4 * h] += q[p][h].x;
+              v[4 * h + 1] += q[p][h].y;
+              v[4 * h + 2] += q[p][h].z;
+              v[4 * h + 3] += q[p][h].w;
+            }
+          }
+        float f[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) f[i] = i8_result(static_cast<int32_t>(v[i]), __shfl_sync(0xffffffffu, sx, i), sw, bias);
+        if (live) i8_store_column<kY>(a.o, f, t, r, a.o.rows - t);
+      }
+    }
+    __syncthreads();
+    cluster_sync();  // nobody ends while another reads its sums
+  }
   if (warp == 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
@@ -429,10 +409,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kI8Threads, 1)
 }
 
 // ------------------------------------------------------------------------------------------------
-// Up to 8 tokens
+// Few tokens
 // ------------------------------------------------------------------------------------------------
 constexpr int kI8GemvRows = 8;
-constexpr int kI8GemvWarps = 8;
 
 // m16n8k32, both signed, 32-bit sums.
 __device__ __forceinline__ void imma16832_s8(int32_t c[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -462,52 +441,58 @@ __device__ __forceinline__ uint4 i8_piece(const int8_t* row, int k, int K, bool 
 
 // A fragment's order along K is free as long as both operands have the same: lane 4g + q takes bytes
 // 32q .. 32q + 31 of every 128 of rows g and g + 8 (and of token g), which are four k32 steps.
-template <int kY>
-__global__ void __launch_bounds__(kI8GemvWarps * 32) i8_gemv_kernel(const int8_t* x, int64_t ldx, const int8_t* w,
-                                                                   int64_t ldw, int32_t K, const I8Out o) {
-  __shared__ int32_t sums[kI8GemvWarps][128];
+template <int kY, int kTok, int kWarps, int kDeep>
+__global__ void __launch_bounds__(kWarps * 32) i8_gemv_kernel(const int8_t* x, int64_t ldx, const int8_t* w, int64_t ldw, int32_t K, const I8Out o) {
+  __shared__ int32_t sums[kWarps][kTok * 128];
   griddep_wait();
   griddep_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int r0 = blockIdx.x * 16;
-  const bool lo = r0 + g < o.M, hi = r0 + g + 8 < o.M, tok = g < o.rows;
+  const bool lo = r0 + g < o.M, hi = r0 + g + 8 < o.M;
   const int8_t* wl = w + static_cast<int64_t>(r0 + g) * ldw;
   const int8_t* wh = wl + 8 * ldw;
   const int8_t* xr = x + static_cast<int64_t>(g) * ldx;
-  int32_t c[4] = {0, 0, 0, 0};
-  constexpr int kStep = 128 * kI8GemvWarps;
-  for (int k0 = 128 * warp; k0 < K; k0 += 2 * kStep) {
-    uint4 a[2][2], b[2][2], t[2][2];
+  int32_t c[kTok][4] = {};
+  constexpr int kStep = 128 * kWarps;
+  for (int k0 = 128 * warp; k0 < K; k0 += kDeep * kStep) {
+    uint4 a[kDeep][2], b[kDeep][2];  // the weights of kDeep steps are under way together; tokens come from L1
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < kDeep; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int at = k0 + j * kStep + 32 * q + 16 * h;
         a[j][h] = i8_piece<true>(wl, at, K, lo);
         b[j][h] = i8_piece<true>(wh, at, K, hi);
-        t[j][h] = i8_piece<false>(xr, at, K, tok);
       }
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int j = 0; j < kDeep; ++j)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        imma16832_s8(c, a[j][h].x, b[j][h].x, a[j][h].y, b[j][h].y, t[j][h].x, t[j][h].y);
-        imma16832_s8(c, a[j][h].z, b[j][h].z, a[j][h].w, b[j][h].w, t[j][h].z, t[j][h].w);
+#pragma unroll
+        for (int n = 0; n < kTok; ++n) {
+          const uint4 t = i8_piece<false>(xr + 8 * n * ldx, k0 + j * kStep + 32 * q + 16 * h, K, g + 8 * n < o.rows);
+          imma16832_s8(c[n], a[j][h].x, b[j][h].x, a[j][h].y, b[j][h].y, t.x, t.y);
+          imma16832_s8(c[n], a[j][h].z, b[j][h].z, a[j][h].w, b[j][h].w, t.z, t.w);
+        }
       }
   }
   // c: channel g (0, 1) and g + 8 (2, 3) of tokens 2q and 2q + 1
-  sums[warp][(2 * q) * 16 + g] = c[0];
-  sums[warp][(2 * q + 1) * 16 + g] = c[1];
-  sums[warp][(2 * q) * 16 + g + 8] = c[2];
-  sums[warp][(2 * q + 1) * 16 + g + 8] = c[3];
+#pragma unroll
+  for (int n = 0; n < kTok; ++n) {
+    int32_t* to = sums[warp] + 128 * n;
+    to[(2 * q) * 16 + g] = c[n][0];
+    to[(2 * q + 1) * 16 + g] = c[n][1];
+    to[(2 * q) * 16 + g + 8] = c[n][2];
+    to[(2 * q + 1) * 16 + g + 8] = c[n][3];
+  }
   __syncthreads();
-  const int t = threadIdx.x >> 4, r = r0 + (threadIdx.x & 15);
-  if (threadIdx.x < 128 && t < o.rows && r < o.M) {
+  for (int i = threadIdx.x; i < kTok * 128; i += kWarps * 32) {
+    const int t = i >> 4, r = r0 + (i & 15);
+    if (t >= o.rows || r >= o.M) continue;
     int32_t s = 0;
 #pragma unroll
-    for (int i = 0; i < kI8GemvWarps; ++i) s += sums[i][threadIdx.x];
-    i8_store1<kY>(o.y, static_cast<int64_t>(t) * o.ldy + r,
-                  i8_result(s, o.sx[t], o.sw[r], i8_bias(o, r)));
+    for (int j = 0; j < kWarps; ++j) s += sums[j][i];
+    i8_store1<kY>(o.y, static_cast<int64_t>(t) * o.ldy + r, i8_result(s, o.sx[t], o.sw[r], i8_bias(o, r)));
   }
 }
 

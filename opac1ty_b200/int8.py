@@ -15,14 +15,13 @@ rows with infinities or NaN give, are in ``include/opc_b200.h``.  Every computat
 from __future__ import annotations
 
 import ctypes
-import functools
 from typing import Optional, Tuple
 
 import torch
 
 from . import _lib
 from . import layer as L
-from .kv import _DTYPES, _call, _check_workspace, _raw_stream, _workspace
+from .kv import _DTYPES, _call, _raw_stream
 
 MAX_WIDTH = 131071  # longest row: no sum of products of two rows leaves 32 bits
 
@@ -214,16 +213,10 @@ def add_rmsnorm(h: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Optio
     return (h if h_out is None else h_out), out
 
 
-@functools.lru_cache(maxsize=1024)
-def linear_workspace_bytes(rows: int, channels: int, k: int, device: int) -> int:
-    return int(_lib.load().opc_i8_gemm_workspace_bytes(rows, channels, k, device))
-
-
 def linear(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
-           out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+           out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """x times weight transposed, with both scales (and a bias [channels]): [rows, channels] in
-    ``dtype``, or in ``out`` and its type.  ``workspace``: zeroed uint8 memory of
-    ``linear_workspace_bytes`` that no other call in flight uses (one per stream by default)."""
+    ``dtype``, or in ``out`` and its type."""
     index, rows, m = x.index, x.rows, weight.rows
     if weight.n != x.n or weight.index != index:
         raise ValueError(f"linear: x has rows of {x.n} on cuda:{index}, the weight of {weight.n} on cuda:{weight.index}")
@@ -241,11 +234,6 @@ def linear(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = None,
     if bias is not None:
         _vector("linear", "bias", bias, m, index)
         b_ptr, b_type = bias.data_ptr(), _DTYPES[bias.dtype]
-    stream = _raw_stream(index)
-    if workspace is None:
-        workspace = _workspace(weight._scales.device, stream, linear_workspace_bytes(rows, m, x.n, index), "i8")
-    else:
-        _check_workspace("linear", workspace, weight.device)
     _call(_lib.load().opc_i8_gemm, index, x._ref, weight._ref, b_ptr, b_type, out.data_ptr(), ldy, _DTYPES[dtype],
-          workspace.data_ptr(), workspace.numel(), stream)
+          _raw_stream(index))
     return out

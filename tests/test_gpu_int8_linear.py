@@ -108,18 +108,6 @@ def test_no_rows(cuda_device):
     assert int8.linear(none, w).shape == (0, 64)
 
 
-@pytest.mark.parametrize("rows", [1, 24, 130, 600])
-def test_one_workspace_for_calls_of_many_sizes(cuda_device, rows):
-    """Calls of other sizes before and after leave a workspace fit for the next."""
-    dev = cuda_device.index
-    sizes = [(rows, 4096, 4096), (3, 333, 999), (rows + 40, 700, 14336), (256, 256, 4096), (rows, 4096, 4096)]
-    need = max(int8.linear_workspace_bytes(r, m, k, dev) for r, m, k in sizes)
-    ws = torch.zeros(need, dtype=torch.uint8, device=cuda_device)
-    for i, (r, m, k) in enumerate(sizes * 2):
-        x, w = operands(r, m, k, cuda_device, seed=i)
-        same(int8.linear(x, w, workspace=ws), x, w)
-
-
 def test_streams_side_by_side(cuda_device):
     x, w = operands(40, 4096, 8192, cuda_device)
     want = int8.linear(x, w)
@@ -206,11 +194,6 @@ def test_refusals(cuda_device):
         int8.linear(x, w, out=torch.empty(1, 64, dtype=F16, device=cuda_device).expand(4, 64))
     with pytest.raises(ValueError, match="bias must be"):
         int8.linear(x, w, bias=torch.zeros(63, device=cuda_device))
-    with pytest.raises(ValueError, match="workspace must be"):
-        int8.linear(x, w, workspace=torch.zeros(64, device=cuda_device))
-    with pytest.raises(_lib.OpcError) as e:
-        int8.linear(x, w, workspace=torch.zeros(4, dtype=torch.uint8, device=cuda_device))
-    assert e.value.code == _lib.OPC_ERR_WORKSPACE
     with pytest.raises(ValueError, match="start on 16 bytes"):
         int8.Int8Rows(torch.zeros(4, 50, dtype=torch.int8, device=cuda_device), torch.ones(4, device=cuda_device))
     with pytest.raises(ValueError, match="start on 16 bytes"):

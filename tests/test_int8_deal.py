@@ -1,115 +1,56 @@
-"""How the 8-bit product deals its tiles to pairs of CTAs, restated on the CPU: every stage of every tile is
-done once, no two parts of cut tiles share a place, and every pair that shares a tile finds the others."""
+"""How the 8-bit product deals its work, restated on the CPU: every tile once, every stage of K once, every
+column of a shared tile by one warp pair of one CTA pair of the cluster."""
 
 import random
 
 import pytest
 
-from opac1ty_b200 import _lib
 
-COUNT_BYTES = 16384
-
-
-def clocks(n):
-    return max(2 * n, 256 + n)
-
-
-def plan(rows, m, k, sms):
-    pairs = min(max(sms // 2, 1), 256)
-    tile_n = min(range(256, 31, -32), key=lambda n: -(-rows // n) * clocks(n))
-    sub = 2 if tile_n <= 64 else 1
-    nk = -(-k // (128 * sub))
-    m_tiles, n_tiles = -(-m // 256), -(-rows // tile_n)
-    tiles = m_tiles * n_tiles
-    full = tiles // pairs * pairs
-    rest = tiles - full
-    stages, least, sharers = rest * nk, 0, rest
-    for s in range(rest, min(pairs, stages) + 1) if rest else ():
-        share = -(-s // rest) + (1 if s % rest else 0)
-        t = -(-stages // s) * clocks(tile_n) * sub + (2000 + share * tile_n * 13 if s > rest else 0)
-        if not least or t < least:
-            least, sharers = t, s
-    if not full:
-        pairs = sharers
-    size = COUNT_BYTES + (sharers * 4 * 128 * tile_n * 4 if sharers > rest else 0)
-    return dict(tile_n=tile_n, m_tiles=m_tiles, n_tiles=n_tiles, nk=nk, full=full, rest=rest, sharers=sharers, pairs=pairs, bytes=size)
-
-
-def items(d, p):
-    for t in range(p, d["full"], d["pairs"]):
-        yield t, 0, d["nk"]
-    if p < d["sharers"]:
-        every = d["rest"] * d["nk"]
-        u, u1 = every * p // d["sharers"], every * (p + 1) // d["sharers"]
-        while u < u1:
-            j = u // d["nk"]
-            k0 = u - j * d["nk"]
-            k1 = min(d["nk"], k0 + u1 - u)
-            yield d["full"] + j, k0, k1
-            u += k1 - k0
-
-
-def place(d, tile, group=8):
-    per = group * d["n_tiles"]
+def place(m_tiles, n_tiles, tile, group=8):
+    per = group * n_tiles
     g, inside = divmod(tile, per)
-    width = min(group, d["m_tiles"] - g * group)
+    width = min(group, m_tiles - g * group)
     return g * group + inside % width, inside // width
 
 
-def slot(d, tile, p):
-    begin = d["rest"] * d["nk"] * p // d["sharers"]
-    return 2 * p + (begin // d["nk"] != tile - d["full"])
+@pytest.mark.parametrize("m_tiles,n_tiles", [(1, 1), (1, 40), (8, 3), (9, 3), (16, 1), (112, 32), (501, 2), (7, 7)])
+def test_every_tile_has_its_place(m_tiles, n_tiles):
+    got = sorted(place(m_tiles, n_tiles, t) for t in range(m_tiles * n_tiles))
+    assert got == [(a, b) for a in range(m_tiles) for b in range(n_tiles)]
 
 
-def check(rows, m, k, sms):
-    d = plan(rows, m, k, sms)
-    assert d["tile_n"] % 32 == 0 and d["rest"] <= 255 and d["rest"] * 16 * 4 <= COUNT_BYTES
-    assert d["rest"] == 0 or d["rest"] <= d["sharers"] <= d["pairs"]
-    assert sorted(place(d, t) for t in range(d["full"] + d["rest"])) == \
-        [(a, b) for a in range(d["m_tiles"]) for b in range(d["n_tiles"])]
-    done, who = {}, {}
-    for p in range(d["pairs"]):
-        for tile, k0, k1 in items(d, p):
-            assert 0 <= k0 < k1 <= d["nk"]
-            done.setdefault(tile, []).append((k0, k1))
-            if k0 > 0 or k1 < d["nk"]:
-                who.setdefault(tile, []).append(p)
-    assert len(done) == d["full"] + d["rest"]
-    for parts in done.values():
-        parts.sort()
-        assert parts[0][0] == 0 and parts[-1][1] == d["nk"]
-        assert all(a[1] == b[0] for a, b in zip(parts, parts[1:]))
-    taken = set()
-    for tile, ps in who.items():
-        every = d["rest"] * d["nk"]
-        a = (tile - d["full"]) * d["nk"]
-        first, last = (((u + 1) * d["sharers"] - 1) // every for u in (a, a + d["nk"] - 1))
-        assert ps == list(range(first, last + 1)) and len(ps) > 1
-        for p in ps:
-            s = slot(d, tile, p)
-            assert s not in taken and s < 2 * d["sharers"]
-            taken.add(s)
-    if who:
-        assert d["bytes"] >= COUNT_BYTES + (max(taken) + 1) * 2 * 128 * d["tile_n"] * 4
-    return d
+def test_pairs_take_every_tile_in_turn():
+    for units in (1, 3, 74):
+        for tiles in (1, 2, 73, 74, 75, 1000):
+            taken = sorted(t for u in range(units) for t in range(u, tiles, units))
+            assert taken == list(range(tiles))
 
 
-@pytest.mark.parametrize("rows,m,k", [(9, 1, 1), (9, 256, 128), (24, 4096, 14336), (512, 6144, 4096), (333, 1011, 1000),
-                                      (8191, 28672, 4096), (17, 128256, 4096), (300, 28672, 4096), (4097, 4096, 131071)])
-def test_layers(rows, m, k):
-    check(rows, m, k, 148)
+@pytest.mark.parametrize("split", [1, 2, 3, 4])
+def test_the_pairs_of_a_cluster_share_k(split):
+    rng = random.Random(split)
+    for nk in [2 * split, 2 * split + 1, 31, 32, 112, 1024] + [rng.randrange(2 * split, 2000) for _ in range(50)]:
+        cuts = [(nk * p // split, nk * (p + 1) // split) for p in range(split)]
+        assert cuts[0][0] == 0 and cuts[-1][1] == nk
+        assert all(a < b for a, b in cuts) and all(x[1] == y[0] for x, y in zip(cuts, cuts[1:]))
 
 
-def test_random_products():
-    rng = random.Random(1)
-    for _ in range(400):
-        rows = max(9, int(2 ** rng.uniform(3, 12)))
-        check(rows, int(2 ** rng.uniform(0, 14)), int(2 ** rng.uniform(0, 17)) or 1, rng.choice([148, 148, 148, 2, 3, 132, 17]))
+@pytest.mark.parametrize("split", [2, 3, 4])
+@pytest.mark.parametrize("tile_n", range(32, 257, 32))
+def test_every_column_of_a_shared_tile_is_added_up_once(split, tile_n):
+    cols = []
+    for p in range(split):
+        for half in range(2):
+            for c in range(8 * (2 * p + half), tile_n, 16 * split):
+                cols += range(c, c + 8)
+    assert sorted(cols) == list(range(tile_n))
 
 
-def test_the_workspace_of_the_library_is_the_plans():
-    """(Without a device the library knows no number of SMs and gives 0.)"""
-    for rows, m, k in ((1, 4096, 4096), (24, 4096, 14336), (512, 6144, 4096)):
-        size = _lib.load().opc_i8_gemm_workspace_bytes(rows, m, k, 0)
-        if size:
-            assert size == (COUNT_BYTES if rows <= 8 else plan(rows, m, k, 148)["bytes"])
+@pytest.mark.parametrize("tile_n", range(32, 257, 32))
+def test_stages_and_sums_fit_in_shared_memory(tile_n):
+    budget, sub = 227 * 1024 - 1024 - 512, 2 if tile_n <= 128 else 1
+    block = 128 * 128 + tile_n * 64
+    stages = min(12, budget // (sub * block))
+    assert stages >= 3 and block % 1024 == 0  # (a tile of the 128-byte swizzle starts on 1024)
+    assert 128 * tile_n * 4 <= stages * sub * block
+    assert 8 * (2 * 12 + 2 + 2 + 1) + 4 <= 512  # barriers and the tensor memory's address

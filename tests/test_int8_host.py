@@ -21,8 +21,8 @@ def norm(out, h=P, ldh=48, ht=_lib.OPC_F32, y=P, ldy=48, yt=_lib.OPC_F16, w=P, w
     return _lib.load().opc_i8_add_rmsnorm(h, ldh, ht, y, ldy, yt, w, wt, eps, ho, ldho, ctypes.byref(out), None, 0, 0, None)
 
 
-def gemm(x, w, bias=None, bt=0, y=P, ldy=64, yt=_lib.OPC_F16, ws=P, ws_bytes=1 << 30):
-    return _lib.load().opc_i8_gemm(ctypes.byref(x), ctypes.byref(w), bias, bt, y, ldy, yt, ws, ws_bytes, None)
+def gemm(x, w, bias=None, bt=0, y=P, ldy=64, yt=_lib.OPC_F16):
+    return _lib.load().opc_i8_gemm(ctypes.byref(x), ctypes.byref(w), bias, bt, y, ldy, yt, None)
 
 
 @pytest.mark.parametrize("kw", [dict(rows=-1), dict(n=0), dict(n=131072), dict(ld=47), dict(ld=32), dict(ld=56),
@@ -72,8 +72,3 @@ def test_gemm_refuses_unlike_widths_and_no_channels():
 def test_no_rows_are_nothing_to_do():
     none = rows(rows=0, codes=None, scales=None)
     assert quantize(none, x=None) == norm(none, h=None) == gemm(none, rows(rows=64), y=None) == _lib.OPC_OK
-
-
-@pytest.mark.parametrize("rows_,m,k", [(-1, 4, 4), (1, 0, 4), (1, 4, 0), (1, 4, 131072)])
-def test_workspace_of_a_refused_request(rows_, m, k):
-    assert _lib.load().opc_i8_gemm_workspace_bytes(rows_, m, k, 0) == 0
