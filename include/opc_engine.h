@@ -103,6 +103,17 @@ BFEngine* bf_engine_create_ex(const char* path, int32_t device, uint32_t max_con
  * instead of 4 * head_dim -- 3.8 times less memory and attention traffic at head_dim 128.  Every
  * call below works alike.  Fails for a head_dim that opc_kv_plan refuses. */
 BFEngine* bf_engine_create_kv4(const char* path, int32_t device, uint32_t max_context);
+/* Same, with any of the options below:
+ *   BF_ENGINE_KV4            the KV cache in 4 bits, as above
+ *   BF_ENGINE_INT8_PROMPTS   the blocks' weights are also laid out in 8 bits (one byte a weight more of
+ *                            device memory; opc_i8_quantize of the dequantized rows), and prompt chunks
+ *                            of more than 64 tokens take their projections from products in 8-bit
+ *                            integers (opc_i8_add_rmsnorm, opc_i8_silu_mul, opc_i8_quantize, opc_i8_gemm),
+ *                            with one scale per token and per output channel.  Shorter chunks, decode
+ *                            steps, the lm_head and layers with element-wise outliers are computed as
+ *                            without it. */
+enum { BF_ENGINE_KV4 = 1, BF_ENGINE_INT8_PROMPTS = 2 };
+BFEngine* bf_engine_create_with(const char* path, int32_t device, uint32_t max_context, uint32_t options);
 void bf_engine_destroy(BFEngine* engine);
 const BFModelConfig* bf_engine_get_config(const BFEngine* engine);
 /* Message of the engine's last error, NULL if none (opacc1ty.h:90-93). */

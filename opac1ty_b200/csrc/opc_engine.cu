@@ -3,7 +3,7 @@
 // and implements them as stubs (runtime/src/inference.c:183-245, bf2_format.c:131-314); this file
 // loads a .bf2 model onto the GPU and runs it.  Projections go through the library's public C ABI
 // (opc_repack_layer, opc_gemv, opc_dequant), and so do the 4-bit cache (opc_kv_append,
-// opc_kv_attention) and the scores (opc_token_logprobs); the small per-token operations (RMSNorm, and
+// opc_kv_attention), prompts in 8 bits (opc_i8_*) and the scores (opc_token_logprobs); the small per-token operations (RMSNorm, and
 // for the fp16 cache rotary embedding and attention, SiLU gating, residual adds) are the kernels below.
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
@@ -23,6 +23,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <initializer_list>
 #include <map>
 #include <numeric>
 #include <random>
@@ -481,6 +482,7 @@ struct DevLayer {
   int32_t *row_ptr = nullptr, *cols = nullptr;
   float* delta = nullptr;
   __half* values = nullptr;
+  opc_i8_rows w8{};  // the same weights in 8 bits, for prompt chunks (codes NULL: none)
 };
 
 struct Block {
@@ -583,6 +585,10 @@ struct BFEngine {
   opc_rope rope{};
   void* kv_ws = nullptr;
   size_t kv_ws_bytes = 0;
+  // prompt chunks in 8 bits: the tokens' codes and scales on the way into one projection
+  bool int8_prompts = false;
+  int8_t* x8 = nullptr;
+  float* x8_scales = nullptr;
   // scoring (allocated by the first bf_engine_score)
   __half* score_logits = nullptr;
   int32_t *score_targets = nullptr, *score_ids = nullptr;
@@ -829,6 +835,22 @@ int load_sparse_part(BFEngine* e, const MappedFile& f, const FileLayer& l, DevLa
     ENG_CUDA(e, cudaMemcpy(d->delta, delta.data(), sizeof(float) * nnz, cudaMemcpyHostToDevice));
     ENG_CUDA(e, cudaMemcpy(d->values, vout.data(), 2 * nnz, cudaMemcpyHostToDevice));
   }
+  return 0;
+}
+
+// The weights of a layer in 8 bits, through an fp16 matrix of them in `full` (room for it given).  A layer
+// with single exact outliers keeps them: it stays on the fp16 products.
+int load_int8(BFEngine* e, DevLayer* d, void* full) {
+  if (!d->present || d->nnz) return 0;
+  const int32_t M = d->L.plan.M, K = d->L.plan.K;
+  void *codes = nullptr, *scales = nullptr;
+  opc_i8_rows w = {M, K, (static_cast<int64_t>(K) + 15) / 16 * 16, nullptr, nullptr};
+  if (dalloc(e, &codes, static_cast<size_t>(M) * w.ld) || dalloc(e, &scales, static_cast<size_t>(M) * sizeof(float))) return -1;
+  w.codes = static_cast<int8_t*>(codes);
+  w.scales = static_cast<float*>(scales);
+  ENG_OPC(e, opc_dequant(&d->L, full, K, e->stream));
+  ENG_OPC(e, opc_i8_quantize(full, K, OPC_F16, &w, nullptr, 0, 0, e->stream));
+  d->w8 = w;
   return 0;
 }
 
@@ -1079,6 +1101,28 @@ int load_model(BFEngine* e, const char* path, uint32_t max_context) {
     ENG_OPC(e, opc_workspace_init(e->kv_ws, e->kv_ws_bytes, e->stream));
   }
 
+  if (e->int8_prompts) {
+    if (!(e->eps >= 1e-12f)) return fail(e, "rms_norm_eps %g is too small for prompts in 8 bits (1e-12 or more)", static_cast<double>(e->eps));
+    size_t most = 0;
+    for (auto& B : e->blocks)
+      for (const DevLayer* d : {&B.q, &B.k, &B.v, &B.o, &B.gate, &B.up, &B.down, &B.qkv, &B.gu})
+        if (d->present && !d->nnz) most = std::max(most, static_cast<size_t>(d->L.plan.M) * d->L.plan.K * 2);
+    void* full = nullptr;
+    if (most) ENG_CUDA(e, cudaMalloc(&full, most));
+    int rc = 0;
+    for (auto& B : e->blocks)
+      for (DevLayer* d : {&B.q, &B.k, &B.v, &B.o, &B.gate, &B.up, &B.down, &B.qkv, &B.gu})
+        if (!rc) rc = load_int8(e, d, full);
+    if (cudaStreamSynchronize(e->stream) != cudaSuccess && !rc) rc = fail(e, "laying out the 8-bit weights: %s", cudaGetErrorString(cudaGetLastError()));
+    cudaFree(full);
+    if (rc) return rc;
+    void *codes = nullptr, *scales = nullptr;
+    const size_t width = (static_cast<size_t>(std::max(std::max(e->hidden, qd), e->inter)) + 15) / 16 * 16;
+    if (dalloc(e, &codes, kChunk * width) || dalloc(e, &scales, kChunk * sizeof(float))) return -1;
+    e->x8 = static_cast<int8_t*>(codes);
+    e->x8_scales = static_cast<float*>(scales);
+  }
+
   // one workspace for every projection and chunk size (calls are ordered on the engine's stream)
   std::vector<const DevLayer*> all;
   for (auto& B : e->blocks)
@@ -1135,6 +1179,33 @@ int enqueue_chunk(BFEngine* e, int n, const Want& want, uint32_t* n_launches) {
     }
     return 0;
   };
+  // Chunks that would run opc_gemm take 8-bit products instead where the engine has them.  Their steps,
+  // each for all n tokens: rows into 8 bits (into x8; and, for a layer that has no 8-bit weights, what
+  // they stand for in fp16), and the product of x8.
+  const bool int8 = e->int8_prompts && n > kGemvMaxBatch;
+  const auto rows8 = [&](int width) {
+    return opc_i8_rows{n, width, (static_cast<int64_t>(width) + 15) / 16 * 16, e->x8, e->x8_scales};
+  };
+  const auto in8 = [](std::initializer_list<const DevLayer*> ds) {
+    for (const DevLayer* d : ds)
+      if (d->present && !d->w8.codes) return false;
+    return true;
+  };
+  const auto norm8 = [&](const __half* y, const __half* w, bool only8) -> int {
+    const opc_i8_rows x = rows8(e->hidden);
+    ++launches;
+    ENG_OPC(e, opc_i8_add_rmsnorm(e->h, e->hidden, OPC_F32, y, e->ld_y, OPC_F16, w, OPC_F16, e->eps, y ? e->h : nullptr, e->hidden, &x,
+                                  only8 ? nullptr : e->xn, e->ld_x, OPC_F16, s));
+    return 0;
+  };
+  // y = x times the layer, x in fp16 or (int8, where the layer has such weights) as it lies in x8
+  const auto project = [&](const DevLayer& d, const __half* x, int ldx, __half* y, int ldy) -> int {
+    if (!int8 || !d.w8.codes) return gemv(d, x, ldx, y, ldy, n);
+    ++launches;
+    const opc_i8_rows x8 = rows8(d.w8.n);
+    ENG_OPC(e, opc_i8_gemm(&x8, &d.w8, nullptr, 0, y, ldy, OPC_F16, s));
+    return 0;
+  };
   ENG_CUDA(e, cudaMemcpyAsync(e->d_tokpos, e->h_tokpos, kTokWords * sizeof(int32_t), cudaMemcpyHostToDevice, s));
   embed_kernel<<<n, 256, 0, s>>>(e->embed_table, e->hidden, e->d_tokpos, e->h);
   ++launches;
@@ -1145,17 +1216,22 @@ int enqueue_chunk(BFEngine* e, int n, const Want& want, uint32_t* n_launches) {
     const Block& B = e->blocks[l];
     const size_t layer_at = static_cast<size_t>(l) * e->kv_heads * e->ctx * e->hd;  // (of the fp16 cache)
     __half *kc = e->kv4 ? nullptr : e->kcache + layer_at, *vc = e->kv4 ? nullptr : e->vcache + layer_at;
-    ENG_CUDA(e, launch_norm(s, n, e->h, e->hidden, res, e->ld_y, 0, B.ln_in, e->eps, e->xn, e->ld_x));
+    if (int8) {
+      if (norm8(res, B.ln_in, in8({&B.qkv, &B.q, &B.k, &B.v}))) return -1;
+    } else {
+      ENG_CUDA(e, launch_norm(s, n, e->h, e->hidden, res, e->ld_y, 0, B.ln_in, e->eps, e->xn, e->ld_x));
+      ++launches;
+    }
     __half *qb = e->q, *kb = e->k, *vb = e->v;
     int ldq = e->ld_q, ldkv = e->ld_kv;
     if (B.qkv.present) {  // one GEMV for q|k|v
-      if (gemv(B.qkv, e->xn, e->ld_x, e->qkv, e->ld_qkv, n)) return -1;
+      if (project(B.qkv, e->xn, e->ld_x, e->qkv, e->ld_qkv)) return -1;
       qb = e->qkv;
       kb = qb + qd;
       vb = kb + e->kv_heads * e->hd;
       ldq = ldkv = e->ld_qkv;
-    } else if (gemv(B.q, e->xn, e->ld_x, e->q, e->ld_q, n) || gemv(B.k, e->xn, e->ld_x, e->k, e->ld_kv, n) ||
-               gemv(B.v, e->xn, e->ld_x, e->v, e->ld_kv, n)) {
+    } else if (project(B.q, e->xn, e->ld_x, e->q, e->ld_q) || project(B.k, e->xn, e->ld_x, e->k, e->ld_kv) ||
+               project(B.v, e->xn, e->ld_x, e->v, e->ld_kv)) {
       return -1;
     }
     if (e->kv4) {
@@ -1171,20 +1247,37 @@ int enqueue_chunk(BFEngine* e, int n, const Want& want, uint32_t* n_launches) {
                              e->heads, e->kv_heads, e->hd, static_cast<int>(e->ctx), pos0, e->att, e->ld_q,
                              e->att_part, e->att_count));
     }
-    if (gemv(B.o, e->att, e->ld_q, e->y, e->ld_y, n)) return -1;
-    ENG_CUDA(e, launch_norm(s, n, e->h, e->hidden, e->y, e->ld_y, 0, B.ln_post, e->eps, e->xn, e->ld_x));
-    if (B.gu.present) {  // one GEMV for gate|up
-      if (gemv(B.gu, e->xn, e->ld_x, e->gu, e->ld_gu, n)) return -1;
-      ENG_CUDA(e, launch_pdl(silu_mul_kernel, dim3(silu_grid), dim3(256), s, e->gu, e->gu + e->inter, e->ld_gu,
-                             e->inter, n, e->a, e->ld_i));
-    } else {
-      if (gemv(B.gate, e->xn, e->ld_x, e->g, e->ld_i, n) || gemv(B.up, e->xn, e->ld_x, e->u, e->ld_i, n)) return -1;
-      ENG_CUDA(e, launch_pdl(silu_mul_kernel, dim3(silu_grid), dim3(256), s, e->g, e->u, e->ld_i, e->inter, n, e->a,
-                             e->ld_i));
+    if (int8 && B.o.w8.codes) {
+      const opc_i8_rows x = rows8(qd);
+      ENG_OPC(e, opc_i8_quantize(e->att, e->ld_q, OPC_F16, &x, nullptr, 0, 0, s));
+      ++launches;
     }
-    if (gemv(B.down, e->a, e->ld_i, e->y, e->ld_y, n)) return -1;
+    if (project(B.o, e->att, e->ld_q, e->y, e->ld_y)) return -1;
+    if (int8) {
+      if (norm8(e->y, B.ln_post, in8({&B.gu, &B.gate, &B.up}))) return -1;
+    } else {
+      ENG_CUDA(e, launch_norm(s, n, e->h, e->hidden, e->y, e->ld_y, 0, B.ln_post, e->eps, e->xn, e->ld_x));
+      ++launches;
+    }
+    const __half *gate = e->gu, *up = e->gu + e->inter;
+    int ldg = e->ld_gu;
+    if (B.gu.present) {  // one GEMV for gate|up
+      if (project(B.gu, e->xn, e->ld_x, e->gu, e->ld_gu)) return -1;
+    } else {
+      if (project(B.gate, e->xn, e->ld_x, e->g, e->ld_i) || project(B.up, e->xn, e->ld_x, e->u, e->ld_i)) return -1;
+      gate = e->g;
+      up = e->u;
+      ldg = e->ld_i;
+    }
+    if (int8 && B.down.w8.codes) {
+      const opc_i8_rows x = rows8(e->inter);
+      ENG_OPC(e, opc_i8_silu_mul(gate, ldg, up, ldg, OPC_F16, &x, nullptr, 0, 0, s));
+    } else {
+      ENG_CUDA(e, launch_pdl(silu_mul_kernel, dim3(silu_grid), dim3(256), s, gate, up, ldg, e->inter, n, e->a, e->ld_i));
+    }
+    if (project(B.down, e->a, e->ld_i, e->y, e->ld_y)) return -1;
     res = e->y;
-    launches += 5;  // two RMSNorms (each with the residual add before it), rotary + cache append, attention, SiLU
+    launches += 3;  // rotary + cache append, attention, SiLU
   }
 
   if (want.score) {  // the final norm of every scored token, then logits and scores kScoreRows at a time
@@ -1384,13 +1477,16 @@ int32_t sample_token(const std::vector<float>& logits_in, const BFSamplingParams
 // ------------------------------------------------------------------------------------------------
 extern "C" {
 
-static BFEngine* create_engine(const char* path, int32_t device, uint32_t max_context, bool kv4) {
+BFEngine* bf_engine_create_with(const char* path, int32_t device, uint32_t max_context, uint32_t options) {
   if (!path) return nullptr;
   BFEngine* e = new (std::nothrow) BFEngine();
   if (!e) return nullptr;
   e->device = device;
-  e->kv4 = kv4;
-  if (load_model(e, path, max_context) != 0) {
+  e->kv4 = (options & BF_ENGINE_KV4) != 0;
+  e->int8_prompts = (options & BF_ENGINE_INT8_PROMPTS) != 0;
+  const bool known = (options & ~static_cast<uint32_t>(BF_ENGINE_KV4 | BF_ENGINE_INT8_PROMPTS)) == 0;
+  if (!known) fail(e, "unknown engine options 0x%x", options);
+  if (!known || load_model(e, path, max_context) != 0) {
     // keep the message; release what was allocated (the handle stays, as in the reference)
     const std::string msg = e->error;
     for (void* p : e->allocs) cudaFree(p);
@@ -1409,10 +1505,10 @@ static BFEngine* create_engine(const char* path, int32_t device, uint32_t max_co
 }
 
 BFEngine* bf_engine_create_ex(const char* path, int32_t device, uint32_t max_context) {
-  return create_engine(path, device, max_context, false);
+  return bf_engine_create_with(path, device, max_context, 0);
 }
 BFEngine* bf_engine_create_kv4(const char* path, int32_t device, uint32_t max_context) {
-  return create_engine(path, device, max_context, true);
+  return bf_engine_create_with(path, device, max_context, BF_ENGINE_KV4);
 }
 
 BFEngine* bf_engine_create(const char* path) { return bf_engine_create_ex(path, 0, 0); }

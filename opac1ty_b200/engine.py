@@ -53,6 +53,9 @@ class Stats(ctypes.Structure):
     ]
 
 
+BF_ENGINE_KV4 = 1
+BF_ENGINE_INT8_PROMPTS = 2
+
 _P = ctypes.c_void_p
 _I32P = ctypes.POINTER(ctypes.c_int32)
 _F32P = ctypes.POINTER(ctypes.c_float)
@@ -62,6 +65,7 @@ PROTOTYPES = {
     "bf_engine_create": (_P, [ctypes.c_char_p]),
     "bf_engine_create_ex": (_P, [ctypes.c_char_p, ctypes.c_int32, ctypes.c_uint32]),
     "bf_engine_create_kv4": (_P, [ctypes.c_char_p, ctypes.c_int32, ctypes.c_uint32]),
+    "bf_engine_create_with": (_P, [ctypes.c_char_p, ctypes.c_int32, ctypes.c_uint32, ctypes.c_uint32]),
     "bf_engine_destroy": (None, [_P]),
     "bf_engine_get_config": (ctypes.POINTER(ModelConfig), [_P]),
     "bf_engine_get_error": (ctypes.c_char_p, [_P]),
@@ -126,15 +130,18 @@ class Score(NamedTuple):
 
 
 class Engine:
-    """One loaded .bf2 model on one GPU (``bf_engine_create_ex``; ``kv_bits`` 4: ``bf_engine_create_kv4``)."""
+    """One loaded .bf2 model on one GPU (``bf_engine_create_with``).  ``kv_bits`` 4: the KV cache in 4
+    bits; ``prompt_bits`` 8: long prompt chunks take products in 8-bit integers."""
 
-    def __init__(self, path: str, device: int = 0, max_context: int = 0, kv_bits: int = 16):
+    def __init__(self, path: str, device: int = 0, max_context: int = 0, kv_bits: int = 16, prompt_bits: int = 16):
         self._h = None
         if kv_bits not in (4, 16):
             raise ValueError(f"Engine: kv_bits must be 16 or 4, got {kv_bits}")
+        if prompt_bits not in (8, 16):
+            raise ValueError(f"Engine: prompt_bits must be 16 or 8, got {prompt_bits}")
         self._L = lib()
-        create = self._L.bf_engine_create_kv4 if kv_bits == 4 else self._L.bf_engine_create_ex
-        self._h = create(str(path).encode(), int(device), int(max_context))
+        options = (BF_ENGINE_KV4 if kv_bits == 4 else 0) | (BF_ENGINE_INT8_PROMPTS if prompt_bits == 8 else 0)
+        self._h = self._L.bf_engine_create_with(str(path).encode(), int(device), int(max_context), options)
         if not self._h:
             raise EngineError("bf_engine_create returned NULL")
         err = self._L.bf_engine_get_error(self._h)

@@ -1,0 +1,203 @@
+"""Prompts in 8-bit products (BF_ENGINE_INT8_PROMPTS) on the GPU, against a float64 forward pass that brings
+weights and tokens into 8 bits by their definition and rounds nothing else.
+
+The engine's own tokens carry fp16 roundings before they are brought into 8 bits, so a share of the codes
+lands on the other side of a rounding boundary.  How much that moves the logits was found in the float64
+pass alone, by disturbing what is brought into 8 bits by 2^-11 of itself (three seeds, Frobenius norm of the
+differences against that of the logits): SEEN below.  The tolerance is three times that, because the
+engine rounds a dozen intermediate results and not one.  The pass without 8 bits is 0.012 (plain), 0.025
+(wide) and 0.024 (mixed) from the one with them; what the engine gives has to be nearer to the latter."""
+
+import json
+
+import numpy as np
+import pytest
+from click.testing import CliRunner
+
+import engine_model
+from engine_model import build, forward64
+from opac1ty_b200 import synthetic
+from opac1ty_b200.engine import Engine, EngineError, lib
+from opac1ty_b200.format import BF2Writer
+
+pytestmark = pytest.mark.gpu
+SEEN = {"plain": 0.0062, "wide": 0.0081, "mixed": 0.0094}
+WIDE = dict(hidden=512, heads=4, kv_heads=1, inter=1376, vocab=500, seed=3)
+MODELS = {"plain": dict(), "wide": WIDE, "mixed": WIDE}
+# "mixed": these layers have element-wise outliers and stay on the fp16 products (the ones after a norm take
+# its 8-bit tokens' values, the others the tokens as they are)
+SPARSE = ("model.layers.0.self_attn.q_proj.weight", "model.layers.0.mlp.up_proj.weight", "model.layers.0.mlp.down_proj.weight",
+          "model.layers.1.self_attn.o_proj.weight")
+CHUNK, LEAST = 512, 65  # tokens of a prompt chunk; the shortest one in 8 bits
+
+
+def q8(x):
+    a = np.abs(x).max(-1, keepdims=True)
+    with np.errstate(all="ignore"):
+        return np.where(a > 0, np.rint(x * (127 / a)) * (a / 127), 0.0)
+
+
+def in_8_bits(n):
+    """Which of n prompt tokens are in chunks long enough."""
+    at = np.arange(n)
+    return np.minimum(n - at // CHUNK * CHUNK, CHUNK) >= LEAST
+
+
+def make(path, name):
+    m = build(path, **MODELS[name])
+    if name == "mixed":
+        for i, layer in enumerate(SPARSE):
+            M, K = m["layers"][layer]["shape"]
+            m["layers"][layer] = engine_model._scaled(synthetic.random_layer_sparse(M, K, 0.01, 900 + i, svs=1, duplicates=2), 2.0)
+        cfg = {"architecture": "llama", "hidden_size": m["hidden"], "num_hidden_layers": m["n_layers"], "vocab_size": m["vocab"],
+               "intermediate_size": MODELS[name]["inter"], "rope_theta": m["theta"], "num_attention_heads": m["heads"],
+               "num_key_value_heads": m["kv_heads"]}
+        BF2Writer(str(path)).write(m["layers"], cfg, {"bits": 2, "sub_vector_size": 1}, progress=False)
+    m["path"] = path
+    return m
+
+
+def forward64_int8(m, tokens, disturb=0.0, seed=0):
+    rng = np.random.default_rng(seed)
+    L = m["layers"]
+    W = {k: engine_model.dequantize_np(v).astype(np.float64) for k, v in L.items() if v["type"] in ("quantized", "sparse_outlier")}
+    vec = {k: np.asarray(v["data"], dtype=np.float64).reshape(-1) for k, v in L.items() if v["type"] == "fp16_passthrough"}
+    hd, H, KV, eps, theta = m["hd"], m["heads"], m["kv_heads"], m["eps"], m["theta"]
+    T = len(tokens)
+    pos, some = np.arange(T, dtype=np.float64), in_8_bits(T)[:, None]
+
+    def mul(x, name):
+        w = W[name]
+        x = x * (1 + disturb * rng.uniform(-1, 1, x.shape))
+        if L[name]["type"] == "sparse_outlier":
+            after_norm = not name.endswith(("o_proj.weight", "down_proj.weight"))
+            return (np.where(some, q8(x), x) if after_norm else x) @ w.T
+        return np.where(some, q8(x) @ q8(w).T, x @ w.T)
+
+    h = W["model.embed_tokens.weight"][np.asarray(tokens)].copy()
+    for i in range(m["n_layers"]):
+        p = f"model.layers.{i}."
+        xn = engine_model._rms(h, vec.get(p + "input_layernorm.weight"), eps)
+        q = engine_model._rope(mul(xn, p + "self_attn.q_proj.weight"), pos, hd, theta).reshape(T, H, hd)
+        k = engine_model._rope(mul(xn, p + "self_attn.k_proj.weight"), pos, hd, theta).reshape(T, KV, hd)
+        v = mul(xn, p + "self_attn.v_proj.weight").reshape(T, KV, hd)
+        att = np.zeros((T, H, hd))
+        for hh in range(H):
+            kh = hh // (H // KV)
+            sc = q[:, hh] @ k[:, kh].T / np.sqrt(hd)
+            sc = np.where(np.tril(np.ones((T, T), dtype=bool)), sc, -np.inf)
+            sc = np.exp(sc - sc.max(axis=1, keepdims=True))
+            att[:, hh] = (sc / sc.sum(axis=1, keepdims=True)) @ v[:, kh]
+        h = h + mul(att.reshape(T, H * hd), p + "self_attn.o_proj.weight")
+        xn = engine_model._rms(h, vec.get(p + "post_attention_layernorm.weight"), eps)
+        g, u = mul(xn, p + "mlp.gate_proj.weight"), mul(xn, p + "mlp.up_proj.weight")
+        h = h + mul(g / (1.0 + np.exp(-g)) * u, p + "mlp.down_proj.weight")
+    return engine_model._rms(h, vec.get("model.norm.weight"), eps) @ W["lm_head.weight"].T
+
+
+def _tokens(n, vocab, seed=1):
+    return np.random.default_rng(seed).integers(1, vocab, size=n).tolist()
+
+
+def _off(a, b):
+    return np.linalg.norm(a - b) / np.linalg.norm(b)
+
+
+@pytest.fixture(scope="module")
+def models(tmp_path_factory, cuda_device):
+    d = tmp_path_factory.mktemp("int8")
+    return {name: make(d / f"{name}.bf2", name) for name in MODELS}
+
+
+@pytest.mark.parametrize("name", list(MODELS))
+def test_prompts_match_float64(models, name):
+    """The last logits of prompts of one chunk, of two (the second long or short enough for fp16), and of tokens after them."""
+    m = models[name]
+    got, want, plain = [], [], []
+    with Engine(m["path"], prompt_bits=8) as eng:
+        for n, seed in ((LEAST, 1), (300, 2), (CHUNK, 3), (CHUNK + 8, 4), (600, 5)):
+            toks = _tokens(n, m["vocab"], seed)
+            ref, ref16 = forward64_int8(m, toks), forward64(m, toks)
+            got.append(eng.forward(toks).astype(np.float64))
+            want.append(ref[-1])
+            plain.append(ref16[-1])
+            assert eng.position == n
+    got, want, plain = np.stack(got), np.stack(want), np.stack(plain)
+    assert _off(got, want) <= 3 * SEEN[name]
+    assert np.linalg.norm(got - want) < np.linalg.norm(got - plain)
+
+
+@pytest.mark.parametrize("name", ["plain", "mixed"])
+def test_every_token_of_a_scored_text(models, name):
+    m = models[name]
+    toks = _tokens(200, m["vocab"], 7)
+    ref = forward64_int8(m, toks)[:-1]
+    with Engine(m["path"], prompt_bits=8) as eng:
+        s = eng.score(toks, top_k=1)
+    lp = ref - ref.max(-1, keepdims=True)
+    lp -= np.log(np.exp(lp).sum(-1, keepdims=True))
+    # a log probability moves by at most twice the largest change of a logit; over all rows by the norm
+    seen = s.logprob.astype(np.float64) - lp[np.arange(199), toks[1:]]
+    assert np.sqrt((seen ** 2).mean()) <= 2 * 3 * SEEN[name] * np.linalg.norm(ref) / np.sqrt(len(ref))
+
+
+def test_short_prompts_and_steps_are_as_without_it(models):
+    m = models["plain"]
+    toks = _tokens(LEAST - 1, m["vocab"], 8)
+    with Engine(m["path"], prompt_bits=8) as a, Engine(m["path"]) as b:
+        assert np.array_equal(a.forward(toks), b.forward(toks))
+        assert np.array_equal(a.forward_step(5), b.forward_step(5))
+        weights = sum(v["shape"][0] * v["shape"][1] for k, v in m["layers"].items() if ".layers." in k and "proj" in k)
+        assert a.stats()["peak_memory_bytes"] >= b.stats()["peak_memory_bytes"] + weights
+        prompt = _tokens(100, m["vocab"], 9)
+        one = a.generate_tokens(prompt, 10, temperature=0.0)
+        assert a.generate_tokens(prompt, 10, temperature=0.0) == one and len(one) >= 1
+
+
+def test_layers_with_element_outliers_keep_their_products(tmp_path, cuda_device):
+    p = tmp_path / "sparse.bf2"
+    m = build(p, element=True)
+    toks = _tokens(150, m["vocab"])
+    with Engine(p, prompt_bits=8) as a, Engine(p) as b:
+        # tokens after a norm are still brought into 8 bits: near, but not the same (tokens and weights of the
+        # plain model change its logits by 0.012, tokens alone by less)
+        x, y = a.forward(toks).astype(np.float64), b.forward(toks).astype(np.float64)
+        assert 0 < _off(x, y) < 0.03
+        assert np.array_equal(a.forward(toks[:20]), b.forward(toks[:20]))
+
+
+def test_with_a_4_bit_cache(models):
+    """Both options: what one changes by about SEEN + 0.012 at most, the other's codes (0.036 of the logits for one
+    such disturbance, as test_gpu_engine_kv4 has it) may follow."""
+    m = models["plain"]
+    toks = _tokens(300, m["vocab"], 11)
+    with Engine(m["path"], kv_bits=4, prompt_bits=8) as a, Engine(m["path"], kv_bits=4) as b:
+        x, y = a.forward(toks).astype(np.float64), b.forward(toks).astype(np.float64)
+        assert 0 < _off(x, y) <= 3 * 0.036
+        assert a.kv_cache_size == b.kv_cache_size and a.position == 300
+
+
+def test_command_line(models):
+    from opac1ty_b200.cli import cli
+
+    m = models["plain"]
+    ids = ",".join(str(t) for t in _tokens(80, m["vocab"], 12))
+    r = CliRunner().invoke(cli, ["score", str(m["path"]), "--tokens", ids, "--prompt-bits", "8"])
+    assert r.exit_code == 0, r.output
+    out = json.loads(r.output)
+    assert out["prompt_bits"] == 8 and len(out["logprobs"]) == 79
+
+
+def test_refusals(models, tmp_path):
+    h = lib().bf_engine_create_with(str(models["plain"]["path"]).encode(), 0, 0, 8)
+    assert b"options" in lib().bf_engine_get_error(h)
+    lib().bf_engine_destroy(h)
+    m = models["plain"]
+    p = tmp_path / "eps.bf2"
+    cfg = {"hidden_size": m["hidden"], "num_hidden_layers": m["n_layers"], "vocab_size": m["vocab"], "rms_norm_eps": 1e-14,
+           "num_attention_heads": m["heads"], "num_key_value_heads": m["kv_heads"]}
+    BF2Writer(str(p)).write(m["layers"], cfg, {"bits": 2, "sub_vector_size": 1}, progress=False)
+    with pytest.raises(EngineError, match="rms_norm_eps"):
+        Engine(p, prompt_bits=8)
+    with Engine(p) as eng:
+        eng.forward([1, 2, 3])
