@@ -17,7 +17,8 @@ using opc_host::fail;
 
 namespace {
 
-constexpr int kMaxWidth = 131071;  // 128 * 128 * 131071 < 2^31: no sum of products leaves 32 bits
+constexpr int kMaxWidth = 131071;           // 128 * 128 * 131071 < 2^31: no sum of products leaves 32 bits
+constexpr int kMaxRows = INT32_MAX - 4095;  // rows rounded up to a tile stay below 2^31
 
 int bytes_of(int32_t dtype) { return dtype == OPC_F32 ? 4 : 2; }
 bool is_type(int32_t dtype) { return dtype == OPC_F16 || dtype == OPC_BF16 || dtype == OPC_F32; }
@@ -33,8 +34,8 @@ int check_matrix(const char* who, const char* name, const void* p, int64_t ld, i
 
 int check_codes(const char* who, const char* name, const opc_i8_rows* m) {
   if (!m) return fail(OPC_ERR_INVALID, "%s: %s is NULL", who, name);
-  if (m->rows < 0 || m->n < 1 || m->n > kMaxWidth)
-    return fail(OPC_ERR_INVALID, "%s: %s is %d x %d (rows of 1 to %d values)", who, name, m->rows, m->n, kMaxWidth);
+  if (m->rows < 0 || m->rows > kMaxRows || m->n < 1 || m->n > kMaxWidth)
+    return fail(OPC_ERR_INVALID, "%s: %s is %d x %d (up to %d rows of 1 to %d values)", who, name, m->rows, m->n, kMaxRows, kMaxWidth);
   if (m->rows == 0) return OPC_OK;
   if (!m->codes || (reinterpret_cast<uintptr_t>(m->codes) & 15u) || m->ld < m->n || (m->ld & 15))
     return fail(OPC_ERR_INVALID, "%s: the codes of %s must start on 16 bytes in rows of a multiple of 16 bytes from %d on, got a leading dimension of %lld",

@@ -214,14 +214,15 @@ __global__ void __launch_bounds__(kI8Threads, 1)
     mbar_init(drain_b, 1);
     fence_mbar_init();
   }
+  __syncthreads();
+  cluster_sync();  // every CTA's barriers are set up
   griddep_wait();  // everything before has ended: its tensor memory is free again, its results are there
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tmem_slot), "r"(cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
-  __syncthreads();
-  cluster_sync();  // both CTAs' barriers are set up
+  __syncthreads();  // (a pair's first MMA waits for both CTAs' loads, which come after this in either)
   tc_fence_after();
   griddep_launch_dependents();  // every CTA that has come this far holds its tensor memory
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot_ptr);

@@ -2,6 +2,9 @@
 products is exact, the operations after it are named in the header)."""
 
 import ctypes
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -100,6 +103,58 @@ def test_nan_zero_and_infinite_scales(cuda_device, rows):
     y = int8.linear(x, w, dtype=F32)
     assert torch.isnan(y[1]).all() and torch.isnan(y[:, 7]).all()
     same(y, x, w)
+
+
+def _random_codes(rows, ld, device, seed):
+    return torch.randint(-128, 128, (rows, ld), dtype=torch.int8, device=device, generator=torch.Generator(device=device).manual_seed(seed))
+
+
+def test_results_past_32_bits(cuda_device):
+    """70001 x 32800 results (their places pass 2^31): those at the end, and at the 2^31st place."""
+    rows, m, k = 70001, 32800, 48
+    x = int8.Int8Rows(_random_codes(rows, k, cuda_device, 1), int8_ref.scales(rows, 1, cuda_device))
+    w = int8.Int8Weight(_random_codes(m, k, cuda_device, 2), int8_ref.scales(m, 2, cuda_device))
+    y = int8.linear(x, w)
+    for a in (0, 2**31 // m - 2, rows - 5):
+        want = int8_ref.linear(x.codes[a:a + 5], x.scales[a:a + 5], w.codes, w.scales, None, F16)
+        assert torch.equal(y[a:a + 5].cpu(), want)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_weights_past_32_bits(cuda_device, rows):
+    m, k = 70001, 65536
+    x = int8.Int8Rows(_random_codes(rows, k, cuda_device, 1), int8_ref.scales(rows, 1, cuda_device))
+    w = int8.Int8Weight(_random_codes(m, k, cuda_device, 2), int8_ref.scales(m, 2, cuda_device))
+    y = int8.linear(x, w, dtype=F32)
+    for a in (0, 2**32 // k - 3, m - 6):
+        want = int8_ref.linear(x.codes, x.scales, w.codes[a:a + 6], w.scales[a:a + 6], None, F32)
+        assert torch.equal(y[:, a:a + 6].cpu(), want)
+
+
+FIRST_CALL = """
+import torch
+from opac1ty_b200 import int8
+dev = torch.device("cuda", 0)
+x = int8.Int8Rows(torch.ones(40, 256, dtype=torch.int8, device=dev), torch.ones(40, device=dev))
+w = int8.Int8Weight(torch.ones(300, 256, dtype=torch.int8, device=dev), torch.ones(300, device=dev))
+t = torch.ones(40, 256, device=dev)
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    y = int8.linear(x, w)
+    h, r = int8.add_rmsnorm(t, t)
+    z = int8.linear(r, w)
+g.replay()
+torch.cuda.synchronize()
+assert (y == 256).all() and (h == 2).all() and (r.codes == 127).all() and ((z - 256).abs() < 0.25).all()
+print("as it should")
+"""
+
+
+def test_a_process_whose_first_calls_are_captured(cuda_device):
+    r = subprocess.run([sys.executable, "-c", FIRST_CALL], capture_output=True, text=True, timeout=300,
+                       cwd=Path(__file__).resolve().parent.parent)
+    assert r.returncode == 0 and "as it should" in r.stdout, r.stderr[-2000:]
 
 
 def test_no_rows(cuda_device):
@@ -214,7 +269,7 @@ def test_refusals(cuda_device):
     assert torch.equal(held.codes, w.codes)
 
 
-def test_gradients_are_refused_silently_by_the_documentation(cuda_device):
+def test_results_carry_no_gradient(cuda_device):
     """Results carry no gradient, whatever their inputs ask for."""
     t = torch.randn(3, 64, device=cuda_device, requires_grad=True)
     r = int8.quantize(t, values=F32)

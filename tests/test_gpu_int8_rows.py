@@ -187,6 +187,20 @@ def test_nothing_is_written_beside_the_rows(cuda_device, n):
     assert (codes == 99).all() and (scales == -1).all() and (vals == -2).all()
 
 
+@pytest.mark.parametrize("n", [1000, 60000])
+def test_rows_past_32_bits(cuda_device, n):
+    """Places in x, the codes and the values beyond 2^31: the rows there are those of a call by themselves."""
+    rows = 2**31 // n + 70
+    x = torch.randint(-30000, 30000, (rows, n), dtype=torch.int16, device=cuda_device,
+                      generator=torch.Generator(device=cuda_device).manual_seed(1)).view(BF16)
+    x = x.nan_to_num_(1.0, 2.0, 3.0)
+    r = int8.quantize(x, values=BF16)
+    for a in (0, rows - 75, rows - 5):
+        want = int8.quantize(x[a:a + 5].clone(), values=BF16)
+        assert torch.equal(r.codes[a:a + 5], want.codes) and torch.equal(r.scales[a:a + 5], want.scales)
+        assert torch.equal(r.values[a:a + 5], want.values)
+
+
 def test_no_rows(cuda_device):
     x = torch.empty(0, 64, dtype=F16, device=cuda_device)
     assert int8.quantize(x, values=F16).values.shape == (0, 64)

@@ -25,7 +25,7 @@ def gemm(x, w, bias=None, bt=0, y=P, ldy=64, yt=_lib.OPC_F16):
     return _lib.load().opc_i8_gemm(ctypes.byref(x), ctypes.byref(w), bias, bt, y, ldy, yt, None)
 
 
-@pytest.mark.parametrize("kw", [dict(rows=-1), dict(n=0), dict(n=131072), dict(ld=47), dict(ld=32), dict(ld=56),
+@pytest.mark.parametrize("kw", [dict(rows=-1), dict(rows=2**31 - 4095), dict(n=0), dict(n=131072), dict(ld=47), dict(ld=32), dict(ld=56),
                                 dict(codes=None), dict(codes=P + 8), dict(scales=None), dict(scales=P + 2)])
 def test_rows_of_codes_are_checked(kw):
     if kw.get("n") == 131072:
