@@ -50,11 +50,10 @@ bool vec_ok(const void* p, int64_t ld, int32_t dtype) {
 }
 
 template <typename... KArgs, typename... Args>
-cudaError_t launch_smem(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y, int threads, size_t smem, void* stream, const Args&... args) {
+cudaError_t launch(void (*kern)(KArgs...), unsigned ctas, int threads, void* stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(grid_x, grid_y);
+  cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];  // the launch overlaps the end of the kernel before, which the kernel waits for
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -63,31 +62,29 @@ cudaError_t launch_smem(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, kern, args...);
 }
-template <typename... KArgs, typename... Args>
-cudaError_t launch(void (*kern)(KArgs...), unsigned grid_x, unsigned grid_y, int threads, void* stream, const Args&... args) {
-  return launch_smem(kern, grid_x, grid_y, threads, 0, stream, args...);
-}
 
 // One warp per row up to 1024 values; beyond, one CTA per row with 16 values a thread, or 8 where there
 // are few rows and a row up to 8192 values (96 x 8192 bf16 norms 3.4 -> 3.2 us, 512 x 4096 fp32 ones 6.1 ->
 // 5.8 us; but 28672 x 4096 quantized 97 -> 111 us), 32 from 16384 values on (shorter rows lose by it:
-// 4097 x 14336 gated 62 -> 83 us).  Rows of more than 32768 values, which no CTA's registers hold, are
-// read twice.
+// 4097 x 14336 gated 62 -> 83 us; longer ones gain over being read twice: 4096 x 28672 152 -> 138 us).  Rows of more than 32768 values, which no CTA's registers hold, are
+// read twice.  (Clusters of CTAs that share a long row were slower than either: 4096 x 28672 gated 141 ->
+// 188 us, 4096 x 40000 quantized 125 -> 181.)
 template <int kOp, int kTX, int kTU>
 cudaError_t launch_rows(const opc::I8RowsArgs& a, int sms, void* stream) {
+  using opc::i8_rows_kernel;
   const int groups = (a.n + 7) / 8;
   if (groups <= 128) {
     const int per = (groups + 31) / 32;
-    auto k = per == 1 ? opc::i8_rows_kernel<kOp, kTX, kTU, 1, true>
-             : per == 2 ? opc::i8_rows_kernel<kOp, kTX, kTU, 2, true> : opc::i8_rows_kernel<kOp, kTX, kTU, 4, true>;
-    return launch(k, (a.rows + 3) / 4, 1, 128, stream, a);
+    auto k = per == 1 ? i8_rows_kernel<kOp, kTX, kTU, 1, true>
+             : per == 2 ? i8_rows_kernel<kOp, kTX, kTU, 2, true> : i8_rows_kernel<kOp, kTX, kTU, 4, true>;
+    return launch(k, (a.rows + 3) / 4, 128, stream, a);
   }
   const int per = groups <= 1024 && a.rows <= 4 * sms ? 1 : groups <= 2048 ? 2 : groups <= 4096 ? 4 : 0;
   const int threads = per ? ((groups + per - 1) / per + 31) / 32 * 32 : 1024;
-  auto k = per == 1 ? opc::i8_rows_kernel<kOp, kTX, kTU, 1, false>
-           : per == 2 ? opc::i8_rows_kernel<kOp, kTX, kTU, 2, false>
-           : per == 4 ? opc::i8_rows_kernel<kOp, kTX, kTU, 4, false> : opc::i8_rows_kernel<kOp, kTX, kTU, 0, false>;
-  return launch(k, a.rows, 1, threads, stream, a);
+  auto k = per == 1 ? i8_rows_kernel<kOp, kTX, kTU, 1, false>
+           : per == 2 ? i8_rows_kernel<kOp, kTX, kTU, 2, false>
+           : per == 4 ? i8_rows_kernel<kOp, kTX, kTU, 4, false> : i8_rows_kernel<kOp, kTX, kTU, 0, false>;
+  return launch(k, a.rows, threads, stream, a);
 }
 
 template <int kOp, int kTU>
@@ -330,7 +327,7 @@ int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, in
     const GemvKernel g = y_dtype == OPC_F16 ? gemv_kernel<opc::kI8F16>(x->rows, w->rows, x->n, dev.sm_count)
                          : y_dtype == OPC_BF16 ? gemv_kernel<opc::kI8BF16>(x->rows, w->rows, x->n, dev.sm_count)
                                                : gemv_kernel<opc::kI8F32>(x->rows, w->rows, x->n, dev.sm_count);
-    return end_rows(who, launch(g.kernel, (w->rows + 15) / 16, 1, g.threads, stream, x->codes, x->ld, w->codes, w->ld, x->n, o));
+    return end_rows(who, launch(g.kernel, (w->rows + 15) / 16, g.threads, stream, x->codes, x->ld, w->codes, w->ld, x->n, o));
   }
   auto k = y_dtype == OPC_F16 ? opc::i8_gemm_kernel<opc::kI8F16>
            : y_dtype == OPC_BF16 ? opc::i8_gemm_kernel<opc::kI8BF16> : opc::i8_gemm_kernel<opc::kI8F32>;

@@ -217,30 +217,30 @@ template <bool kWarpRow>
 __device__ __forceinline__ I8Row i8_reduce(const I8Stat& p, bool norm) {
   I8Row s;
   s.big = p.big;
+  s.ss = s.small = 0.f;
   if (norm) {
     const float2 a = i8_both(p.ss), b = i8_both(p.small);
     s.ss = a.x + a.y;
     s.small = b.x + b.y;
   }
   i8_warp_reduce(s, norm);
-  if constexpr (!kWarpRow) {
-    __shared__ float part_big[32], part_ss[32], part_small[32];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
-    if (lane == 0) {
-      part_big[warp] = s.big;
-      if (norm) {
-        part_ss[warp] = s.ss;
-        part_small[warp] = s.small;
-      }
-    }
-    __syncthreads();
-    s.big = lane < warps ? part_big[lane] : 0.f;
+  if constexpr (kWarpRow) return s;
+  __shared__ float part_big[32], part_ss[32], part_small[32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  if (lane == 0) {
+    part_big[warp] = s.big;
     if (norm) {
-      s.ss = lane < warps ? part_ss[lane] : 0.f;
-      s.small = lane < warps ? part_small[lane] : 0.f;
+      part_ss[warp] = s.ss;
+      part_small[warp] = s.small;
     }
-    i8_warp_reduce(s, norm);
   }
+  __syncthreads();
+  s.big = lane < warps ? part_big[lane] : 0.f;
+  if (norm) {
+    s.ss = lane < warps ? part_ss[lane] : 0.f;
+    s.small = lane < warps ? part_small[lane] : 0.f;
+  }
+  i8_warp_reduce(s, norm);
   return s;
 }
 
@@ -332,9 +332,9 @@ __device__ __forceinline__ float i8_silu_mul(float g, float u) {
 }
 
 // 8 values of a row before its scale from what was loaded, their part of the statistics, and (norm) h_out.
-template <int kOp, int kTX, int kTU>
+template <int kOp, int kTX, int kTU, bool kWriteH>
 __device__ __forceinline__ void i8_make8(const I8RowsArgs& a, int row, int i, const I8Raw<kTX>& rx, const I8Raw<kTU>& ru, I8Pair (&v)[4],
-                                         I8Stat& s, bool write_h) {
+                                         I8Stat& s) {
   const int left = a.n - i;
   i8_open8(rx, v);
   if constexpr (kTU != kI8None) {
@@ -351,7 +351,7 @@ __device__ __forceinline__ void i8_make8(const I8RowsArgs& a, int row, int i, co
     }
   }
   if constexpr (kOp == kI8Norm) {
-    if (write_h && a.h_out) i8_store8<kTX>(a.h_out, static_cast<int64_t>(row) * a.ldh + i, left, a.vec_h, v);
+    if (kWriteH && a.h_out) i8_store8<kTX>(a.h_out, static_cast<int64_t>(row) * a.ldh + i, left, a.vec_h, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       s.ss = i8_fma2(v[e], v[e], s.ss);
@@ -372,10 +372,16 @@ __device__ __forceinline__ void i8_make8(const I8RowsArgs& a, int row, int i, co
   }
 }
 
+// CTAs of 1024 threads that an SM is to hold, where 32 registers a thread do for that: a CTA alone leaves
+// the memory idle while it reduces (4097 x 14336 gated: 72 us with one CTA an SM, 48 with two).
+constexpr int i8_resident(int op, int x, int per, bool warp_row) {
+  return !warp_row && per < 4 && (op == kI8Quant || (op == kI8Silu && x != kI8F32)) ? 2 : 1;
+}
+
 // One row per CTA (kWarpRow: per warp), kPer groups of 8 values per thread in registers; kPer 0: rows
 // of any length, read once for the statistics and once more for the codes.
 template <int kOp, int kTX, int kTU, int kPer, bool kWarpRow>
-__global__ void __launch_bounds__(kWarpRow ? 128 : 1024) i8_rows_kernel(const I8RowsArgs a) {
+__global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, kPer, kWarpRow)) i8_rows_kernel(const I8RowsArgs a) {
   griddep_wait();
   griddep_launch_dependents();
   const int threads = kWarpRow ? 32 : blockDim.x;
@@ -384,28 +390,28 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024) i8_rows_kernel(const I8
   if (kWarpRow && row >= a.rows) return;
   constexpr bool kNorm = kOp == kI8Norm;
   constexpr bool kExact = kOp != kI8Silu && kTU == kI8None;
-  const int64_t at_x = static_cast<int64_t>(row) * a.ldx, at_u = static_cast<int64_t>(row) * a.ldu;
   I8Stat s{0.f, 0ull, 0ull};
+  // groups whose loads are all under way before the first is used (two of 64 registers would not stay in them)
+  constexpr int kBatch = kPer < 2 || (kPer == 4 && kTX == kI8F32 && kTU == kI8F32) ? 1 : 2;
+  I8Raw<kTX> rx[kBatch];
+  I8Raw<kTU> ru[kBatch];
+  const auto load = [&](int i, int j) {
+    i8_load8(a.x, static_cast<int64_t>(row) * a.ldx + i, a.n - i, a.vec_x, rx[j]);
+    if constexpr (kTU != kI8None) i8_load8(a.u, static_cast<int64_t>(row) * a.ldu + i, a.n - i, a.vec_u, ru[j]);
+  };
   if constexpr (kPer > 0) {
-    // groups whose loads are all under way before the first is used (two of 64 registers would not stay in them)
-    constexpr int kBatch = kPer < 2 || (kPer == 4 && kTX == kI8F32 && kTU == kI8F32) ? 1 : 2;
     I8Pair v[kPer][4];
 #pragma unroll
     for (int j0 = 0; j0 < kPer; j0 += kBatch) {
-      I8Raw<kTX> rx[kBatch];
-      I8Raw<kTU> ru[kBatch];
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int i = 8 * (t + (j0 + j) * threads);
-        if (i < a.n) {
-          i8_load8(a.x, at_x + i, a.n - i, a.vec_x, rx[j]);
-          if constexpr (kTU != kI8None) i8_load8(a.u, at_u + i, a.n - i, a.vec_u, ru[j]);
-        }
+        if (i < a.n) load(i, j);
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
         const int i = 8 * (t + (j0 + j) * threads);
-        if (i < a.n) i8_make8<kOp, kTX, kTU>(a, row, i, rx[j], ru[j], v[j0 + j], s, true);
+        if (i < a.n) i8_make8<kOp, kTX, kTU, true>(a, row, i, rx[j], ru[j], v[j0 + j], s);
       }
     }
     const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), a, kNorm);
@@ -421,23 +427,17 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024) i8_rows_kernel(const I8
       for (int i = 8 * t; i < a.n; i += 8 * threads) i8_write8<false, kExact>(a, row, i, a.n - i, v[0], sc);
     }
   } else {
-    I8Raw<kTX> rx;
-    I8Raw<kTU> ru;
     I8Pair v[4];
-    auto load = [&](int i) {
-      i8_load8(a.x, at_x + i, a.n - i, a.vec_x, rx);
-      if constexpr (kTU != kI8None) i8_load8(a.u, at_u + i, a.n - i, a.vec_u, ru);
-    };
     for (int i = 8 * t; i < a.n; i += 8 * threads) {
-      load(i);
-      i8_make8<kOp, kTX, kTU>(a, row, i, rx, ru, v, s, false);
+      load(i, 0);
+      i8_make8<kOp, kTX, kTU, false>(a, row, i, rx[0], ru[0], v, s);
     }
     const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), a, kNorm);
     if (t == 0) a.scales[row] = sc.scale;
     I8Stat none{0.f, 0ull, 0ull};
     for (int i = 8 * t; i < a.n; i += 8 * threads) {  // (h_out may be h: each thread reads a place before it writes it)
-      load(i);
-      i8_make8<kOp, kTX, kTU>(a, row, i, rx, ru, v, none, true);
+      load(i, 0);
+      i8_make8<kOp, kTX, kTU, true>(a, row, i, rx[0], ru[0], v, none);
       if (sc.live) i8_write8<true, kExact>(a, row, i, a.n - i, v, sc);
       else i8_write8<false, kExact>(a, row, i, a.n - i, v, sc);
     }

@@ -63,9 +63,9 @@ class Int8Rows:
         elif values not in _DTYPES:
             raise ValueError(f"values must be float16, bfloat16 or float32, got {values}")
         elif like.shape[1] == n:  # (rows are like's everywhere)
-            self.values = torch.empty_like(like, dtype=values, memory_format=torch.contiguous_format)
+            self.values = torch.empty_like(like, dtype=values)  # (contiguous: like has unit stride)
         else:
-            self.values = like.new_empty((rows, n), dtype=values)
+            self.values = like.new_empty(rows, n, dtype=values)
         ld = -(-n // 16) * 16
         held = like.new_empty(rows * (ld // 4 + 1), dtype=torch.float32)
         self._codes = self._scales = None
@@ -86,7 +86,7 @@ class Int8Rows:
     @property
     def scales(self) -> torch.Tensor:
         if self._scales is None:
-            self._scales = self._held.narrow(0, self.rows * (self.c.ld // 4), self.rows)
+            self._scales = self._held[self.rows * (self.c.ld // 4):]
         return self._scales
 
     @property
@@ -194,7 +194,7 @@ def add_rmsnorm(h: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Optio
         if y_type != h_type and h_type != _lib.OPC_F32:
             raise ValueError(f"add_rmsnorm: y is {y.dtype} beside an h of {h.dtype}")
         if h_out is None:
-            h_out = torch.empty_like(h, memory_format=torch.contiguous_format)
+            h_out = torch.empty_like(h)  # (contiguous: h has unit stride)
             o_ptr, ldo = h_out.data_ptr(), n
     if h_out is not None and o_ptr is None:
         ldo = _matrix("add_rmsnorm", "h_out", h_out, rows, n, index)
@@ -223,7 +223,7 @@ def linear(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = None,
     if out is None:
         if dtype not in _DTYPES:
             raise ValueError(f"linear: results are float16, bfloat16 or float32, not {dtype}")
-        out = weight._scales.new_empty((rows, m), dtype=dtype)
+        out = weight._scales.new_empty(rows, m, dtype=dtype)
         ldy = m
     else:
         ldy = _matrix("linear", "out", out, rows, m, index)
