@@ -157,6 +157,25 @@ GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, const int (&clusters)[5])
   return p;
 }
 
+// The same, remembered by its sizes (a thread's last few; the choice costs about a microsecond).
+GemmPlan plan_of(int32_t rows, int32_t M, int32_t K, const int (&clusters)[5]) {
+  struct Known {
+    int32_t rows, M, K;
+    int clusters[5];
+    GemmPlan plan;
+  };
+  thread_local Known known[8] = {};
+  Known& k = known[(static_cast<uint32_t>(rows) * 31u + static_cast<uint32_t>(M) * 7u + static_cast<uint32_t>(K)) / 32u % 8u];
+  if (k.rows != rows || k.M != M || k.K != K || !std::equal(clusters + 1, clusters + 5, k.clusters + 1)) {
+    k.plan = plan_gemm(rows, M, K, clusters);
+    k.rows = rows;
+    k.M = M;
+    k.K = K;
+    std::copy(clusters + 1, clusters + 5, k.clusters + 1);
+  }
+  return k.plan;
+}
+
 // Rows of codes as a tensor of bytes, in boxes of 128 bytes x box rows, zeros beyond its edges.
 int map_codes(const char* who, const opc_i8_rows* m, int box, CUtensorMap* map) {
   auto encode = opc_host::tensor_map_encoder();
@@ -334,7 +353,7 @@ int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, in
   int clusters[5];
   cudaError_t e = gemm_setup(k, y_dtype, &clusters);
   if (e != cudaSuccess) return cuda_fail(e, "opc_i8_gemm: setting up");
-  const GemmPlan p = plan_gemm(x->rows, w->rows, x->n, clusters);
+  const GemmPlan p = plan_of(x->rows, w->rows, x->n, clusters);
   if (!p.ctas) return fail(OPC_ERR_UNSUPPORTED, "%s: %d tokens times %d channels are too many tiles for one call", who, x->rows, w->rows);
   opc::I8GemmArgs a = {o, p.deal, dev.error_word};
   CUtensorMap tw, tx;
