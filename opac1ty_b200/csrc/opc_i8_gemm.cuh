@@ -15,7 +15,16 @@
 //                   warp 1     tensor memory; in a pair's first CTA it issues the MMAs
 //                   warps 2-9  epilogue: two warps per TMEM lane quarter, half of the columns each;
 //                              it reads one accumulator while the MMAs fill the other
+//                 Measured (device time in a graph, weights from memory): 8191 tokens 4096 -> 28672 581 us,
+//                 3.31 PFLOP/s at the clocks of a short run; in a loop the power limit brings the clock to
+//                 1.27 GHz, of whose 3.07 PFLOP/s it reaches 2.87.  512 tokens 4096 -> 6144 14.7 us: 72 of 74
+//                 pairs for one tile of 192 tokens, 8 us of MMAs behind 4 us of launch and first loads,
+//                 then 2 us of results.  24 tokens 14336 -> 4096 15.2 us, 3.9 TB/s: the reading of W at
+//                 6.8 TB/s, behind the same and the exchange of sums.
 // i8_gemv_kernel  few tokens: mma.sync fragments straight from global memory; bound by the reading of W.
+//                 One token 4096 -> 28672 20.6 us, 5.7 TB/s; 4096 -> 128256 77 us, 6.8 TB/s.  (tcgen05
+//                 would wait for tensor memory, barriers and a transposed staging of W: 8.7 us instead of
+//                 5.3 for 4096 -> 4096.)
 #pragma once
 
 #include <cuda.h>
@@ -101,7 +110,7 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // The asynchronous operations are issued by one lane (`leader`) of a converged warp: outside a divergent
-// branch their operands can stay in uniform registers.
+// branch their operands can stay in uniform registers (8191 tokens 4096 -> 28672: 725 -> 647 us).
 __device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -169,7 +178,7 @@ struct I8Walk {
 template <int kY, int kNum>
 __device__ __forceinline__ void i8_store_column(const I8Out& o, const float (&f)[kNum], int32_t t, int32_t r, int32_t left) {
   const int64_t at = static_cast<int64_t>(t) * o.ldy + r;
-  if (left >= kNum) {  // (without a branch per value, so that their chains overlap)
+  if (left >= kNum) {  // (without a branch per value, so that their chains overlap: 256 tokens of a tile 6 -> 2 us)
 #pragma unroll
     for (int i = 0; i < kNum; ++i) i8_store1<kY>(o.y, at + i * o.ldy, f[i]);
   } else {
