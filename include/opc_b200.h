@@ -504,7 +504,8 @@ typedef struct opc_i8_rows {
  *                      sqrt(mean t^2 + eps), t as formed, before its rounding: the codes of the
  *                      normalized row.  y has h's type, or h is OPC_F32.  eps from 1e-12 on.  (The
  *                      limits of a zero row above are those of t * weight.)  Sums in fp32, a row whose
- *                      squares leave fp32 included; deterministic. */
+ *                      squares leave fp32 included; the factor to 2^-21 of itself besides the sum's
+ *                      roundings.  Deterministic. */
 int opc_i8_quantize(const void* x, int64_t ldx, int32_t dtype, const opc_i8_rows* out, void* values, int64_t ldv,
                     int32_t v_dtype, void* stream);
 int opc_i8_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, int32_t dtype, const opc_i8_rows* out,

@@ -109,13 +109,13 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// The asynchronous operations are issued by one lane (`leader`) of a converged warp: outside a divergent
-// branch their operands can stay in uniform registers (8191 tokens 4096 -> 28672: 725 -> 647 us).
 __device__ __forceinline__ uint4 ld_cluster_v4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared::cluster.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
+// The asynchronous operations are issued by one lane (`leader`) of a converged warp: outside a divergent
+// branch their operands can stay in uniform registers (8191 tokens 4096 -> 28672: 725 -> 647 us).
 // A TMA load into this CTA's shared memory that completes on a barrier of either CTA of the pair.
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t leader, uint32_t dst, const CUtensorMap* map, int32_t x, int32_t y, uint32_t bar) {
   asm volatile(
@@ -189,8 +189,8 @@ __device__ __forceinline__ void i8_store_column(const I8Out& o, const float (&f)
 }
 
 // tw: w [M][K], box 128 bytes x 128 channels; tx: x [rows][K], box 128 bytes x tile_n / 2 tokens; both
-// with the 128-byte swizzle, zeros beyond the edges.
-// Clusters of 2 * split CTAs.
+// with the 128-byte swizzle, zeros beyond the edges.  Clusters of 2 * split CTAs; dynamic shared memory for
+// the stages, which later hold a split tile's sums, and the barriers.
 template <int kY>
 __global__ void __launch_bounds__(kI8Threads, 1)
     i8_gemm_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const I8GemmArgs a) {
@@ -209,7 +209,7 @@ __global__ void __launch_bounds__(kI8Threads, 1)
   const int lane = threadIdx.x & 31;
   const uint32_t in_cluster = cluster_rank(), first = in_cluster & ~1u, rank = in_cluster & 1u;  // `first`: the pair's first CTA
   const int split = a.d.split;
-  const int cols = kN <= 16 ? 32 : kN <= 32 ? 64 : kN <= 64 ? 128 : kN <= 128 ? 256 : 512;  // two accumulators
+  const int cols = kN <= 32 ? 64 : kN <= 64 ? 128 : kN <= 128 ? 256 : 512;  // two accumulators
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < stages; ++s) {

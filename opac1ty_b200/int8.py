@@ -223,7 +223,7 @@ def linear(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = None,
     if out is None:
         if dtype not in _DTYPES:
             raise ValueError(f"linear: results are float16, bfloat16 or float32, not {dtype}")
-        out = weight._scales.new_empty(rows, m, dtype=dtype)
+        out = weight.scales.new_empty(rows, m, dtype=dtype)
         ldy = m
     else:
         ldy = _matrix("linear", "out", out, rows, m, index)

@@ -6,7 +6,8 @@ lands on the other side of a rounding boundary.  How much that moves the logits 
 pass alone, by disturbing what is brought into 8 bits by 2^-11 of itself (three seeds, Frobenius norm of the
 differences against that of the logits): SEEN below.  The tolerance is three times that, because the
 engine rounds a dozen intermediate results and not one.  The pass without 8 bits is 0.012 (plain), 0.025
-(wide) and 0.024 (mixed) from the one with them; what the engine gives has to be nearer to the latter."""
+(wide) and 0.024 (mixed) from the one with them; what the engine gives has to be nearer to the latter.  (0.034
+with vectors of 8, too little beside what one disturbance does there.)"""
 
 import json
 
@@ -21,9 +22,9 @@ from opac1ty_b200.engine import Engine, EngineError, lib
 from opac1ty_b200.format import BF2Writer
 
 pytestmark = pytest.mark.gpu
-SEEN = {"plain": 0.0062, "wide": 0.0081, "mixed": 0.0094}
+SEEN = {"plain": 0.0062, "wide": 0.0081, "mixed": 0.0094, "vectors": 0.0266}
 WIDE = dict(hidden=512, heads=4, kv_heads=1, inter=1376, vocab=500, seed=3)
-MODELS = {"plain": dict(), "wide": WIDE, "mixed": WIDE}
+MODELS = {"plain": dict(), "wide": WIDE, "mixed": WIDE, "vectors": dict(svs=8, seed=2)}
 # "mixed": these layers have element-wise outliers and stay on the fp16 products (the ones after a norm take
 # its 8-bit tokens' values, the others the tokens as they are)
 SPARSE = ("model.layers.0.self_attn.q_proj.weight", "model.layers.0.mlp.up_proj.weight", "model.layers.0.mlp.down_proj.weight",
@@ -124,7 +125,7 @@ def test_prompts_match_float64(models, name):
             assert eng.position == n
     got, want, plain = np.stack(got), np.stack(want), np.stack(plain)
     assert _off(got, want) <= 3 * SEEN[name]
-    assert np.linalg.norm(got - want) < np.linalg.norm(got - plain)
+    assert name == "vectors" or np.linalg.norm(got - want) < np.linalg.norm(got - plain)
 
 
 @pytest.mark.parametrize("name", ["plain", "mixed"])
