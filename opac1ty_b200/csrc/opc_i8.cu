@@ -45,8 +45,9 @@ int check_codes(const char* who, const char* name, const opc_i8_rows* m) {
   return OPC_OK;
 }
 
-bool vec_ok(const void* p, int64_t ld, int32_t dtype) {
-  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (ld * bytes_of(dtype)) % 16 == 0;
+// Whether every row starts on 16 bytes (a matrix that is not there: yes).
+bool vec_ok(const void* p, int64_t ld, int32_t dtype, int32_t rows) {
+  return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (!p || rows == 1 || (ld * bytes_of(dtype)) % 16 == 0);
 }
 
 template <typename... KArgs, typename... Args>
@@ -65,33 +66,36 @@ cudaError_t launch(void (*kern)(KArgs...), unsigned ctas, int threads, void* str
 
 // One warp per row up to 1024 values; beyond, one CTA per row with 16 values a thread, or 8 where there
 // are few rows and a row up to 8192 values (96 x 8192 bf16 norms 3.4 -> 3.2 us, 512 x 4096 fp32 ones 6.1 ->
-// 5.8 us; but 28672 x 4096 quantized 97 -> 111 us), 32 from 16384 values on (shorter rows lose by it:
-// 4097 x 14336 gated 62 -> 83 us; longer ones gain over being read twice: 4096 x 28672 152 -> 138 us).  Rows of more than 32768 values, which no CTA's registers hold, are
-// read twice.  (Clusters of CTAs that share a long row were slower than either: 4096 x 28672 gated 141 ->
-// 188 us, 4096 x 40000 quantized 125 -> 181.)
+// 5.8 us; but 28672 x 4096 quantized 97 -> 111 us), 32 from 16384 values on (shorter rows lose by it: 4097 x
+// 14336 gated 62 -> 83 us; longer ones gain over being read twice: 4096 x 28672 152 -> 138 us).  Rows of more
+// than 32768 values, which no CTA's registers hold, are read twice.  (Clusters of CTAs that share a long row
+// were slower than either: 4096 x 28672 gated 141 -> 188 us, 4096 x 40000 quantized 125 -> 181.)  Rows that do
+// not all start on 16 bytes are moved value by value.
 template <int kOp, int kTX, int kTU>
-cudaError_t launch_rows(const opc::I8RowsArgs& a, int sms, void* stream) {
+cudaError_t launch_rows(const opc::I8RowsArgs& a, bool vec, int sms, void* stream) {
   using opc::i8_rows_kernel;
   const int groups = (a.n + 7) / 8;
   if (groups <= 128) {
     const int per = (groups + 31) / 32;
-    auto k = per == 1 ? i8_rows_kernel<kOp, kTX, kTU, 1, true>
-             : per == 2 ? i8_rows_kernel<kOp, kTX, kTU, 2, true> : i8_rows_kernel<kOp, kTX, kTU, 4, true>;
+    auto k = !vec ? i8_rows_kernel<kOp, kTX, kTU, 4, true, false>
+             : per == 1 ? i8_rows_kernel<kOp, kTX, kTU, 1, true, true>
+             : per == 2 ? i8_rows_kernel<kOp, kTX, kTU, 2, true, true> : i8_rows_kernel<kOp, kTX, kTU, 4, true, true>;
     return launch(k, (a.rows + 3) / 4, 128, stream, a);
   }
-  const int per = groups <= 1024 && a.rows <= 4 * sms ? 1 : groups <= 2048 ? 2 : groups <= 4096 ? 4 : 0;
+  const int per = vec && groups <= 1024 && a.rows <= 4 * sms ? 1 : groups <= 2048 ? 2 : vec && groups <= 4096 ? 4 : 0;
   const int threads = per ? ((groups + per - 1) / per + 31) / 32 * 32 : 1024;
-  auto k = per == 1 ? i8_rows_kernel<kOp, kTX, kTU, 1, false>
-           : per == 2 ? i8_rows_kernel<kOp, kTX, kTU, 2, false>
-           : per == 4 ? i8_rows_kernel<kOp, kTX, kTU, 4, false> : i8_rows_kernel<kOp, kTX, kTU, 0, false>;
+  auto k = !vec ? (per == 2 ? i8_rows_kernel<kOp, kTX, kTU, 2, false, false> : i8_rows_kernel<kOp, kTX, kTU, 0, false, false>)
+           : per == 1 ? i8_rows_kernel<kOp, kTX, kTU, 1, false, true>
+           : per == 2 ? i8_rows_kernel<kOp, kTX, kTU, 2, false, true>
+           : per == 4 ? i8_rows_kernel<kOp, kTX, kTU, 4, false, true> : i8_rows_kernel<kOp, kTX, kTU, 0, false, true>;
   return launch(k, a.rows, threads, stream, a);
 }
 
 template <int kOp, int kTU>
-cudaError_t launch_rows_x(int32_t x_type, const opc::I8RowsArgs& a, int sms, void* stream) {
-  if (x_type == OPC_F16) return launch_rows<kOp, opc::kI8F16, kTU == 4 ? opc::kI8F16 : kTU>(a, sms, stream);
-  if (x_type == OPC_BF16) return launch_rows<kOp, opc::kI8BF16, kTU == 4 ? opc::kI8BF16 : kTU>(a, sms, stream);
-  return launch_rows<kOp, opc::kI8F32, kTU == 4 ? opc::kI8F32 : kTU>(a, sms, stream);
+cudaError_t launch_rows_x(int32_t x_type, const opc::I8RowsArgs& a, bool vec, int sms, void* stream) {
+  if (x_type == OPC_F16) return launch_rows<kOp, opc::kI8F16, kTU == 4 ? opc::kI8F16 : kTU>(a, vec, sms, stream);
+  if (x_type == OPC_BF16) return launch_rows<kOp, opc::kI8BF16, kTU == 4 ? opc::kI8BF16 : kTU>(a, vec, sms, stream);
+  return launch_rows<kOp, opc::kI8F32, kTU == 4 ? opc::kI8F32 : kTU>(a, vec, sms, stream);
 }
 constexpr int kSame = 4;  // launch_rows_x: the second operand has the first one's type
 
@@ -112,7 +116,6 @@ int start_rows(const char* who, const opc_i8_rows* out, void* values, int64_t ld
   a->values = values;
   a->ldv = ldv;
   a->v_type = v_dtype;
-  a->vec_v = values && vec_ok(values, ldv, v_dtype);
   return OPC_OK;
 }
 
@@ -263,10 +266,10 @@ int opc_i8_quantize(const void* x, int64_t ldx, int32_t dtype, const opc_i8_rows
   if ((rc = check_matrix(who, "x", x, ldx, dtype, out->n)) != OPC_OK) return rc;
   a.x = x;
   a.ldx = ldx;
-  a.vec_x = vec_ok(x, ldx, dtype);
+  const bool vec = vec_ok(x, ldx, dtype, out->rows) && vec_ok(values, ldv, v_dtype, out->rows);
   opc_host::Device dev;
   if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
-  return end_rows(who, launch_rows_x<opc::kI8Quant, opc::kI8None>(dtype, a, dev.sm_count, stream));
+  return end_rows(who, launch_rows_x<opc::kI8Quant, opc::kI8None>(dtype, a, vec, dev.sm_count, stream));
 }
 
 int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* y, int64_t ldy, int32_t y_dtype,
@@ -286,25 +289,24 @@ int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* 
   if (!(eps >= 1e-12f) || !std::isfinite(eps)) return fail(OPC_ERR_INVALID, "%s: eps %g (1e-12 or more)", who, static_cast<double>(eps));
   a.x = h;
   a.ldx = ldh;
-  a.vec_x = vec_ok(h, ldh, h_dtype);
   a.u = y;
   a.ldu = ldy;
-  a.vec_u = y && vec_ok(y, ldy, y_dtype);
   a.w = weight;
   a.w_type = w_dtype;
-  a.vec_w = weight && vec_ok(weight, 8, w_dtype);
   a.h_out = h_out;
   a.ldh = ldho;
-  a.vec_h = h_out && vec_ok(h_out, ldho, h_dtype);
   a.eps = eps;
   a.inv_n = 1.0f / static_cast<float>(n);
+  const int32_t rows = out->rows;
+  const bool vec = vec_ok(h, ldh, h_dtype, rows) && vec_ok(y, ldy, y_dtype, rows) && vec_ok(weight, n, w_dtype, 1) &&
+                   vec_ok(h_out, ldho, h_dtype, rows) && vec_ok(values, ldv, v_dtype, rows);
   opc_host::Device dev;
   if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
   cudaError_t e;
-  if (!y) e = launch_rows_x<opc::kI8Norm, opc::kI8None>(h_dtype, a, dev.sm_count, stream);
-  else if (y_dtype == h_dtype) e = launch_rows_x<opc::kI8Norm, kSame>(h_dtype, a, dev.sm_count, stream);
-  else if (y_dtype == OPC_F16) e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8F16>(a, dev.sm_count, stream);
-  else e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8BF16>(a, dev.sm_count, stream);
+  if (!y) e = launch_rows_x<opc::kI8Norm, opc::kI8None>(h_dtype, a, vec, dev.sm_count, stream);
+  else if (y_dtype == h_dtype) e = launch_rows_x<opc::kI8Norm, kSame>(h_dtype, a, vec, dev.sm_count, stream);
+  else if (y_dtype == OPC_F16) e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8F16>(a, vec, dev.sm_count, stream);
+  else e = launch_rows<opc::kI8Norm, opc::kI8F32, opc::kI8BF16>(a, vec, dev.sm_count, stream);
   return end_rows(who, e);
 }
 
@@ -318,13 +320,12 @@ int opc_i8_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, 
   if ((rc = check_matrix(who, "up", up, ldu, dtype, out->n)) != OPC_OK) return rc;
   a.x = gate;
   a.ldx = ldg;
-  a.vec_x = vec_ok(gate, ldg, dtype);
   a.u = up;
   a.ldu = ldu;
-  a.vec_u = vec_ok(up, ldu, dtype);
+  const bool vec = vec_ok(gate, ldg, dtype, out->rows) && vec_ok(up, ldu, dtype, out->rows) && vec_ok(values, ldv, v_dtype, out->rows);
   opc_host::Device dev;
   if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
-  return end_rows(who, launch_rows_x<opc::kI8Silu, kSame>(dtype, a, dev.sm_count, stream));
+  return end_rows(who, launch_rows_x<opc::kI8Silu, kSame>(dtype, a, vec, dev.sm_count, stream));
 }
 
 int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, int32_t bias_dtype, void* y, int64_t ldy,

@@ -10,14 +10,15 @@
 // in registers between the reduction and the rounding.  Bound by memory for large calls, which takes
 // few enough instructions per value that it stays so: pairs of values in packed fp32 operations, one
 // maximum of three per two values (device time with L2 flushed by the inputs: 8191 x 4096 fp32 + fp16 norms
-// with values 66 us, 6.6 TB/s; 4097 x 14336 fp16 gated with values 62 us, 6.6 TB/s; 28672 x 4096 fp16
-// quantized with values 97 us, 6.1 TB/s).  opc_i8.cu has how rows are dealt to threads.
+// with values 66 us, 6.6 TB/s; 4097 x 14336 fp16 gated with values 61 us, 6.8 TB/s; 28672 x 4096 fp16
+// quantized with values 86 us, 6.8 TB/s).  opc_i8.cu has how rows are dealt to threads.
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "opc_device.cuh"
 
@@ -38,8 +39,6 @@ struct I8RowsArgs {
   void* values;       // what the codes stand for (or NULL), element type v_type
   int64_t ldx, ldu, ldh, ldc, ldv;
   int32_t rows, n, w_type, v_type;
-  // whether groups of 8 values may be moved 16 bytes at a time (else one value at a time)
-  int32_t vec_x, vec_u, vec_w, vec_h, vec_v;
   float eps, inv_n;   // norm: 1 / n
 };
 
@@ -77,38 +76,52 @@ __device__ __forceinline__ float i8_max3(float a, float b, float c) {
   return d;
 }
 
+// A thread's group of 8 values: with kVec, 8 in a row, moved 16 bytes at a time (every row of every operand
+// starts on 16 bytes); else every 32nd of 256, so that a warp's loads and stores of single values are still
+// of neighbours (4096 x 4097 fp16 quantized: 47.8 us with 8 in a row, 20.8 so).
+template <bool kVec>
+__device__ __forceinline__ int i8_first(int group) {
+  return kVec ? 8 * group : 256 * (group >> 5) + (group & 31);
+}
+template <bool kVec>
+constexpr int i8_stride() {
+  return kVec ? 1 : 32;
+}
+template <bool kVec>
+__device__ __forceinline__ bool i8_whole(int left) {  // `left`: values of the row from the group's first on
+  return left > 7 * i8_stride<kVec>();
+}
+
 // 8 values as they lie in memory.
 template <int kT>
 struct I8Raw {
   uint4 a, b;  // (b: the second half of 32-bit values)
 };
 
-// With !vec, or fewer than 8 left, one at a time, zeros after them.
-template <int kT>
-__device__ __forceinline__ void i8_load8(const void* base, int64_t at, int left, bool vec, I8Raw<kT>& r) {
-  if constexpr (kT == kI8F32) {
-    const uint32_t* p = static_cast<const uint32_t*>(base) + at;
-    if (vec && left >= 8) {
-      r.a = *reinterpret_cast<const uint4*>(p);
-      r.b = *reinterpret_cast<const uint4*>(p + 4);
-    } else {
-      uint32_t v[8];
+// Zeros for those beyond the row.
+template <int kT, bool kVec>
+__device__ __forceinline__ void i8_load8(const void* base, int64_t at, int left, I8Raw<kT>& r) {
+  constexpr int kStep = i8_stride<kVec>();
+  using T = typename std::conditional<kT == kI8F32, uint32_t, uint16_t>::type;
+  const T* p = static_cast<const T*>(base) + at;
+  if (kVec && i8_whole<kVec>(left)) {
+    r.a = *reinterpret_cast<const uint4*>(p);
+    if constexpr (kT == kI8F32) r.b = *reinterpret_cast<const uint4*>(p + 4);
+    return;
+  }
+  uint32_t v[8];
+  if (i8_whole<kVec>(left)) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = i < left ? p[i] : 0u;
-      r.a = make_uint4(v[0], v[1], v[2], v[3]);
-      r.b = make_uint4(v[4], v[5], v[6], v[7]);
-    }
+    for (int i = 0; i < 8; ++i) v[i] = p[kStep * i];
   } else {
-    const uint16_t* p = static_cast<const uint16_t*>(base) + at;
-    if (vec && left >= 8) {
-      r.a = *reinterpret_cast<const uint4*>(p);
-    } else {
-      uint32_t h[4];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        h[i] = (2 * i < left ? p[2 * i] : 0u) | (2 * i + 1 < left ? static_cast<uint32_t>(p[2 * i + 1]) << 16 : 0u);
-      r.a = make_uint4(h[0], h[1], h[2], h[3]);
-    }
+    for (int i = 0; i < 8; ++i) v[i] = kStep * i < left ? p[kStep * i] : 0u;
+  }
+  if constexpr (kT == kI8F32) {
+    r.a = make_uint4(v[0], v[1], v[2], v[3]);
+    r.b = make_uint4(v[4], v[5], v[6], v[7]);
+  } else {
+    r.a = make_uint4(v[0] | v[1] << 16, v[2] | v[3] << 16, v[4] | v[5] << 16, v[6] | v[7] << 16);
   }
 }
 template <int kT>
@@ -132,64 +145,61 @@ __device__ __forceinline__ void i8_open8(const I8Raw<kT>& r, I8Pair (&v)[4]) {
     }
   }
 }
-__device__ __forceinline__ void i8_load8_of(int type, const void* base, int64_t at, int left, bool vec, I8Pair (&v)[4]) {
+template <bool kVec>
+__device__ __forceinline__ void i8_load8_of(int type, const void* base, int64_t at, int left, I8Pair (&v)[4]) {
   if (type == kI8F16) {
     I8Raw<kI8F16> r;
-    i8_load8(base, at, left, vec, r);
+    i8_load8<kI8F16, kVec>(base, at, left, r);
     i8_open8(r, v);
   } else if (type == kI8BF16) {
     I8Raw<kI8BF16> r;
-    i8_load8(base, at, left, vec, r);
+    i8_load8<kI8BF16, kVec>(base, at, left, r);
     i8_open8(r, v);
   } else {
     I8Raw<kI8F32> r;
-    i8_load8(base, at, left, vec, r);
+    i8_load8<kI8F32, kVec>(base, at, left, r);
     i8_open8(r, v);
   }
 }
 
-template <int kT>
-__device__ __forceinline__ void i8_store8(void* base, int64_t at, int left, bool vec, const I8Pair (&v)[4]) {
-  if constexpr (kT == kI8F32) {
-    float* p = static_cast<float*>(base) + at;
-    if (vec && left >= 8) {
-      const float2 a = i8_both(v[0]), b = i8_both(v[1]), c = i8_both(v[2]), d = i8_both(v[3]);
-      *reinterpret_cast<float4*>(p) = make_float4(a.x, a.y, b.x, b.y);
-      *reinterpret_cast<float4*>(p + 4) = make_float4(c.x, c.y, d.x, d.y);
+template <int kT, bool kVec>
+__device__ __forceinline__ void i8_store8(void* base, int64_t at, int left, const I8Pair (&v)[4]) {
+  constexpr int kStep = i8_stride<kVec>();
+  using T = typename std::conditional<kT == kI8F32, uint32_t, uint16_t>::type;
+  T* p = static_cast<T*>(base) + at;
+  uint32_t w[8];  // fp32 values, or pairs of 16-bit ones in the first four
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = i8_both(v[i]);
+    if constexpr (kT == kI8F32) {
+      w[2 * i] = __float_as_uint(f.x);
+      w[2 * i + 1] = __float_as_uint(f.y);
+    } else if constexpr (kT == kI8BF16) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
     } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float2 f = i8_both(v[i >> 1]);
-        if (i < left) p[i] = (i & 1) ? f.y : f.x;
-      }
-    }
-  } else {
-    uint16_t* p = static_cast<uint16_t*>(base) + at;
-    uint32_t h[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = i8_both(v[i]);
-      if constexpr (kT == kI8BF16) {
-        const __nv_bfloat162 b = __floats2bfloat162_rn(f.x, f.y);
-        h[i] = *reinterpret_cast<const uint32_t*>(&b);
-      } else {
-        const __half2 b = __floats2half2_rn(f.x, f.y);
-        h[i] = *reinterpret_cast<const uint32_t*>(&b);
-      }
-    }
-    if (vec && left >= 8) {
-      *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
-    } else {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (i < left) p[i] = static_cast<uint16_t>(h[i >> 1] >> (16 * (i & 1)));
+      const __half2 b = __floats2half2_rn(f.x, f.y);
+      w[i] = *reinterpret_cast<const uint32_t*>(&b);
     }
   }
+  const bool whole = i8_whole<kVec>(left);
+  if (kVec && whole) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+    if constexpr (kT == kI8F32) *reinterpret_cast<uint4*>(p + 4) = make_uint4(w[4], w[5], w[6], w[7]);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (whole || kStep * i < left) {
+      if constexpr (kT == kI8F32) p[kStep * i] = w[i];
+      else p[kStep * i] = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
+    }
 }
-__device__ __forceinline__ void i8_store8_of(int type, void* base, int64_t at, int left, bool vec, const I8Pair (&v)[4]) {
-  if (type == kI8F16) i8_store8<kI8F16>(base, at, left, vec, v);
-  else if (type == kI8BF16) i8_store8<kI8BF16>(base, at, left, vec, v);
-  else i8_store8<kI8F32>(base, at, left, vec, v);
+template <bool kVec>
+__device__ __forceinline__ void i8_store8_of(int type, void* base, int64_t at, int left, const I8Pair (&v)[4]) {
+  if (type == kI8F16) i8_store8<kI8F16, kVec>(base, at, left, v);
+  else if (type == kI8BF16) i8_store8<kI8BF16, kVec>(base, at, left, v);
+  else i8_store8<kI8F32, kVec>(base, at, left, v);
 }
 
 // What a row's reduction carries: max |v| (NaN if a value is), and for the norm two sums of squares,
@@ -284,7 +294,7 @@ __device__ __forceinline__ I8Scale i8_scale_of(const I8Row& s, const I8RowsArgs&
 // byte is the code.  Exact: the quotient is corrected once by its remainder, so it is the nearest fp32,
 // and a half that 16-bit inputs often meet is a half and goes to even (with v * (127 / a) every half of
 // a row goes the way that 127 / a was rounded); where v itself is a rounded result there are none.
-template <bool kLive, bool kExact>
+template <bool kLive, bool kExact, bool kVec>
 __device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, int left, const I8Pair (&v)[4], const I8Scale& s) {
   constexpr float kMagic = 12582912.0f;
   const I8Pair magic = i8_pair(kMagic, kMagic);
@@ -308,18 +318,19 @@ __device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, i
                        __byte_perm(__float_as_uint(hi.x), __float_as_uint(hi.y), 0x0040), 0x5410);
   }
   int8_t* c = a.codes + static_cast<int64_t>(row) * a.ldc + i;
-  if (left >= 8) {
+  const bool whole = i8_whole<kVec>(left);
+  if (kVec && whole) {
     *reinterpret_cast<uint2*>(c) = make_uint2(q[0], q[1]);  // (codes start on 16 bytes, rows too)
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
-      if (e < left) c[e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
+      if (whole || i8_stride<kVec>() * e < left) c[i8_stride<kVec>() * e] = static_cast<int8_t>(q[e >> 2] >> (8 * (e & 3)));
   }
   if (a.values) {
     I8Pair o[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) o[e] = i8_mul2(i8_add2(f[e], i8_pair(-kMagic, -kMagic)), i8_pair(s.scale, s.scale));
-    i8_store8_of(a.v_type, a.values, static_cast<int64_t>(row) * a.ldv + i, left, a.vec_v, o);
+    i8_store8_of<kVec>(a.v_type, a.values, static_cast<int64_t>(row) * a.ldv + i, left, o);
   }
 }
 
@@ -332,7 +343,7 @@ __device__ __forceinline__ float i8_silu_mul(float g, float u) {
 }
 
 // 8 values of a row before its scale from what was loaded, their part of the statistics, and (norm) h_out.
-template <int kOp, int kTX, int kTU, bool kWriteH>
+template <int kOp, int kTX, int kTU, bool kVec, bool kWriteH>
 __device__ __forceinline__ void i8_make8(const I8RowsArgs& a, int row, int i, const I8Raw<kTX>& rx, const I8Raw<kTU>& ru, I8Pair (&v)[4],
                                          I8Stat& s) {
   const int left = a.n - i;
@@ -351,7 +362,7 @@ __device__ __forceinline__ void i8_make8(const I8RowsArgs& a, int row, int i, co
     }
   }
   if constexpr (kOp == kI8Norm) {
-    if (kWriteH && a.h_out) i8_store8<kTX>(a.h_out, static_cast<int64_t>(row) * a.ldh + i, left, a.vec_h, v);
+    if (kWriteH && a.h_out) i8_store8<kTX, kVec>(a.h_out, static_cast<int64_t>(row) * a.ldh + i, left, v);
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       s.ss = i8_fma2(v[e], v[e], s.ss);
@@ -360,7 +371,7 @@ __device__ __forceinline__ void i8_make8(const I8RowsArgs& a, int row, int i, co
     }
     if (a.w) {
       I8Pair w[4];
-      i8_load8_of(a.w_type, a.w, i, left, a.vec_w, w);
+      i8_load8_of<kVec>(a.w_type, a.w, i, left, w);
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = i8_mul2(v[e], w[e]);
     }
@@ -380,7 +391,7 @@ constexpr int i8_resident(int op, int x, int per, bool warp_row) {
 
 // One row per CTA (kWarpRow: per warp), kPer groups of 8 values per thread in registers; kPer 0: rows
 // of any length, read once for the statistics and once more for the codes.
-template <int kOp, int kTX, int kTU, int kPer, bool kWarpRow>
+template <int kOp, int kTX, int kTU, int kPer, bool kWarpRow, bool kVec>
 __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, kPer, kWarpRow)) i8_rows_kernel(const I8RowsArgs a) {
   griddep_wait();
   griddep_launch_dependents();
@@ -396,8 +407,8 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, k
   I8Raw<kTX> rx[kBatch];
   I8Raw<kTU> ru[kBatch];
   const auto load = [&](int i, int j) {
-    i8_load8(a.x, static_cast<int64_t>(row) * a.ldx + i, a.n - i, a.vec_x, rx[j]);
-    if constexpr (kTU != kI8None) i8_load8(a.u, static_cast<int64_t>(row) * a.ldu + i, a.n - i, a.vec_u, ru[j]);
+    i8_load8<kTX, kVec>(a.x, static_cast<int64_t>(row) * a.ldx + i, a.n - i, rx[j]);
+    if constexpr (kTU != kI8None) i8_load8<kTU, kVec>(a.u, static_cast<int64_t>(row) * a.ldu + i, a.n - i, ru[j]);
   };
   if constexpr (kPer > 0) {
     I8Pair v[kPer][4];
@@ -405,13 +416,13 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, k
     for (int j0 = 0; j0 < kPer; j0 += kBatch) {
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int i = 8 * (t + (j0 + j) * threads);
+        const int i = i8_first<kVec>(t + (j0 + j) * threads);
         if (i < a.n) load(i, j);
       }
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int i = 8 * (t + (j0 + j) * threads);
-        if (i < a.n) i8_make8<kOp, kTX, kTU, true>(a, row, i, rx[j], ru[j], v[j0 + j], s);
+        const int i = i8_first<kVec>(t + (j0 + j) * threads);
+        if (i < a.n) i8_make8<kOp, kTX, kTU, kVec, true>(a, row, i, rx[j], ru[j], v[j0 + j], s);
       }
     }
     const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), a, kNorm);
@@ -419,27 +430,27 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, k
     if (sc.live) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
-        const int i = 8 * (t + j * threads);
-        if (i < a.n) i8_write8<true, kExact>(a, row, i, a.n - i, v[j], sc);
+        const int i = i8_first<kVec>(t + j * threads);
+        if (i < a.n) i8_write8<true, kExact, kVec>(a, row, i, a.n - i, v[j], sc);
       }
     } else {
 #pragma unroll 1
-      for (int i = 8 * t; i < a.n; i += 8 * threads) i8_write8<false, kExact>(a, row, i, a.n - i, v[0], sc);
+      for (int g = t, i; (i = i8_first<kVec>(g)) < a.n; g += threads) i8_write8<false, kExact, kVec>(a, row, i, a.n - i, v[0], sc);
     }
   } else {
     I8Pair v[4];
-    for (int i = 8 * t; i < a.n; i += 8 * threads) {
+    for (int g = t, i; (i = i8_first<kVec>(g)) < a.n; g += threads) {
       load(i, 0);
-      i8_make8<kOp, kTX, kTU, false>(a, row, i, rx[0], ru[0], v, s);
+      i8_make8<kOp, kTX, kTU, kVec, false>(a, row, i, rx[0], ru[0], v, s);
     }
     const I8Scale sc = i8_scale_of(i8_reduce<kWarpRow>(s, kNorm), a, kNorm);
     if (t == 0) a.scales[row] = sc.scale;
     I8Stat none{0.f, 0ull, 0ull};
-    for (int i = 8 * t; i < a.n; i += 8 * threads) {  // (h_out may be h: each thread reads a place before it writes it)
+    for (int g = t, i; (i = i8_first<kVec>(g)) < a.n; g += threads) {  // (h_out may be h: each thread reads a place before it writes it)
       load(i, 0);
-      i8_make8<kOp, kTX, kTU, true>(a, row, i, rx[0], ru[0], v, none);
-      if (sc.live) i8_write8<true, kExact>(a, row, i, a.n - i, v, sc);
-      else i8_write8<false, kExact>(a, row, i, a.n - i, v, sc);
+      i8_make8<kOp, kTX, kTU, kVec, true>(a, row, i, rx[0], ru[0], v, none);
+      if (sc.live) i8_write8<true, kExact, kVec>(a, row, i, a.n - i, v, sc);
+      else i8_write8<false, kExact, kVec>(a, row, i, a.n - i, v, sc);
     }
   }
 }
