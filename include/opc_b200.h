@@ -488,7 +488,8 @@ int opc_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int32_t ro
 typedef struct opc_i8_rows {
   int32_t rows, n;                /* rows up to 2^31 - 4096; n 1 .. 131071 (no sum of products of two rows
                                      leaves 32 bits) */
-  int64_t ld;                     /* bytes from a row to the next: a multiple of 16, at least n */
+  int64_t ld;                     /* bytes from a row to the next: a multiple of 16, at least n (products read
+                                     rows that start on 128 bytes fastest) */
   int8_t* codes;                  /* device, 16-byte aligned: [rows][ld]; bytes from n on are neither read nor written */
   float* scales;                  /* device [rows] */
 } opc_i8_rows;

@@ -844,7 +844,7 @@ int load_int8(BFEngine* e, DevLayer* d, void* full) {
   if (!d->present || d->nnz) return 0;
   const int32_t M = d->L.plan.M, K = d->L.plan.K;
   void *codes = nullptr, *scales = nullptr;
-  opc_i8_rows w = {M, K, (static_cast<int64_t>(K) + 15) / 16 * 16, nullptr, nullptr};
+  opc_i8_rows w = {M, K, (static_cast<int64_t>(K) + 127) / 128 * 128, nullptr, nullptr};  // (rows on whole lines are read fastest)
   if (dalloc(e, &codes, static_cast<size_t>(M) * w.ld) || dalloc(e, &scales, static_cast<size_t>(M) * sizeof(float))) return -1;
   w.codes = static_cast<int8_t*>(codes);
   w.scales = static_cast<float*>(scales);
@@ -1117,7 +1117,7 @@ int load_model(BFEngine* e, const char* path, uint32_t max_context) {
     cudaFree(full);
     if (rc) return rc;
     void *codes = nullptr, *scales = nullptr;
-    const size_t width = (static_cast<size_t>(std::max(std::max(e->hidden, qd), e->inter)) + 15) / 16 * 16;
+    const size_t width = (static_cast<size_t>(std::max(std::max(e->hidden, qd), e->inter)) + 127) / 128 * 128;
     if (dalloc(e, &codes, kChunk * width) || dalloc(e, &scales, kChunk * sizeof(float))) return -1;
     e->x8 = static_cast<int8_t*>(codes);
     e->x8_scales = static_cast<float*>(scales);
@@ -1184,7 +1184,7 @@ int enqueue_chunk(BFEngine* e, int n, const Want& want, uint32_t* n_launches) {
   // they stand for in fp16), and the product of x8.
   const bool int8 = e->int8_prompts && n > kGemvMaxBatch;
   const auto rows8 = [&](int width) {
-    return opc_i8_rows{n, width, (static_cast<int64_t>(width) + 15) / 16 * 16, e->x8, e->x8_scales};
+    return opc_i8_rows{n, width, (static_cast<int64_t>(width) + 127) / 128 * 128, e->x8, e->x8_scales};
   };
   const auto in8 = [](std::initializer_list<const DevLayer*> ds) {
     for (const DevLayer* d : ds)
