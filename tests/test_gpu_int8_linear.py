@@ -105,6 +105,18 @@ def test_nan_zero_and_infinite_scales(cuda_device, rows):
     same(y, x, w)
 
 
+@pytest.mark.parametrize("rows", [1, 5, 12, 40, 300])
+@pytest.mark.parametrize("k,ldx,ldw", [(777, 784, 800), (777, 1024, 784), (40, 48, 400), (4100, 4112, 4128)])
+def test_rows_that_start_on_16_bytes_only(cuda_device, rows, k, ldx, ldw):
+    """Weights as they are given (Int8Weight would lay them out anew)."""
+    m = 515
+    x = int8.Int8Rows(int8_ref.codes(rows, k, 1, cuda_device, ld=ldx), int8_ref.scales(rows, 1, cuda_device))
+    held = int8_ref.codes(m + 1, k, 2, cuda_device, ld=ldw)
+    w = int8.Int8Rows(held[1:], int8_ref.scales(m, 2, cuda_device))
+    assert w.c.ld == ldw and w.c.codes % 128
+    same(int8.linear(x, w), x, w)
+
+
 def _random_codes(rows, ld, device, seed):
     return torch.randint(-128, 128, (rows, ld), dtype=torch.int8, device=device, generator=torch.Generator(device=device).manual_seed(seed))
 
