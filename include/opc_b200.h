@@ -481,7 +481,8 @@ int opc_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int32_t ro
  *   code  = round(v * 127 / a)     (to even; -127 .. 127)
  * and stands for scale * code.  A row with a < 2^-100 counts as zeros (scale 0, codes 0).  A row with
  * an infinity or NaN has a NaN scale and codes 0: everything made of it is NaN.  v is formed in fp32
- * from the inputs (silu's exponential to |g| 2^-23 of itself), and so is v * 127 / a before it is rounded
+ * from the inputs (silu's exponential to (|g| + 2) 2^-23 of itself, at gates far below 0 too, which a large u
+ * brings back into range), and so is v * 127 / a before it is rounded
  * to a whole number.  Where nothing was added or gated, that quotient is the nearest fp32: codes of 16-bit
  * inputs taken as they are are exact, halves included.
  * --------------------------------------------------------------------------------------------- */
