@@ -482,9 +482,10 @@ int opc_token_logprobs(const void* logits, int64_t ld, int32_t dtype, int32_t ro
  * and stands for scale * code.  A row with a < 2^-100 counts as zeros (scale 0, codes 0).  A row with
  * an infinity or NaN has a NaN scale and codes 0: everything made of it is NaN.  v is formed in fp32
  * from the inputs (silu's exponential to (|g| + 2) 2^-23 of itself, at gates far below 0 too, which a large u
- * brings back into range), and so is v * 127 / a before it is rounded
- * to a whole number.  Where nothing was added or gated, that quotient is the nearest fp32: codes of 16-bit
- * inputs taken as they are are exact, halves included.
+ * brings back into range), and so is v * 127 / a before it is rounded to a whole number: opc_i8_quantize takes the
+ * fp32 nearest to the quotient (either of two that are as near to 2^-21 steps), so codes of 16-bit inputs are exact,
+ * halves included; a norm to which nothing was added rounds v * 127 before; where something was added or gated, the
+ * quotient is v times 127 / a, to 2^-22 of itself.
  * --------------------------------------------------------------------------------------------- */
 typedef struct opc_i8_rows {
   int32_t rows, n;                /* rows up to 2^31 - 4096; n 1 .. 131071 (no sum of products of two rows

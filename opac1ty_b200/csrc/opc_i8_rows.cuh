@@ -64,6 +64,11 @@ __device__ __forceinline__ I8Pair i8_add2(I8Pair a, I8Pair b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
   return d;
 }
+__device__ __forceinline__ I8Pair i8_sub2(I8Pair a, I8Pair b) {
+  I8Pair d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 __device__ __forceinline__ I8Pair i8_fma2(I8Pair a, I8Pair b, I8Pair c) {
   I8Pair d;
   asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
@@ -254,8 +259,11 @@ __device__ __forceinline__ I8Row i8_reduce(const I8Stat& p, bool norm) {
   return s;
 }
 
-// What the codes are made with.  `exact`: code = round((v * c) / a) with c = 127 and a the largest
-// magnitude, or both times 2^-32 where v * 127 could leave fp32; inv = 1 / a.  Else round(v * mul).
+// How a code is made of a value.  kI8Product: round(v * mul).  The others: round(q), q nearly the quotient (v * c) / a with
+// c = 127 and a the largest magnitude, or both times 2^-32 where v * 127 could leave fp32; inv = 1 / a.  kI8Quotient
+// takes v * c as rounded to fp32 (v of 16 bits: it needs no rounding), kI8Quotient2 with what the rounding left out.
+enum : int { kI8Product = 0, kI8Quotient = 1, kI8Quotient2 = 2 };
+// What the codes are made with.
 // `live` is false for rows of zeros and rows that hold an infinity or NaN, whose codes are 0 whatever v is.
 // Every thread forms them, so they cost as much as several values do: reciprocals to a step or two of
 // fp32 and their products instead of divisions (4097 x 14336 gated 77 -> 47 us).
@@ -291,10 +299,15 @@ __device__ __forceinline__ I8Scale i8_scale_of(const I8Row& s, const I8RowsArgs&
 }
 
 // Codes (and values) of 8 values.  Adding 1.5 * 2^23 rounds to a whole number, to even, whose lowest
-// byte is the code.  Exact: the quotient is corrected once by its remainder, so it is the nearest fp32,
-// and a half that 16-bit inputs often meet is a half and goes to even (with v * (127 / a) every half of
-// a row goes the way that 127 / a was rounded); where v itself is a rounded result there are none.
-template <bool kLive, bool kExact, bool kVec>
+// byte is the code.  A quotient is v * c times inv, off by two steps at most, corrected once by its remainder: within
+// 2^-21 steps of the true one before its last rounding, so the nearest fp32 but where two are that nearly as near.  For
+// values of 16 bits, whose quotients are halves or 2^-12 away from them, a half is a half and goes to even (with v *
+// (127 / a) every half of a row goes the way that 127 / a was rounded).  kI8Quotient2 costs nothing where rows are
+// read from memory and quantized (16384 x 4096 fp32: 69.4 us with and without), but two registers a thread, which a
+// norm of fp32 rows would pay with a CTA an SM (8191 x 4096: 38.6 -> 41.3 us): its v * c keeps its rounding.  Rows
+// that were added or gated, whose values are rounded themselves, take the product; so do 16-bit rows whose sum happened
+// to be exact.
+template <bool kLive, int kHow, bool kVec>
 __device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, int left, const I8Pair (&v)[4], const I8Scale& s) {
   constexpr float kMagic = 12582912.0f;
   const I8Pair magic = i8_pair(kMagic, kMagic);
@@ -303,9 +316,11 @@ __device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, i
   for (int e = 0; e < 4; ++e) {
     if constexpr (!kLive) {
       f[e] = magic;
-    } else if constexpr (kExact) {
+    } else if constexpr (kHow != kI8Product) {
       const I8Pair inv = i8_pair(s.inv, s.inv), t = i8_mul2(v[e], i8_pair(s.c, s.c)), q = i8_mul2(t, inv);
-      f[e] = i8_add2(i8_fma2(i8_fma2(q, i8_pair(-s.a, -s.a), t), inv, q), magic);
+      I8Pair r = i8_fma2(q, i8_pair(-s.a, -s.a), t);
+      if constexpr (kHow == kI8Quotient2) r = i8_sub2(r, i8_fma2(v[e], i8_pair(-s.c, -s.c), t));
+      f[e] = i8_add2(i8_fma2(r, inv, q), magic);
     } else {
       f[e] = i8_fma2(v[e], i8_pair(s.mul, s.mul), magic);
     }
@@ -417,7 +432,7 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, k
   const int row = kWarpRow ? blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5) : blockIdx.x;
   if (kWarpRow && row >= a.rows) return;
   constexpr bool kNorm = kOp == kI8Norm;
-  constexpr bool kExact = kOp != kI8Silu && kTU == kI8None;
+  constexpr int kHow = kOp == kI8Silu || kTU != kI8None ? kI8Product : kOp == kI8Quant && kTX == kI8F32 ? kI8Quotient2 : kI8Quotient;
   I8Stat s{0.f, 0ull, 0ull};
   // groups whose loads are all under way before the first is used (two of 64 registers would not stay in them)
   constexpr int kBatch = kPer < 2 || (kPer == 4 && kTX == kI8F32 && kTU == kI8F32) ? 1 : 2;
@@ -448,11 +463,11 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, k
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const int i = i8_first<kVec>(t + j * threads);
-        if (i < a.n) i8_write8<true, kExact, kVec>(a, row, i, a.n - i, v[j], sc);
+        if (i < a.n) i8_write8<true, kHow, kVec>(a, row, i, a.n - i, v[j], sc);
       }
     } else {
 #pragma unroll 1
-      for (int g = t, i; (i = i8_first<kVec>(g)) < a.n; g += threads) i8_write8<false, kExact, kVec>(a, row, i, a.n - i, v[0], sc);
+      for (int g = t, i; (i = i8_first<kVec>(g)) < a.n; g += threads) i8_write8<false, kHow, kVec>(a, row, i, a.n - i, v[0], sc);
     }
   } else {
     I8Pair v[4];
@@ -466,8 +481,8 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, k
     for (int g = t, i; (i = i8_first<kVec>(g)) < a.n; g += threads) {  // (h_out may be h: each thread reads a place before it writes it)
       load(i, 0);
       i8_make8<kOp, kTX, kTU, kVec, true>(a, row, i, rx[0], ru[0], v, none);
-      if (sc.live) i8_write8<true, kExact, kVec>(a, row, i, a.n - i, v, sc);
-      else i8_write8<false, kExact, kVec>(a, row, i, a.n - i, v, sc);
+      if (sc.live) i8_write8<true, kHow, kVec>(a, row, i, a.n - i, v, sc);
+      else i8_write8<false, kHow, kVec>(a, row, i, a.n - i, v, sc);
     }
   }
 }
