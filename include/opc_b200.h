@@ -508,7 +508,10 @@ typedef struct opc_i8_rows {
  *                      normalized row.  y has h's type, or h is OPC_F32.  eps from 1e-12 on.  (The
  *                      limits of a zero row above are those of t * weight.)  Sums in fp32, a row whose
  *                      squares leave fp32 included; the factor to 2^-21 of itself besides the sum's
- *                      roundings.  Deterministic. */
+ *                      roundings.  With OPC_I8_UNROUNDED added to v_dtype, `values` takes the normalized rows as
+ *                      formed instead (t * weight times the factor, rounded to the type alone): tokens for a
+ *                      layer that is to have them in 16 bits.  Deterministic. */
+enum { OPC_I8_UNROUNDED = 0x100 };
 int opc_i8_quantize(const void* x, int64_t ldx, int32_t dtype, const opc_i8_rows* out, void* values, int64_t ldv,
                     int32_t v_dtype, void* stream);
 int opc_i8_silu_mul(const void* gate, int64_t ldg, const void* up, int64_t ldu, int32_t dtype, const opc_i8_rows* out,

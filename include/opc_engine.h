@@ -110,8 +110,9 @@ BFEngine* bf_engine_create_kv4(const char* path, int32_t device, uint32_t max_co
  *                            of more than 64 tokens take their projections from products in 8-bit
  *                            integers (opc_i8_add_rmsnorm, opc_i8_silu_mul, opc_i8_quantize, opc_i8_gemm),
  *                            with one scale per token and per output channel.  Shorter chunks, decode
- *                            steps, the lm_head and layers with element-wise outliers are computed as
- *                            without it. */
+ *                            steps and the lm_head are computed as without it; layers with element-wise
+ *                            outliers keep their fp16 products, of tokens that are not rounded to 8 bits.
+ */
 enum { BF_ENGINE_KV4 = 1, BF_ENGINE_INT8_PROMPTS = 2 };
 BFEngine* bf_engine_create_with(const char* path, int32_t device, uint32_t max_context, uint32_t options);
 void bf_engine_destroy(BFEngine* engine);

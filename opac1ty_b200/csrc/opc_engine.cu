@@ -1180,8 +1180,8 @@ int enqueue_chunk(BFEngine* e, int n, const Want& want, uint32_t* n_launches) {
     return 0;
   };
   // Chunks that would run opc_gemm take 8-bit products instead where the engine has them.  Their steps,
-  // each for all n tokens: rows into 8 bits (into x8; and, for a layer that has no 8-bit weights, what
-  // they stand for in fp16), and the product of x8.
+  // each for all n tokens: rows into 8 bits (into x8; the norm's also in fp16, not rounded to 8 bits, where a
+  // layer behind it has no 8-bit weights), and the product of x8.
   const bool int8 = e->int8_prompts && n > kGemvMaxBatch;
   const auto rows8 = [&](int width) {
     return opc_i8_rows{n, width, (static_cast<int64_t>(width) + 127) / 128 * 128, e->x8, e->x8_scales};
@@ -1195,7 +1195,7 @@ int enqueue_chunk(BFEngine* e, int n, const Want& want, uint32_t* n_launches) {
     const opc_i8_rows x = rows8(e->hidden);
     ++launches;
     ENG_OPC(e, opc_i8_add_rmsnorm(e->h, e->hidden, OPC_F32, y, e->ld_y, OPC_F16, w, OPC_F16, e->eps, y ? e->h : nullptr, e->hidden, &x,
-                                  only8 ? nullptr : e->xn, e->ld_x, OPC_F16, s));
+                                  only8 ? nullptr : e->xn, e->ld_x, OPC_F16 | OPC_I8_UNROUNDED, s));
     return 0;
   };
   // y = x times the layer, x in fp16 or (int8, where the layer has such weights) as it lies in x8

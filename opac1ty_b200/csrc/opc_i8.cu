@@ -6,6 +6,7 @@
 #include <atomic>
 #include <climits>
 #include <cmath>
+#include <utility>
 
 #include "../../include/opc_b200.h"
 #include "opc_i8_gemm.cuh"
@@ -75,6 +76,14 @@ template <int kOp, int kTX, int kTU>
 cudaError_t launch_rows(const opc::I8RowsArgs& a, bool vec, int sms, void* stream) {
   using opc::i8_rows_kernel;
   const int groups = (a.n + 7) / 8;
+  if constexpr (kOp == opc::kI8Norm) {
+    // Normalized rows beside their codes (tokens for layers of either kind): one kernel for every width, which reads
+    // them twice.  In the others two more values to write for a place would take registers from every call (8191 x
+    // 4096: 44 a thread would be 54, a CTA an SM less).
+    if (a.plain)
+      return launch(vec ? i8_rows_kernel<kOp, kTX, kTU, 0, false, true, true> : i8_rows_kernel<kOp, kTX, kTU, 0, false, false, true>, a.rows,
+                    std::min(1024, (groups + 31) / 32 * 32), stream, a);
+  }
   if (groups <= 128) {
     const int per = (groups + 31) / 32;
     auto k = !vec ? i8_rows_kernel<kOp, kTX, kTU, 4, true, false>
@@ -277,8 +286,11 @@ int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* 
                        void* values, int64_t ldv, int32_t v_dtype, void* stream) {
   const char* who = "opc_i8_add_rmsnorm";
   opc::I8RowsArgs a;
+  const bool unrounded = values && (v_dtype & OPC_I8_UNROUNDED);
+  if (unrounded) v_dtype &= ~OPC_I8_UNROUNDED;
   int rc = start_rows(who, out, values, ldv, v_dtype, &a);
   if (rc != OPC_OK || out->rows == 0) return rc;
+  if (unrounded) std::swap(a.values, a.plain);
   const int32_t n = out->n;
   if ((rc = check_matrix(who, "h", h, ldh, h_dtype, n)) != OPC_OK) return rc;
   if (y && (rc = check_matrix(who, "y", y, ldy, y_dtype, n)) != OPC_OK) return rc;

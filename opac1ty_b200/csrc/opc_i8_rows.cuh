@@ -37,6 +37,7 @@ struct I8RowsArgs {
   int8_t* codes;
   float* scales;
   void* values;       // what the codes stand for (or NULL), element type v_type
+  void* plain;        // norm (kPlain): the normalized row as formed, element type v_type, rows ldv apart
   int64_t ldx, ldu, ldh, ldc, ldv;
   int32_t rows, n, w_type, v_type;
   float eps, inv_n;   // norm: 1 / n
@@ -269,6 +270,7 @@ enum : int { kI8Product = 0, kI8Quotient = 1, kI8Quotient2 = 2 };
 // fp32 and their products instead of divisions (4097 x 14336 gated 77 -> 47 us).
 struct I8Scale {
   float scale, mul, c, a, inv;
+  float factor;  // norm: 1 / sqrt(mean t^2 + eps)
   bool live;
 };
 __device__ __forceinline__ float i8_recip(float x) {
@@ -292,7 +294,8 @@ __device__ __forceinline__ I8Scale i8_scale_of(const I8Row& s, const I8RowsArgs&
     const bool far = !(s.ss < __uint_as_float(0x7f800000u));
     float root;
     asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(far ? s.small * a.inv_n : fmaf(s.ss, a.inv_n, a.eps)));
-    r.scale *= far ? root * 0x1p-80f : root;
+    r.factor = far ? root * 0x1p-80f : root;
+    r.scale *= r.factor;
   }
   r.scale = bad ? __uint_as_float(0x7fffffffu) : r.live ? r.scale : 0.f;
   return r;
@@ -347,6 +350,15 @@ __device__ __forceinline__ void i8_write8(const I8RowsArgs& a, int row, int i, i
     for (int e = 0; e < 4; ++e) o[e] = i8_mul2(i8_add2(f[e], i8_pair(-kMagic, -kMagic)), i8_pair(s.scale, s.scale));
     i8_store8_of<kVec>(a.v_type, a.values, static_cast<int64_t>(row) * a.ldv + i, left, o);
   }
+}
+
+// 8 normalized values, not brought into 8 bits.
+template <bool kVec>
+__device__ __forceinline__ void i8_write_plain(const I8RowsArgs& a, int row, int i, int left, const I8Pair (&v)[4], float factor) {
+  I8Pair o[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = i8_mul2(v[e], i8_pair(factor, factor));
+  i8_store8_of<kVec>(a.v_type, a.plain, static_cast<int64_t>(row) * a.ldv + i, left, o);
 }
 
 __device__ __forceinline__ float i8_ex2(float x) {
@@ -422,8 +434,9 @@ constexpr int i8_resident(int op, int x, int per, bool warp_row) {
 }
 
 // One row per CTA (kWarpRow: per warp), kPer groups of 8 values per thread in registers; kPer 0: rows
-// of any length, read once for the statistics and once more for the codes.
-template <int kOp, int kTX, int kTU, int kPer, bool kWarpRow, bool kVec>
+// of any length, read once for the statistics and once more for the codes.  kPlain (kPer 0): the normalized row is
+// written too, as formed.
+template <int kOp, int kTX, int kTU, int kPer, bool kWarpRow, bool kVec, bool kPlain = false>
 __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, kPer, kWarpRow)) i8_rows_kernel(const I8RowsArgs a) {
   griddep_wait();
   griddep_launch_dependents();
@@ -481,6 +494,7 @@ __global__ void __launch_bounds__(kWarpRow ? 128 : 1024, i8_resident(kOp, kTX, k
     for (int g = t, i; (i = i8_first<kVec>(g)) < a.n; g += threads) {  // (h_out may be h: each thread reads a place before it writes it)
       load(i, 0);
       i8_make8<kOp, kTX, kTU, kVec, true>(a, row, i, rx[0], ru[0], v, none);
+      if constexpr (kPlain) i8_write_plain<kVec>(a, row, i, a.n - i, v, sc.factor);
       if (sc.live) i8_write8<true, kHow, kVec>(a, row, i, a.n - i, v, sc);
       else i8_write8<false, kHow, kVec>(a, row, i, a.n - i, v, sc);
     }
