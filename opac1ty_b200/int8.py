@@ -36,6 +36,7 @@ def _empty(like: torch.Tensor, index: int, shape: Tuple[int, ...], strides: Tupl
 
 
 MAX_WIDTH = 131071  # longest row: no sum of products of two rows leaves 32 bits
+MAX_ROWS = 2**31 - 4096
 
 
 def _row_bytes(n: int) -> int:
@@ -55,8 +56,8 @@ class Int8Rows:
             raise ValueError(f"Int8Rows: codes must be int8 [rows, n] on a CUDA device, got {codes.dtype} "
                              f"{tuple(codes.shape)} on {codes.device}")
         rows, n = codes.shape
-        if n < 1 or n > MAX_WIDTH:
-            raise ValueError(f"Int8Rows: rows of {n} values (1 to {MAX_WIDTH})")
+        if n < 1 or n > MAX_WIDTH or rows > MAX_ROWS:
+            raise ValueError(f"Int8Rows: {rows} rows of {n} values (up to {MAX_ROWS} rows of 1 to {MAX_WIDTH})")
         if scales.dtype != torch.float32 or tuple(scales.shape) != (rows,) or scales.device != codes.device or \
                 (rows > 1 and scales.stride(0) != 1):
             raise ValueError(f"Int8Rows: scales must be contiguous float32 [{rows}] on {codes.device}, got {scales.dtype} "
@@ -73,8 +74,8 @@ class Int8Rows:
     def _new(cls, like: torch.Tensor, rows: int, n: int, values: Optional[torch.dtype]) -> "Int8Rows":
         """Memory for rows of n values on like's device: codes and then scales in one piece (a tensor costs
         more to make than the quantization of a token)."""
-        if n < 1 or n > MAX_WIDTH:
-            raise ValueError(f"rows of {n} values (1 to {MAX_WIDTH})")
+        if n < 1 or n > MAX_WIDTH or rows > MAX_ROWS:  # (the C struct's 32 bits would take more modulo 2^32)
+            raise ValueError(f"{rows} rows of {n} values (up to {MAX_ROWS} rows of 1 to {MAX_WIDTH})")
         if values is not None and values not in _DTYPES:
             raise ValueError(f"values must be float16, bfloat16 or float32, got {values}")
         self = cls.__new__(cls)
