@@ -10,6 +10,8 @@
 A row stands for ``scale * codes`` with scale = max / 127; the definitions, and what rows of zeros and
 rows with infinities or NaN give, are in ``include/opc_b200.h``.  Every computation is a call into
 ``libopc_b200.so``.  There is no backward pass: results carry no gradient, whatever their inputs ask for.
+Tensors given to be written (``out``, ``h_out``) count as changed in place: a backward pass that needs what they
+held before is an error, as after torch's own in-place operations.
 """
 
 from __future__ import annotations
@@ -18,6 +20,7 @@ import ctypes
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib
 from . import layer as L
@@ -204,6 +207,7 @@ def add_rmsnorm(h: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Optio
     index, h_type = h.get_device(), _DTYPES[h.dtype]
     y_ptr = w_ptr = o_ptr = None
     ldy = y_type = w_type = ldo = 0
+    given = h_out is not None
     if y is not None:
         ldy = _matrix("add_rmsnorm", "y", y, rows, n, index)
         y_ptr, y_type = y.data_ptr(), _DTYPES[y.dtype]
@@ -212,7 +216,7 @@ def add_rmsnorm(h: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Optio
         if h_out is None:
             h_out = _empty(h, index, (rows, n), (n, 1), h.dtype)
             o_ptr, ldo = h_out.data_ptr(), n
-    if h_out is not None and o_ptr is None:
+    if given:
         ldo = _matrix("add_rmsnorm", "h_out", h_out, rows, n, index)
         if h_out.dtype != h.dtype:
             raise ValueError(f"add_rmsnorm: h_out is {h_out.dtype}, h {h.dtype}")
@@ -226,7 +230,11 @@ def add_rmsnorm(h: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Optio
     v = out.values
     _call(_lib.load().opc_i8_add_rmsnorm, index, h.data_ptr(), ldh, h_type, y_ptr, ldy, y_type, w_ptr, w_type, eps, o_ptr, ldo,
           out._ref, None if v is None else v.data_ptr(), n, 0 if v is None else _DTYPES[values], _raw_stream(index))
-    return (h if h_out is None else h_out), out
+    if h_out is None:
+        return h, out
+    if given:
+        increment_version(h_out)
+    return h_out, out
 
 
 def linear(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.float16,
@@ -239,9 +247,10 @@ def linear(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = None,
     if out is None:
         if dtype not in _DTYPES:
             raise ValueError(f"linear: results are float16, bfloat16 or float32, not {dtype}")
-        out = _empty(weight.scales, index, (rows, m), (m, 1), dtype)
+        result = _empty(weight.scales, index, (rows, m), (m, 1), dtype)
         ldy = m
     else:
+        result = out
         ldy = _matrix("linear", "out", out, rows, m, index)
         if rows > 1 and ldy < m:
             raise ValueError(f"linear: the rows of out overlap (strides {out.stride()})")
@@ -250,6 +259,8 @@ def linear(x: Int8Rows, weight: Int8Weight, bias: Optional[torch.Tensor] = None,
     if bias is not None:
         _vector("linear", "bias", bias, m, index)
         b_ptr, b_type = bias.data_ptr(), _DTYPES[bias.dtype]
-    _call(_lib.load().opc_i8_gemm, index, x._ref, weight._ref, b_ptr, b_type, out.data_ptr(), ldy, _DTYPES[dtype],
+    _call(_lib.load().opc_i8_gemm, index, x._ref, weight._ref, b_ptr, b_type, result.data_ptr(), ldy, _DTYPES[dtype],
           _raw_stream(index))
-    return out
+    if out is not None:
+        increment_version(out)
+    return result
