@@ -352,7 +352,7 @@ int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, in
   if (bias && (rc = check_matrix(who, "bias", bias, w->rows, bias_dtype, w->rows)) != OPC_OK) return rc;
   opc_host::Device dev;
   if ((rc = opc_host::current_device(&dev)) != OPC_OK) return rc;
-  const opc::I8Out o = {x->scales, w->scales, bias, y, ldy, x->rows, w->rows, bias_dtype, y_dtype};
+  const opc::I8Out o = {x->scales, w->scales, bias, y, ldy, x->rows, w->rows, bias_dtype};
   // Few tokens by mma.sync; beyond 8, which it reads twice as often, only where the weights are few (16 tokens,
   // 4096 -> 4096: 6.7 us instead of 9.0; 4096 -> 28672: 31.7 instead of 22.6).
   if (x->rows <= 8 || (x->rows <= 16 && static_cast<int64_t>(w->rows) * w->n <= 1 << 24)) {

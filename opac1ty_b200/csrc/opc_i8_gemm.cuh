@@ -53,7 +53,7 @@ struct I8Out {
   const void* bias;
   void* y;
   int64_t ldy;
-  int32_t rows, M, bias_type, y_type;
+  int32_t rows, M, bias_type;
 };
 
 // How the tiles are dealt to the pairs of CTAs.
