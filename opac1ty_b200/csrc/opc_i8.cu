@@ -129,57 +129,17 @@ int start_rows(const char* who, const opc_i8_rows* out, void* values, int64_t ld
 }
 
 // ---- the product's plan
-struct GemmPlan {
-  opc::I8Deal deal;
-  int ctas;  // 0: too many tiles
-};
-
-// clusters[s]: how many clusters of s pairs run at once.  The choice is by a model of the time in clocks,
-// fitted to 5 widths and 3 splits of 14 products (in the comments: what was measured, at 1.9 GHz).
-GemmPlan plan_gemm(int32_t rows, int32_t M, int32_t K, const int (&clusters)[5]) {
-  GemmPlan p = {};
-  const int64_t m_tiles = (static_cast<int64_t>(M) + 255) / 256;
-  int64_t best = 0;
-  for (int n = 256; n >= 32; n -= 32) {
-    // Narrow tiles: two blocks a stage, since the barriers of a stage outlast its small MMAs (96 tokens,
-    // 14336 -> 4096: 25.1 -> 21.5 us; 512 tokens, 4096 -> 6144 with tiles of 128: 18.5 -> 17.3; four blocks,
-    // or two in wide tiles, no better).
-    const int sub = n <= 128 ? 2 : 1;
-    const int nk = (K + opc::kI8Block * sub - 1) / (opc::kI8Block * sub);
-    const int64_t n_tiles = (static_cast<int64_t>(rows) + n - 1) / n, tiles = m_tiles * n_tiles;
-    if (tiles > INT32_MAX / 2) continue;
-    for (int split = 1; split <= 4; ++split) {
-      if (split > 1 && (tiles > clusters[split] || nk < 2 * split)) continue;
-      const int64_t rounds = (tiles + clusters[1] - 1) / clusters[1];
-      const int64_t busy = 2 * split * std::min<int64_t>(tiles, clusters[1]);  // CTAs
-      // One block: its MMAs at 2 clocks a token, its loads at 75 bytes a clock into an SM (57 when every SM
-      // loads), the weights' part of them at 3580 a clock from memory.
-      const int64_t rate = 75 - 18 * busy / (2 * clusters[1]);
-      const int64_t block = std::max<int64_t>(std::max<int64_t>(2 * n + 12, (16384 + 64 * n) / rate),
-                                              16384 * busy / (3580 * std::min<int64_t>(n_tiles, 8)));
-      // Then the results of a tile, and for a split tile the exchange of sums (1.2 us for 32 tokens, 2.4 for 256).
-      const int64_t t = rounds * ((nk + split - 1) / split) * sub * block + 19 * n / split + (split > 1 ? 2200 + 10 * n : 0);
-      if (!best || t < best) {
-        best = t;
-        p.deal = {n, static_cast<int32_t>(m_tiles), static_cast<int32_t>(n_tiles), sub, nk, split};
-        p.ctas = static_cast<int>(2 * split * (split > 1 ? tiles : std::min<int64_t>(tiles, clusters[1])));
-      }
-    }
-  }
-  return p;
-}
-
-// The same, remembered by its sizes (a thread's last few; the choice costs about a microsecond).
-GemmPlan plan_of(int32_t rows, int32_t M, int32_t K, const int (&clusters)[5]) {
+// i8_plan, remembered by its sizes (a thread's last few; the choice costs about a microsecond).
+opc::I8Plan plan_of(int32_t rows, int32_t M, int32_t K, const int (&clusters)[5]) {
   struct Known {
     int32_t rows, M, K;
     int clusters[5];
-    GemmPlan plan;
+    opc::I8Plan plan;
   };
   thread_local Known known[8] = {};
   Known& k = known[(static_cast<uint32_t>(rows) * 31u + static_cast<uint32_t>(M) * 7u + static_cast<uint32_t>(K)) / 32u % 8u];
   if (k.rows != rows || k.M != M || k.K != K || !std::equal(clusters + 1, clusters + 5, k.clusters + 1)) {
-    k.plan = plan_gemm(rows, M, K, clusters);
+    k.plan = opc::i8_plan(rows, M, K, clusters);
     k.rows = rows;
     k.M = M;
     k.K = K;
@@ -366,7 +326,7 @@ int opc_i8_gemm(const opc_i8_rows* x, const opc_i8_rows* w, const void* bias, in
   int clusters[5];
   cudaError_t e = gemm_setup(k, y_dtype, &clusters);
   if (e != cudaSuccess) return cuda_fail(e, "opc_i8_gemm: setting up");
-  const GemmPlan p = plan_of(x->rows, w->rows, x->n, clusters);
+  const opc::I8Plan p = plan_of(x->rows, w->rows, x->n, clusters);
   if (!p.ctas) return fail(OPC_ERR_UNSUPPORTED, "%s: %d tokens times %d channels are too many tiles for one call", who, x->rows, w->rows);
   opc::I8GemmArgs a = {o, p.deal, dev.error_word};
   CUtensorMap tw, tx;

@@ -29,24 +29,14 @@
 
 #include <cuda.h>
 
+#include "opc_i8_plan.h"
 #include "opc_i8_rows.cuh"
 #include "opc_tcgen05.cuh"
 
 namespace opc {
 
-constexpr int kI8Block = 128;                 // values of K per stage (one 128-byte swizzled row)
-constexpr int kI8ABytes = 128 * kI8Block;     // a CTA's channels of a stage
 constexpr int kI8Epi = 8;                     // epilogue warps of a CTA
 constexpr int kI8Threads = 64 + 32 * kI8Epi;
-constexpr int kI8Group = 8;                   // channel tiles taken together
-constexpr int kI8MaxStages = 12;
-constexpr int kI8SmemBudget = 227 * 1024 - 1024 - 512;  // less alignment slack and barriers
-
-// A stage holds `sub` blocks of 128 values of K: the channels' block, then half of the tokens'.
-__host__ __device__ constexpr int i8_block_bytes(int n) { return kI8ABytes + n * (kI8Block / 2); }
-__host__ __device__ constexpr int i8_stages(int n, int sub) {
-  return kI8SmemBudget / (sub * i8_block_bytes(n)) > kI8MaxStages ? kI8MaxStages : kI8SmemBudget / (sub * i8_block_bytes(n));
-}
 
 struct I8Out {
   const float *sx, *sw;
@@ -54,15 +44,6 @@ struct I8Out {
   void* y;
   int64_t ldy;
   int32_t rows, M, bias_type;
-};
-
-// How the tiles are dealt to the pairs of CTAs.
-struct I8Deal {
-  int32_t tile_n;              // tokens of a tile
-  int32_t m_tiles, n_tiles;    // tiles of 256 channels, of tile_n tokens
-  int32_t sub;                 // blocks of 128 values of K in a stage
-  int32_t nk;                  // stages of a tile
-  int32_t split;               // 1: a pair does whole tiles in turn; 2 .. 4: so many pairs (a cluster) do one
 };
 
 struct I8GemmArgs {
@@ -156,8 +137,8 @@ struct I8Walk {
   int32_t next, step_, tile, k0, k1;
   // `unit`: the pair, or with split > 1 the cluster, of `units`; `part`: the pair's place in its cluster
   __device__ I8Walk(const I8Deal& deal, int32_t unit, int32_t units, int32_t part) : d(deal), next(unit), step_(units), tile(0) {
-    k0 = d.nk * part / d.split;
-    k1 = d.nk * (part + 1) / d.split;
+    k0 = i8_cut(d, part);
+    k1 = i8_cut(d, part + 1);
   }
   __device__ bool step() {
     if (next >= d.m_tiles * d.n_tiles) return false;
@@ -165,13 +146,7 @@ struct I8Walk {
     next += step_;
     return true;
   }
-  // Channel and token tile: groups of kI8Group channel tiles, channels first.
-  __device__ void place(int32_t* mi, int32_t* ni) const {
-    const int32_t per = kI8Group * d.n_tiles, g = tile / per, in = tile - g * per;
-    const int32_t width = min(kI8Group, d.m_tiles - g * kI8Group);
-    *mi = g * kI8Group + in % width;
-    *ni = in / width;
-  }
+  __device__ void place(int32_t* mi, int32_t* ni) const { i8_place(d, tile, mi, ni); }
 };
 
 // kNum results of one channel, for tokens t, t + 1, ... of which `left` exist.
