@@ -68,7 +68,8 @@ cudaError_t launch(void (*kern)(KArgs...), unsigned ctas, int threads, void* str
 // One warp per row up to 1024 values; beyond, one CTA per row with 16 values a thread, or 8 where there
 // are few rows and a row up to 8192 values (96 x 8192 bf16 norms 3.4 -> 3.2 us, 512 x 4096 fp32 ones 6.1 ->
 // 5.8 us; but 28672 x 4096 quantized 97 -> 111 us), 32 from 16384 values on (shorter rows lose by it: 4097 x
-// 14336 gated 62 -> 83 us; longer ones gain over being read twice: 4096 x 28672 152 -> 138 us).  Rows of more
+// 14336 gated 62 -> 83 us; longer ones gain over being read twice: 4096 x 28672 gated 152 -> 143 us, normalized 322 ->
+// 226; quantized alone they lose by it, 90 -> 108).  Rows of more
 // than 32768 values, which no CTA's registers hold, are read twice.  (Clusters of CTAs that share a long row
 // were slower than either: 4096 x 28672 gated 141 -> 188 us, 4096 x 40000 quantized 125 -> 181.)  Rows that do
 // not all start on 16 bytes are moved value by value.

@@ -10,8 +10,9 @@
 // in registers between the reduction and the rounding.  Bound by memory for large calls, which takes
 // few enough instructions per value that it stays so: pairs of values in packed fp32 operations, one
 // maximum of three per two values (device time with L2 flushed by the inputs: 8191 x 4096 fp32 + fp16 norms
-// with values 66 us, 6.6 TB/s; 4097 x 14336 fp16 gated with values 61 us, 6.8 TB/s; 28672 x 4096 fp16
-// quantized with values 86 us, 6.8 TB/s).  opc_i8.cu has how rows are dealt to threads.
+// with values 67 us, 6.5 TB/s; 4097 x 14336 fp16 gated with values 61 us, 6.8 TB/s; 28672 x 4096 fp16
+// quantized with values 87 us, 6.8 TB/s: of bytes read and written, part of which are still in L2 at the end; memory
+// itself moves 5.8 to 6.0).  opc_i8.cu has how rows are dealt to threads.
 #pragma once
 
 #include <cuda_bf16.h>
