@@ -503,7 +503,8 @@ typedef struct opc_i8_rows {
  * opc_i8_quantize      v = x                      activations, or a layer's weights (row = channel)
  * opc_i8_silu_mul      v = g / (1 + exp(-g)) * u
  * opc_i8_add_rmsnorm   t = h + y (y may be NULL), written to h_out rounded to h's type (h_out may be
- *                      h itself, or NULL); v = t * weight (NULL: ones), and the scale is also divided by
+ *                      h itself, or y of its type, place for place, or NULL; another overlap with what is
+ *                      read is refused); v = t * weight (NULL: ones), and the scale is also divided by
  *                      sqrt(mean t^2 + eps), t as formed, before its rounding: the codes of the
  *                      normalized row.  y has h's type, or h is OPC_F32.  eps from 1e-12 on.  (The
  *                      limits of a zero row above are those of t * weight.)  Sums in fp32, a row whose

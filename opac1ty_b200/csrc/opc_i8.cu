@@ -51,6 +51,18 @@ bool vec_ok(const void* p, int64_t ld, int32_t dtype, int32_t rows) {
   return (reinterpret_cast<uintptr_t>(p) & 15u) == 0 && (!p || rows == 1 || (ld * bytes_of(dtype)) % 16 == 0);
 }
 
+// Whether `rows` rows of wa bytes, pa bytes apart from a on, and rows of wb bytes at b (as many as far apart, or one: pb 0)
+// have no byte in common.
+bool apart(const void* a, int64_t pa, int64_t wa, const void* b, int64_t pb, int64_t wb, int32_t rows) {
+  using i128 = __int128;
+  const i128 from_a = reinterpret_cast<uintptr_t>(a), from_b = reinterpret_cast<uintptr_t>(b);
+  const i128 to_a = from_a + static_cast<i128>(rows - 1) * pa + wa, to_b = from_b + static_cast<i128>(pb ? rows - 1 : 0) * pb + wb;
+  if (to_a <= from_b || to_b <= from_a) return true;
+  if (rows == 1 || (pb && pb != pa)) return false;
+  const i128 in = ((from_b - from_a) % pa + pa) % pa;  // where b's rows begin in a's
+  return in >= wa && pa - in >= wb;
+}
+
 template <typename... KArgs, typename... Args>
 cudaError_t launch(void (*kern)(KArgs...), unsigned ctas, int threads, void* stream, const Args&... args) {
   cudaLaunchConfig_t cfg = {};
@@ -259,6 +271,14 @@ int opc_i8_add_rmsnorm(const void* h, int64_t ldh, int32_t h_dtype, const void* 
     return fail(OPC_ERR_UNSUPPORTED, "%s: y of type %d beside h of type %d (the same, or h of type %d)", who, y_dtype, h_dtype, OPC_F32);
   if (weight && (rc = check_matrix(who, "weight", weight, n, w_dtype, n)) != OPC_OK) return rc;
   if (h_out && (rc = check_matrix(who, "h_out", h_out, ldho, h_dtype, n)) != OPC_OK) return rc;
+  if (h_out) {  // written row by row while others are read: place for place over h or y, or apart from what is read
+    const int64_t size = bytes_of(h_dtype), p = ldho * size, bytes = n * size, y_size = bytes_of(y_dtype);
+    const auto same = [&](const void* q, int64_t ldq) { return h_out == q && (ldho == ldq || out->rows == 1); };
+    if (!(same(h, ldh) || apart(h_out, p, bytes, h, ldh * size, bytes, out->rows)) ||
+        (y && !((y_dtype == h_dtype && same(y, ldy)) || apart(h_out, p, bytes, y, ldy * y_size, n * y_size, out->rows))) ||
+        (weight && !apart(h_out, p, bytes, weight, 0, static_cast<int64_t>(n) * bytes_of(w_dtype), out->rows)))
+      return fail(OPC_ERR_INVALID, "%s: h_out overlaps h, y or the weight (it may be h, or y of its type, place for place)", who);
+  }
   if (!(eps >= 1e-12f) || !std::isfinite(eps)) return fail(OPC_ERR_INVALID, "%s: eps %g (1e-12 or more)", who, static_cast<double>(eps));
   a.x = h;
   a.ldx = ldh;

@@ -200,8 +200,8 @@ def silu_mul(gate: torch.Tensor, up: Optional[torch.Tensor] = None, values: Opti
 def add_rmsnorm(h: torch.Tensor, y: Optional[torch.Tensor] = None, weight: Optional[torch.Tensor] = None, eps: float = 1e-5,
                 h_out: Optional[torch.Tensor] = None, values: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, Int8Rows]:
     """(h + y, the rows of its root-mean-square norm times ``weight`` in 8 bits).  y has h's type, or
-    any beside an h of float32.  The sum goes to ``h_out`` (which may be h) or a new tensor; without y
-    the first result is h itself (or h copied into ``h_out``)."""
+    any beside an h of float32.  The sum goes to ``h_out`` (which may be h, or a y of its type; no other
+    overlap) or a new tensor; without y the first result is h itself (or h copied into ``h_out``)."""
     ldh = _matrix("add_rmsnorm", "h", h)
     rows, n = h.shape
     index, h_type = h.get_device(), _DTYPES[h.dtype]

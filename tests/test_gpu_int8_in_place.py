@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import int8_ref
-from opac1ty_b200 import int8
+from opac1ty_b200 import _lib, int8
 
 pytestmark = pytest.mark.gpu
 F16, F32 = torch.float16, torch.float32
@@ -50,3 +50,26 @@ def test_inputs_are_not_changed(cuda_device):
     int8.quantize(h)
     int8.linear(r, int8.Int8Weight.quantize(h), dtype=F32)
     assert same is h and (h._version, y._version) == versions and new._version == 0
+
+
+@pytest.mark.parametrize("n", [60, 1011, 4096, 14336, 28672, 40000])
+def test_the_sum_over_either_of_its_parts(cuda_device, n):
+    g = torch.Generator(device=cuda_device).manual_seed(n)
+    wide = torch.randn(50, 2 * n + 8, generator=g, device=cuda_device)
+    for h, y in ((wide[:, :n], wide[:, n:2 * n]), (wide[:, :n].half(), wide[:, n:2 * n].half())):
+        want, r = int8.add_rmsnorm(h, y)
+        for first in (True, False):
+            hh, yy = (h.clone(), y.clone()) if h.dtype == F16 else (lambda c: (c[:, :n], c[:, n:2 * n]))(wide.clone())
+            out = hh if first else yy
+            got, s = int8.add_rmsnorm(hh, yy, h_out=out)
+            assert got is out and torch.equal(out, want) and torch.equal(yy if first else hh, y if first else h)
+            assert torch.equal(s.codes, r.codes) and torch.equal(s.scales, r.scales)
+
+
+def test_other_overlaps_are_refused(cuda_device):
+    t = torch.randn(8, 64, device=cuda_device)
+    before = t.clone()
+    for h, y, w, h_out in ((t[:4], None, None, t[1:5]), (t[:4], t[4:], t[0], t[:4]), (t[:2], t[2:4].half(), None, t[1:3])):
+        with pytest.raises(_lib.OpcError, match="overlaps"):
+            int8.add_rmsnorm(h, y, w, h_out=h_out)
+    assert torch.equal(t, before)
